@@ -14,6 +14,7 @@ from .array import (ARRAY_OF_TYPE, ArrowArrayGPU, ArrowType, BooleanArrayGPU, Bo
                     broadcast_dyn, broadcast_op_dyn)
 from .gpu_utils import ArrowComputePipeline, CmpQuery, DeviceBuffer, GpuDevice  # noqa: F401
 from .gpu_utils import gpu_device as GPU_DEVICE  # noqa: F401
+from .rows import BeamSelection, PageMap, QuantisedRowsGPU, RowsGPU  # noqa: F401
 from .kernels import *  # noqa: F401,F403
 from . import interop, ipc, sharding  # noqa: F401,E402
 from .interop import PinnedStaging, from_arrow, from_arrow_batch, from_arrow_chunked, from_arrow_reader, to_arrow  # noqa: F401,E402

@@ -30,6 +30,10 @@ RED_SUM, RED_MIN, RED_MAX = range(3)
 # agpu_comm_dtype
 COMM_F32, COMM_F64, COMM_I32, COMM_U32, COMM_I64, COMM_U64 = range(6)
 COMM_ID_BYTES = 128
+# agpu_row_type, agpu_code_type
+ROW_F32, ROW_F16, ROW_BF16 = range(3)
+CODE_I8, CODE_I4, CODE_E4M3 = range(3)
+NO_ROW = 0xFFFFFFFF
 
 _vp, _u64, _i32, _u32, _i64, _sz = C.c_void_p, C.c_uint64, C.c_int32, C.c_uint32, C.c_int64, C.c_size_t
 _pp = C.POINTER(C.c_void_p)
@@ -161,6 +165,13 @@ SIGNATURES = {
     "agpu_put_bits_bounded": [_vp, _vp, _u64, _vp, _vp, _u64, _vp, _u64],
     "agpu_put": [_vp, _i32, _vp, _vp, _vp, _vp, _u64],
     "agpu_put_bits": [_vp, _vp, _vp, _vp, _vp, _u64],
+    "agpu_put_quantised": [_vp, _i32, _vp, _vp, _vp, _u64],
+    "agpu_put_quantised_pages": [_vp, _i32, _vp, _vp, _vp, _u64],
+    "agpu_take_quantised": [_vp, _i32, _vp, _vp, _vp, _u64],
+    "agpu_take_quantised_pages": [_vp, _i32, _vp, _vp, _vp, _u64],
+    "agpu_take_rows": [_vp, _i32, _vp, _u64, _vp, _vp, _u64],
+    "agpu_select_beams_workspace": [_u32, _u32, _u32, _u32, C.POINTER(_u64)],
+    "agpu_select_beams": [_vp, _vp],
     "agpu_merge": [_vp, _i32, _vp, _vp, _vp, _vp, _u64],
     "agpu_merge_bits": [_vp, _vp, _vp, _vp, _vp, _u64],
     "agpu_index_max": [_vp, _vp, _u64, _vp],
@@ -217,6 +228,33 @@ class ArrowColumnStruct(C.Structure):  # agpu_arrow_column
 
 class IpcFieldStruct(C.Structure):  # agpu_ipc_field
     _fields_ = [("name", C.c_char_p), ("format", C.c_char_p), ("dtype", C.c_int32), ("nullable", C.c_int32)]
+
+
+class RowsStruct(C.Structure):  # agpu_rows
+    _fields_ = [("data", C.c_void_p), ("row_stride", C.c_uint64), ("head_stride", C.c_uint64), ("type", C.c_int32)]
+
+
+class QuantisedRowsStruct(C.Structure):  # agpu_quantised_rows
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("n_slots", C.c_uint64), ("heads", C.c_uint32), ("dim", C.c_uint32),
+                ("group", C.c_uint32), ("code", C.c_int32)]
+
+
+class PageMapStruct(C.Structure):  # agpu_page_map
+    _fields_ = [("tables", C.c_void_p), ("table_stride", C.c_uint64), ("offsets", C.c_void_p), ("first", C.c_void_p), ("n_seqs", C.c_uint32),
+                ("max_pages", C.c_uint32), ("page_rows", C.c_uint32)]
+
+
+class StateStruct(C.Structure):  # agpu_state
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("src_row_stride", C.c_uint64), ("src_piece_stride", C.c_uint64),
+                ("dst_row_stride", C.c_uint64), ("dst_piece_stride", C.c_uint64), ("n_pieces", C.c_uint64), ("piece_bytes", C.c_uint64),
+                ("position_bytes", C.c_uint64)]
+
+
+class BeamsStruct(C.Structure):  # agpu_beams
+    _fields_ = [("logits", C.c_void_p), ("row_stride", C.c_uint64), ("type", C.c_int32), ("batch", C.c_uint32), ("beams", C.c_uint32),
+                ("vocab", C.c_uint32), ("k", C.c_uint32), ("end_token", C.c_uint32), ("scores", C.c_void_p), ("allowed", C.c_void_p),
+                ("allowed_stride", C.c_uint64), ("finished", C.c_void_p), ("out_scores", C.c_void_p), ("out_parents", C.c_void_p),
+                ("out_tokens", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
 
 
 class ArrowErrorGPU(RuntimeError):

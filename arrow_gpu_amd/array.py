@@ -16,7 +16,7 @@ import numpy as np
 
 from . import _capi as capi
 from ._capi import ArrowErrorGPU, CastingNotSupported
-from .gpu_utils import ArrowComputePipeline, DeviceBuffer, GpuDevice
+from .gpu_utils import ArrowComputePipeline, DeviceBuffer, GpuDevice, borrow_tensor, tensor_type
 
 
 class ArrowType(enum.Enum):
@@ -249,6 +249,18 @@ class PrimitiveArrayGpu(ArrowArrayGPU):
         return cls(gpu_device.create_gpu_buffer_with_data(host), gpu_device, len(host), None)
 
     @classmethod
+    def of_tensor(cls, tensor, gpu_device: GpuDevice):
+        """The array over a contiguous tensor's memory, without a copy (integers of one width may change their sign: an int32 tensor is a
+        UInt32ArrayGPU's memory too).  `values()` and the ops see what the tensor holds when they run."""
+        t = tensor_type(tensor)
+        if (t[0] == "f") != (cls.NP_DTYPE is np.float32) or tensor.element_size() != cls.ITEM_SIZE or t == "bf16":
+            raise capi.ArrowErrorGPU("ArgumentError", f"{cls.__name__} over a tensor of {tensor.dtype}", capi.ERR_ARG)
+        if not tensor.is_contiguous():
+            raise capi.ArrowErrorGPU("ShapeError", f"{cls.__name__} over a tensor that is not contiguous", capi.ERR_SHAPE)
+        n = tensor.numel()
+        return cls(borrow_tensor(tensor, gpu_device, n * cls.ITEM_SIZE), gpu_device, n, None)
+
+    @classmethod
     def _to_native(cls, v):
         if np.issubdtype(cls.NP_DTYPE, np.integer):
             info = np.iinfo(cls.NP_DTYPE)
@@ -350,6 +362,15 @@ class BooleanArrayGPU(ArrowArrayGPU):
         """NB: like the reference, `len` is the BYTE count of the slice (boolean_gpu.rs:70-81)."""
         data = np.ascontiguousarray(value, dtype=np.uint8)
         return cls(_upload_bitmap(gpu_device, data, len(data) * 8), gpu_device, len(data), None)
+
+    @classmethod
+    def of_tensor(cls, tensor, gpu_device: GpuDevice, n_bits: Optional[int] = None):
+        """The bitmap over a contiguous 8-bit tensor's memory, without a copy; n_bits: its length (all bits if left out)."""
+        held = tensor.numel()
+        n_bits = 8 * held if n_bits is None else int(n_bits)
+        if tensor.element_size() != 1 or not tensor.is_contiguous() or bitmap_bytes(n_bits) > held:
+            raise capi.ArrowErrorGPU("ShapeError", f"a bitmap of {n_bits} bits needs {bitmap_bytes(n_bits)} contiguous bytes", capi.ERR_SHAPE)
+        return cls(borrow_tensor(tensor, gpu_device, held), gpu_device, n_bits, None)
 
     def raw_bytes(self) -> np.ndarray:
         return self.gpu_device.retrive_data(self.data, (self.len + 7) // 8)

@@ -41,6 +41,45 @@ class DeviceBuffer:
             self.ptr = 0
 
 
+class BorrowedBuffer(DeviceBuffer):
+    """Device memory of somebody else's (a torch tensor's, …).  `owner` is held as long as the buffer is, never freed here."""
+
+    __slots__ = ("owner",)
+
+    def __init__(self, device: "GpuDevice", ptr: int, nbytes: int, owner=None):
+        self.device = device
+        self.ptr = ptr
+        self.nbytes = nbytes
+        self._owned = False
+        self.owner = owner
+
+
+_TENSOR_TYPES = {"float32": "f32", "float16": "f16", "bfloat16": "bf16", "int8": "i8", "uint8": "u8", "int16": "i16", "uint16": "u16", "int32": "i32",
+                 "uint32": "u32", "int64": "i64", "float64": "f64", "float8_e4m3fn": "u8"}
+_TENSOR_TYPE_OF = {}  # dtype object → name
+
+
+def tensor_type(tensor) -> str:
+    """Element type name of a tensor-like object ("f32", "bf16", "i32", …)."""
+    t = _TENSOR_TYPE_OF.get(tensor.dtype)
+    if t is None:
+        t = _TENSOR_TYPES.get(str(tensor.dtype).rsplit(".", 1)[-1])
+        if t is None:
+            raise capi.OperationNotSupported(f"tensors of {tensor.dtype}")
+        _TENSOR_TYPE_OF[tensor.dtype] = t
+    return t
+
+
+def borrow_tensor(tensor, device: "GpuDevice", nbytes: int) -> BorrowedBuffer:
+    """The memory of a tensor on `device` (anything with data_ptr() and device: torch is not needed here).  The rules of torch's own streams hold:
+    the tensor's memory may be given back to its allocator when no work on ANOTHER stream than the tensor's still uses it.  A program that uses
+    torch on the GPU imports it before this library's first call: then both run on the one GPU runtime that torch has loaded."""
+    where = tensor.device
+    if where.type != "cuda" or (where.index or 0) != device.ordinal:
+        raise capi.ArrowErrorGPU("ArgumentError", f"a tensor on {where} for a buffer on GPU {device.ordinal}", capi.ERR_ARG)
+    return BorrowedBuffer(device, tensor.data_ptr(), nbytes, tensor)
+
+
 class GpuDevice:
     """One gfx950 device.  [ref: GpuDevice::new, gpu_device.rs:46-85]"""
 

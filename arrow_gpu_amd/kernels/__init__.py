@@ -8,4 +8,5 @@ from .fused import FusedChain  # noqa: F401
 from .logical import *  # noqa: F401,F403
 from .math import *  # noqa: F401,F403
 from .routines import *  # noqa: F401,F403
+from .rows import *  # noqa: F401,F403
 from .trigonometry import *  # noqa: F401,F403

@@ -1,0 +1,227 @@
+"""Operators on whole rows (include/arrow_gpu.h "rows"): put_quantised / take_quantised — take and put with a cast to 8 or 4 bits between them —
+select_beams, whose parents are an index column, and take_rows, which reorders the states by it.  No counterpart in the reference.
+
+As everywhere here the `*_op` forms enqueue on a pipeline and return without waiting; the plain forms run on a pipeline of their own and wait, so
+that an index out of range is raised by the call.  `out` writes into memory the caller has (a torch tensor's, last step's)."""
+from __future__ import annotations
+
+import ctypes as C
+
+from .. import _capi as capi
+from ..array import BooleanArrayGPU, Float32ArrayGPU, UInt32ArrayGPU
+from ..gpu_utils import ArrowComputePipeline
+from ..rows import ROW_TYPE, BeamSelection, PageMap, QuantisedRowsGPU, RowsGPU, shape_error
+
+_MAX_COLUMNS = 64
+
+
+def _keep(pipeline, *buffers) -> None:
+    """Buffers of this library's own: a borrowed one's lifetime is its owner's affair."""
+    pipeline.keep(*[b for b in buffers if b is not None and b._owned])
+
+
+def _on(pipeline, *things) -> None:
+    dev = pipeline.device
+    for t in things:
+        if t is not None and t.gpu_device is not dev and t.gpu_device.ordinal != dev.ordinal:
+            raise capi.ArrowErrorGPU("ArgumentError", f"memory of GPU {t.gpu_device.ordinal} in a pipeline of GPU {dev.ordinal}", capi.ERR_ARG)
+
+
+def _u32(array, what: str):
+    if not isinstance(array, UInt32ArrayGPU) or array.null_buffer is not None:
+        raise capi.OperationNotSupported(f"{what}: a UInt32ArrayGPU without nulls")
+    return array
+
+
+def _quantised(name: str, stores, rows, where, n: int, pipeline) -> None:
+    k = len(stores)
+    if k > _MAX_COLUMNS:
+        raise shape_error(f"{k} caches in one call: at most {_MAX_COLUMNS}")
+    s, r = (capi.QuantisedRowsStruct * k)(), (capi.RowsStruct * k)()
+    for i, (store, x) in enumerate(zip(stores, rows)):
+        shape, strides = x.shape, x.strides
+        if x.type not in ROW_TYPE:
+            raise capi.OperationNotSupported(f"rows of {x.type} in a quantised cache")
+        if shape[1:] != (store.heads, store.dim) and (store.heads != 1 or shape[1:] != (store.dim,)) or shape[0] != n:
+            raise shape_error(f"rows {shape} for {n} rows of {store.heads} x {store.dim}")
+        s[i] = store.struct
+        v = r[i]
+        v.data, v.row_stride, v.head_stride, v.type = x.ptr, strides[0], strides[1], ROW_TYPE[x.type]
+    _on(pipeline, *stores, *rows)
+    if isinstance(where, PageMap):
+        _on(pipeline, where.tables, where.offsets, where.first)
+        capi.call(name + "_pages", pipeline._handle, k, s, r, C.byref(where.struct), n)
+        _keep(pipeline, where.tables.data, where.offsets.data, where.first.data if where.first is not None else None)
+    else:
+        _on(pipeline, where)
+        capi.call(name, pipeline._handle, k, s, r, where.data.ptr, n)
+        _keep(pipeline, where.data)
+    for store, x in zip(stores, rows):
+        _keep(pipeline, store.codes, store.scales, x.data)
+
+
+def put_quantised_op(stores, rows, where, pipeline: ArrowComputePipeline) -> None:
+    """stores[c] row where[i] = rows[c] row i, quantised: the columns of one table (keys and values, of one layer or of all) by one slot column.
+
+    where: a UInt32ArrayGPU of slots (0xFFFFFFFF: not stored) or a PageMap.  A slot out of range is dropped, and ShapeError at the next sync."""
+    stores = [stores] if isinstance(stores, QuantisedRowsGPU) else stores
+    rows = [rows] if isinstance(rows, RowsGPU) else rows
+    if len(stores) != len(rows):
+        raise shape_error(f"{len(rows)} rows for {len(stores)} caches")
+    if not stores:
+        return
+    n = len(rows[0])
+    if not isinstance(where, PageMap) and _u32(where, "slots").len != n:
+        raise shape_error(f"{where.len} slots for {n} rows")
+    _quantised("agpu_put_quantised", stores, rows, where, n, pipeline)
+
+
+def take_quantised_op(stores, where, pipeline: ArrowComputePipeline, type_: str = "f32", n_rows: int | None = None, out=None) -> list:
+    """[rows of every store], row i = the values of row where[i], in `type_` ("f32", "f16", "bf16").
+
+    where: a UInt32ArrayGPU of slots or a PageMap; with a PageMap `n_rows` (or `out`) says how many rows there are.  A row that `where` names none
+    for (0xFFFFFFFF, behind the last sequence) is left as it was — in `out`; in memory allocated here it is unspecified.  A slot out of range gives
+    zeros, and ShapeError at the next sync."""
+    stores = [stores] if isinstance(stores, QuantisedRowsGPU) else stores
+    out = [out] if isinstance(out, RowsGPU) else out
+    if not stores:
+        return []
+    if out is not None:
+        if len(out) != len(stores):
+            raise shape_error(f"{len(out)} outputs for {len(stores)} caches")
+        n = len(out[0])
+    elif isinstance(where, PageMap):
+        if n_rows is None:
+            raise shape_error("take_quantised through a page map: how many rows? (n_rows or out)")
+        n = int(n_rows)
+    else:
+        n = _u32(where, "slots").len
+    if not isinstance(where, PageMap) and _u32(where, "slots").len != n:
+        raise shape_error(f"{where.len} slots for {n} rows")
+    if out is None:
+        out = [RowsGPU.empty((n, s.heads, s.dim), type_, s.gpu_device) for s in stores]
+    _quantised("agpu_take_quantised", stores, out, where, n, pipeline)
+    return out
+
+
+def take_rows_op(states, indexes: UInt32ArrayGPU, pipeline: ArrowComputePipeline, lengths: UInt32ArrayGPU | None = None, out=None) -> list:
+    """[row indexes[i] of every state]: the states reordered by a selection's parents (any element type, 2 to 4 axes: rows, (pieces,) (positions,)
+    values).  lengths: per row how many positions (the axis before the last) hold anything; what lies behind them is left as it was in `out` (in
+    memory allocated here: unspecified).  An index out of range gives a row of zeros, and ShapeError at the next sync; 0xFFFFFFFF leaves it."""
+    states = [states] if isinstance(states, RowsGPU) else states
+    out = [out] if isinstance(out, RowsGPU) else out
+    n = _u32(indexes, "indexes").len
+    if lengths is not None and _u32(lengths, "lengths").len != n:
+        raise shape_error(f"{lengths.len} lengths for {n} rows")
+    if not states:
+        return []
+    if len(states) > _MAX_COLUMNS:
+        raise shape_error(f"{len(states)} states in one call: at most {_MAX_COLUMNS}")
+    if out is None:
+        out = [RowsGPU.empty((n,) + tuple(s.shape[1:]), s.type, s.gpu_device) for s in states]
+    if len(out) != len(states):
+        raise shape_error(f"{len(out)} outputs for {len(states)} states")
+    v = (capi.StateStruct * len(states))()
+    n_src = len(states[0])
+    for e, s, o in zip(v, states, out):
+        if len(s) != n_src or o.shape[1:] != s.shape[1:] or len(o) != n or o.item_size != s.item_size:
+            raise shape_error(f"rows {o.shape} from a state {s.shape} by {n} indexes, in a call over {n_src} rows")
+        if lengths is not None and len(s.shape) < 3:
+            raise shape_error("lengths count positions: the axis before the last")
+        _state(e, s, o, lengths is not None)
+    _on(pipeline, indexes, lengths, *states, *out)
+    capi.call("agpu_take_rows", pipeline._handle, len(states), v, n_src, indexes.data.ptr, lengths.data.ptr if lengths is not None else None, n)
+    _keep(pipeline, indexes.data, lengths.data if lengths is not None else None, *[s.data for s in states], *[o.data for o in out])
+    return out
+
+
+def _state(e, s: RowsGPU, o: RowsGPU, counted: bool) -> None:
+    """Axes after the first: the trailing ones that lie densely in both are one piece, what is left (at most one axis) are the pieces."""
+    item, shape = s.item_size, s.shape
+    inner, axis = shape[-1], len(shape) - 1
+    e.position_bytes = inner * item
+    while axis > 1 and (shape[axis - 1] == 1 or s.strides[axis - 1] == o.strides[axis - 1] == inner) and not (axis == 2 and len(shape) == 4):
+        axis -= 1
+        inner *= shape[axis]
+    if axis > 2 or (counted and axis > len(shape) - 2):
+        raise shape_error(f"the positions and values of a state lie next to each other: got strides {s.strides} and {o.strides}")
+    e.src, e.dst = s.ptr, o.ptr
+    e.piece_bytes, e.n_pieces = inner * item, shape[1] if axis == 2 else 1
+    e.src_row_stride, e.dst_row_stride = s.strides[0] * item, o.strides[0] * item
+    e.src_piece_stride, e.dst_piece_stride = (s.strides[1] * item, o.strides[1] * item) if axis == 2 else (0, 0)
+
+
+def select_beams_op(logits: RowsGPU, beams: int, k: int, pipeline: ArrowComputePipeline, scores: Float32ArrayGPU | None = None,
+                    allowed: BooleanArrayGPU | None = None, finished: BooleanArrayGPU | None = None, end_token: int = 0,
+                    out: BeamSelection | None = None) -> BeamSelection:
+    """Per request the k best of its beams x tokens by scores[row] + log_softmax(logits[row])[token], best first.
+
+    logits: rows of (batch * beams, vocab).  scores: the rows' running scores (none: 0).  allowed: a bitmap of one row's, or of every row's,
+    vocab bits, each row's on a multiple of 64 bits.  finished: a bitmap of the rows; a finished row's one candidate is (end_token, its score)."""
+    if logits.type not in ROW_TYPE:
+        raise capi.OperationNotSupported(f"logits of {logits.type}")
+    if len(logits.shape) != 2 or beams < 1 or logits.shape[0] % beams:
+        raise shape_error(f"logits {logits.shape} of {beams} beams a request")
+    rows, vocab = logits.shape
+    batch, pitch = rows // beams, (vocab + 63) // 64 * 64
+    if scores is not None and (not isinstance(scores, Float32ArrayGPU) or scores.null_buffer is not None or scores.len != rows):
+        raise shape_error(f"scores: a Float32ArrayGPU of {rows} values without nulls")
+    stride = 0
+    if allowed is not None:
+        if not isinstance(allowed, BooleanArrayGPU) or allowed.null_buffer is not None or allowed.len not in (rows * pitch, pitch, vocab):
+            raise shape_error(f"allowed: a BooleanArrayGPU of {rows} x {pitch} bits, or of one row's, without nulls")
+        stride = pitch // 8 if allowed.len == rows * pitch else 0
+    if finished is not None and (not isinstance(finished, BooleanArrayGPU) or finished.null_buffer is not None or finished.len != rows):
+        raise shape_error(f"finished: a BooleanArrayGPU of {rows} bits without nulls")
+    if not 0 <= end_token < vocab:
+        raise shape_error(f"end_token {end_token} of {vocab} tokens")
+    if not 1 <= k <= 64 or k > beams * vocab:
+        raise shape_error(f"k {k}: 1 to 64, at most {beams} x {vocab}")
+    if out is None:
+        out = BeamSelection.empty(batch, k, pipeline.device)
+    elif (out.batch, out.k) != (batch, k):
+        raise shape_error(f"a selection of {out.batch} x {out.k} for {batch} x {k}")
+    _on(pipeline, logits, scores, allowed, finished, out)
+    if batch == 0:
+        return out
+    need = C.c_uint64()
+    capi.call("agpu_select_beams_workspace", batch, beams, vocab, k, C.byref(need))
+    work = out.ensure_workspace(need.value)
+    args = capi.BeamsStruct(logits.ptr, logits.strides[0], ROW_TYPE[logits.type], batch, beams, vocab, k, end_token,
+                            scores.data.ptr if scores is not None else None, allowed.data.ptr if allowed is not None else None, stride,
+                            finished.data.ptr if finished is not None else None, out.scores.data.ptr, out.parents.data.ptr, out.tokens.data.ptr,
+                            work.ptr, work.nbytes)
+    capi.call("agpu_select_beams", pipeline._handle, C.byref(args))
+    _keep(pipeline, logits.data, scores.data if scores is not None else None, allowed.data if allowed is not None else None,
+          finished.data if finished is not None else None, out.scores.data, out.parents.data, out.tokens.data, work)
+    return out
+
+
+def _waited(device, label: str, op):
+    p = ArrowComputePipeline(device, label)
+    got = op(p)
+    p.finish()
+    p.sync()  # surfaces an index out of range here
+    return got
+
+
+def put_quantised(stores, rows, where) -> None:
+    first = stores if isinstance(stores, QuantisedRowsGPU) else stores[0]
+    _waited(first.gpu_device, "put_quantised", lambda p: put_quantised_op(stores, rows, where, p))
+
+
+def take_quantised(stores, where, type_: str = "f32", n_rows: int | None = None, out=None) -> list:
+    first = stores if isinstance(stores, QuantisedRowsGPU) else stores[0]
+    return _waited(first.gpu_device, "take_quantised", lambda p: take_quantised_op(stores, where, p, type_, n_rows, out))
+
+
+def take_rows(states, indexes: UInt32ArrayGPU, lengths: UInt32ArrayGPU | None = None, out=None) -> list:
+    return _waited(indexes.gpu_device, "take_rows", lambda p: take_rows_op(states, indexes, p, lengths, out))
+
+
+def select_beams(logits: RowsGPU, beams: int, k: int, scores: Float32ArrayGPU | None = None, allowed: BooleanArrayGPU | None = None,
+                 finished: BooleanArrayGPU | None = None, end_token: int = 0, out: BeamSelection | None = None) -> BeamSelection:
+    return _waited(logits.gpu_device, "select_beams", lambda p: select_beams_op(logits, beams, k, p, scores, allowed, finished, end_token, out))
+
+
+__all__ = ["put_quantised", "put_quantised_op", "take_quantised", "take_quantised_op", "take_rows", "take_rows_op", "select_beams", "select_beams_op"]

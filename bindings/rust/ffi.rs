@@ -74,6 +74,14 @@ pub type agpu_chain_kind = i32;
 pub const AGPU_CHAIN_UNARY: agpu_chain_kind = 0;
 pub const AGPU_CHAIN_SCALAR: agpu_chain_kind = 1;
 pub const AGPU_CHAIN_ARRAY: agpu_chain_kind = 2;
+pub type agpu_row_type = i32;
+pub const AGPU_ROW_F32: agpu_row_type = 0;
+pub const AGPU_ROW_F16: agpu_row_type = 1;
+pub const AGPU_ROW_BF16: agpu_row_type = 2;
+pub type agpu_code_type = i32;
+pub const AGPU_CODE_I8: agpu_code_type = 0;
+pub const AGPU_CODE_I4: agpu_code_type = 1;
+pub const AGPU_CODE_E4M3: agpu_code_type = 2;
 pub type agpu_comm_dtype = i32;
 pub const AGPU_COMM_F32: agpu_comm_dtype = 0;
 pub const AGPU_COMM_F64: agpu_comm_dtype = 1;
@@ -103,6 +111,65 @@ pub struct agpu_f32_stats {
     pub max: f32,
     pub reserved: u32,
     pub sum_f64: f64,
+}
+#[repr(C)]
+pub struct agpu_rows {
+    pub data: *mut c_void,
+    pub row_stride: u64,
+    pub head_stride: u64,
+    pub type: i32,
+}
+#[repr(C)]
+pub struct agpu_quantised_rows {
+    pub codes: *mut c_void,
+    pub scales: *mut f32,
+    pub n_slots: u64,
+    pub heads: u32,
+    pub dim: u32,
+    pub group: u32,
+    pub code: i32,
+}
+#[repr(C)]
+pub struct agpu_page_map {
+    pub tables: *const u32,
+    pub table_stride: u64,
+    pub offsets: *const u32,
+    pub first: *const u32,
+    pub n_seqs: u32,
+    pub max_pages: u32,
+    pub page_rows: u32,
+}
+#[repr(C)]
+pub struct agpu_state {
+    pub src: *const c_void,
+    pub dst: *mut c_void,
+    pub src_row_stride: u64,
+    pub src_piece_stride: u64,
+    pub dst_row_stride: u64,
+    pub dst_piece_stride: u64,
+    pub n_pieces: u64,
+    pub piece_bytes: u64,
+    pub position_bytes: u64,
+}
+#[repr(C)]
+pub struct agpu_beams {
+    pub logits: *const c_void,
+    pub row_stride: u64,
+    pub type: i32,
+    pub batch: u32,
+    pub beams: u32,
+    pub vocab: u32,
+    pub k: u32,
+    pub end_token: u32,
+    pub scores: *const f32,
+    pub allowed: *const c_void,
+    pub allowed_stride: u64,
+    pub finished: *const c_void,
+    pub out_scores: *mut f32,
+    pub out_parents: *mut u32,
+    pub out_tokens: *mut u32,
+    pub workspace: *mut c_void,
+    pub workspace_bytes: u64,
 }
 #[repr(C)]
 pub struct agpu_comm_peer {
@@ -258,6 +325,13 @@ extern "C" {
     pub fn agpu_merge(p: *mut agpu_pipeline, width: i32, a: *const c_void, b: *const c_void, mask_bits: *const c_void, out: *mut c_void, n: u64) -> agpu_status;
     pub fn agpu_merge_bits(p: *mut agpu_pipeline, a: *const c_void, b: *const c_void, mask_bits: *const c_void, out: *mut c_void, n_bits: u64) -> agpu_status;
     pub fn agpu_index_max(p: *mut agpu_pipeline, idx: *const u32, n: u64, out_max_dev: *mut u32) -> agpu_status;
+    pub fn agpu_put_quantised(p: *mut agpu_pipeline, n_cols: i32, stores: *const agpu_quantised_rows, rows: *const agpu_rows, slots: *const u32, n: u64) -> agpu_status;
+    pub fn agpu_put_quantised_pages(p: *mut agpu_pipeline, n_cols: i32, stores: *const agpu_quantised_rows, rows: *const agpu_rows, pages: *const agpu_page_map, n: u64) -> agpu_status;
+    pub fn agpu_take_quantised(p: *mut agpu_pipeline, n_cols: i32, stores: *const agpu_quantised_rows, rows: *const agpu_rows, slots: *const u32, n: u64) -> agpu_status;
+    pub fn agpu_take_quantised_pages(p: *mut agpu_pipeline, n_cols: i32, stores: *const agpu_quantised_rows, rows: *const agpu_rows, pages: *const agpu_page_map, n: u64) -> agpu_status;
+    pub fn agpu_take_rows(p: *mut agpu_pipeline, n_states: i32, states: *const agpu_state, n_src: u64, idx: *const u32, lengths: *const u32, n: u64) -> agpu_status;
+    pub fn agpu_select_beams_workspace(batch: u32, beams: u32, vocab: u32, k: u32, out_bytes: *mut u64) -> agpu_status;
+    pub fn agpu_select_beams(p: *mut agpu_pipeline, args: *const agpu_beams) -> agpu_status;
     pub fn agpu_comm_get_unique_id(out_id: *mut c_void) -> agpu_status;
     pub fn agpu_comm_init_rank(dev: *mut agpu_device, unique_id: *const c_void, rank: i32, world: i32, out_comm: *mut *mut agpu_comm) -> agpu_status;
     pub fn agpu_comm_init_rank_timeout(dev: *mut agpu_device, unique_id: *const c_void, rank: i32, world: i32, timeout_ms: i64, out_comm: *mut *mut agpu_comm) -> agpu_status;

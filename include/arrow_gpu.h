@@ -517,6 +517,114 @@ agpu_status agpu_merge_bits(agpu_pipeline* p, const void* a, const void* b, cons
 /* *out_max (device u32) = max(idx[0..n)) — lets a host wrapper reject out-of-range indices (HIP has no robust access) */
 agpu_status agpu_index_max(agpu_pipeline* p, const uint32_t* idx, uint64_t n, uint32_t* out_max_dev);
 
+/* ---------------------------------------------------------------- rows: quantised caches, beam selection, states
+ * Not in the reference, whose widest element is 4 bytes: take and put for WHOLE ROWS (heads x dim values, or any number of bytes), with the
+ * cast that a cache wants between them, and the selection whose result names the rows that the next step keeps.  One step of a beam search
+ * over a cache is  agpu_put_quantised (the new rows) -> agpu_take_quantised_pages (what attention reads) -> agpu_select_beams ->
+ * agpu_take_rows (tables, caches, states by the parents).  Like every kernel call these are asynchronous on the pipeline and copy nothing to
+ * the host; all arguments that are structs are read during the call. */
+typedef enum { AGPU_ROW_F32 = 0, AGPU_ROW_F16 = 1, AGPU_ROW_BF16 = 2 } agpu_row_type;
+typedef enum { AGPU_CODE_I8 = 0, AGPU_CODE_I4 = 1, AGPU_CODE_E4M3 = 2 } agpu_code_type;
+#define AGPU_NO_ROW 0xFFFFFFFFu /* a slot or a page that stands for none: the row is neither stored nor written, and nothing is reported */
+
+/* Rows of heads x dim values: value (i, h, d) is data[i * row_stride + h * head_stride + d], strides in elements (a slice of a fused
+ * projection is such rows).  data is aligned to its element. */
+typedef struct agpu_rows {
+  void* data;
+  uint64_t row_stride;
+  uint64_t head_stride;
+  int32_t type; /* agpu_row_type */
+} agpu_rows;
+
+/* A cache of n_slots rows in 8 or 4 bits.  codes: [n_slots, heads, dim], contiguous, one byte a value; AGPU_CODE_I4: two values a byte, the
+ * even one in the low half (dim and group even).  scales: [n_slots, heads, dim / group] f32; AGPU_CODE_I4: pairs (scale, lowest).
+ * For the values x of one group, in f32:
+ *   I8    span = max |x|,  scale = span / 127, code = rint(x * (127 / span)),  value = code * scale
+ *   E4M3  span = max |x|,  scale = span / 448, code = e4m3(x * (448 / span)),  value = code * scale   (OCP e4m3, ties to even)
+ *   I4    span = max x - min x, scale = span / 15, code = rint((x - min x) * (15 / span)) in 0..15,   value = code * scale + lowest
+ * each quotient rounded to f32; the product of I8 and I4 rounded once, to the nearest whole number, ties to even.  span < top * 2^-126:
+ * scale and codes are 0 (the values come back as 0; I4: as the lowest).  A group with a NaN or an infinity, or an I4 span that overflows:
+ * scale NaN, every value of the group comes back NaN.  group divides dim; 1 <= group <= 65536. */
+typedef struct agpu_quantised_rows {
+  void* codes;
+  float* scales;
+  uint64_t n_slots;
+  uint32_t heads, dim, group;
+  int32_t code; /* agpu_code_type */
+} agpu_quantised_rows;
+
+/* Where the rows of ragged sequences lie in a paged cache: row i belongs to the sequence s with offsets[s] <= i < offsets[s + 1] (offsets:
+ * n_seqs + 1 ascending values), is its position t = first[s] + i - offsets[s] (first NULL: 0) and lies in slot
+ * tables[s * table_stride + t / page_rows] * page_rows + t % page_rows.  Rows before offsets[0] or from offsets[n_seqs] on are AGPU_NO_ROW, and
+ * so is every row of a page AGPU_NO_ROW; a position behind max_pages pages is out of range. */
+typedef struct agpu_page_map {
+  const uint32_t* tables;
+  uint64_t table_stride;
+  const uint32_t* offsets;
+  const uint32_t* first;
+  uint32_t n_seqs, max_pages, page_rows;
+} agpu_page_map;
+
+/* stores[c] row slots[i] = rows[c] row i, quantised, for i < n and c < n_cols <= 64: the columns of one table (keys, values, of one layer or
+ * of all) by one slot column.  A slot >= n_slots is dropped and reported by the next agpu_pipeline_sync (AGPU_ERR_SHAPE), as for put.  The slots of
+ * one call are distinct (AGPU_NO_ROW aside): of a slot named twice the codes and scales may come from either row. */
+agpu_status agpu_put_quantised(agpu_pipeline* p, int32_t n_cols, const agpu_quantised_rows* stores, const agpu_rows* rows,
+                               const uint32_t* slots, uint64_t n);
+agpu_status agpu_put_quantised_pages(agpu_pipeline* p, int32_t n_cols, const agpu_quantised_rows* stores, const agpu_rows* rows,
+                                     const agpu_page_map* pages, uint64_t n);
+/* rows[c] row i = the values of stores[c] row slots[i], rounded once to the rows' type from f32.  A slot >= n_slots gives a row of zeros and is
+ * reported; a row whose slot is AGPU_NO_ROW is left as it was. */
+agpu_status agpu_take_quantised(agpu_pipeline* p, int32_t n_cols, const agpu_quantised_rows* stores, const agpu_rows* rows,
+                                const uint32_t* slots, uint64_t n);
+agpu_status agpu_take_quantised_pages(agpu_pipeline* p, int32_t n_cols, const agpu_quantised_rows* stores, const agpu_rows* rows,
+                                      const agpu_page_map* pages, uint64_t n);
+
+/* The states of take_rows: a row is n_pieces pieces of piece_bytes (a key cache [rows, heads, positions, dim] has heads pieces of
+ * positions * dim values), strides in bytes. */
+typedef struct agpu_state {
+  const void* src;
+  void* dst;
+  uint64_t src_row_stride, src_piece_stride;
+  uint64_t dst_row_stride, dst_piece_stride;
+  uint64_t n_pieces, piece_bytes;
+  uint64_t position_bytes; /* with lengths: bytes of one position inside a piece */
+} agpu_state;
+/* dst row i = src row idx[i], i < n, of every state (n_states <= 64): the reordering of the states by a selection's parents, whatever the bytes
+ * are.  lengths (may be NULL): only the first lengths[i] positions of row i's pieces are copied (all, if they are more than a piece holds), what
+ * lies behind them is left as it was.  idx[i] >= n_src: a row of zeros (of that length), reported by the next sync; AGPU_NO_ROW: the row is left as
+ * it was.  No dst may overlap a src (AGPU_ERR_ARG): rows are not reordered in place. */
+agpu_status agpu_take_rows(agpu_pipeline* p, int32_t n_states, const agpu_state* states, uint64_t n_src, const uint32_t* idx,
+                           const uint32_t* lengths, uint64_t n);
+
+/* Beam search's selection.  logits: [batch * beams, vocab] of an agpu_row_type, row_stride elements apart.  For row r of request b
+ *   score(r, v) = scores[r] + logits[r, v] - log sum_u exp(logits[r, u]),   u over the row's allowed tokens, in 64 bits,
+ * and the k largest of the request's beams * vocab scores go to out_scores / out_parents / out_tokens [batch, k], largest first; parents are
+ * rows r (indices for agpu_take_rows).  Equal scores: the lower row, then the higher logit, then the lower token.  scores NULL: 0.
+ * allowed: per row a bitmap of vocab bits, allowed_stride bytes apart (a multiple of 8, 0: one bitmap for all rows), NULL: every token.  What the
+ * logits of other tokens hold does not matter.  finished: a bitmap of batch * beams rows; a finished row has one candidate, (end_token,
+ * scores[r]), its logits are not read.  A row with a NaN or +infinity among its allowed logits, or with none above -infinity, and a row whose
+ * score is NaN, has scores of -infinity.  Where fewer than k scores are above -infinity, the rest of the k are the other (row, token) in
+ * ascending order with score -infinity.  1 <= k <= 64, k <= beams * vocab, beams <= 1024, batch * beams < 2^24, vocab < 2^31.
+ * workspace: agpu_select_beams_workspace bytes, 16-byte aligned, not shared with a call that may run at the same time (two captured graphs that
+ * hold the same workspace must not be replayed at the same time); its contents need no preparation and are nothing to keep. */
+typedef struct agpu_beams {
+  const void* logits;
+  uint64_t row_stride;
+  int32_t type; /* agpu_row_type */
+  uint32_t batch, beams, vocab, k, end_token;
+  const float* scores;
+  const void* allowed;
+  uint64_t allowed_stride;
+  const void* finished;
+  float* out_scores;
+  uint32_t* out_parents;
+  uint32_t* out_tokens;
+  void* workspace;
+  uint64_t workspace_bytes;
+} agpu_beams;
+agpu_status agpu_select_beams_workspace(uint32_t batch, uint32_t beams, uint32_t vocab, uint32_t k, uint64_t* out_bytes);
+agpu_status agpu_select_beams(agpu_pipeline* p, const agpu_beams* args);
+
 /* ---------------------------------------------------------------- multi-GPU: chunk-sharded columns, RCCL final reduce
  * Not in the reference (single device + single queue [ref: crates/array/src/gpu_utils/gpu_device.rs:29-33]); this is
  * north_star config 5.  One host thread or process per GPU, each with its own agpu_device + pipeline + communicator

@@ -1,0 +1,279 @@
+"""CPU: the row operators' refusals (argument checks come before anything touches a device: with valid arguments the only complaint left is the
+missing pipeline), the Python host's, and the slot arithmetic of the page tables — broken tables too — compiled for the host."""
+import ctypes as C
+import os
+import subprocess
+import types
+
+import numpy as np
+import pytest
+
+import rows_ref as R
+from arrow_gpu_amd import _capi as capi
+
+ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+NO_PIPELINE = (capi.ERR_ARG, "null pipeline")
+
+
+def status(name, *args):
+    st = getattr(capi.lib(), name)(*args)
+    return st, capi.last_error()
+
+
+def store(**kw):
+    a = dict(codes=1 << 20, scales=1 << 21, n_slots=8, heads=2, dim=64, group=32, code=capi.CODE_I8)
+    a.update(kw)
+    return capi.QuantisedRowsStruct(**a)
+
+
+def rows(**kw):
+    a = dict(data=1 << 22, row_stride=128, head_stride=64, type=capi.ROW_BF16)
+    a.update(kw)
+    return capi.RowsStruct(**a)
+
+
+@pytest.mark.parametrize("name", ["agpu_put_quantised", "agpu_take_quantised"])
+@pytest.mark.parametrize("kw,rw,code,text", [
+    ({}, {}, *NO_PIPELINE),
+    (dict(code=3), {}, capi.ERR_ARG, "code type"), (dict(code=-1), {}, capi.ERR_ARG, "code type"),
+    ({}, dict(type=3), capi.ERR_ARG, "row type"),
+    (dict(heads=0), {}, capi.ERR_SHAPE, "heads"), (dict(dim=0), {}, capi.ERR_SHAPE, "heads"), (dict(heads=1 << 20, dim=1 << 12, group=1 << 12), {}, capi.ERR_SHAPE, "heads"),
+    (dict(group=0), {}, capi.ERR_SHAPE, "group"), (dict(group=48), {}, capi.ERR_SHAPE, "group"), (dict(heads=1, dim=1 << 17, group=1 << 17), {}, capi.ERR_SHAPE, "group"),
+    (dict(code=capi.CODE_I4, dim=9, group=9), {}, capi.ERR_SHAPE, "even"),
+    (dict(n_slots=(1 << 32) + 1), {}, capi.ERR_SHAPE, "n_slots"),
+    (dict(codes=0), {}, capi.ERR_ARG, "null"), (dict(scales=0), {}, capi.ERR_ARG, "null"), ({}, dict(data=0), capi.ERR_ARG, "null"),
+    ({}, dict(data=(1 << 22) + 1), capi.ERR_SHAPE, "alignment"), ({}, dict(data=(1 << 22) + 2, type=capi.ROW_F32), capi.ERR_SHAPE, "alignment"),
+    (dict(scales=(1 << 21) + 2), {}, capi.ERR_SHAPE, "alignment")])
+def test_quantised_arguments(name, kw, rw, code, text):
+    st, msg = status(name, None, 1, C.byref(store(**kw)), C.byref(rows(**rw)), 1 << 23, 4)
+    assert st == code and text in msg, msg
+
+
+def test_quantised_calls():
+    s, r = store(), rows()
+    for name in ("agpu_put_quantised", "agpu_take_quantised"):
+        assert status(name, None, 65, C.byref(s), C.byref(r), 1 << 23, 4)[0] == capi.ERR_ARG
+        assert status(name, None, -1, C.byref(s), C.byref(r), 1 << 23, 4)[0] == capi.ERR_ARG
+        assert "null pointer" in status(name, None, 1, C.byref(s), C.byref(r), None, 4)[1]
+        assert "null pointer" in status(name, None, 1, None, C.byref(r), 1 << 23, 4)[1]
+        assert "alignment" in status(name, None, 1, C.byref(s), C.byref(r), (1 << 23) + 1, 4)[1]
+        assert status(name, None, 1, C.byref(s), C.byref(r), 1 << 23, (1 << 32) + 1)[0] == capi.ERR_SHAPE
+        assert NO_PIPELINE[1] in status(name, None, 0, None, None, None, 4)[1]  # nothing to do, but still a pipeline's call
+        assert NO_PIPELINE[1] in status(name, None, 1, None, None, None, 0)[1]
+    # rows that are written may not lie on each other; read ones may (a broadcast row)
+    for kw in (dict(head_stride=63), dict(row_stride=63), dict(head_stride=0)):
+        assert "overlap" in status("agpu_take_quantised", None, 1, C.byref(s), C.byref(rows(**kw)), 1 << 23, 4)[1]
+        assert NO_PIPELINE[1] in status("agpu_put_quantised", None, 1, C.byref(s), C.byref(rows(**kw)), 1 << 23, 4)[1]
+
+
+def test_page_arguments():
+    def pages(**kw):
+        a = dict(tables=1 << 24, table_stride=4, offsets=1 << 25, first=None, n_seqs=3, max_pages=4, page_rows=16)
+        a.update(kw)
+        return capi.PageMapStruct(**a)
+
+    s, r = store(), rows()
+    for name in ("agpu_put_quantised_pages", "agpu_take_quantised_pages"):
+        call = lambda m: status(name, None, 1, C.byref(s), C.byref(r), C.byref(m), 4)  # noqa: E731, B023
+        assert NO_PIPELINE[1] in call(pages())[1]
+        assert NO_PIPELINE[1] in call(pages(tables=None, max_pages=0))[1]
+        assert call(pages(tables=None))[0] == capi.ERR_ARG
+        assert call(pages(offsets=None))[0] == capi.ERR_ARG
+        for kw in (dict(n_seqs=0), dict(n_seqs=1 << 31), dict(page_rows=0), dict(tables=(1 << 24) + 1), dict(offsets=(1 << 25) + 2), dict(first=3)):
+            assert call(pages(**kw))[0] == capi.ERR_SHAPE, kw
+        assert status(name, None, 1, C.byref(s), C.byref(r), None, 4)[0] == capi.ERR_ARG
+
+
+def test_take_rows_arguments():
+    def state(**kw):
+        a = dict(src=1 << 30, dst=1 << 40, src_row_stride=4096, src_piece_stride=1024, dst_row_stride=4096, dst_piece_stride=1024, n_pieces=4, piece_bytes=1024, position_bytes=64)
+        a.update(kw)
+        return capi.StateStruct(**a)
+
+    def call(*states, n_src=8, idx=1 << 20, lengths=None, n=8):
+        v = (capi.StateStruct * max(len(states), 1))(*states)
+        return status("agpu_take_rows", None, len(states), v, n_src, idx, lengths, n)
+
+    assert NO_PIPELINE[1] in call(state())[1] and NO_PIPELINE[1] in call()[1] and NO_PIPELINE[1] in call(state(), n=0)[1]
+    assert NO_PIPELINE[1] in call(state(), lengths=1 << 21)[1]
+    assert call(*[state()] * 65)[0] == capi.ERR_ARG
+    assert call(state(), idx=None)[0] == capi.ERR_ARG
+    assert call(state(src=None))[0] == capi.ERR_ARG and call(state(dst=None))[0] == capi.ERR_ARG
+    assert NO_PIPELINE[1] in call(state(src=None), n_src=0)[1]  # no rows to take from: every index is out of range
+    assert call(state(), idx=(1 << 20) + 2)[0] == capi.ERR_SHAPE and call(state(), lengths=(1 << 20) + 2)[0] == capi.ERR_SHAPE
+    assert "overlap" in call(state(dst_piece_stride=1023))[1] and "overlap" in call(state(dst_row_stride=100))[1]
+    assert "position_bytes" in call(state(position_bytes=0), lengths=1 << 21)[1]
+    assert NO_PIPELINE[1] in call(state(position_bytes=0))[1]
+    assert "address space" in call(state(src_row_stride=1 << 62))[1] and "address space" in call(state(n_pieces=1 << 40, piece_bytes=1 << 30, dst_piece_stride=1 << 30))[1]
+    assert "address space" in call(state(piece_bytes=(1 << 64) - 1, dst_piece_stride=(1 << 64) - 1, dst_row_stride=(1 << 64) - 1))[1]
+    # in place, by one byte, and one state's dst on another's src
+    assert call(state(dst=1 << 30))[0] == capi.ERR_ARG
+    assert call(state(dst=(1 << 30) + 8 * 4096 - 1))[0] == capi.ERR_ARG and NO_PIPELINE[1] in call(state(dst=(1 << 30) + 8 * 4096))[1]
+    assert call(state(dst=(1 << 30) - 8 * 4096 + 1))[0] == capi.ERR_ARG and NO_PIPELINE[1] in call(state(dst=(1 << 30) - 8 * 4096))[1]
+    assert call(state(), state(src=1 << 40, dst=1 << 41))[0] == capi.ERR_ARG
+
+
+def test_select_beams_arguments():
+    def beams(**kw):
+        a = dict(logits=1 << 20, row_stride=1000, type=capi.ROW_F16, batch=2, beams=4, vocab=1000, k=8, end_token=0, scores=1 << 21, allowed=1 << 22, allowed_stride=128,
+                 finished=1 << 23, out_scores=1 << 24, out_parents=1 << 25, out_tokens=1 << 26, workspace=1 << 27, workspace_bytes=1 << 30)
+        a.update(kw)
+        return status("agpu_select_beams", None, C.byref(capi.BeamsStruct(**a)))
+
+    assert NO_PIPELINE[1] in beams()[1] and NO_PIPELINE[1] in beams(batch=0, logits=0)[1]
+    assert NO_PIPELINE[1] in beams(scores=0, allowed=0, finished=0, allowed_stride=0)[1]
+    assert status("agpu_select_beams", None, None)[0] == capi.ERR_ARG
+    for kw in (dict(type=3), dict(logits=0), dict(out_scores=0), dict(out_parents=0), dict(out_tokens=0), dict(workspace=0)):
+        assert beams(**kw)[0] == capi.ERR_ARG, kw
+    for kw in (dict(k=0), dict(k=65), dict(beams=0), dict(beams=1025), dict(vocab=0), dict(vocab=1 << 31), dict(k=9, beams=1, vocab=8), dict(batch=1 << 22),
+               dict(workspace_bytes=8), dict(end_token=1000), dict(row_stride=999), dict(allowed_stride=120), dict(allowed_stride=132), dict(logits=(1 << 20) + 1),
+               dict(scores=(1 << 21) + 1), dict(allowed=(1 << 22) + 4), dict(finished=(1 << 23) + 4), dict(out_scores=(1 << 24) + 2), dict(out_tokens=(1 << 26) + 2),
+               dict(workspace=(1 << 27) + 8)):
+        assert beams(**kw)[0] == capi.ERR_SHAPE, kw
+    n = C.c_uint64(1)
+    assert status("agpu_select_beams_workspace", 0, 0, 0, 0, C.byref(n))[0] == 0 and n.value == 0
+    assert status("agpu_select_beams_workspace", 2, 4, 1000, 8, C.byref(n))[0] == 0 and n.value > 0
+    assert status("agpu_select_beams_workspace", 2, 4, 1000, 8, None)[0] == capi.ERR_ARG
+
+
+# ---------------------------------------------------------------------------------------------------------- the Python host
+class _Device:
+    ordinal = 0
+    _handle = None
+
+
+def _host():
+    import arrow_gpu_amd as ag
+
+    dev = _Device()
+    buf = lambda n: ag.DeviceBuffer(dev, 4096, n, owned=False)  # noqa: E731
+    pipe = types.SimpleNamespace(device=dev, _handle=None, keep=lambda *a: None)
+    return ag, dev, buf, pipe
+
+
+def test_python_refusals():
+    ag, dev, buf, pipe = _host()
+    idx = lambda n: ag.UInt32ArrayGPU(buf(4 * n), dev, n, None)  # noqa: E731
+    view = lambda shape, t="f32", strides=None: ag.RowsGPU(buf(1), dev, shape, t, strides)  # noqa: E731
+    cache = lambda **kw: ag.QuantisedRowsGPU(buf(1), buf(1), dev, **{**dict(n_slots=4, heads=2, dim=8, group=4, code="i8"), **kw})  # noqa: E731
+    for bad in (lambda: view((3,)), lambda: view((1, 2, 3, 4, 5)), lambda: view((2, 2), strides=(1, 2)), lambda: view((2, 2), strides=(-2, 1)),
+                lambda: cache(group=3), lambda: cache(dim=6, group=3, code="i4"), lambda: cache(heads=0),
+                lambda: ag.put_quantised_op(cache(), view((3, 2, 8)), idx(4), pipe), lambda: ag.put_quantised_op(cache(), view((3, 16)), idx(3), pipe),
+                lambda: ag.put_quantised_op([cache(), cache()], [view((3, 2, 8))], idx(3), pipe),
+                lambda: ag.put_quantised_op([cache(), cache()], [view((3, 2, 8)), view((4, 2, 8))], idx(3), pipe),
+                lambda: ag.take_quantised_op(cache(), idx(3), pipe, out=view((4, 2, 8))), lambda: ag.put_quantised_op([cache()] * 65, [view((3, 2, 8))] * 65, idx(3), pipe),
+                lambda: ag.PageMap(view((3, 2), "u32"), 4, idx(3)), lambda: ag.PageMap(view((3, 2), "u32"), 0, idx(4)), lambda: ag.PageMap(view((3, 2)), 4, idx(4)),
+                lambda: ag.PageMap(view((3, 2), "u32"), 4, idx(4), idx(4)),
+                lambda: ag.take_quantised_op(cache(), ag.PageMap(view((3, 2), "u32"), 4, idx(4)), pipe),
+                lambda: ag.take_rows_op(view((3, 4)), idx(3), pipe, lengths=idx(3), out=view((3, 4))), lambda: ag.take_rows_op(view((3, 2, 4)), idx(3), pipe, lengths=idx(2), out=view((3, 2, 4))),
+                lambda: ag.take_rows_op(view((3, 4)), idx(3), pipe, out=view((2, 4))), lambda: ag.take_rows_op([view((3, 4)), view((2, 4))], idx(3), pipe, out=[view((3, 4))] * 2),
+                lambda: ag.take_rows_op(view((3, 4)), idx(3), pipe, out=view((3, 4), "f16")),
+                lambda: ag.take_rows_op(view((3, 2, 5, 4), strides=(100, 50, 8, 1)), idx(3), pipe, out=view((3, 2, 5, 4))),
+                lambda: ag.take_rows_op(view((3, 5, 4), strides=(100, 8, 1)), idx(3), pipe, lengths=idx(3), out=view((3, 5, 4))),
+                lambda: ag.select_beams_op(view((7, 10)), 2, 4, pipe), lambda: ag.select_beams_op(view((6, 10)), 2, 0, pipe), lambda: ag.select_beams_op(view((6, 10)), 2, 65, pipe),
+                lambda: ag.select_beams_op(view((6, 10)), 2, 21, pipe), lambda: ag.select_beams_op(view((6, 10)), 2, 4, pipe, end_token=10),
+                lambda: ag.select_beams_op(view((6, 10)), 2, 4, pipe, scores=ag.Float32ArrayGPU(buf(4), dev, 5, None)),
+                lambda: ag.select_beams_op(view((6, 10)), 2, 4, pipe, allowed=ag.BooleanArrayGPU(buf(8), dev, 60, None)),
+                lambda: ag.select_beams_op(view((6, 10)), 2, 4, pipe, finished=ag.BooleanArrayGPU(buf(8), dev, 64, None)),
+                lambda: ag.select_beams_op(view((6, 10)), 2, 4, pipe, out=ag.BeamSelection(*[t(buf(4), dev, 9, None) for t in (ag.Float32ArrayGPU, ag.UInt32ArrayGPU, ag.UInt32ArrayGPU)], dev, 3, 3))):
+        with pytest.raises(ag.ArrowErrorGPU) as e:
+            bad()
+        assert e.value.status == capi.ERR_SHAPE, e.value
+    for bad in (lambda: view((2, 2), "c64"), lambda: cache(code="i5"), lambda: ag.put_quantised_op(cache(), view((3, 2, 8), "i32"), idx(3), pipe),
+                lambda: ag.take_rows_op(view((3, 4)), ag.Int32ArrayGPU(buf(12), dev, 3, None), pipe), lambda: ag.select_beams_op(view((6, 10), "i32"), 2, 4, pipe)):
+        with pytest.raises(ag.OperationNotSupported):
+            bad()
+    other = _Device()
+    other.ordinal = 1
+    with pytest.raises(ag.ArrowErrorGPU) as e:  # memory of another GPU
+        ag.take_rows_op(ag.RowsGPU(buf(1), other, (3, 4), "f32"), idx(3), pipe, out=view((3, 4)))
+    assert e.value.status == capi.ERR_ARG
+
+
+# ------------------------------------------------------------------------------------------------- slots, broken tables too
+SRC = r"""
+#include "%s/arrow_gpu_amd/csrc/row_address.hpp"
+extern "C" void slots(const uint32_t* slot_column, const uint32_t* tables, uint64_t stride, const uint32_t* offsets, const uint32_t* first, uint32_t n_seqs,
+                      uint32_t max_pages, uint32_t page_rows, uint64_t n, uint64_t n_slots, int64_t* out) {
+  const RowAddr a = {slot_column, tables, stride, offsets, first, n_seqs, max_pages, page_rows};
+  for (uint64_t i = 0; i < n; i++) out[i] = (int64_t)row_slot(a, i, n_slots);
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def slots_lib(tmp_path_factory):
+    d = tmp_path_factory.mktemp("rows")
+    (d / "s.cpp").write_text(SRC % ROOT)
+    subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-shared", "-fPIC", "-o", str(d / "s.so"), str(d / "s.cpp")], check=True, timeout=120)
+    return C.CDLL(str(d / "s.so"))
+
+
+def _slots(lib, n, n_slots, column=None, tables=None, offsets=None, first=None, page_rows=1):
+    ptr = lambda a: a.ctypes.data_as(C.c_void_p) if a is not None else None  # noqa: E731
+    got = np.zeros(n, np.int64)
+    lib.slots(ptr(column), ptr(tables), C.c_uint64(tables.shape[1] if tables is not None else 0), ptr(offsets), ptr(first), C.c_uint32(len(offsets) - 1 if offsets is not None else 0),
+              C.c_uint32(tables.shape[1] if tables is not None else 0), C.c_uint32(page_rows), C.c_uint64(n), C.c_uint64(n_slots), ptr(got))
+    return got
+
+
+def test_slots_of_a_column(slots_lib):
+    c = np.array([0, 7, 8, R.NO_ROW, 0xFFFFFFFE, 3], np.uint32)
+    assert _slots(slots_lib, 6, 8, c).tolist() == [0, 7, -2, -1, -2, 3]
+    assert _slots(slots_lib, 6, 1 << 32, c).tolist() == [0, 7, 8, -1, 0xFFFFFFFE, 3]
+    assert _slots(slots_lib, 6, 0, c).tolist() == [-2, -2, -2, -1, -2, -2]
+
+
+@pytest.mark.parametrize("seed", range(30))
+def test_slots_of_pages(slots_lib, seed):
+    rng = np.random.default_rng(seed)
+    seqs, page = int(rng.integers(1, 20)), int(rng.choice([1, 2, 5, 16, 1000]))
+    lens = rng.integers(0, 40, seqs) * (rng.random(seqs) < 0.7)
+    offsets = (int(rng.integers(0, 4)) + np.concatenate([[0], np.cumsum(lens)])).astype(np.uint32)
+    first = rng.integers(0, 50, seqs).astype(np.uint32) if seed % 2 else None
+    tables = rng.integers(0, 60, (seqs, int(rng.integers(1, 30)))).astype(np.uint32)
+    tables[rng.random(tables.shape) < 0.1] = R.NO_ROW
+    tables[rng.random(tables.shape) < 0.05] = 0xFFFFFFFE
+    n = int(offsets[-1]) + 5
+    assert np.array_equal(_slots(slots_lib, n, 50 * page, None, tables, offsets, first, page), R.slots_of(tables, page, offsets, n, 50 * page, first))
+
+
+@pytest.mark.parametrize("seed", range(30))
+def test_broken_offsets_stay_inside_the_tables(slots_lib, seed):
+    """offsets in any order: every answer is a slot of the cache, none, or out of range — and no table is read past its end (the tables end in front
+    of a guard that would give a slot of its own)"""
+    rng = np.random.default_rng(seed)
+    seqs, most, page = int(rng.integers(1, 12)), int(rng.integers(1, 6)), int(rng.integers(1, 9))
+    tables = np.zeros((seqs + 1, most), np.uint32)
+    tables[:seqs] = rng.integers(0, 9, (seqs, most))
+    tables[seqs] = 10  # the guard: slots 10 * page and up
+    offsets = rng.integers(0, 30, seqs + 1).astype(np.uint32)
+    first = rng.choice(np.array([0, 1, 7, 0xFFFFFFFF], np.uint32), seqs)
+    got = _slots(slots_lib, 40, 20 * page, None, tables[:seqs], offsets, first, page)
+    assert ((got >= -2) & (got < 10 * page)).all()
+
+
+def test_the_reference_agrees_with_torch():
+    """rows_ref's 8-bit type and quantiser against torch's conversion and a formula written apart"""
+    torch = pytest.importorskip("torch")
+    v = R.e4m3_values()
+    t = torch.arange(256, dtype=torch.uint8).view(torch.float8_e4m3fn).double().numpy()
+    assert np.array_equal(v[~np.isnan(v)], t[~np.isnan(t)]) and np.array_equal(np.isnan(v), np.isnan(t))
+    x = np.concatenate([np.random.default_rng(0).uniform(-448, 448, 20000), np.random.default_rng(1).normal(0, 0.02, 20000), (v[:126] + v[1:127]) / 2, v[:127], -v[:127]]).astype(np.float32)
+    got = torch.from_numpy(x).to(torch.float8_e4m3fn).view(torch.uint8).numpy()
+    assert np.array_equal(R.to_e4m3(x) & 127, got & 127)
+    y = np.random.default_rng(2).standard_normal((3, 2, 8)).astype(np.float32)
+    c, s = R.quantise(y, "i8", 4)
+    a = np.abs(y.reshape(3, 2, 2, 4)).max(-1)
+    assert np.array_equal(s, a / np.float32(127)) and np.abs(R.values(c, s, "i8", 4) - y).max() <= a.max() / 127 * 0.5001
+
+
+def test_the_reference_selection_agrees_with_torch():
+    torch = pytest.importorskip("torch")
+    x = np.random.default_rng(0).standard_normal((6, 40))
+    cum = np.random.default_rng(1).standard_normal(6).astype(np.float32)
+    s, r, t = R.select(x, 3, 5, cum)
+    z = (torch.log_softmax(torch.from_numpy(x), -1) + torch.from_numpy(cum).double()[:, None]).reshape(2, -1)
+    v, i = torch.topk(z, 5)
+    assert np.allclose(s, v.numpy(), rtol=1e-13, atol=1e-13)
+    assert np.array_equal(r, (i // 40).numpy() + np.array([[0], [3]])) and np.array_equal(t, (i % 40).numpy())
