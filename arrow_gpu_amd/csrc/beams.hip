@@ -1,13 +1,14 @@
 // beams.hip — beam search's selection: log-softmax over every row's vocabulary and the k best of a request's rows x tokens.
 //
-// One pass over the logits.  A row is cut into segments of one block each, whose logits stay in registers: the segment's maximum M, the sum of
-// exp(x − M), and its k best tokens go to the workspace; a block a request joins the segments (log-sum-exp as M + log S, sums rescaled by
-// exp(M' − M)) and selects among the segments' bests by score.
+// One pass over the logits.  A row is cut into segments of one WAVE each; the wave streams its segment, adding up exp(x) and keeping the tokens that
+// can be among its k best, and leaves (sum, k best) in the workspace.  A block a request joins the sums and selects among the segments' bests.
+// No wave waits for another before the join, and none needs the maximum first: f64 holds exp(x − first tile's maximum) for all x of a row
+// whose logits are less than 600 apart; a segment that holds others is read again.
 //
 // Why 64 bits: the result is whole numbers, and rows that compete differ by their log-sums only — a log-sum 1e-7 off swaps tokens of two beams.
-// The f64 unit runs at the rate of the f32 one here, so exp is made there: x − M = (256 e + j + r) · c, c = ln 2 / 256, |r| <= 1/2, exp = 2^e · 2^(j/256) ·
-// (1 + r c + r² c² / 2), the middle factor from a table in LDS.  The cubic term that is left out is at most 4.2e-10 and odd: over many tokens it
-// cancels.
+// The f64 unit runs at the rate of the f32 one here, so exp is made there: with c = ln 2 / 256, x = (256 e + j + r) c, |r| <= 1/2,
+// exp(x) = 2^e · 2^(j/256) · (1 + r c + r² c² / 2), the middle factor from a table in LDS.  The cubic term that is left out is at most 4.2e-10, and
+// odd: over many tokens it cancels.
 #include "common.hpp"
 
 namespace {
@@ -28,14 +29,11 @@ struct BeamArgs {
   uint32_t* out_tokens;
   uint32_t segs;
 };
-// a segment's part of its row; count: how many of its k entries there are, BAD: it holds a NaN or +infinity
+// a segment's part of its row: sum = Σ exp(x − ref), NaN where it holds a NaN or +infinity, 0 where nothing is above −infinity
 struct SegSum {
-  double sum;
-  float max;
-  uint32_t count;
+  double sum, ref;
 };
-constexpr uint32_t BAD = 0xFFFFFFFFu;
-struct Entry {
+struct Entry {  // logit −infinity: none
   float logit;
   uint32_t token;
 };
@@ -59,18 +57,17 @@ constexpr ExpTable make_exp_table() {
 }
 __device__ const ExpTable exp_table = make_exp_table();
 
-// exp(d), d = x − M <= 0
-__device__ __forceinline__ double exp_of(double d, const double* table) {
-  const double magic = 0x1.8p52, scale = EXP_STEPS / 0.69314718055994530942, c = 0.69314718055994530942 / EXP_STEPS;
-  d = fmax(d, -690.0);  // 1e-300, nothing beside the maximum's 1; −infinity too
-  const double z = __builtin_fma(d, scale, magic);  // its low word: the whole number nearest to d · 256 / ln 2
+constexpr double EXP_C = 0.69314718055994530942 / EXP_STEPS, EXP_SCALE = EXP_STEPS / 0.69314718055994530942, EXP_MAGIC = 0x1.8p52;
+// exp(x − ref), ref = (EXP_MAGIC − k) · EXP_C a whole number of steps: no subtraction, the steps of ref leave with the whole number.  |x| <= 2^30
+__device__ __forceinline__ void add_exp(double& sum, double x, double k, const double* table) {
+  const double z = __builtin_fma(x, EXP_SCALE, k);  // its low word: steps of x, less those of ref
   const int n = (int)__builtin_bit_cast(uint64_t, z);
-  const double r = __builtin_fma(d, scale, magic - z), f = table[n & (EXP_STEPS - 1)];
-  const double p = __builtin_fma(r, __builtin_fma(r, c * c / 2, c), 1.0);
-  return __builtin_ldexp(p * f, n >> 8);
+  const double r = __builtin_fma(x, EXP_SCALE, k - z), f = __builtin_ldexp(table[n & (EXP_STEPS - 1)], n >> 8);
+  sum = __builtin_fma(f, __builtin_fma(r, __builtin_fma(r, EXP_C * EXP_C / 2, EXP_C), 1.0), sum);
 }
 
 // ---------------------------------------------------------------- order
+constexpr float LOWEST = -__builtin_inff();
 // u32 that grows with the value; −0 counts as +0
 __device__ __forceinline__ uint32_t order_of(float x) {
   const uint32_t b = __builtin_bit_cast(uint32_t, x + 0.0f);
@@ -78,140 +75,208 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 }
 __device__ __forceinline__ float value_of(uint32_t o) { return __builtin_bit_cast(float, o ^ ((o >> 31) ? 0x80000000u : 0xFFFFFFFFu)); }
 
-// the k-th largest of a wave's values: bit by bit, how many lanes reach the prefix.  `low`: bits that are 0 in every value, or do not matter
-__device__ __forceinline__ uint32_t wave_kth(uint32_t v, uint32_t k, int low) {
-  uint32_t t = 0;
-  for (int b = 31; b >= low; b--)
-    if ((uint32_t)__popcll(__ballot(v >= (t | 1u << b))) >= k) t |= 1u << b;
-  return t;
+// a value that at least k of the wave's 64 (x[0], … x[N − 1] of every lane) reach, −infinity if there are none: the k-th largest, its bits below
+// `low` cleared — found bit by bit, by how many reach the prefix
+template <int N>
+__device__ __forceinline__ float wave_kth(const float (&x)[N], uint32_t k, int low) {
+  uint32_t o[N], t = 0;
+#pragma unroll
+  for (int i = 0; i < N; i++) o[i] = order_of(x[i]);
+  for (int b = 31; b >= low; b--) {
+    const uint32_t up = t | 1u << b;
+    uint32_t n = 0;
+#pragma unroll
+    for (int i = 0; i < N; i++) n += (uint32_t)__popcll(__ballot(o[i] >= up));
+    t = n >= k ? up : t;
+  }
+  return t > order_of(LOWEST) ? value_of(t) : LOWEST;
 }
 
 // ---------------------------------------------------------------- a segment
-template <typename T> struct Raw;  // what an order's low bits hold
-template <> struct Raw<float> { static constexpr int low = 0; };
-template <> struct Raw<f16_t> { static constexpr int low = 13; };  // (of negative values these bits are all set: the prefix lies below, and still above the next)
-template <> struct Raw<bf16_t> { static constexpr int low = 16; };
+template <typename T> struct Raw;  // low: bits of an order that are equal in all values of the type of one sign
+template <> struct Raw<float> {
+  static constexpr int low = 0;
+  static __device__ __forceinline__ float at(u32x4 w, int i) {
+    const uint32_t b = w[i];  // (a bit cast of w[i] itself takes element 0)
+    return __builtin_bit_cast(float, b);
+  }
+};
+template <> struct Raw<f16_t> {
+  static constexpr int low = 13;
+  static __device__ __forceinline__ float at(u32x4 w, int i) { return (float)__builtin_bit_cast(f16_t, (uint16_t)(w[i / 2] >> (i & 1) * 16)); }
+};
+template <> struct Raw<bf16_t> {
+  static constexpr int low = 16;
+  static __device__ __forceinline__ float at(u32x4 w, int i) { return __builtin_bit_cast(float, (i & 1) ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16); }
+};
 
-constexpr int LIST = 512;
+constexpr int TILE = 1024;  // logits a wave takes at a time: 16 a lane
+constexpr int LIST = 512;   // tokens it can keep: 18 + 9 + 6 + … for k = 16 and logits in no order, 230 for k = 64
 
-template <typename T, int VPT>
-__global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, SegSum* sums, Entry* entries) {
-  constexpr int VE = 16 / sizeof(T), EPT = VPT * VE;
+template <typename T, bool MASK>
+struct Segment {
+  static constexpr int VE = 16 / sizeof(T), U = TILE / 64 / VE;
+  const T* x;           // the row
+  const uint8_t* bits;  // its allowed tokens
+  uint32_t vocab, lead, lane;
+
+  // first token of vector u of tile t: vectors lie on 16 bytes, the row starts `lead` elements into its first
+  __device__ __forceinline__ int64_t token(uint32_t t, int u) const { return (int64_t)t * TILE + u * (64 * VE) + lane * VE - lead; }
+
+  __device__ __forceinline__ void load(uint32_t t, u32x4 (&w)[U], uint32_t (&m)[U]) const {
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+      const int64_t at = token(t, u);
+      if (at >= 0 && at + VE <= vocab) {
+        w[u] = *reinterpret_cast<const u32x4*>(x + at);
+        m[u] = ~0u;
+      } else {  // the row's ends
+        T e[VE] = {};
+        m[u] = 0;
+#pragma unroll
+        for (int i = 0; i < VE; i++)
+          if (at + i >= 0 && at + i < vocab) e[i] = x[at + i], m[u] |= 1u << i;
+        w[u] = __builtin_bit_cast(u32x4, e);
+      }
+      if (MASK && m[u]) {
+        const uint32_t first = at < 0 ? 0u : (uint32_t)at, byte = first >> 3, last = (vocab - 1) >> 3;
+        const uint32_t b = (bits[byte] | (uint32_t)bits[byte < last ? byte + 1 : last] << 8) >> (first & 7);
+        m[u] &= at < 0 ? b << -at : b;
+      }
+    }
+  }
+  // the logits, −infinity for what is not allowed
+  __device__ __forceinline__ void values(const u32x4 (&w)[U], const uint32_t (&m)[U], float (&v)[U * VE]) const {
+#pragma unroll
+    for (int u = 0; u < U; u++) {
+#pragma unroll
+      for (int i = 0; i < VE; i++) v[u * VE + i] = Raw<T>::at(w[u], i);
+      if (MASK || !__all(m[u] == ~0u)) {
+#pragma unroll
+        for (int i = 0; i < VE; i++) v[u * VE + i] = (m[u] >> i & 1) ? v[u * VE + i] : LOWEST;
+      }
+    }
+  }
+};
+
+template <typename T, bool MASK>
+__global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, uint32_t tiles, uint32_t n_segs, SegSum* sums, Entry* entries) {
+  typedef Segment<T, MASK> S;
+  constexpr int VE = S::VE, U = S::U, EPT = U * VE;
   __shared__ double table[EXP_STEPS];
-  __shared__ double wave_sum[AGPU_BLOCK / 64];
-  __shared__ uint64_t list[LIST];
-  __shared__ float wave_max[AGPU_BLOCK / 64];
-  __shared__ uint32_t wave_t[AGPU_BLOCK / 64], wave_bad[AGPU_BLOCK / 64], count;
-  const uint32_t row = blockIdx.x / a.segs, seg = blockIdx.x - row * a.segs, wave = threadIdx.x >> 6;
-  if (is_finished(a, row)) return;
+  __shared__ uint64_t lists[AGPU_BLOCK / 64][LIST];
   table[threadIdx.x] = exp_table.v[threadIdx.x];
-  if (threadIdx.x == 0) count = 0;
+  __syncthreads();  // the only one: from here on every wave is by itself
+  const uint32_t id = __builtin_amdgcn_readfirstlane(blockIdx.x * (AGPU_BLOCK / 64) + (threadIdx.x >> 6)), lane = threadIdx.x & 63;
+  if (id >= n_segs) return;
+  const uint32_t row = id / a.segs, seg = id - row * a.segs;
+  if (is_finished(a, row)) return;
+  uint64_t* list = lists[threadIdx.x >> 6];
 
-  // vectors on 16 bytes; the row starts `lead` elements into the first
-  const T* x = static_cast<const T*>(a.logits) + row * a.row_stride;
-  const uint32_t lead = (uint32_t)(reinterpret_cast<uintptr_t>(x) & 15) / sizeof(T);
-  const uint8_t* bits = a.allowed ? a.allowed + row * a.allowed_stride : nullptr;
-  const uint32_t last_byte = (a.vocab - 1) >> 3;
-  float v[EPT];
-  bool bad = false;
-  float tm = -__builtin_inff();
+  S s;
+  s.x = static_cast<const T*>(a.logits) + row * a.row_stride;
+  s.bits = MASK ? a.allowed + row * a.allowed_stride : nullptr;
+  s.vocab = a.vocab;
+  s.lead = (uint32_t)(reinterpret_cast<uintptr_t>(s.x) & 15) / sizeof(T);
+  s.lane = lane;
+  const uint32_t t0 = seg * tiles, row_tiles = (uint32_t)(((uint64_t)a.vocab + s.lead + TILE - 1) / TILE), t1 = t0 + tiles < row_tiles ? t0 + tiles : row_tiles;
+
+  float top[2] = {LOWEST, LOWEST};  // the largest of the lane's first and second eight logits of every tile
+  float floor_v = LOWEST, ref_v = 0.0f;
+  double sum = 0.0, k = EXP_MAGIC;
+  uint32_t count = 0, negative_nan = 0;
+  u32x4 w[U], next[U];
+  uint32_t m[U], next_m[U];
+  if (t0 < t1) s.load(t0, w, m);
+  for (uint32_t t = t0; t < t1; t++) {
+    if (t + 1 < t1) s.load(t + 1, next, next_m);
+    float v[EPT];
+    s.values(w, m, v);
+    float tm[2] = {v[0], v[EPT / 2]};
 #pragma unroll
-  for (int u = 0; u < VPT; u++) {
-    const int64_t at = ((int64_t)seg * VPT + u) * AGPU_BLOCK * VE + threadIdx.x * VE - lead;
-    if (at >= 0 && at + VE <= a.vocab) {
-      typedef T vec __attribute__((ext_vector_type(VE)));
-      const vec w = *reinterpret_cast<const vec*>(x + at);
-#pragma unroll
-      for (int i = 0; i < VE; i++) v[u * VE + i] = (float)w[i];
-    } else {
-#pragma unroll
-      for (int i = 0; i < VE; i++) v[u * VE + i] = at + i >= 0 && at + i < a.vocab ? (float)x[at + i] : -__builtin_inff();
+    for (int i = 1; i < EPT / 2; i++) tm[0] = fmaxf(tm[0], v[i]), tm[1] = fmaxf(tm[1], v[EPT / 2 + i]);
+    top[0] = fmaxf(top[0], tm[0]), top[1] = fmaxf(top[1], tm[1]);
+    if (t == t0) {  // the reference: the tile's maximum, as far as it is an ordinary number
+      float f = fmaxf(tm[0], tm[1]);
+      for (int d = 32; d; d >>= 1) f = fmaxf(f, __shfl_xor(f, d));
+      ref_v = __builtin_fabsf(f) <= 16384.0f ? f : 0.0f;
+      k = EXP_MAGIC - __builtin_rint((double)ref_v * EXP_SCALE);
     }
-    if (bits && at + VE > 0 && at < a.vocab) {
-      const uint32_t t = at < 0 ? 0u : (uint32_t)at, byte = t >> 3;
-      uint32_t m = (bits[byte] | (uint32_t)bits[byte < last_byte ? byte + 1 : byte] << 8) >> (t & 7);
-      if (at < 0) m <<= -at;
+    if (__any(fmaxf(tm[0], tm[1]) >= floor_v)) {
+      if (((t - t0) & (t - t0 + 1)) == 0) floor_v = wave_kth(top, a.k, Raw<T>::low);  // tiles 0, 1, 3, 7 …
+      const float above = fmaxf(floor_v, -0x1.fffffep127f);
 #pragma unroll
-      for (int i = 0; i < VE; i++) v[u * VE + i] = (m >> i & 1) ? v[u * VE + i] : -__builtin_inff();
-    }
-#pragma unroll
-    for (int i = 0; i < VE; i++) {
-      bad |= !(v[u * VE + i] < __builtin_inff());
-      tm = fmaxf(tm, v[u * VE + i]);
-    }
-  }
-
-  // the wave's maximum, and a value that at least k of its logits reach: the k-th largest of the lanes' maxima
-  float m = tm;
-  for (int d = 32; d; d >>= 1) m = fmaxf(m, __shfl_xor(m, d));
-  const uint32_t t = wave_kth(order_of(tm), a.k, Raw<T>::low);
-  bad = __any(bad);
-  if ((threadIdx.x & 63) == 0) wave_max[wave] = m, wave_t[wave] = t, wave_bad[wave] = bad;
-  __syncthreads();
-  m = wave_max[0];
-  uint32_t least = wave_t[0], any_bad = wave_bad[0];
-#pragma unroll
-  for (int w = 1; w < AGPU_BLOCK / 64; w++) {
-    m = fmaxf(m, wave_max[w]);
-    least = least > wave_t[w] ? least : wave_t[w];
-    any_bad |= wave_bad[w];
-  }
-  SegSum* mine = sums + (uint64_t)row * a.segs + seg;
-  if (any_bad || m == -__builtin_inff()) {  // nothing to select here
-    if (threadIdx.x == 0) *mine = {0.0, m, any_bad ? BAD : 0u};
-    return;
-  }
-
-  const double top = m;
-  double sum = 0.0;
-#pragma unroll
-  for (int i = 0; i < EPT; i++) sum += exp_of((double)v[i] - top, table);
-  for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
-  if ((threadIdx.x & 63) == 0) wave_sum[wave] = sum;
-
-  // what reaches the block's threshold, as (logit, token) in one number: larger is better
-  const float floor_v = least > order_of(-__builtin_inff()) ? value_of(least) : -__builtin_inff();
-  if (order_of(tm) >= least && tm > -__builtin_inff()) {
-#pragma unroll
-    for (int u = 0; u < VPT; u++)
-#pragma unroll
-      for (int i = 0; i < VE; i++)
-        if (v[u * VE + i] >= floor_v && v[u * VE + i] > -__builtin_inff()) {
-          const uint32_t at = atomicAdd(&count, 1u);
-          if (at < LIST) list[at] = (uint64_t)order_of(v[u * VE + i]) << 32 | ~(((seg * VPT + u) * AGPU_BLOCK + threadIdx.x) * VE + i - lead);
+      for (int i = 0; i < EPT; i++) {
+        const uint64_t who = __ballot(v[i] >= above);
+        if (who) {
+          const uint32_t at = count + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+          if (v[i] >= above && at < LIST) list[at] = (uint64_t)order_of(v[i]) << 32 | ~(uint32_t)(s.token(t, i / VE) + i % VE);
+          count += (uint32_t)__popcll(who);
         }
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < EPT; i++) {
+      // at least −2^30: the unsigned order of negative numbers grows downwards.  It keeps +infinity and positive NaN, which make the sum NaN
+      const uint32_t b = __builtin_bit_cast(uint32_t, v[i]), low = 0xCE800000u;
+      negative_nan = b > negative_nan ? b : negative_nan;
+      add_exp(sum, (double)__builtin_bit_cast(float, b < low ? b : low), k, table);
+    }
+#pragma unroll
+    for (int u = 0; u < U; u++) w[u] = next[u], m[u] = next_m[u];
   }
-  __syncthreads();
-  const uint32_t n = count;
-  Entry* out = entries + ((uint64_t)row * a.segs + seg) * a.k;
-  if (threadIdx.x == 0) *mine = {wave_sum[0] + wave_sum[1] + wave_sum[2] + wave_sum[3], m, n < a.k ? n : a.k};
-  if (n <= LIST) {
-    for (uint32_t i = threadIdx.x; i < n; i += AGPU_BLOCK) {
+
+  for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+  float most = fmaxf(top[0], top[1]);
+  for (int d = 32; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
+  double ref = (EXP_MAGIC - k) * EXP_C;
+  if (most > LOWEST && most < __builtin_inff() && __builtin_fabsf(most - ref_v) > 600.0f) {  // again, below the maximum that is now known
+    ref = most;
+    sum = 0.0;
+    for (uint32_t t = t0; t < t1; t++) {
+      float v[EPT];
+      s.load(t, w, m);
+      s.values(w, m, v);
+#pragma unroll
+      for (int i = 0; i < EPT; i++) {
+        const double d = (double)v[i] - ref;
+        add_exp(sum, d < -0x1p30 ? -0x1p30 : d, EXP_MAGIC, table);
+      }
+    }
+    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+  }
+  if (__any(negative_nan > 0xFF800000u) || most == __builtin_inff()) sum = __builtin_nan("");
+  if (lane == 0) sums[id] = {most > LOWEST || sum != sum ? sum : 0.0, ref};
+
+  Entry* out = entries + (uint64_t)id * a.k;
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the list was written by other lanes
+  if (count <= LIST) {
+    if (lane >= count && lane < a.k) out[lane] = {LOWEST, 0};
+    for (uint32_t i = lane; i < count; i += 64) {
       const uint64_t e = list[i];
       uint32_t rank = 0;
-      for (uint32_t j = 0; j < n; j++) rank += list[j] > e;
+      for (uint32_t j = 0; j < count; j++) rank += list[j] > e;
       if (rank < a.k) out[rank] = {value_of((uint32_t)(e >> 32)), ~(uint32_t)e};
     }
-  } else {  // very many equal logits: the best, then the best behind it, k times
+  } else {  // very many equal logits, or ascending ones: the best, then the best behind it, k times
     uint64_t before = ~0ull;
     for (uint32_t r = 0; r < a.k; r++) {
       uint64_t best = 0;
+      for (uint32_t t = t0; t < t1; t++) {
+        float v[EPT];
+        s.load(t, w, m);
+        s.values(w, m, v);
 #pragma unroll
-      for (int u = 0; u < VPT; u++)
-#pragma unroll
-        for (int i = 0; i < VE; i++) {
-          const uint64_t e = (uint64_t)order_of(v[u * VE + i]) << 32 | ~(((seg * VPT + u) * AGPU_BLOCK + threadIdx.x) * VE + i - lead);
-          if (e < before && e > best && v[u * VE + i] > -__builtin_inff()) best = e;
+        for (int i = 0; i < EPT; i++) {
+          const uint64_t e = (uint64_t)order_of(v[i]) << 32 | ~(uint32_t)(s.token(t, i / VE) + i % VE);
+          if (e < before && e > best && v[i] > LOWEST) best = e;
         }
+      }
       for (int d = 32; d; d >>= 1) {
         const uint64_t o = __shfl_xor(best, d);
         best = o > best ? o : best;
       }
-      __syncthreads();
-      if ((threadIdx.x & 63) == 0) list[wave] = best;
-      __syncthreads();
-      for (int w = 0; w < AGPU_BLOCK / 64; w++) best = list[w] > best ? list[w] : best;
-      if (threadIdx.x == 0) out[r] = {value_of((uint32_t)(best >> 32)), ~(uint32_t)best};
+      if (lane == 0) out[r] = {value_of((uint32_t)(best >> 32)), ~(uint32_t)best};
       before = best;
     }
   }
@@ -230,70 +295,82 @@ __device__ __forceinline__ bool better(const Candidate& x, const Candidate& y) {
   return x.token < y.token;
 }
 
-constexpr int MERGE_LIST = 512;
+constexpr int MERGE_BLOCK = 1024, MERGE_LIST = 512, HELD = 4;
 
-__global__ __launch_bounds__(AGPU_BLOCK) void beam_merge_kernel(BeamArgs a, const SegSum* sums, const Entry* entries) {
+// Lists of k entries, best first: the largest scores among a few heads of them give a bound that k candidates reach; what reaches it goes to LDS and
+// is ranked there by counting.
+__global__ __launch_bounds__(MERGE_BLOCK) void beam_merge_kernel(BeamArgs a, const SegSum* sums, const Entry* entries) {
   __shared__ double lse[1024];  // per beam: its log-sum, NaN for a row whose scores are −infinity
+  __shared__ float cum[1024];
   __shared__ Candidate list[MERGE_LIST];
   __shared__ uint64_t chosen[64];
-  __shared__ uint32_t wave_t[AGPU_BLOCK / 64], count;
+  __shared__ uint32_t count;
   const uint32_t r0 = blockIdx.x * a.beams, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, per_row = a.segs * a.k, n = a.beams * per_row;
   const double none = -__builtin_inf();
+  entries += (uint64_t)r0 * per_row;
+  Entry held[HELD], heads[HELD];
+#pragma unroll
+  for (int i = 0; i < HELD; i++) {
+    const uint32_t e = threadIdx.x + i * MERGE_BLOCK;
+    held[i] = e < n ? entries[e] : Entry{LOWEST, 0};
+  }
+  // a sample of the lists' heads, one wave's: `deep` of each
+  const uint32_t lists = a.beams * a.segs, deep = lists < a.k ? (a.k + lists - 1) / lists : 1;
+#pragma unroll
+  for (int i = 0; i < HELD; i++) {
+    const uint32_t h = lane + i * 64;
+    heads[i] = h < lists * deep ? entries[h / deep * a.k + h % deep] : Entry{LOWEST, 0};
+  }
   if (threadIdx.x == 0) count = 0;
-  for (uint32_t b = wave; b < a.beams; b += AGPU_BLOCK / 64) {
-    double m = none, s = 0.0;
-    bool bad = false;
-    if (!is_finished(a, r0 + b))
+  for (uint32_t b = wave; b < a.beams; b += MERGE_BLOCK / 64) {
+    const bool done = is_finished(a, r0 + b);
+    double s = 0.0, ref = none;
+    if (!done)
       for (uint32_t i = lane; i < a.segs; i += 64) {
         const SegSum g = sums[(uint64_t)(r0 + b) * a.segs + i];
-        bad |= g.count == BAD;
-        if (g.max > m) s = s * exp(m - (double)g.max) + g.sum, m = g.max;
-        else if (g.max > -__builtin_inff()) s += g.sum * exp((double)g.max - m);
+        if (g.sum == 0.0) continue;
+        if (g.ref > ref) s = s * exp(ref - g.ref) + g.sum, ref = g.ref;
+        else s += g.sum * exp(g.ref - ref);
       }
-    double top = m;
+    double top = ref;
     for (int d = 32; d; d >>= 1) top = fmax(top, __shfl_xor(top, d));
-    if (m > none) s *= exp(m - top);
+    s = ref > none ? s * exp(ref - top) : 0.0;
     for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
-    if (lane == 0) lse[b] = top + log(s);  // (nothing allowed: NaN or −infinity, and no entries)
-    if (__any(bad) && lane == 0) lse[b] = __builtin_nan("");
+    if (lane == 0) lse[b] = done ? __builtin_nan("") : top + log(s), cum[b] = a.scores ? a.scores[r0 + b] : 0.0f;
   }
   __syncthreads();
 
-  // entry e → its candidate; score −infinity: none
-  const auto candidate = [&](uint32_t e) {
-    const uint32_t b = e / per_row, i = e - b * per_row, row = r0 + b;
-    Candidate c = {none, b, 0, 0.0f};
-    const double cum = a.scores ? (double)a.scores[row] : 0.0;
-    double s = none;
-    if (is_finished(a, row)) {
-      if (i == 0) s = cum, c.token = a.end_token;
-    } else {
-      const uint32_t seg = i / a.k, held = sums[(uint64_t)row * a.segs + seg].count;
-      if (held != BAD && i - seg * a.k < held) {
-        const Entry x = entries[(uint64_t)row * per_row + i];
-        s = cum + ((double)x.logit - lse[b]);
-        c.token = x.token, c.logit = x.logit;
-      }
-    }
-    if (s > none) c.score = s;  // (NaN: none)
+  const auto candidate = [&](uint32_t e, Entry x) {
+    const uint32_t b = e / per_row;
+    Candidate c = {none, b, x.token, x.logit};
+    const double s = (double)cum[b] + ((double)x.logit - lse[b]);
+    if (x.logit > LOWEST && s > none) c.score = s;  // (NaN: none)
     return c;
   };
-
-  float best = -__builtin_inff();  // rounding to f32 keeps the order, but for ties
-  for (uint32_t e = threadIdx.x; e < n; e += AGPU_BLOCK) best = fmaxf(best, (float)candidate(e).score);
-  const uint32_t t = wave_kth(order_of(best), a.k, 0);
-  if (lane == 0) wave_t[wave] = t;
-  __syncthreads();
-  uint32_t least = wave_t[0];
-  for (int w = 1; w < AGPU_BLOCK / 64; w++) least = least > wave_t[w] ? least : wave_t[w];
-  const float floor_v = value_of(least);
-  for (uint32_t e = threadIdx.x; e < n; e += AGPU_BLOCK) {
-    const Candidate c = candidate(e);
+  float best[1] = {LOWEST};  // rounding to f32 keeps the order, but for ties
+#pragma unroll
+  for (int i = 0; i < HELD; i++) {
+    const uint32_t h = lane + i * 64;
+    if (h < lists * deep) best[0] = fmaxf(best[0], (float)candidate(h / deep * a.k, heads[i]).score);
+  }
+  for (uint32_t h = lane + HELD * 64; h < lists * deep; h += 64) {
+    const uint32_t e = h / deep * a.k + h % deep;
+    best[0] = fmaxf(best[0], (float)candidate(e, entries[e]).score);
+  }
+  const float floor_v = wave_kth(best, a.k, 0);
+  const auto offer = [&](const Candidate& c) {
     if (c.score > none && (float)c.score >= floor_v) {
       const uint32_t at = atomicAdd(&count, 1u);
       if (at < MERGE_LIST) list[at] = c;
     }
-  }
+  };
+#pragma unroll
+  for (int i = 0; i < HELD; i++)
+    if (threadIdx.x + i * MERGE_BLOCK < n) offer(candidate(threadIdx.x + i * MERGE_BLOCK, held[i]));
+  for (uint32_t e = threadIdx.x + HELD * MERGE_BLOCK; e < n; e += MERGE_BLOCK) offer(candidate(e, entries[e]));
+  // a finished row's one candidate (of its entries none was: its log-sum is NaN)
+  for (uint32_t b = threadIdx.x; b < a.beams; b += MERGE_BLOCK)
+    if (is_finished(a, r0 + b)) offer({cum[b] == cum[b] ? (double)cum[b] : none, b, a.end_token, 0.0f});
   __syncthreads();
   const uint32_t found = count < a.k ? count : a.k;
   const auto put = [&](uint32_t rank, const Candidate& c) {
@@ -304,7 +381,7 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_merge_kernel(BeamArgs a, cons
     chosen[rank] = (uint64_t)c.beam * a.vocab + c.token;
   };
   if (count <= MERGE_LIST) {
-    for (uint32_t i = threadIdx.x; i < count; i += AGPU_BLOCK) {
+    for (uint32_t i = threadIdx.x; i < count; i += MERGE_BLOCK) {
       const Candidate c = list[i];
       uint32_t rank = 0;
       for (uint32_t j = 0; j < count; j++) rank += better(list[j], c);
@@ -314,10 +391,12 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_merge_kernel(BeamArgs a, cons
     Candidate before = {__builtin_inf(), 0, 0, 0.0f};
     for (uint32_t r = 0; r < a.k; r++) {
       Candidate top = {none, ~0u, 0, 0.0f};
-      for (uint32_t e = threadIdx.x; e < n; e += AGPU_BLOCK) {
-        const Candidate c = candidate(e);
+      const auto take = [&](const Candidate& c) {
         if (c.score > none && (r == 0 || better(before, c)) && better(c, top)) top = c;
-      }
+      };
+      for (uint32_t e = threadIdx.x; e < n; e += MERGE_BLOCK) take(candidate(e, entries[e]));
+      for (uint32_t b = threadIdx.x; b < a.beams; b += MERGE_BLOCK)
+        if (is_finished(a, r0 + b)) take({cum[b] == cum[b] ? (double)cum[b] : none, b, a.end_token, 0.0f});
       for (int d = 32; d; d >>= 1) {
         const Candidate o = {__shfl_xor(top.score, d), __shfl_xor(top.beam, d), __shfl_xor(top.token, d), __shfl_xor(top.logit, d)};
         if (better(o, top)) top = o;
@@ -325,7 +404,7 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_merge_kernel(BeamArgs a, cons
       __syncthreads();
       if (lane == 0) list[wave] = top;
       __syncthreads();
-      for (int w = 0; w < AGPU_BLOCK / 64; w++)
+      for (int w = 0; w < MERGE_BLOCK / 64; w++)
         if (better(list[w], top)) top = list[w];
       if (threadIdx.x == 0) put(r, top);
       before = top;
@@ -345,15 +424,15 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_merge_kernel(BeamArgs a, cons
 }
 
 // ---------------------------------------------------------------- host
-// Segments of a row: the type does not enter, so that the workspace does not depend on it
-constexpr uint32_t SEG_MOST = 8192, SEG_LEAST = 2048;
-uint32_t segment_elements(uint64_t rows, uint64_t vocab) {
-  uint32_t e = SEG_MOST;
-  while (e > SEG_LEAST && rows * ((vocab + 7 + e - 1) / e) < 512) e /= 2;
-  return e;
+// Tiles of a segment: the fewer, the more waves share the work; the more, the fewer lists there are to join.  As many as leave 4096 waves (16 a
+// CU), at most 8.  (The type does not enter: the workspace does not depend on it.)
+uint32_t segment_tiles(uint64_t rows, uint64_t vocab) {
+  uint32_t t = 8;
+  while (t > 1 && rows * ((vocab + 7 + t * TILE - 1) / (t * TILE)) < 4096) t /= 2;
+  return t;
 }
 uint32_t segments(uint64_t rows, uint64_t vocab) {
-  const uint32_t e = segment_elements(rows, vocab);
+  const uint64_t e = (uint64_t)segment_tiles(rows, vocab) * TILE;
   return (uint32_t)((vocab + 7 + e - 1) / e);  // + 7: a row may start anywhere in a vector
 }
 
@@ -367,13 +446,10 @@ bool workspace_bytes(uint64_t batch, uint64_t beams, uint64_t vocab, uint64_t k,
 
 template <typename T>
 void launch_segments(agpu_pipeline* p, const BeamArgs& a, SegSum* sums, Entry* entries) {
-  constexpr int E = 16 / sizeof(T) * AGPU_BLOCK;
-  const dim3 grid(a.batch * a.beams * a.segs);
-  switch (segment_elements((uint64_t)a.batch * a.beams, a.vocab)) {
-    case SEG_MOST: hipLaunchKernelGGL((beam_segment_kernel<T, SEG_MOST / E>), grid, dim3(AGPU_BLOCK), 0, p->stream, a, sums, entries); break;
-    case SEG_MOST / 2: hipLaunchKernelGGL((beam_segment_kernel<T, SEG_MOST / 2 / E>), grid, dim3(AGPU_BLOCK), 0, p->stream, a, sums, entries); break;
-    default: hipLaunchKernelGGL((beam_segment_kernel<T, SEG_LEAST / E>), grid, dim3(AGPU_BLOCK), 0, p->stream, a, sums, entries); break;
-  }
+  const uint32_t rows = a.batch * a.beams, n = rows * a.segs, tiles = segment_tiles(rows, a.vocab);
+  const dim3 grid((n + AGPU_BLOCK / 64 - 1) / (AGPU_BLOCK / 64));
+  if (a.allowed) hipLaunchKernelGGL((beam_segment_kernel<T, true>), grid, dim3(AGPU_BLOCK), 0, p->stream, a, tiles, n, sums, entries);
+  else hipLaunchKernelGGL((beam_segment_kernel<T, false>), grid, dim3(AGPU_BLOCK), 0, p->stream, a, tiles, n, sums, entries);
 }
 
 }  // namespace
@@ -418,7 +494,7 @@ agpu_status agpu_select_beams(agpu_pipeline* p, const agpu_beams* args) {
   else if (b.type == AGPU_ROW_F16) launch_segments<f16_t>(p, a, sums, entries);
   else launch_segments<bf16_t>(p, a, sums, entries);
   AGPU_LAUNCH_CHECK();
-  hipLaunchKernelGGL(beam_merge_kernel, dim3(b.batch), dim3(AGPU_BLOCK), 0, p->stream, a, sums, entries);
+  hipLaunchKernelGGL(beam_merge_kernel, dim3(b.batch), dim3(MERGE_BLOCK), 0, p->stream, a, sums, entries);
   AGPU_LAUNCH_CHECK();
   return AGPU_OK;
 }
