@@ -2,13 +2,13 @@
 //
 // One pass over the logits.  A row is cut into segments of one WAVE each; the wave streams its segment, adding up exp(x) and keeping the tokens that
 // can be among its k best, and leaves (sum, k best) in the workspace.  A block a request joins the sums and selects among the segments' bests.
-// No wave waits for another before the join, and none needs the maximum first: f64 holds exp(x − first tile's maximum) for all x of a row
-// whose logits are less than 600 apart; a segment that holds others is read again.
+// No wave waits for another before the join, and none needs the maximum first: exp is taken relative to the first tile's, and f32 holds it as long as
+// a segment's maximum is within 60 of that; a segment of another kind is read again.
 //
-// Why 64 bits: the result is whole numbers, and rows that compete differ by their log-sums only — a log-sum 1e-7 off swaps tokens of two beams.
-// The f64 unit runs at the rate of the f32 one here, so exp is made there: with c = ln 2 / 256, x = (256 e + j + r) c, |r| <= 1/2,
-// exp(x) = 2^e · 2^(j/256) · (1 + r c + r² c² / 2), the middle factor from a table in LDS.  The cubic term that is left out is at most 4.2e-10, and
-// odd: over many tokens it cancels.
+// Precision.  The result is whole numbers, and rows that compete differ by their log-sums only: a log-sum 1e-7 off swaps tokens of two beams.  The tokens that
+// are kept (about the 3 k largest of a segment) hold the largest terms: theirs are taken in f64, from the list, and left out of the f32 ones.  Those are
+// many and small, each 1e-7 off at random: 1e-8 and less in the sum.  A term is 2^f · 2^n with x log2 e = n + f, |f| <= 1/2: one fma rounds x log2 e to n, the
+// next gives f exactly, a third adds x times what log2 e has beyond f32; n goes into the exponent.
 #include "common.hpp"
 
 namespace {
@@ -41,29 +41,15 @@ struct Entry {  // logit −infinity: none
 __device__ __forceinline__ bool is_finished(const BeamArgs& a, uint32_t row) { return a.finished && (a.finished[row >> 6] >> (row & 63) & 1); }
 
 // ---------------------------------------------------------------- exp
-constexpr int EXP_STEPS = 256;
-struct ExpTable {
-  double v[EXP_STEPS];
-};
-constexpr ExpTable make_exp_table() {
-  ExpTable t = {};
-  for (int j = 0; j < EXP_STEPS; j++) {  // Taylor's series of exp(j ln 2 / 256), arguments below 0.7: 20 terms
-    const double y = 0.69314718055994530942 * j / EXP_STEPS;
-    double term = 1.0, sum = 0.0;
-    for (int n = 1; n <= 20; n++) sum += term, term = term * y / n;
-    t.v[j] = sum;
-  }
-  return t;
-}
-__device__ const ExpTable exp_table = make_exp_table();
-
-constexpr double EXP_C = 0.69314718055994530942 / EXP_STEPS, EXP_SCALE = EXP_STEPS / 0.69314718055994530942, EXP_MAGIC = 0x1.8p52;
-// exp(x − ref), ref = (EXP_MAGIC − k) · EXP_C a whole number of steps: no subtraction, the steps of ref leave with the whole number.  |x| <= 2^30
-__device__ __forceinline__ void add_exp(double& sum, double x, double k, const double* table) {
-  const double z = __builtin_fma(x, EXP_SCALE, k);  // its low word: steps of x, less those of ref
-  const int n = (int)__builtin_bit_cast(uint64_t, z);
-  const double r = __builtin_fma(x, EXP_SCALE, k - z), f = __builtin_ldexp(table[n & (EXP_STEPS - 1)], n >> 8);
-  sum = __builtin_fma(f, __builtin_fma(r, __builtin_fma(r, EXP_C * EXP_C / 2, EXP_C), 1.0), sum);
+constexpr float LOG2E = 0x1.715476p+0f, LOG2E_LOW = 0x1.4ae0cp-26f, MAGIC = 0x1.8p23f;
+constexpr double LN2 = 0.69314718055994530942;
+constexpr float REF_MOST = 16384.0f;  // of a reference: MAGIC − k holds its steps
+constexpr float APART = 60.0f;        // of a segment's maximum from its reference
+// exp(x) / 2^N, k = MAGIC − N; x log2 e − N within 2^±126
+__device__ __forceinline__ float exp_term(float x, float k) {
+  const float z = __builtin_fmaf(x, LOG2E, k);  // its low bits: n − N
+  const float f = __builtin_fmaf(x, LOG2E_LOW, __builtin_fmaf(x, LOG2E, k - z));
+  return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, __builtin_amdgcn_exp2f(f)) + (__builtin_bit_cast(uint32_t, z) << 23));
 }
 
 // ---------------------------------------------------------------- order
@@ -111,7 +97,8 @@ template <> struct Raw<bf16_t> {
 };
 
 constexpr int TILE = 1024;  // logits a wave takes at a time: 16 a lane
-constexpr int LIST = 512;   // tokens it can keep: 18 + 9 + 6 + … for k = 16 and logits in no order, 230 for k = 64
+constexpr int RANKED = 8;
+constexpr int LIST = 512;   // tokens it can keep; logits in no order: about 3 k + 10
 
 template <typename T, bool MASK>
 struct Segment {
@@ -163,10 +150,7 @@ template <typename T, bool MASK>
 __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, uint32_t tiles, uint32_t n_segs, SegSum* sums, Entry* entries) {
   typedef Segment<T, MASK> S;
   constexpr int VE = S::VE, U = S::U, EPT = U * VE;
-  __shared__ double table[EXP_STEPS];
-  __shared__ uint64_t lists[AGPU_BLOCK / 64][LIST];
-  table[threadIdx.x] = exp_table.v[threadIdx.x];
-  __syncthreads();  // the only one: from here on every wave is by itself
+  __shared__ uint64_t lists[AGPU_BLOCK / 64][LIST + RANKED];
   const uint32_t id = __builtin_amdgcn_readfirstlane(blockIdx.x * (AGPU_BLOCK / 64) + (threadIdx.x >> 6)), lane = threadIdx.x & 63;
   if (id >= n_segs) return;
   const uint32_t row = id / a.segs, seg = id - row * a.segs;
@@ -182,9 +166,10 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
   const uint32_t t0 = seg * tiles, row_tiles = (uint32_t)(((uint64_t)a.vocab + s.lead + TILE - 1) / TILE), t1 = t0 + tiles < row_tiles ? t0 + tiles : row_tiles;
 
   float top[2] = {LOWEST, LOWEST};  // the largest of the lane's first and second eight logits of every tile
-  float floor_v = LOWEST, ref_v = 0.0f;
-  double sum = 0.0, k = EXP_MAGIC;
-  uint32_t count = 0, negative_nan = 0;
+  float floor_v = LOWEST, ref_v = 0.0f, k = MAGIC, least = 0.0f;
+  double sum = 0.0;
+  uint32_t count = 0;
+  bool nan = false;
   u32x4 w[U], next[U];
   uint32_t m[U], next_m[U];
   if (t0 < t1) s.load(t0, w, m);
@@ -195,12 +180,15 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
     float tm[2] = {v[0], v[EPT / 2]};
 #pragma unroll
     for (int i = 1; i < EPT / 2; i++) tm[0] = fmaxf(tm[0], v[i]), tm[1] = fmaxf(tm[1], v[EPT / 2 + i]);
+#pragma unroll
+    for (int i = 0; i < EPT; i += 2) nan |= __builtin_isunordered(v[i], v[i + 1]);
     top[0] = fmaxf(top[0], tm[0]), top[1] = fmaxf(top[1], tm[1]);
     if (t == t0) {  // the reference: the tile's maximum, as far as it is an ordinary number
       float f = fmaxf(tm[0], tm[1]);
       for (int d = 32; d; d >>= 1) f = fmaxf(f, __shfl_xor(f, d));
-      ref_v = __builtin_fabsf(f) <= 16384.0f ? f : 0.0f;
-      k = EXP_MAGIC - __builtin_rint((double)ref_v * EXP_SCALE);
+      ref_v = __builtin_fabsf(f) <= REF_MOST ? f : 0.0f;
+      k = MAGIC - __builtin_rintf(ref_v * LOG2E);
+      least = ref_v - 80.0f;
     }
     if (__any(fmaxf(tm[0], tm[1]) >= floor_v)) {
       if (((t - t0) & (t - t0 + 1)) == 0) floor_v = wave_kth(top, a.k, Raw<T>::low);  // tiles 0, 1, 3, 7 …
@@ -210,52 +198,60 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
         const uint64_t who = __ballot(v[i] >= above);
         if (who) {
           const uint32_t at = count + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
-          if (v[i] >= above && at < LIST) list[at] = (uint64_t)order_of(v[i]) << 32 | ~(uint32_t)(s.token(t, i / VE) + i % VE);
+          if (v[i] >= above) {
+            if (at < LIST) list[at] = (uint64_t)order_of(v[i]) << 32 | ~(uint32_t)(s.token(t, i / VE) + i % VE);
+            v[i] = LOWEST;  // its term is taken from the list
+          }
           count += (uint32_t)__popcll(who);
         }
       }
     }
+    float part = 0.0f;
 #pragma unroll
-    for (int i = 0; i < EPT; i++) {
-      // at least −2^30: the unsigned order of negative numbers grows downwards.  It keeps +infinity and positive NaN, which make the sum NaN
-      const uint32_t b = __builtin_bit_cast(uint32_t, v[i]), low = 0xCE800000u;
-      negative_nan = b > negative_nan ? b : negative_nan;
-      add_exp(sum, (double)__builtin_bit_cast(float, b < low ? b : low), k, table);
-    }
+    for (int i = 0; i < EPT; i++) part += exp_term(fmaxf(v[i], least), k);  // (e^-80 for what is less, −infinity too: nothing beside the largest)
+    sum += (double)part;
 #pragma unroll
     for (int u = 0; u < U; u++) w[u] = next[u], m[u] = next_m[u];
   }
 
-  for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the list was written by other lanes
   float most = fmaxf(top[0], top[1]);
   for (int d = 32; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
-  double ref = (EXP_MAGIC - k) * EXP_C;
-  if (most > LOWEST && most < __builtin_inff() && __builtin_fabsf(most - ref_v) > 600.0f) {  // again, below the maximum that is now known
-    ref = most;
-    sum = 0.0;
-    for (uint32_t t = t0; t < t1; t++) {
-      float v[EPT];
-      s.load(t, w, m);
-      s.values(w, m, v);
-#pragma unroll
-      for (int i = 0; i < EPT; i++) {
-        const double d = (double)v[i] - ref;
-        add_exp(sum, d < -0x1p30 ? -0x1p30 : d, EXP_MAGIC, table);
+  double ref = (double)(MAGIC - k) * LN2;
+  if (most > LOWEST && most < __builtin_inff()) {
+    if (count > LIST || __builtin_fabsf(most - ref_v) > APART) {  // again, in f64, below the maximum that is now known
+      ref = most;
+      sum = 0.0;
+      for (uint32_t t = t0; t < t1; t++) {
+        float v[EPT];
+        s.load(t, w, m);
+        s.values(w, m, v);
+#pragma unroll 1
+        for (int i = 0; i < EPT; i++) sum += exp((double)v[i] - ref);
       }
+    } else {
+      for (uint32_t i = lane; i < count; i += 64) sum += exp((double)value_of((uint32_t)(list[i] >> 32)) - ref);
     }
-    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
   }
-  if (__any(negative_nan > 0xFF800000u) || most == __builtin_inff()) sum = __builtin_nan("");
+  for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+  if (__any(nan) || most == __builtin_inff()) sum = __builtin_nan("");
   if (lane == 0) sums[id] = {most > LOWEST || sum != sum ? sum : 0.0, ref};
 
   Entry* out = entries + (uint64_t)id * a.k;
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the list was written by other lanes
   if (count <= LIST) {
     if (lane >= count && lane < a.k) out[lane] = {LOWEST, 0};
+    if (lane < RANKED) list[count + lane] = 0;
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     for (uint32_t i = lane; i < count; i += 64) {
       const uint64_t e = list[i];
       uint32_t rank = 0;
-      for (uint32_t j = 0; j < count; j++) rank += list[j] > e;
+      for (uint32_t j = 0; j < count; j += RANKED) {  // (many reads at a time: one after the other they are all latency)
+        uint64_t o[RANKED];
+#pragma unroll
+        for (int q = 0; q < RANKED; q++) o[q] = list[j + q];
+#pragma unroll
+        for (int q = 0; q < RANKED; q++) rank += o[q] > e;
+      }
       if (rank < a.k) out[rank] = {value_of((uint32_t)(e >> 32)), ~(uint32_t)e};
     }
   } else {  // very many equal logits, or ascending ones: the best, then the best behind it, k times
@@ -295,39 +291,40 @@ __device__ __forceinline__ bool better(const Candidate& x, const Candidate& y) {
   return x.token < y.token;
 }
 
-constexpr int MERGE_BLOCK = 1024, MERGE_LIST = 512, HELD = 4;
+constexpr int MERGE_BLOCK = 512, MERGE_WAVES = MERGE_BLOCK / 64, MERGE_LIST = 512, HELD = 8;
 
-// Lists of k entries, best first: the largest scores among a few heads of them give a bound that k candidates reach; what reaches it goes to LDS and
-// is ranked there by counting.
+// A wave a beam: its log-sum, its entries' scores, and a bound that k of them reach.  What reaches the best of the beams' bounds goes to LDS and is
+// ranked there by counting.
 __global__ __launch_bounds__(MERGE_BLOCK) void beam_merge_kernel(BeamArgs a, const SegSum* sums, const Entry* entries) {
   __shared__ double lse[1024];  // per beam: its log-sum, NaN for a row whose scores are −infinity
-  __shared__ float cum[1024];
+  __shared__ float cum[1024], wave_floor[MERGE_WAVES];
+  __shared__ double scores[MERGE_LIST + RANKED];
   __shared__ Candidate list[MERGE_LIST];
   __shared__ uint64_t chosen[64];
   __shared__ uint32_t count;
-  const uint32_t r0 = blockIdx.x * a.beams, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, per_row = a.segs * a.k, n = a.beams * per_row;
+  const uint32_t r0 = blockIdx.x * a.beams, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, per_row = a.segs * a.k;
   const double none = -__builtin_inf();
-  entries += (uint64_t)r0 * per_row;
-  Entry held[HELD], heads[HELD];
-#pragma unroll
-  for (int i = 0; i < HELD; i++) {
-    const uint32_t e = threadIdx.x + i * MERGE_BLOCK;
-    held[i] = e < n ? entries[e] : Entry{LOWEST, 0};
-  }
-  // a sample of the lists' heads, one wave's: `deep` of each
-  const uint32_t lists = a.beams * a.segs, deep = lists < a.k ? (a.k + lists - 1) / lists : 1;
-#pragma unroll
-  for (int i = 0; i < HELD; i++) {
-    const uint32_t h = lane + i * 64;
-    heads[i] = h < lists * deep ? entries[h / deep * a.k + h % deep] : Entry{LOWEST, 0};
-  }
   if (threadIdx.x == 0) count = 0;
-  for (uint32_t b = wave; b < a.beams; b += MERGE_BLOCK / 64) {
-    const bool done = is_finished(a, r0 + b);
+
+  const auto score = [&](Entry x, double c, double l) {
+    const double s = c + ((double)x.logit - l);
+    return x.logit > LOWEST && s > none ? s : none;  // (NaN: none)
+  };
+  float floor_v = LOWEST;
+  Entry held[HELD];  // of the wave's first beam
+  for (uint32_t b = wave; b < a.beams; b += MERGE_WAVES) {
+    const uint32_t row = r0 + b;
+    const Entry* mine = entries + (uint64_t)row * per_row;
+    const bool done = is_finished(a, row);
+    const float c = a.scores ? a.scores[row] : 0.0f;
+    if (b == wave) {
+#pragma unroll
+      for (int i = 0; i < HELD; i++) held[i] = !done && lane + i * 64 < per_row ? mine[lane + i * 64] : Entry{LOWEST, 0};
+    }
     double s = 0.0, ref = none;
     if (!done)
       for (uint32_t i = lane; i < a.segs; i += 64) {
-        const SegSum g = sums[(uint64_t)(r0 + b) * a.segs + i];
+        const SegSum g = sums[(uint64_t)row * a.segs + i];
         if (g.sum == 0.0) continue;
         if (g.ref > ref) s = s * exp(ref - g.ref) + g.sum, ref = g.ref;
         else s += g.sum * exp(g.ref - ref);
@@ -336,43 +333,48 @@ __global__ __launch_bounds__(MERGE_BLOCK) void beam_merge_kernel(BeamArgs a, con
     for (int d = 32; d; d >>= 1) top = fmax(top, __shfl_xor(top, d));
     s = ref > none ? s * exp(ref - top) : 0.0;
     for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
-    if (lane == 0) lse[b] = done ? __builtin_nan("") : top + log(s), cum[b] = a.scores ? a.scores[r0 + b] : 0.0f;
-  }
-  __syncthreads();
-
-  const auto candidate = [&](uint32_t e, Entry x) {
-    const uint32_t b = e / per_row;
-    Candidate c = {none, b, x.token, x.logit};
-    const double s = (double)cum[b] + ((double)x.logit - lse[b]);
-    if (x.logit > LOWEST && s > none) c.score = s;  // (NaN: none)
-    return c;
-  };
-  float best[1] = {LOWEST};  // rounding to f32 keeps the order, but for ties
+    const double l = done ? __builtin_nan("") : top + log(s);
+    if (lane == 0) lse[b] = l, cum[b] = c;
+    float best[1] = {LOWEST};  // rounding to f32 keeps the order, but for ties
+    if (b == wave) {
 #pragma unroll
-  for (int i = 0; i < HELD; i++) {
-    const uint32_t h = lane + i * 64;
-    if (h < lists * deep) best[0] = fmaxf(best[0], (float)candidate(h / deep * a.k, heads[i]).score);
+      for (int i = 0; i < HELD; i++) best[0] = fmaxf(best[0], (float)score(held[i], c, l));
+    }
+    for (uint32_t e = lane + (b == wave ? HELD * 64 : 0); e < per_row && !done; e += 64) best[0] = fmaxf(best[0], (float)score(mine[e], c, l));
+    floor_v = fmaxf(floor_v, wave_kth(best, a.k, 0));
   }
-  for (uint32_t h = lane + HELD * 64; h < lists * deep; h += 64) {
-    const uint32_t e = h / deep * a.k + h % deep;
-    best[0] = fmaxf(best[0], (float)candidate(e, entries[e]).score);
-  }
-  const float floor_v = wave_kth(best, a.k, 0);
-  const auto offer = [&](const Candidate& c) {
-    if (c.score > none && (float)c.score >= floor_v) {
+  if (lane == 0) wave_floor[wave] = floor_v;
+  __syncthreads();
+#pragma unroll
+  for (int w = 0; w < MERGE_WAVES; w++) floor_v = fmaxf(floor_v, wave_floor[w]);
+
+  const auto offer = [&](double s, uint32_t b, Entry x) {
+    if (s > none && (float)s >= floor_v) {
       const uint32_t at = atomicAdd(&count, 1u);
-      if (at < MERGE_LIST) list[at] = c;
+      if (at < MERGE_LIST) scores[at] = s, list[at] = {s, b, x.token, x.logit};
     }
   };
+  // every beam's entries, and a finished one's only candidate: f(score, beam, entry)
+  const auto each = [&](const auto& f) {
+    for (uint32_t b = wave; b < a.beams; b += MERGE_WAVES) {
+      if (is_finished(a, r0 + b)) {
+        if (lane == 0 && cum[b] == cum[b]) f((double)cum[b], b, Entry{0.0f, a.end_token});
+        continue;
+      }
+      const double l = lse[b], c = cum[b];
+      if (b == wave) {
 #pragma unroll
-  for (int i = 0; i < HELD; i++)
-    if (threadIdx.x + i * MERGE_BLOCK < n) offer(candidate(threadIdx.x + i * MERGE_BLOCK, held[i]));
-  for (uint32_t e = threadIdx.x + HELD * MERGE_BLOCK; e < n; e += MERGE_BLOCK) offer(candidate(e, entries[e]));
-  // a finished row's one candidate (of its entries none was: its log-sum is NaN)
-  for (uint32_t b = threadIdx.x; b < a.beams; b += MERGE_BLOCK)
-    if (is_finished(a, r0 + b)) offer({cum[b] == cum[b] ? (double)cum[b] : none, b, a.end_token, 0.0f});
+        for (int i = 0; i < HELD; i++) f(score(held[i], c, l), b, held[i]);
+      }
+      for (uint32_t e = lane + (b == wave ? HELD * 64 : 0); e < per_row; e += 64) {
+        const Entry x = entries[(uint64_t)(r0 + b) * per_row + e];
+        f(score(x, c, l), b, x);
+      }
+    }
+  };
+  each(offer);
   __syncthreads();
-  const uint32_t found = count < a.k ? count : a.k;
+  const uint32_t n = count, found = n < a.k ? n : a.k;
   const auto put = [&](uint32_t rank, const Candidate& c) {
     const uint64_t o = (uint64_t)blockIdx.x * a.k + rank;
     a.out_scores[o] = (float)c.score;
@@ -380,23 +382,31 @@ __global__ __launch_bounds__(MERGE_BLOCK) void beam_merge_kernel(BeamArgs a, con
     a.out_tokens[o] = c.token;
     chosen[rank] = (uint64_t)c.beam * a.vocab + c.token;
   };
-  if (count <= MERGE_LIST) {
-    for (uint32_t i = threadIdx.x; i < count; i += MERGE_BLOCK) {
+  if (n <= MERGE_LIST) {
+    if (threadIdx.x < RANKED) scores[n + threadIdx.x] = none;
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < n; i += MERGE_BLOCK) {
       const Candidate c = list[i];
-      uint32_t rank = 0;
-      for (uint32_t j = 0; j < count; j++) rank += better(list[j], c);
+      uint32_t rank = 0, equal = 0;
+      for (uint32_t j = 0; j < n; j += RANKED) {
+        double o[RANKED];
+#pragma unroll
+        for (int q = 0; q < RANKED; q++) o[q] = scores[j + q];
+#pragma unroll
+        for (int q = 0; q < RANKED; q++) rank += o[q] > c.score, equal += o[q] == c.score;
+      }
+      if (equal > 1)
+        for (uint32_t j = 0; j < n; j++) rank += scores[j] == c.score && better(list[j], c);
       if (rank < a.k) put(rank, c);
     }
   } else {  // very many equal scores: the best, then the best behind it, k times
     Candidate before = {__builtin_inf(), 0, 0, 0.0f};
     for (uint32_t r = 0; r < a.k; r++) {
       Candidate top = {none, ~0u, 0, 0.0f};
-      const auto take = [&](const Candidate& c) {
-        if (c.score > none && (r == 0 || better(before, c)) && better(c, top)) top = c;
-      };
-      for (uint32_t e = threadIdx.x; e < n; e += MERGE_BLOCK) take(candidate(e, entries[e]));
-      for (uint32_t b = threadIdx.x; b < a.beams; b += MERGE_BLOCK)
-        if (is_finished(a, r0 + b)) take({cum[b] == cum[b] ? (double)cum[b] : none, b, a.end_token, 0.0f});
+      each([&](double s, uint32_t b, Entry x) {
+        const Candidate c = {s, b, x.token, x.logit};
+        if (s > none && (r == 0 || better(before, c)) && better(c, top)) top = c;
+      });
       for (int d = 32; d; d >>= 1) {
         const Candidate o = {__shfl_xor(top.score, d), __shfl_xor(top.beam, d), __shfl_xor(top.token, d), __shfl_xor(top.logit, d)};
         if (better(o, top)) top = o;
@@ -404,7 +414,7 @@ __global__ __launch_bounds__(MERGE_BLOCK) void beam_merge_kernel(BeamArgs a, con
       __syncthreads();
       if (lane == 0) list[wave] = top;
       __syncthreads();
-      for (int w = 0; w < MERGE_BLOCK / 64; w++)
+      for (int w = 0; w < MERGE_WAVES; w++)
         if (better(list[w], top)) top = list[w];
       if (threadIdx.x == 0) put(r, top);
       before = top;
