@@ -97,6 +97,7 @@ template <> struct Raw<bf16_t> {
 };
 
 constexpr int TILE = 1024;  // logits a wave takes at a time: 16 a lane
+constexpr int HITS = 2048; // and may look at twice
 constexpr int RANKED = 8;
 constexpr int LIST = 512;   // tokens it can keep; logits in no order: about 3 k + 10
 
@@ -109,15 +110,19 @@ struct Segment {
 
   // first token of vector u of tile t: vectors lie on 16 bytes, the row starts `lead` elements into its first
   __device__ __forceinline__ int64_t token(uint32_t t, int u) const { return (int64_t)t * TILE + u * (64 * VE) + lane * VE - lead; }
+  // whether all of a tile are the row's (the same in all lanes)
+  __device__ __forceinline__ bool whole(uint32_t t) const { return (uint64_t)t * TILE >= lead && (uint64_t)(t + 1) * TILE <= (uint64_t)vocab + lead; }
 
+  // m: bit i: element i of the vector counts
   __device__ __forceinline__ void load(uint32_t t, u32x4 (&w)[U], uint32_t (&m)[U]) const {
+    if (whole(t)) {
+      const u32x4* at = reinterpret_cast<const u32x4*>(x - lead) + (uint64_t)t * (TILE / VE) + lane;
 #pragma unroll
-    for (int u = 0; u < U; u++) {
-      const int64_t at = token(t, u);
-      if (at >= 0 && at + VE <= vocab) {
-        w[u] = *reinterpret_cast<const u32x4*>(x + at);
-        m[u] = ~0u;
-      } else {  // the row's ends
+      for (int u = 0; u < U; u++) w[u] = at[u * 64];
+    } else {  // the row's ends
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const int64_t at = token(t, u);
         T e[VE] = {};
         m[u] = 0;
 #pragma unroll
@@ -125,26 +130,42 @@ struct Segment {
           if (at + i >= 0 && at + i < vocab) e[i] = x[at + i], m[u] |= 1u << i;
         w[u] = __builtin_bit_cast(u32x4, e);
       }
-      if (MASK && m[u]) {
-        const uint32_t first = at < 0 ? 0u : (uint32_t)at, byte = first >> 3, last = (vocab - 1) >> 3;
-        const uint32_t b = (bits[byte] | (uint32_t)bits[byte < last ? byte + 1 : last] << 8) >> (first & 7);
-        m[u] &= at < 0 ? b << -at : b;
+    }
+    if (MASK) {
+#pragma unroll
+      for (int u = 0; u < U; u++) {
+        const int64_t at = token(t, u);
+        uint32_t b = 0;
+        if (at + VE > 0 && at < vocab) {
+          const uint32_t first = at < 0 ? 0u : (uint32_t)at, byte = first >> 3, last = (vocab - 1) >> 3;
+          b = (bits[byte] | (uint32_t)bits[byte < last ? byte + 1 : last] << 8) >> (first & 7) << (at < 0 ? -at : 0);
+        }
+        m[u] = whole(t) ? b : m[u] & b;
       }
     }
   }
   // the logits, −infinity for what is not allowed
-  __device__ __forceinline__ void values(const u32x4 (&w)[U], const uint32_t (&m)[U], float (&v)[U * VE]) const {
+  __device__ __forceinline__ void values(uint32_t t, const u32x4 (&w)[U], const uint32_t (&m)[U], float (&v)[U * VE]) const {
 #pragma unroll
-    for (int u = 0; u < U; u++) {
+    for (int u = 0; u < U; u++)
 #pragma unroll
       for (int i = 0; i < VE; i++) v[u * VE + i] = Raw<T>::at(w[u], i);
-      if (MASK || !__all(m[u] == ~0u)) {
+    if (MASK || !whole(t)) {
+#pragma unroll
+      for (int u = 0; u < U; u++)
 #pragma unroll
         for (int i = 0; i < VE; i++) v[u * VE + i] = (m[u] >> i & 1) ? v[u * VE + i] : LOWEST;
-      }
     }
   }
 };
+
+// the larger, without the instruction that would quiet a NaN first (of a NaN either: rows that hold one are found by themselves)
+__device__ __forceinline__ float max_of(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, __builtin_inff()); }
+__device__ __forceinline__ float max_of(float a, float b, float c) {
+  float r;
+  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
 
 template <typename T, bool MASK>
 __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, uint32_t tiles, uint32_t n_segs, SegSum* sums, Entry* entries) {
@@ -168,20 +189,21 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
   float top[2] = {LOWEST, LOWEST};  // the largest of the lane's first and second eight logits of every tile
   float floor_v = LOWEST, ref_v = 0.0f, k = MAGIC, least = 0.0f;
   double sum = 0.0;
-  uint32_t count = 0;
-  bool nan = false;
+  uint64_t nan = 0;
+  uint32_t hits[4] = {0, 0, 0, 0};  // a bit a logit of the lane's: it reached the floor; the last tile's first in the lowest
   u32x4 w[U], next[U];
   uint32_t m[U], next_m[U];
   if (t0 < t1) s.load(t0, w, m);
   for (uint32_t t = t0; t < t1; t++) {
     if (t + 1 < t1) s.load(t + 1, next, next_m);
     float v[EPT];
-    s.values(w, m, v);
+    s.values(t, w, m, v);
     float tm[2] = {v[0], v[EPT / 2]};
 #pragma unroll
-    for (int i = 1; i < EPT / 2; i++) tm[0] = fmaxf(tm[0], v[i]), tm[1] = fmaxf(tm[1], v[EPT / 2 + i]);
+    for (int i = 1; i < EPT / 2 - 1; i += 2) tm[0] = max_of(tm[0], v[i], v[i + 1]), tm[1] = max_of(tm[1], v[EPT / 2 + i], v[EPT / 2 + i + 1]);
+    tm[0] = max_of(tm[0], v[EPT / 2 - 1]), tm[1] = max_of(tm[1], v[EPT - 1]);
 #pragma unroll
-    for (int i = 0; i < EPT; i += 2) nan |= __builtin_isunordered(v[i], v[i + 1]);
+    for (int i = 0; i < EPT; i += 2) nan |= __ballot(__builtin_isunordered(v[i], v[i + 1]));
     top[0] = fmaxf(top[0], tm[0]), top[1] = fmaxf(top[1], tm[1]);
     if (t == t0) {  // the reference: the tile's maximum, as far as it is an ordinary number
       float f = fmaxf(tm[0], tm[1]);
@@ -190,51 +212,72 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
       k = MAGIC - __builtin_rintf(ref_v * LOG2E);
       least = ref_v - 80.0f;
     }
-    if (__any(fmaxf(tm[0], tm[1]) >= floor_v)) {
-      if (((t - t0) & (t - t0 + 1)) == 0) floor_v = wave_kth(top, a.k, Raw<T>::low);  // tiles 0, 1, 3, 7 …
-      const float above = fmaxf(floor_v, -0x1.fffffep127f);
+    if (((t - t0) & (t - t0 + 1)) == 0) floor_v = wave_kth(top, a.k, Raw<T>::low);  // tiles 0, 1, 3, 7
+    const float above = fmaxf(floor_v, -0x1.fffffep127f);
+    hits[3] = hits[3] << EPT | hits[2] >> (32 - EPT), hits[2] = hits[2] << EPT | hits[1] >> (32 - EPT), hits[1] = hits[1] << EPT | hits[0] >> (32 - EPT);
+    hits[0] <<= EPT;
+    if (__any(max_of(tm[0], tm[1]) >= above)) {
+      uint32_t h = 0;
 #pragma unroll
-      for (int i = 0; i < EPT; i++) {
-        const uint64_t who = __ballot(v[i] >= above);
-        if (who) {
-          const uint32_t at = count + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
-          if (v[i] >= above) {
-            if (at < LIST) list[at] = (uint64_t)order_of(v[i]) << 32 | ~(uint32_t)(s.token(t, i / VE) + i % VE);
-            v[i] = LOWEST;  // its term is taken from the list
-          }
-          count += (uint32_t)__popcll(who);
-        }
+      for (int i = EPT - 1; i >= 0; i--) {
+        const bool hit = v[i] >= above;
+        h = h + h + hit;
+        v[i] = hit ? LOWEST : v[i];  // its term is taken in f64
       }
+      hits[0] |= h;
     }
     float part = 0.0f;
 #pragma unroll
-    for (int i = 0; i < EPT; i++) part += exp_term(fmaxf(v[i], least), k);  // (e^-80 for what is less, −infinity too: nothing beside the largest)
+    for (int i = 0; i < EPT; i++) part += exp_term(max_of(v[i], least), k);  // (e^-80 for what is less, −infinity too: nothing beside the largest)
     sum += (double)part;
 #pragma unroll
     for (int u = 0; u < U; u++) w[u] = next[u], m[u] = next_m[u];
   }
 
-  __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");  // the list was written by other lanes
   float most = fmaxf(top[0], top[1]);
   for (int d = 32; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
   double ref = (double)(MAGIC - k) * LN2;
-  if (most > LOWEST && most < __builtin_inff()) {
-    if (count > LIST || __builtin_fabsf(most - ref_v) > APART) {  // again, in f64, below the maximum that is now known
-      ref = most;
-      sum = 0.0;
-      for (uint32_t t = t0; t < t1; t++) {
-        float v[EPT];
-        s.load(t, w, m);
-        s.values(w, m, v);
-#pragma unroll 1
-        for (int i = 0; i < EPT; i++) sum += exp((double)v[i] - ref);
+  // the logits that reached a floor, one of each lane at a time (read again: the lane's registers cannot be indexed): their terms, and into the list
+  // what reaches the last floor
+  uint32_t count = 0, all = 0;
+#pragma unroll
+  for (int i = 0; i < 4; i++) all += (uint32_t)__builtin_popcount(hits[i]);
+  for (int d = 32; d; d >>= 1) all += __shfl_xor(all, d);
+  const bool again = most > LOWEST && most < __builtin_inff() && (all > HITS || __builtin_fabsf(most - ref_v) > APART);
+  if (!again) {
+    while (__any((hits[0] | hits[1] | hits[2] | hits[3]) != 0)) {
+      const int word = hits[0] ? 0 : hits[1] ? 1 : hits[2] ? 2 : 3;
+      const uint32_t h = word == 0 ? hits[0] : word == 1 ? hits[1] : word == 2 ? hits[2] : hits[3];
+      float y = LOWEST;
+      uint32_t token = 0;
+      if (h) {
+        const uint32_t bit = word * 32 + __builtin_ctz(h), t = t1 - 1 - bit / EPT, i = bit % EPT;
+        token = t * TILE + i / VE * (64 * VE) + lane * VE + i % VE - s.lead;
+        y = (float)s.x[token];
+        sum += exp((double)y - ref);
       }
-    } else {
-      for (uint32_t i = lane; i < count; i += 64) sum += exp((double)value_of((uint32_t)(list[i] >> 32)) - ref);
+      const uint32_t rest = h & (h - 1);
+      hits[0] = word == 0 ? rest : hits[0], hits[1] = word == 1 ? rest : hits[1], hits[2] = word == 2 ? rest : hits[2], hits[3] = word == 3 ? rest : hits[3];
+      const bool keep = y >= floor_v && y > LOWEST;
+      const uint64_t who = __ballot(keep);
+      const uint32_t at = count + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+      if (keep && at < LIST) list[at] = (uint64_t)order_of(y) << 32 | ~token;
+      count += (uint32_t)__popcll(who);
+    }
+  } else {  // in f64, below the maximum that is now known
+    ref = most;
+    sum = 0.0;
+    count = LIST + 1;
+    for (uint32_t t = t0; t < t1; t++) {
+      float v[EPT];
+      s.load(t, w, m);
+      s.values(t, w, m, v);
+#pragma unroll 1
+      for (int i = 0; i < EPT; i++) sum += exp((double)v[i] - ref);
     }
   }
   for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
-  if (__any(nan) || most == __builtin_inff()) sum = __builtin_nan("");
+  if (nan || most == __builtin_inff()) sum = __builtin_nan("");
   if (lane == 0) sums[id] = {most > LOWEST || sum != sum ? sum : 0.0, ref};
 
   Entry* out = entries + (uint64_t)id * a.k;
@@ -261,7 +304,7 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
       for (uint32_t t = t0; t < t1; t++) {
         float v[EPT];
         s.load(t, w, m);
-        s.values(w, m, v);
+        s.values(t, w, m, v);
 #pragma unroll
         for (int i = 0; i < EPT; i++) {
           const uint64_t e = (uint64_t)order_of(v[i]) << 32 | ~(uint32_t)(s.token(t, i / VE) + i % VE);
@@ -291,7 +334,7 @@ __device__ __forceinline__ bool better(const Candidate& x, const Candidate& y) {
   return x.token < y.token;
 }
 
-constexpr int MERGE_BLOCK = 512, MERGE_WAVES = MERGE_BLOCK / 64, MERGE_LIST = 512, HELD = 8;
+constexpr int MERGE_BLOCK = 512, MERGE_WAVES = MERGE_BLOCK / 64, MERGE_LIST = 512, HELD = 4;
 
 // A wave a beam: its log-sum, its entries' scores, and a bound that k of them reach.  What reaches the best of the beams' bounds goes to LDS and is
 // ranked there by counting.
@@ -302,7 +345,7 @@ __global__ __launch_bounds__(MERGE_BLOCK) void beam_merge_kernel(BeamArgs a, con
   __shared__ Candidate list[MERGE_LIST];
   __shared__ uint64_t chosen[64];
   __shared__ uint32_t count;
-  const uint32_t r0 = blockIdx.x * a.beams, lane = threadIdx.x & 63, wave = threadIdx.x >> 6, per_row = a.segs * a.k;
+  const uint32_t r0 = blockIdx.x * a.beams, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), per_row = a.segs * a.k;
   const double none = -__builtin_inf();
   if (threadIdx.x == 0) count = 0;
 
@@ -315,23 +358,22 @@ __global__ __launch_bounds__(MERGE_BLOCK) void beam_merge_kernel(BeamArgs a, con
   for (uint32_t b = wave; b < a.beams; b += MERGE_WAVES) {
     const uint32_t row = r0 + b;
     const Entry* mine = entries + (uint64_t)row * per_row;
-    const bool done = is_finished(a, row);
-    const float c = a.scores ? a.scores[row] : 0.0f;
-    if (b == wave) {
+    if (b == wave) {  // (a finished row's are what an earlier call left: its log-sum, NaN, keeps them out)
 #pragma unroll
-      for (int i = 0; i < HELD; i++) held[i] = !done && lane + i * 64 < per_row ? mine[lane + i * 64] : Entry{LOWEST, 0};
+      for (int i = 0; i < HELD; i++) held[i] = lane + i * 64 < per_row ? mine[lane + i * 64] : Entry{LOWEST, 0};
     }
-    double s = 0.0, ref = none;
-    if (!done)
-      for (uint32_t i = lane; i < a.segs; i += 64) {
-        const SegSum g = sums[(uint64_t)row * a.segs + i];
-        if (g.sum == 0.0) continue;
-        if (g.ref > ref) s = s * exp(ref - g.ref) + g.sum, ref = g.ref;
-        else s += g.sum * exp(g.ref - ref);
-      }
-    double top = ref;
+    const SegSum* parts = sums + (uint64_t)row * a.segs;
+    const SegSum first = lane < a.segs ? parts[lane] : SegSum{0.0, none};
+    const float c = a.scores ? a.scores[row] : 0.0f;
+    const bool done = is_finished(a, row);
+    double top = first.sum != 0.0 ? first.ref : none;
+    for (uint32_t i = lane + 64; i < a.segs; i += 64) top = fmax(top, parts[i].sum != 0.0 ? parts[i].ref : none);
     for (int d = 32; d; d >>= 1) top = fmax(top, __shfl_xor(top, d));
-    s = ref > none ? s * exp(ref - top) : 0.0;
+    double s = 0.0;
+    for (uint32_t i = lane; i < a.segs; i += 64) {
+      const SegSum g = i < 64 ? first : parts[i];
+      if (g.sum != 0.0) s += g.sum * exp(g.ref - top);
+    }
     for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
     const double l = done ? __builtin_nan("") : top + log(s);
     if (lane == 0) lse[b] = l, cum[b] = c;
@@ -355,24 +397,24 @@ __global__ __launch_bounds__(MERGE_BLOCK) void beam_merge_kernel(BeamArgs a, con
     }
   };
   // every beam's entries, and a finished one's only candidate: f(score, beam, entry)
-  const auto each = [&](const auto& f) {
+  const auto each = [&](uint32_t from, const auto& f) {  // from: entries of the wave's first beam that f has had
     for (uint32_t b = wave; b < a.beams; b += MERGE_WAVES) {
       if (is_finished(a, r0 + b)) {
         if (lane == 0 && cum[b] == cum[b]) f((double)cum[b], b, Entry{0.0f, a.end_token});
         continue;
       }
       const double l = lse[b], c = cum[b];
-      if (b == wave) {
-#pragma unroll
-        for (int i = 0; i < HELD; i++) f(score(held[i], c, l), b, held[i]);
-      }
-      for (uint32_t e = lane + (b == wave ? HELD * 64 : 0); e < per_row; e += 64) {
+      for (uint32_t e = lane + (b == wave ? from : 0); e < per_row; e += 64) {
         const Entry x = entries[(uint64_t)(r0 + b) * per_row + e];
         f(score(x, c, l), b, x);
       }
     }
   };
-  each(offer);
+  if (wave < a.beams) {
+#pragma unroll
+    for (int i = 0; i < HELD; i++) offer(score(held[i], cum[wave], lse[wave]), wave, held[i]);
+  }
+  each(HELD * 64, offer);
   __syncthreads();
   const uint32_t n = count, found = n < a.k ? n : a.k;
   const auto put = [&](uint32_t rank, const Candidate& c) {
@@ -403,7 +445,7 @@ __global__ __launch_bounds__(MERGE_BLOCK) void beam_merge_kernel(BeamArgs a, con
     Candidate before = {__builtin_inf(), 0, 0, 0.0f};
     for (uint32_t r = 0; r < a.k; r++) {
       Candidate top = {none, ~0u, 0, 0.0f};
-      each([&](double s, uint32_t b, Entry x) {
+      each(0, [&](double s, uint32_t b, Entry x) {
         const Candidate c = {s, b, x.token, x.logit};
         if (s > none && (r == 0 || better(before, c)) && better(c, top)) top = c;
       });
