@@ -322,26 +322,26 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
 }
 
 // ---------------------------------------------------------------- a request
+// Candidates in order: score, then the lower beam, the higher logit (`tie`: smaller is better), the lower token
 struct Candidate {
   double score;
-  uint32_t beam, token;
-  float logit;
+  uint64_t tie;
+  uint32_t token;
 };
-__device__ __forceinline__ bool better(const Candidate& x, const Candidate& y) {
-  if (x.score != y.score) return x.score > y.score;
-  if (x.beam != y.beam) return x.beam < y.beam;
-  if (x.logit != y.logit) return x.logit > y.logit;
-  return x.token < y.token;
+__device__ __forceinline__ Candidate candidate_of(double score, uint32_t beam, Entry x) {
+  return {score, (uint64_t)beam << 32 | ~order_of(x.logit), x.token};
 }
+__device__ __forceinline__ bool before_equal(const Candidate& x, const Candidate& y) { return x.tie < y.tie || (x.tie == y.tie && x.token < y.token); }
+__device__ __forceinline__ bool better(const Candidate& x, const Candidate& y) { return x.score > y.score || (x.score == y.score && before_equal(x, y)); }
 
-constexpr int MERGE_BLOCK = 512, MERGE_WAVES = MERGE_BLOCK / 64, MERGE_LIST = 512, HELD = 4;
+constexpr int MERGE_BLOCK = 512, MERGE_WAVES = MERGE_BLOCK / 64, MERGE_LIST = 512, HELD = 4, PARTS = 4;
 
 // A wave a beam: its log-sum, its entries' scores, and a bound that k of them reach.  What reaches the best of the beams' bounds goes to LDS and is
 // ranked there by counting.
 __global__ __launch_bounds__(MERGE_BLOCK) void beam_merge_kernel(BeamArgs a, const SegSum* sums, const Entry* entries) {
   __shared__ double lse[1024];  // per beam: its log-sum, NaN for a row whose scores are −infinity
   __shared__ float cum[1024], wave_floor[MERGE_WAVES];
-  __shared__ double scores[MERGE_LIST + RANKED];
+  __shared__ double scores[MERGE_LIST + PARTS * RANKED];
   __shared__ Candidate list[MERGE_LIST];
   __shared__ uint64_t chosen[64];
   __shared__ uint32_t count;
@@ -393,7 +393,7 @@ __global__ __launch_bounds__(MERGE_BLOCK) void beam_merge_kernel(BeamArgs a, con
   const auto offer = [&](double s, uint32_t b, Entry x) {
     if (s > none && (float)s >= floor_v) {
       const uint32_t at = atomicAdd(&count, 1u);
-      if (at < MERGE_LIST) scores[at] = s, list[at] = {s, b, x.token, x.logit};
+      if (at < MERGE_LIST) scores[at] = s, list[at] = candidate_of(s, b, x);
     }
   };
   // every beam's entries, and a finished one's only candidate: f(score, beam, entry)
@@ -419,38 +419,46 @@ __global__ __launch_bounds__(MERGE_BLOCK) void beam_merge_kernel(BeamArgs a, con
   const uint32_t n = count, found = n < a.k ? n : a.k;
   const auto put = [&](uint32_t rank, const Candidate& c) {
     const uint64_t o = (uint64_t)blockIdx.x * a.k + rank;
+    const uint32_t beam = (uint32_t)(c.tie >> 32);
     a.out_scores[o] = (float)c.score;
-    a.out_parents[o] = r0 + c.beam;
+    a.out_parents[o] = r0 + beam;
     a.out_tokens[o] = c.token;
-    chosen[rank] = (uint64_t)c.beam * a.vocab + c.token;
+    chosen[rank] = (uint64_t)beam * a.vocab + c.token;
   };
   if (n <= MERGE_LIST) {
-    if (threadIdx.x < RANKED) scores[n + threadIdx.x] = none;
+    if (threadIdx.x < PARTS * RANKED) scores[n + threadIdx.x] = none;
     __syncthreads();
-    for (uint32_t i = threadIdx.x; i < n; i += MERGE_BLOCK) {
+    // PARTS lanes a candidate, each counts among its share
+    const uint32_t part = threadIdx.x % PARTS;
+    for (uint32_t i = threadIdx.x / PARTS; i < n; i += MERGE_BLOCK / PARTS) {
       const Candidate c = list[i];
       uint32_t rank = 0, equal = 0;
-      for (uint32_t j = 0; j < n; j += RANKED) {
+      for (uint32_t j = part * RANKED; j < n; j += PARTS * RANKED) {
         double o[RANKED];
 #pragma unroll
         for (int q = 0; q < RANKED; q++) o[q] = scores[j + q];
 #pragma unroll
-        for (int q = 0; q < RANKED; q++) rank += o[q] > c.score, equal += o[q] == c.score;
+        for (int q = 0; q < RANKED; q++) rank += o[q] > c.score, equal |= (uint32_t)(o[q] == c.score) << q;
+        while (equal) {  // (itself, and tokens of one logit)
+          const int q = __builtin_ctz(equal);
+          equal &= equal - 1;
+          rank += before_equal(list[j + q], c);
+        }
       }
-      if (equal > 1)
-        for (uint32_t j = 0; j < n; j++) rank += scores[j] == c.score && better(list[j], c);
-      if (rank < a.k) put(rank, c);
+#pragma unroll
+      for (int d = 1; d < PARTS; d *= 2) rank += __shfl_xor(rank, d);
+      if (part == 0 && rank < a.k) put(rank, c);
     }
   } else {  // very many equal scores: the best, then the best behind it, k times
-    Candidate before = {__builtin_inf(), 0, 0, 0.0f};
+    Candidate before = {__builtin_inf(), 0, 0};
     for (uint32_t r = 0; r < a.k; r++) {
-      Candidate top = {none, ~0u, 0, 0.0f};
+      Candidate top = {none, ~0ull, 0};
       each(0, [&](double s, uint32_t b, Entry x) {
-        const Candidate c = {s, b, x.token, x.logit};
+        const Candidate c = candidate_of(s, b, x);
         if (s > none && (r == 0 || better(before, c)) && better(c, top)) top = c;
       });
       for (int d = 32; d; d >>= 1) {
-        const Candidate o = {__shfl_xor(top.score, d), __shfl_xor(top.beam, d), __shfl_xor(top.token, d), __shfl_xor(top.logit, d)};
+        const Candidate o = {__shfl_xor(top.score, d), __shfl_xor(top.tie, d), __shfl_xor(top.token, d)};
         if (better(o, top)) top = o;
       }
       __syncthreads();
@@ -462,17 +470,25 @@ __global__ __launch_bounds__(MERGE_BLOCK) void beam_merge_kernel(BeamArgs a, con
       before = top;
     }
   }
+  if (found == a.k) return;
+  // the rest: (row, token) in ascending order, without the chosen ones — of the first found + (k − found) < 128 pairs as many are free
   __syncthreads();
-  if (threadIdx.x == 0)  // the rest: (row, token) in ascending order, without the chosen ones
-    for (uint64_t f = 0, i = found; i < a.k; f++) {
+  if (wave == 0) {
+    uint32_t at = found;
+    for (uint32_t f = lane; at < a.k; f += 64) {
       bool taken = false;
       for (uint32_t j = 0; j < found; j++) taken |= chosen[j] == f;
-      if (taken) continue;
-      const uint64_t o = (uint64_t)blockIdx.x * a.k + i++;
-      a.out_scores[o] = -__builtin_inff();
-      a.out_parents[o] = r0 + (uint32_t)(f / a.vocab);
-      a.out_tokens[o] = (uint32_t)(f % a.vocab);
+      const uint64_t free = __ballot(!taken);
+      const uint32_t mine = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(free >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)free, 0));
+      if (!taken && mine < a.k) {
+        const uint64_t o = (uint64_t)blockIdx.x * a.k + mine;
+        a.out_scores[o] = LOWEST;
+        a.out_parents[o] = r0 + f / a.vocab;
+        a.out_tokens[o] = f % a.vocab;
+      }
+      at += (uint32_t)__popcll(free);
     }
+  }
 }
 
 // ---------------------------------------------------------------- host
