@@ -23,16 +23,18 @@ struct Factors {
 // span: max |x| or max − min; bad: the group holds a NaN or an infinity
 template <int CODE>
 __device__ __forceinline__ Factors factors(float span, float lo, bool bad) {
-  const float top = Top<CODE>::v;
+  constexpr float top = Top<CODE>::v;
   if (bad || !(span < __builtin_inff())) return {__builtin_nanf(""), 0.0f, lo};
   if (span < top * 0x1p-126f) return {0.0f, 0.0f, lo};  // span / top would be subnormal and top / span could overflow
-  return {span / top, top / span, lo};
+  // span / top, rounded once: the remainder of span · (1 / top) is exact and corrects it (compared with the division for all 2^23 mantissas)
+  constexpr float r = 1.0f / top;
+  const float q = span * r;
+  return {__builtin_fmaf(__builtin_fmaf(-q, top, span), r, q), top / span, lo};
 }
 __device__ __forceinline__ uint32_t whole(float x, float inv) {  // low byte: the code in two's complement
   return __builtin_bit_cast(uint32_t, __builtin_fmaf(x, inv, 0x1.8p23f));
 }
 
-// ---------------------------------------------------------------- one wave a group: any group, stride and alignment
 struct QuantCol {
   void* x;
   uint64_t row_stride, head_stride;
@@ -44,6 +46,180 @@ struct QuantShape {
   uint32_t heads, dim, group, groups_per_head, groups_per_row;
 };
 
+// ---------------------------------------------------------------- eight values a lane
+// Both ways stream: 16-byte accesses (32 of f32) on the rows' side, 8 or 4 on the codes'.  A group is `lanes` neighbouring lanes (a power of two, those
+// past the group's end idle), its span found with data-parallel moves inside the wave.  A block takes whole rows, looks their slots up once and
+// keeps them in LDS: a search of the sequence through memory costs microseconds, so it is shared by up to 16 passes of the block.
+constexpr int MAX_COLS = 8, MAX_ROWS = 256;
+struct QuantCols {
+  QuantCol c[MAX_COLS];
+};
+// x / d by a product, x < 2^31
+struct Divide {
+  uint32_t d, m, s;
+};
+__device__ __forceinline__ uint32_t operator/(uint32_t x, Divide d) { return __umulhi(x << 1, d.m) >> d.s; }
+Divide divide_by(uint32_t d) {
+  uint32_t s = 0;
+  while ((1ull << s) < d) s++;
+  return {d, (uint32_t)(((1ull << (31 + s)) + d - 1) / d), s};
+}
+struct FastShape {
+  uint32_t group, dim, groups_per_row, lanes, log_lanes, rows;  // rows of a block
+  Divide by_row, by_head;                                      // groups a row, groups a head
+};
+
+typedef uint32_t u32x8 __attribute__((ext_vector_type(8)));
+template <typename T> struct Eight;  // eight values as they lie in memory
+template <> struct Eight<float> {
+  typedef float type __attribute__((ext_vector_type(8)));
+};
+template <> struct Eight<f16_t> {
+  typedef f16_t type __attribute__((ext_vector_type(8)));
+};
+template <> struct Eight<bf16_t> {
+  typedef bf16_t type __attribute__((ext_vector_type(8)));
+};
+
+template <int CTRL>
+__device__ __forceinline__ float moved(float x) {  // another lane's of the row of 16
+  return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, x), CTRL, 0xF, 0xF, true));
+}
+// f over the `lanes` lanes of a group: neighbour, pair, then mirrored halves — after the steps before them all lanes of a half agree
+template <typename F>
+__device__ __forceinline__ float over_group(float x, uint32_t lanes, F f) {
+  if (lanes > 1) x = f(x, moved<0xB1>(x));   // quad_perm 1 0 3 2
+  if (lanes > 2) x = f(x, moved<0x4E>(x));   // quad_perm 2 3 0 1
+  if (lanes > 4) x = f(x, moved<0x141>(x));  // row_half_mirror
+  if (lanes > 8) x = f(x, moved<0x140>(x));  // row_mirror
+  if (lanes > 16) x = f(x, __shfl_xor(x, 16));
+  if (lanes > 32) x = f(x, __shfl_xor(x, 32));
+  return x;
+}
+
+// the block's rows' slots; false: nothing to do in this block
+__device__ __forceinline__ uint32_t block_slots(const RowAddr& addr, uint64_t row0, uint64_t n, uint32_t rows, uint64_t n_slots, uint64_t* slots, uint32_t* flags) {
+  const uint32_t mine = (uint32_t)(n - row0 < rows ? n - row0 : rows);
+  if (threadIdx.x < mine) {
+    const uint64_t s = row_slot(addr, row0 + threadIdx.x, n_slots);
+    slots[threadIdx.x] = s;
+    if (s == ROW_BAD) *reinterpret_cast<volatile uint32_t*>(flags) = AGPU_FLAG_INDEX_RANGE;
+  }
+  __syncthreads();
+  return mine;
+}
+
+template <typename T, int CODE>
+__global__ __launch_bounds__(AGPU_BLOCK) void put_eight_kernel(QuantCols cols, FastShape q, RowAddr addr, uint64_t n, uint32_t* flags) {
+  __shared__ uint64_t slots[MAX_ROWS];
+  const QuantCol& c = cols.c[blockIdx.y];
+  const uint64_t row0 = (uint64_t)blockIdx.x * q.rows;
+  const uint32_t rows = block_slots(addr, row0, n, q.rows, c.n_slots, slots, flags);
+  const uint32_t total = (rows * q.groups_per_row) << q.log_lanes;
+  for (uint32_t i = threadIdx.x; i < total; i += AGPU_BLOCK) {
+    const uint32_t g = i >> q.log_lanes, sub = i & (q.lanes - 1), row = g / q.by_row, in_row = g - row * q.groups_per_row, head = in_row / q.by_head;
+    const uint64_t slot = slots[row];
+    const uint32_t off = (in_row - head * q.by_head.d) * q.group + sub * 8;
+    const bool live = sub * 8 < q.group && slot < ROW_BAD;
+    float v[8] = {};
+    if (live) {
+      const T* x = static_cast<const T*>(c.x) + (row0 + row) * c.row_stride + head * c.head_stride + off;
+      const typename Eight<T>::type w = *reinterpret_cast<const typename Eight<T>::type*>(x);
+#pragma unroll
+      for (int j = 0; j < 8; j++) v[j] = (float)w[j];
+    }
+    // the largest magnitude by its bits: a NaN's lie above infinity's, and stay
+    uint32_t most = 0;
+#pragma unroll
+    for (int j = 0; j < 8; j++) {
+      const uint32_t b = __builtin_bit_cast(uint32_t, v[j]) & 0x7FFFFFFFu;
+      most = b > most ? b : most;
+    }
+    const auto higher = [](float a, float b) {
+      const uint32_t x = __builtin_bit_cast(uint32_t, a), y = __builtin_bit_cast(uint32_t, b);
+      return __builtin_bit_cast(float, x > y ? x : y);
+    };
+    const float mag = over_group(__builtin_bit_cast(float, most), q.lanes, higher);
+    const bool bad = __builtin_bit_cast(uint32_t, mag) >= 0x7F800000u;
+    float span = mag, lo = 0.0f;
+    if (CODE == AGPU_CODE_I4) {
+      float l = live ? v[0] : __builtin_inff(), h = live ? v[0] : -__builtin_inff();
+#pragma unroll
+      for (int j = 1; j < 8; j++) l = live ? fminf(l, v[j]) : l, h = live ? fmaxf(h, v[j]) : h;
+      lo = over_group(l, q.lanes, [](float a, float b) { return fminf(a, b); });
+      span = over_group(h, q.lanes, [](float a, float b) { return fmaxf(a, b); }) - lo;
+    }
+    const Factors f = factors<CODE>(span, lo, bad);
+    if (!live) continue;
+    const uint64_t at = slot * q.groups_per_row + in_row;
+    if (CODE == AGPU_CODE_I4) {
+      if (sub == 0) reinterpret_cast<float2*>(c.scales)[at] = {f.scale, f.lo};
+      uint32_t w = 0;
+#pragma unroll
+      for (int j = 0; j < 8; j++) w |= (whole(v[j] - f.lo, f.inv) & 15) << 4 * j;
+      *reinterpret_cast<uint32_t*>(c.codes + at * (q.group / 2) + sub * 4) = w;
+    } else {
+      if (sub == 0) c.scales[at] = f.scale;
+      u32x2 w;
+#pragma unroll
+      for (int h = 0; h < 2; h++) {
+        if (CODE == AGPU_CODE_I8) {
+          w[h] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(whole(v[4 * h + 3], f.inv), whole(v[4 * h + 2], f.inv), 0x0C0C0400u),
+                                       __builtin_amdgcn_perm(whole(v[4 * h + 1], f.inv), whole(v[4 * h], f.inv), 0x0C0C0400u), 0x05040100u);
+        } else {
+          const int low = __builtin_amdgcn_cvt_pk_fp8_f32(v[4 * h] * f.inv, v[4 * h + 1] * f.inv, 0, false);
+          w[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[4 * h + 2] * f.inv, v[4 * h + 3] * f.inv, low, true);
+        }
+      }
+      *reinterpret_cast<u32x2*>(c.codes + at * q.group + sub * 8) = w;
+    }
+  }
+}
+
+template <typename T, int CODE>
+__global__ __launch_bounds__(AGPU_BLOCK) void take_eight_kernel(QuantCols cols, FastShape q, RowAddr addr, uint64_t n, uint32_t* flags) {
+  __shared__ uint64_t slots[MAX_ROWS];
+  const QuantCol& c = cols.c[blockIdx.y];
+  const uint64_t row0 = (uint64_t)blockIdx.x * q.rows;
+  const uint32_t rows = block_slots(addr, row0, n, q.rows, c.n_slots, slots, flags);
+  const uint32_t total = (rows * q.groups_per_row) << q.log_lanes;
+  for (uint32_t i = threadIdx.x; i < total; i += AGPU_BLOCK) {
+    const uint32_t g = i >> q.log_lanes, sub = i & (q.lanes - 1), row = g / q.by_row, in_row = g - row * q.groups_per_row, head = in_row / q.by_head;
+    const uint64_t slot = slots[row];
+    if (sub * 8 >= q.group || slot == ROW_NONE) continue;
+    const uint64_t at = slot * q.groups_per_row + in_row;
+    float v[8] = {};
+    if (slot != ROW_BAD) {
+      if (CODE == AGPU_CODE_I4) {
+        const float2 f = reinterpret_cast<const float2*>(c.scales)[at];
+        const uint32_t w = *reinterpret_cast<const uint32_t*>(c.codes + at * (q.group / 2) + sub * 4);
+#pragma unroll
+        for (int j = 0; j < 8; j++) v[j] = __builtin_fmaf((float)(w >> 4 * j & 15), f.x, f.y);
+      } else {
+        const float scale = c.scales[at];
+        const u32x2 w = *reinterpret_cast<const u32x2*>(c.codes + at * q.group + sub * 8);
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const uint32_t b = w[h];
+          if (CODE == AGPU_CODE_I8) {
+#pragma unroll
+            for (int j = 0; j < 4; j++) v[4 * h + j] = (float)(int8_t)(b >> 8 * j) * scale;
+          } else {
+            const auto low = __builtin_amdgcn_cvt_pk_f32_fp8(b, false), high = __builtin_amdgcn_cvt_pk_f32_fp8(b, true);
+            v[4 * h] = low[0] * scale, v[4 * h + 1] = low[1] * scale, v[4 * h + 2] = high[0] * scale, v[4 * h + 3] = high[1] * scale;
+          }
+        }
+      }
+    }
+    typename Eight<T>::type o;
+#pragma unroll
+    for (int j = 0; j < 8; j++) o[j] = (T)v[j];
+    T* x = static_cast<T*>(c.x) + (row0 + row) * c.row_stride + head * c.head_stride + (in_row - head * q.by_head.d) * q.group + sub * 8;
+    *reinterpret_cast<typename Eight<T>::type*>(x) = o;
+  }
+}
+
+// ---------------------------------------------------------------- one wave a group: any group, stride and alignment
 template <typename T, int CODE>
 __global__ __launch_bounds__(AGPU_BLOCK) void put_group_kernel(QuantCol c, QuantShape q, RowAddr addr, uint64_t n_groups, uint32_t* flags) {
   const uint32_t lane = threadIdx.x & 63;
@@ -132,22 +308,50 @@ agpu_status check_columns(int32_t n_cols, const agpu_quantised_rows* stores, con
   return AGPU_OK;
 }
 
+// Eight values a lane: a group of whole eights in one wave, everything on its vectors' alignment
+bool by_eights(const QuantCol& c, const QuantShape& q, int type, int code) {
+  const uint64_t item = type == AGPU_ROW_F32 ? 4 : 2, strides = (c.row_stride | (q.heads > 1 ? c.head_stride : 0)) * item;
+  return q.group % 8 == 0 && q.group <= 512 && strides % 16 == 0 && aligned16(c.x) && aligned_to(c.codes, code == AGPU_CODE_I4 ? 4 : 8) &&
+         aligned_to(c.scales, code == AGPU_CODE_I4 ? 8 : 4);
+}
+
+// Rows of a block: 16 passes of its lanes, fewer where that would leave less than 2048 blocks (8 a CU)
+FastShape fast_shape(const QuantShape& q, uint64_t n, uint32_t n_cols) {
+  FastShape f = {};
+  f.group = q.group, f.dim = q.dim, f.groups_per_row = q.groups_per_row;
+  while (8u << f.log_lanes < q.group) f.log_lanes++;
+  f.lanes = 1u << f.log_lanes;
+  const uint64_t row_lanes = (uint64_t)q.groups_per_row << f.log_lanes;
+  uint64_t rows = 16 * AGPU_BLOCK / row_lanes;
+  if (rows * 2048 > n * n_cols) rows = n * n_cols / 2048;
+  if (rows * row_lanes < AGPU_BLOCK) rows = AGPU_BLOCK / row_lanes;
+  f.rows = (uint32_t)(rows < 1 ? 1 : rows > MAX_ROWS ? MAX_ROWS : rows);
+  f.by_row = divide_by(q.groups_per_row), f.by_head = divide_by(q.groups_per_head);
+  return f;
+}
+
 template <typename T, int CODE>
-agpu_status launch_groups(agpu_pipeline* p, bool put, const QuantCol& c, const QuantShape& q, const RowAddr& addr, uint64_t n) {
-  const uint64_t n_groups = n * q.groups_per_row;
-  const uint64_t blocks = (n_groups + 3) / 4;
-  const int grid = (int)(blocks > (1u << 20) ? (1u << 20) : blocks);
-  if (put) hipLaunchKernelGGL((put_group_kernel<T, CODE>), dim3(grid), dim3(AGPU_BLOCK), 0, p->stream, c, q, addr, n_groups, p->flags);
-  else hipLaunchKernelGGL((take_group_kernel<T, CODE>), dim3(grid), dim3(AGPU_BLOCK), 0, p->stream, c, q, addr, n_groups, p->flags);
-  AGPU_LAUNCH_CHECK();
-  return AGPU_OK;
+void launch_code(agpu_pipeline* p, bool put, bool eights, const QuantCols& cols, uint32_t n_cols, const QuantShape& q, const RowAddr& addr, uint64_t n) {
+  if (eights) {
+    const FastShape f = fast_shape(q, n, n_cols);
+    const dim3 grid((uint32_t)((n + f.rows - 1) / f.rows), n_cols);
+    if (put) hipLaunchKernelGGL((put_eight_kernel<T, CODE>), grid, dim3(AGPU_BLOCK), 0, p->stream, cols, f, addr, n, p->flags);
+    else hipLaunchKernelGGL((take_eight_kernel<T, CODE>), grid, dim3(AGPU_BLOCK), 0, p->stream, cols, f, addr, n, p->flags);
+    return;
+  }
+  for (uint32_t k = 0; k < n_cols; k++) {
+    const uint64_t n_groups = n * q.groups_per_row, blocks = (n_groups + 3) / 4;
+    const int grid = (int)(blocks > (1u << 20) ? (1u << 20) : blocks);
+    if (put) hipLaunchKernelGGL((put_group_kernel<T, CODE>), dim3(grid), dim3(AGPU_BLOCK), 0, p->stream, cols.c[k], q, addr, n_groups, p->flags);
+    else hipLaunchKernelGGL((take_group_kernel<T, CODE>), dim3(grid), dim3(AGPU_BLOCK), 0, p->stream, cols.c[k], q, addr, n_groups, p->flags);
+  }
 }
 template <typename T>
-agpu_status launch_code(agpu_pipeline* p, bool put, int code, const QuantCol& c, const QuantShape& q, const RowAddr& addr, uint64_t n) {
+void launch_type(agpu_pipeline* p, bool put, bool eights, int code, const QuantCols& cols, uint32_t n_cols, const QuantShape& q, const RowAddr& addr, uint64_t n) {
   switch (code) {
-    case AGPU_CODE_I8: return launch_groups<T, AGPU_CODE_I8>(p, put, c, q, addr, n);
-    case AGPU_CODE_I4: return launch_groups<T, AGPU_CODE_I4>(p, put, c, q, addr, n);
-    default: return launch_groups<T, AGPU_CODE_E4M3>(p, put, c, q, addr, n);
+    case AGPU_CODE_I8: return launch_code<T, AGPU_CODE_I8>(p, put, eights, cols, n_cols, q, addr, n);
+    case AGPU_CODE_I4: return launch_code<T, AGPU_CODE_I4>(p, put, eights, cols, n_cols, q, addr, n);
+    default: return launch_code<T, AGPU_CODE_E4M3>(p, put, eights, cols, n_cols, q, addr, n);
   }
 }
 
@@ -155,15 +359,25 @@ agpu_status quantised(agpu_pipeline* p, bool put, int32_t n_cols, const agpu_qua
                       uint64_t n, const char* name) {
   AGPU_BIND_AS(p, name);
   if (n == 0) return AGPU_OK;
-  for (int32_t k = 0; k < n_cols; k++) {
+  // neighbouring columns of one kind go into one launch
+  for (int32_t k = 0; k < n_cols;) {
     const agpu_quantised_rows& s = stores[k];
-    const agpu_rows& r = rows[k];
-    const QuantCol c = {r.data, r.row_stride, r.head_stride, static_cast<uint8_t*>(s.codes), s.scales, s.n_slots};
+    const int type = rows[k].type;
     const QuantShape q = {s.heads, s.dim, s.group, s.dim / s.group, s.heads * (s.dim / s.group)};
-    const agpu_status st = r.type == AGPU_ROW_F32   ? launch_code<float>(p, put, s.code, c, q, addr, n)
-                           : r.type == AGPU_ROW_F16 ? launch_code<f16_t>(p, put, s.code, c, q, addr, n)
-                                                    : launch_code<bf16_t>(p, put, s.code, c, q, addr, n);
-    if (st != AGPU_OK) return st;
+    QuantCols cols;
+    uint32_t m = 0;
+    bool eights = true;
+    for (; k < n_cols && m < MAX_COLS; k++, m++) {
+      const agpu_quantised_rows& o = stores[k];
+      const agpu_rows& r = rows[k];
+      if (o.heads != s.heads || o.dim != s.dim || o.group != s.group || o.code != s.code || r.type != type) break;
+      cols.c[m] = {r.data, r.row_stride, r.head_stride, static_cast<uint8_t*>(o.codes), o.scales, o.n_slots};
+      eights = eights && by_eights(cols.c[m], q, type, s.code);
+    }
+    if (type == AGPU_ROW_F32) launch_type<float>(p, put, eights, s.code, cols, m, q, addr, n);
+    else if (type == AGPU_ROW_F16) launch_type<f16_t>(p, put, eights, s.code, cols, m, q, addr, n);
+    else launch_type<bf16_t>(p, put, eights, s.code, cols, m, q, addr, n);
+    AGPU_LAUNCH_CHECK();
   }
   return AGPU_OK;
 }
