@@ -230,33 +230,6 @@ class IpcFieldStruct(C.Structure):  # agpu_ipc_field
     _fields_ = [("name", C.c_char_p), ("format", C.c_char_p), ("dtype", C.c_int32), ("nullable", C.c_int32)]
 
 
-class RowsStruct(C.Structure):  # agpu_rows
-    _fields_ = [("data", C.c_void_p), ("row_stride", C.c_uint64), ("head_stride", C.c_uint64), ("type", C.c_int32)]
-
-
-class QuantisedRowsStruct(C.Structure):  # agpu_quantised_rows
-    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("n_slots", C.c_uint64), ("heads", C.c_uint32), ("dim", C.c_uint32),
-                ("group", C.c_uint32), ("code", C.c_int32)]
-
-
-class PageMapStruct(C.Structure):  # agpu_page_map
-    _fields_ = [("tables", C.c_void_p), ("table_stride", C.c_uint64), ("offsets", C.c_void_p), ("first", C.c_void_p), ("n_seqs", C.c_uint32),
-                ("max_pages", C.c_uint32), ("page_rows", C.c_uint32)]
-
-
-class StateStruct(C.Structure):  # agpu_state
-    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("src_row_stride", C.c_uint64), ("src_piece_stride", C.c_uint64),
-                ("dst_row_stride", C.c_uint64), ("dst_piece_stride", C.c_uint64), ("n_pieces", C.c_uint64), ("piece_bytes", C.c_uint64),
-                ("position_bytes", C.c_uint64)]
-
-
-class BeamsStruct(C.Structure):  # agpu_beams
-    _fields_ = [("logits", C.c_void_p), ("row_stride", C.c_uint64), ("type", C.c_int32), ("batch", C.c_uint32), ("beams", C.c_uint32),
-                ("vocab", C.c_uint32), ("k", C.c_uint32), ("end_token", C.c_uint32), ("scores", C.c_void_p), ("allowed", C.c_void_p),
-                ("allowed_stride", C.c_uint64), ("finished", C.c_void_p), ("out_scores", C.c_void_p), ("out_parents", C.c_void_p),
-                ("out_tokens", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
-
-
 class ArrowErrorGPU(RuntimeError):
     """Mirror of `enum ArrowErrorGPU` (crates/array/src/lib.rs:11-14) plus device/runtime failures."""
 
@@ -313,4 +286,12 @@ def check(status: int, what: str = "") -> None:
 
 def call(name: str, *args) -> None:
     """Call a status-returning entry point and raise on failure."""
-    check(getattr(lib(), name)(*args), name)
+    status = getattr(_lib or lib(), name)(*args)
+    if status != OK:
+        check(status, name)
+
+
+def select_beams_workspace(batch: int, beams: int, vocab: int, k: int) -> int:
+    need = C.c_uint64()
+    call("agpu_select_beams_workspace", batch, beams, vocab, k, C.byref(need))
+    return need.value

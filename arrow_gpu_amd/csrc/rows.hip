@@ -412,20 +412,43 @@ agpu_status quantised_pages(agpu_pipeline* p, bool put, int32_t n_cols, const ag
 }
 
 // ---------------------------------------------------------------- take_rows
+// A copy with one indirection: lanes run over the states' accesses of V bytes in the order of the destination, four of a lane in flight, all states in
+// one launch (blockIdx.y).
+constexpr int MAX_STATES = 8, ROWS_UNROLL = 4;
+struct State {
+  const char* src;
+  char* dst;
+  uint64_t src_row_stride, src_piece_stride, dst_row_stride, dst_piece_stride, position_bytes;
+  uint32_t n_vecs, vecs_per_row;
+  Divide by_row, by_piece;
+};
+struct States {
+  State s[MAX_STATES];
+};
+
 template <typename V>
-__global__ __launch_bounds__(AGPU_BLOCK) void take_rows_kernel(agpu_state s, uint64_t n_src, const uint32_t* idx, const uint32_t* lengths, uint64_t n_vecs,
-                                                               uint64_t vecs_per_piece, uint32_t* flags) {
-  const uint64_t stride = (uint64_t)gridDim.x * AGPU_BLOCK, vecs_per_row = vecs_per_piece * s.n_pieces;
-  for (uint64_t v = (uint64_t)blockIdx.x * AGPU_BLOCK + threadIdx.x; v < n_vecs; v += stride) {
-    const uint64_t row = v / vecs_per_row, in_row = v - row * vecs_per_row, piece = in_row / vecs_per_piece, off = (in_row - piece * vecs_per_piece) * sizeof(V);
+__global__ __launch_bounds__(AGPU_BLOCK) void take_rows_kernel(States states, uint64_t n_src, const uint32_t* idx, const uint32_t* lengths, uint32_t* flags) {
+  const State& s = states.s[blockIdx.y];
+  const uint32_t v0 = blockIdx.x * (AGPU_BLOCK * ROWS_UNROLL) + threadIdx.x;
+  V w[ROWS_UNROLL];
+  char* to[ROWS_UNROLL];
+#pragma unroll
+  for (int u = 0; u < ROWS_UNROLL; u++) {
+    const uint32_t v = v0 + u * AGPU_BLOCK;
+    to[u] = nullptr;
+    w[u] = V{};
+    if (v >= s.n_vecs) continue;
+    const uint32_t row = v / s.by_row, in_row = v - row * s.vecs_per_row, piece = in_row / s.by_piece, off = (in_row - piece * s.by_piece.d) * (uint32_t)sizeof(V);
     if (lengths && off >= lengths[row] * s.position_bytes) continue;
     const uint32_t from = idx[row];
     if (from == AGPU_NO_ROW) continue;
-    V w = {};
-    if (from < n_src) w = *reinterpret_cast<const V*>(static_cast<const char*>(s.src) + from * s.src_row_stride + piece * s.src_piece_stride + off);
+    to[u] = s.dst + row * s.dst_row_stride + piece * s.dst_piece_stride + off;
+    if (from < n_src) w[u] = *reinterpret_cast<const V*>(s.src + from * s.src_row_stride + piece * s.src_piece_stride + off);
     else *reinterpret_cast<volatile uint32_t*>(flags) = AGPU_FLAG_INDEX_RANGE;
-    *reinterpret_cast<V*>(static_cast<char*>(s.dst) + row * s.dst_row_stride + piece * s.dst_piece_stride + off) = w;
   }
+#pragma unroll
+  for (int u = 0; u < ROWS_UNROLL; u++)
+    if (to[u]) *reinterpret_cast<V*>(to[u]) = w[u];
 }
 
 // bytes from the first to behind the last of n rows; 0: none.  false: past 2^63
@@ -450,6 +473,7 @@ agpu_status check_states(int32_t n_states, const agpu_state* states, uint64_t n_
                  AGPU_ERR_SHAPE, "a state past the address space");
     AGPU_REQUIRE((s.n_pieces == 1 || s.dst_piece_stride >= s.piece_bytes) && (n == 1 || s.dst_row_stride >= s.piece_bytes), AGPU_ERR_SHAPE,
                  "rows that are written may not overlap");
+    AGPU_REQUIRE(row_bytes < (1ull << 31), AGPU_ERR_SHAPE, "a row holds less than 2^31 bytes");
     AGPU_REQUIRE(!lengths || s.position_bytes > 0, AGPU_ERR_SHAPE, "lengths need position_bytes");
     for (int32_t j = 0; j < n_states; j++) {
       const agpu_state& o = states[j];
@@ -491,20 +515,41 @@ agpu_status agpu_take_rows(agpu_pipeline* p, int32_t n_states, const agpu_state*
   }
   AGPU_BIND(p);
   if (!any) return AGPU_OK;
+  // the widest access that everything is a multiple of, the same for the states of one launch
+  uint64_t all = 0, longest = 0;
   for (int32_t k = 0; k < n_states; k++) {
     const agpu_state& s = states[k];
     if (s.n_pieces == 0 || s.piece_bytes == 0) continue;
-    // the widest access that everything is a multiple of
-    const uint64_t all = reinterpret_cast<uintptr_t>(s.src) | reinterpret_cast<uintptr_t>(s.dst) | s.src_row_stride | s.src_piece_stride | s.dst_row_stride |
-                         s.dst_piece_stride | s.piece_bytes | (lengths ? s.position_bytes : 0);
-    const uint64_t width = (all & 15) == 0 ? 16 : (all & 3) == 0 ? 4 : 1;
-    const uint64_t vecs_per_piece = s.piece_bytes / width, n_vecs = n * s.n_pieces * vecs_per_piece;
-    const uint64_t blocks = (n_vecs + AGPU_BLOCK - 1) / AGPU_BLOCK;
-    const int grid = (int)(blocks > (1u << 20) ? (1u << 20) : blocks);
-    if (width == 16) hipLaunchKernelGGL((take_rows_kernel<u32x4>), dim3(grid), dim3(AGPU_BLOCK), 0, p->stream, s, n_src, idx, lengths, n_vecs, vecs_per_piece, p->flags);
-    else if (width == 4) hipLaunchKernelGGL((take_rows_kernel<uint32_t>), dim3(grid), dim3(AGPU_BLOCK), 0, p->stream, s, n_src, idx, lengths, n_vecs, vecs_per_piece, p->flags);
-    else hipLaunchKernelGGL((take_rows_kernel<uint8_t>), dim3(grid), dim3(AGPU_BLOCK), 0, p->stream, s, n_src, idx, lengths, n_vecs, vecs_per_piece, p->flags);
-    AGPU_LAUNCH_CHECK();
+    all |= reinterpret_cast<uintptr_t>(s.src) | reinterpret_cast<uintptr_t>(s.dst) | s.src_row_stride | s.src_piece_stride | s.dst_row_stride | s.dst_piece_stride |
+           s.piece_bytes | (lengths ? s.position_bytes : 0);
+    if (s.n_pieces * s.piece_bytes > longest) longest = s.n_pieces * s.piece_bytes;
+  }
+  if (longest == 0) return AGPU_OK;
+  const uint32_t width = (all & 15) == 0 ? 16 : (all & 3) == 0 ? 4 : 1;
+  // accesses are counted in 31 bits: as many rows at a time as that holds
+  const uint64_t at_once = ((1ull << 31) - 1) / (longest / width);
+  for (uint64_t r0 = 0; r0 < n; r0 += at_once) {
+    const uint64_t rows = n - r0 < at_once ? n - r0 : at_once;
+    for (int32_t k = 0; k < n_states;) {
+      States held;
+      uint32_t m = 0, most = 0;
+      for (; k < n_states && m < MAX_STATES; k++) {
+        const agpu_state& s = states[k];
+        if (s.n_pieces == 0 || s.piece_bytes == 0) continue;
+        const uint32_t per_piece = (uint32_t)(s.piece_bytes / width), per_row = (uint32_t)s.n_pieces * per_piece, n_vecs = (uint32_t)rows * per_row;
+        held.s[m++] = {static_cast<const char*>(s.src), static_cast<char*>(s.dst) + r0 * s.dst_row_stride, s.src_row_stride, s.src_piece_stride, s.dst_row_stride,
+                       s.dst_piece_stride, s.position_bytes, n_vecs, per_row, divide_by(per_row), divide_by(per_piece)};
+        most = n_vecs > most ? n_vecs : most;
+      }
+      if (m == 0) break;
+      const dim3 grid((most + AGPU_BLOCK * ROWS_UNROLL - 1) / (AGPU_BLOCK * ROWS_UNROLL), m);
+      const uint32_t* at = idx + r0;
+      const uint32_t* len = lengths ? lengths + r0 : nullptr;
+      if (width == 16) hipLaunchKernelGGL((take_rows_kernel<u32x4>), grid, dim3(AGPU_BLOCK), 0, p->stream, held, n_src, at, len, p->flags);
+      else if (width == 4) hipLaunchKernelGGL((take_rows_kernel<uint32_t>), grid, dim3(AGPU_BLOCK), 0, p->stream, held, n_src, at, len, p->flags);
+      else hipLaunchKernelGGL((take_rows_kernel<uint8_t>), grid, dim3(AGPU_BLOCK), 0, p->stream, held, n_src, at, len, p->flags);
+      AGPU_LAUNCH_CHECK();
+    }
   }
   return AGPU_OK;
 }

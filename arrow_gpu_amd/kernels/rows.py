@@ -5,7 +5,7 @@ As everywhere here the `*_op` forms enqueue on a pipeline and return without wai
 that an index out of range is raised by the call.  `out` writes into memory the caller has (a torch tensor's, last step's)."""
 from __future__ import annotations
 
-import ctypes as C
+import struct
 
 from .. import _capi as capi
 from ..array import BooleanArrayGPU, Float32ArrayGPU, UInt32ArrayGPU
@@ -13,17 +13,21 @@ from ..gpu_utils import ArrowComputePipeline
 from ..rows import ROW_TYPE, BeamSelection, PageMap, QuantisedRowsGPU, RowsGPU, shape_error
 
 _MAX_COLUMNS = 64
+_PACK_STATE = struct.Struct("=QQQQQQQQQ")            # agpu_state
+_PACK_BEAMS = struct.Struct("=QQiIIIIIQQQQQQQQQ")  # agpu_beams
 
 
 def _keep(pipeline, *buffers) -> None:
     """Buffers of this library's own: a borrowed one's lifetime is its owner's affair."""
-    pipeline.keep(*[b for b in buffers if b is not None and b._owned])
+    for b in buffers:
+        if b._owned:
+            pipeline.keep(b)
 
 
 def _on(pipeline, *things) -> None:
     dev = pipeline.device
     for t in things:
-        if t is not None and t.gpu_device is not dev and t.gpu_device.ordinal != dev.ordinal:
+        if t.gpu_device is not dev and t.gpu_device.ordinal != dev.ordinal:
             raise capi.ArrowErrorGPU("ArgumentError", f"memory of GPU {t.gpu_device.ordinal} in a pipeline of GPU {dev.ordinal}", capi.ERR_ARG)
 
 
@@ -34,27 +38,22 @@ def _u32(array, what: str):
 
 
 def _quantised(name: str, stores, rows, where, n: int, pipeline) -> None:
-    k = len(stores)
-    if k > _MAX_COLUMNS:
-        raise shape_error(f"{k} caches in one call: at most {_MAX_COLUMNS}")
-    s, r = (capi.QuantisedRowsStruct * k)(), (capi.RowsStruct * k)()
-    for i, (store, x) in enumerate(zip(stores, rows)):
-        shape, strides = x.shape, x.strides
-        if x.type not in ROW_TYPE:
-            raise capi.OperationNotSupported(f"rows of {x.type} in a quantised cache")
-        if shape[1:] != (store.heads, store.dim) and (store.heads != 1 or shape[1:] != (store.dim,)) or shape[0] != n:
-            raise shape_error(f"rows {shape} for {n} rows of {store.heads} x {store.dim}")
-        s[i] = store.struct
-        v = r[i]
-        v.data, v.row_stride, v.head_stride, v.type = x.ptr, strides[0], strides[1], ROW_TYPE[x.type]
-    _on(pipeline, *stores, *rows)
+    if len(stores) > _MAX_COLUMNS:
+        raise shape_error(f"{len(stores)} caches in one call: at most {_MAX_COLUMNS}")
+    for store, x in zip(stores, rows):
+        shape = x.shape
+        if shape[0] != n or (shape[1:] != store.shape and (store.heads != 1 or shape[1:] != store.shape[1:])):
+            raise shape_error(f"rows {tuple(shape)} for {n} rows of {store.heads} x {store.dim}")
+        _on(pipeline, store, x)
+    s, r = b"".join([store.packed for store in stores]), b"".join([x.as_rows() for x in rows])
     if isinstance(where, PageMap):
-        _on(pipeline, where.tables, where.offsets, where.first)
-        capi.call(name + "_pages", pipeline._handle, k, s, r, C.byref(where.struct), n)
-        _keep(pipeline, where.tables.data, where.offsets.data, where.first.data if where.first is not None else None)
+        held = [where.tables, where.offsets] if where.first is None else [where.tables, where.offsets, where.first]
+        _on(pipeline, *held)
+        capi.call(name + "_pages", pipeline._handle, len(stores), s, r, where.packed, n)
+        _keep(pipeline, *[x.data for x in held])
     else:
         _on(pipeline, where)
-        capi.call(name, pipeline._handle, k, s, r, where.data.ptr, n)
+        capi.call(name, pipeline._handle, len(stores), s, r, where.data.ptr, n)
         _keep(pipeline, where.data)
     for store, x in zip(stores, rows):
         _keep(pipeline, store.codes, store.scales, x.data)
@@ -121,34 +120,28 @@ def take_rows_op(states, indexes: UInt32ArrayGPU, pipeline: ArrowComputePipeline
         out = [RowsGPU.empty((n,) + tuple(s.shape[1:]), s.type, s.gpu_device) for s in states]
     if len(out) != len(states):
         raise shape_error(f"{len(out)} outputs for {len(states)} states")
-    v = (capi.StateStruct * len(states))()
     n_src = len(states[0])
-    for e, s, o in zip(v, states, out):
-        if len(s) != n_src or o.shape[1:] != s.shape[1:] or len(o) != n or o.item_size != s.item_size:
-            raise shape_error(f"rows {o.shape} from a state {s.shape} by {n} indexes, in a call over {n_src} rows")
-        if lengths is not None and len(s.shape) < 3:
-            raise shape_error("lengths count positions: the axis before the last")
-        _state(e, s, o, lengths is not None)
-    _on(pipeline, indexes, lengths, *states, *out)
-    capi.call("agpu_take_rows", pipeline._handle, len(states), v, n_src, indexes.data.ptr, lengths.data.ptr if lengths is not None else None, n)
-    _keep(pipeline, indexes.data, lengths.data if lengths is not None else None, *[s.data for s in states], *[o.data for o in out])
+    packed = []
+    for s, o in zip(states, out):
+        if s.shape[0] != n_src or o.shape[1:] != s.shape[1:] or o.shape[0] != n or o.item_size != s.item_size:
+            raise shape_error(f"rows {tuple(o.shape)} from a state {tuple(s.shape)} by {n} indexes, in a call over {n_src} rows")
+        row, step, pieces, size, position = s.as_pieces()
+        out_row, out_step, out_pieces, out_size, _ = o.as_pieces()
+        if (pieces, size) != (out_pieces, out_size):
+            raise shape_error(f"the pieces of {tuple(s.shape)}: strides {s.strides} and {o.strides}")
+        if lengths is not None and not position:
+            raise shape_error("lengths count positions, the axis before the last: they lie next to each other")
+        packed.append(_PACK_STATE.pack(s.ptr, o.ptr, row, step, out_row, out_step, pieces, size, position))
+        _on(pipeline, s, o)
+    _on(pipeline, indexes)
+    if lengths is not None:
+        _on(pipeline, lengths)
+        _keep(pipeline, lengths.data)
+    capi.call("agpu_take_rows", pipeline._handle, len(states), b"".join(packed), n_src, indexes.data.ptr, lengths.data.ptr if lengths is not None else None, n)
+    _keep(pipeline, indexes.data)
+    for s, o in zip(states, out):
+        _keep(pipeline, s.data, o.data)
     return out
-
-
-def _state(e, s: RowsGPU, o: RowsGPU, counted: bool) -> None:
-    """Axes after the first: the trailing ones that lie densely in both are one piece, what is left (at most one axis) are the pieces."""
-    item, shape = s.item_size, s.shape
-    inner, axis = shape[-1], len(shape) - 1
-    e.position_bytes = inner * item
-    while axis > 1 and (shape[axis - 1] == 1 or s.strides[axis - 1] == o.strides[axis - 1] == inner) and not (axis == 2 and len(shape) == 4):
-        axis -= 1
-        inner *= shape[axis]
-    if axis > 2 or (counted and axis > len(shape) - 2):
-        raise shape_error(f"the positions and values of a state lie next to each other: got strides {s.strides} and {o.strides}")
-    e.src, e.dst = s.ptr, o.ptr
-    e.piece_bytes, e.n_pieces = inner * item, shape[1] if axis == 2 else 1
-    e.src_row_stride, e.dst_row_stride = s.strides[0] * item, o.strides[0] * item
-    e.src_piece_stride, e.dst_piece_stride = (s.strides[1] * item, o.strides[1] * item) if axis == 2 else (0, 0)
 
 
 def select_beams_op(logits: RowsGPU, beams: int, k: int, pipeline: ArrowComputePipeline, scores: Float32ArrayGPU | None = None,
@@ -181,19 +174,17 @@ def select_beams_op(logits: RowsGPU, beams: int, k: int, pipeline: ArrowComputeP
         out = BeamSelection.empty(batch, k, pipeline.device)
     elif (out.batch, out.k) != (batch, k):
         raise shape_error(f"a selection of {out.batch} x {out.k} for {batch} x {k}")
-    _on(pipeline, logits, scores, allowed, finished, out)
+    given = [x for x in (scores, allowed, finished) if x is not None]
+    _on(pipeline, logits, out, *given)
     if batch == 0:
         return out
-    need = C.c_uint64()
-    capi.call("agpu_select_beams_workspace", batch, beams, vocab, k, C.byref(need))
-    work = out.ensure_workspace(need.value)
-    args = capi.BeamsStruct(logits.ptr, logits.strides[0], ROW_TYPE[logits.type], batch, beams, vocab, k, end_token,
-                            scores.data.ptr if scores is not None else None, allowed.data.ptr if allowed is not None else None, stride,
-                            finished.data.ptr if finished is not None else None, out.scores.data.ptr, out.parents.data.ptr, out.tokens.data.ptr,
+    work = out.ensure_workspace(beams, vocab)
+    args = _PACK_BEAMS.pack(logits.ptr, logits.strides[0], ROW_TYPE[logits.type], batch, beams, vocab, k, end_token,
+                            scores.data.ptr if scores is not None else 0, allowed.data.ptr if allowed is not None else 0, stride,
+                            finished.data.ptr if finished is not None else 0, out.scores.data.ptr, out.parents.data.ptr, out.tokens.data.ptr,
                             work.ptr, work.nbytes)
-    capi.call("agpu_select_beams", pipeline._handle, C.byref(args))
-    _keep(pipeline, logits.data, scores.data if scores is not None else None, allowed.data if allowed is not None else None,
-          finished.data if finished is not None else None, out.scores.data, out.parents.data, out.tokens.data, work)
+    capi.call("agpu_select_beams", pipeline._handle, args)
+    _keep(pipeline, logits.data, out.scores.data, out.parents.data, out.tokens.data, work, *[x.data for x in given])
     return out
 
 

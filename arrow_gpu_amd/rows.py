@@ -3,7 +3,7 @@ values).  RowsGPU is a strided view of a tensor in HBM, QuantisedRowsGPU a cache
 sequences lie in a paged cache, BeamSelection holds what select_beams found.  The operators are in kernels/rows.py."""
 from __future__ import annotations
 
-import ctypes as C
+import struct
 from typing import Optional
 
 import numpy as np
@@ -17,6 +17,12 @@ ROW_TYPE = {"f32": capi.ROW_F32, "f16": capi.ROW_F16, "bf16": capi.ROW_BF16}
 CODE_TYPE = {"i8": capi.CODE_I8, "i4": capi.CODE_I4, "e4m3": capi.CODE_E4M3}
 _NUMPY = {"f32": np.float32, "f16": np.float16, "bf16": np.uint16, "i8": np.int8, "u8": np.uint8, "i16": np.int16, "u16": np.uint16, "i32": np.int32,
           "u32": np.uint32, "i64": np.int64, "f64": np.float64}
+
+
+# The ABI's structs (include/arrow_gpu.h) as bytes: a serving loop makes them anew in every call, and packing costs a fifth of filling ctypes fields
+_PACK_ROWS = struct.Struct("=QQQi4x").pack          # agpu_rows
+_PACK_STORE = struct.Struct("=QQQIIIi").pack        # agpu_quantised_rows
+_PACK_PAGES = struct.Struct("=QQQQIII4x").pack      # agpu_page_map
 
 
 def shape_error(message: str) -> capi.ArrowErrorGPU:
@@ -34,7 +40,7 @@ def _dense(shape):
 class RowsGPU:
     """Rows of values in HBM: shape (n, …) of 2 to 4 axes, strides in elements, the values of the last axis next to each other."""
 
-    __slots__ = ("data", "gpu_device", "shape", "strides", "type", "ptr", "item_size")
+    __slots__ = ("data", "gpu_device", "shape", "strides", "type", "ptr", "item_size", "_rows", "_pieces")
 
     def __init__(self, data: DeviceBuffer, gpu_device: GpuDevice, shape, type_: str, strides=None, ptr: Optional[int] = None):
         if type_ not in ITEM_SIZE:
@@ -44,6 +50,7 @@ class RowsGPU:
         self.strides = _dense(self.shape)[0] if strides is None else tuple(strides)
         self.item_size = ITEM_SIZE[type_]
         self.ptr = data.ptr if ptr is None else ptr
+        self._rows = self._pieces = None
         if not 2 <= len(self.shape) <= 4 or len(self.strides) != len(self.shape):
             raise shape_error(f"rows have 2 to 4 axes: got {self.shape}")
         if min(self.strides) < 0 or (self.strides[-1] != 1 and self.shape[-1] > 1):
@@ -55,6 +62,30 @@ class RowsGPU:
         """The rows over a tensor's memory, without a copy (a slice of a bigger tensor keeps its strides)."""
         t = tensor_type(tensor)
         return cls(borrow_tensor(tensor, gpu_device, tensor.numel() * ITEM_SIZE[t]), gpu_device, tensor.shape, t, tensor.stride())
+
+    # -- what the ABI's calls take
+    def as_rows(self) -> bytes:
+        """agpu_rows of (n, heads, dim)"""
+        if self._rows is None:
+            if self.type not in ROW_TYPE:
+                raise capi.OperationNotSupported(f"rows of {self.type} in a quantised cache")
+            self._rows = _PACK_ROWS(self.ptr, self.strides[0], self.strides[1], ROW_TYPE[self.type])
+        return self._rows
+
+    def as_pieces(self):
+        """(row stride, piece stride, pieces, piece bytes, position bytes) for agpu_state: the trailing axes that lie densely are one piece, the axis
+        that is left, if any, are the pieces; position bytes 0: the positions (the axis before the last) are not inside one."""
+        if self._pieces is None:
+            item, shape, strides = self.item_size, self.shape, self.strides
+            inner, axis = shape[-1], len(shape) - 1
+            while axis > 1 and (shape[axis - 1] == 1 or strides[axis - 1] == inner) and not (axis == 2 and len(shape) == 4):
+                axis -= 1
+                inner *= shape[axis]
+            if axis > 2:
+                raise shape_error(f"the positions and values of a state lie next to each other: got strides {strides}")
+            counted = shape[-1] * item if len(shape) > 2 and axis <= len(shape) - 2 else 0
+            self._pieces = (strides[0] * item, strides[1] * item if axis == 2 else 0, shape[1] if axis == 2 else 1, inner * item, counted)
+        return self._pieces
 
     @classmethod
     def empty(cls, shape, type_: str, gpu_device: GpuDevice) -> "RowsGPU":
@@ -106,7 +137,7 @@ class QuantisedRowsGPU:
     code "i8": whole numbers -127..127, "e4m3": 8-bit floating, "i4": whole numbers 0..15 above the group's lowest value.  An empty cache's rows
     read back as zeros."""
 
-    __slots__ = ("codes", "scales", "gpu_device", "n_slots", "heads", "dim", "group", "code", "struct")
+    __slots__ = ("codes", "scales", "gpu_device", "n_slots", "heads", "dim", "group", "code", "shape", "packed")
 
     def __init__(self, codes: DeviceBuffer, scales: DeviceBuffer, gpu_device: GpuDevice, n_slots: int, heads: int, dim: int, group: int, code: str):
         if code not in CODE_TYPE:
@@ -115,7 +146,8 @@ class QuantisedRowsGPU:
             raise shape_error(f"group {group} of {code} codes in rows of {heads} x {dim}")
         self.codes, self.scales, self.gpu_device = codes, scales, gpu_device
         self.n_slots, self.heads, self.dim, self.group, self.code = n_slots, heads, dim, group, code
-        self.struct = capi.QuantisedRowsStruct(codes.ptr, scales.ptr, n_slots, heads, dim, group, CODE_TYPE[code])
+        self.shape = (heads, dim)  # of a row
+        self.packed = _PACK_STORE(codes.ptr, scales.ptr, n_slots, heads, dim, group, CODE_TYPE[code])
 
     @staticmethod
     def bytes_of(n_slots: int, heads: int, dim: int, group: int, code: str):
@@ -158,7 +190,7 @@ class PageMap:
 
     tables: RowsGPU of u32 / i32, (sequences, pages); offsets: UInt32ArrayGPU of sequences + 1; first: UInt32ArrayGPU of sequences, or none."""
 
-    __slots__ = ("tables", "page_rows", "offsets", "first", "struct")
+    __slots__ = ("tables", "page_rows", "offsets", "first", "packed")
 
     def __init__(self, tables: RowsGPU, page_rows: int, offsets: UInt32ArrayGPU, first: Optional[UInt32ArrayGPU] = None):
         if tables.type not in ("u32", "i32") or len(tables.shape) != 2:
@@ -169,8 +201,8 @@ class PageMap:
         if page_rows < 1:
             raise shape_error(f"pages of {page_rows} rows")
         self.tables, self.page_rows, self.offsets, self.first = tables, page_rows, offsets, first
-        self.struct = capi.PageMapStruct(tables.ptr, tables.strides[0], offsets.data.ptr, first.data.ptr if first is not None else None, n,
-                                         tables.shape[1], page_rows)
+        self.packed = _PACK_PAGES(tables.ptr, tables.strides[0], offsets.data.ptr, first.data.ptr if first is not None else 0, n, tables.shape[1],
+                                  page_rows)
 
 
 class BeamSelection:
@@ -178,14 +210,14 @@ class BeamSelection:
     tokens (UInt32ArrayGPU), best first.  It holds the selection's workspace too: a selection that is passed as `out` again is not in use by two
     calls at one time, and lives as long as a captured graph that writes it."""
 
-    __slots__ = ("scores", "parents", "tokens", "gpu_device", "batch", "k", "workspace")
+    __slots__ = ("scores", "parents", "tokens", "gpu_device", "batch", "k", "workspace", "_workspace_of")
 
     def __init__(self, scores: Float32ArrayGPU, parents: UInt32ArrayGPU, tokens: UInt32ArrayGPU, gpu_device: GpuDevice, batch: int, k: int):
         if not (scores.len == parents.len == tokens.len == batch * k):
             raise shape_error(f"a selection of {batch} x {k} has that many scores, parents and tokens")
         self.scores, self.parents, self.tokens, self.gpu_device = scores, parents, tokens, gpu_device
         self.batch, self.k = batch, k
-        self.workspace = None
+        self.workspace = self._workspace_of = None
 
     @classmethod
     def empty(cls, batch: int, k: int, gpu_device: GpuDevice) -> "BeamSelection":
@@ -200,9 +232,13 @@ class BeamSelection:
         return cls(Float32ArrayGPU.of_tensor(scores, gpu_device), UInt32ArrayGPU.of_tensor(parents, gpu_device),
                    UInt32ArrayGPU.of_tensor(tokens, gpu_device), gpu_device, scores.shape[0], scores.shape[1])
 
-    def ensure_workspace(self, nbytes: int) -> DeviceBuffer:
-        if self.workspace is None or self.workspace.nbytes < nbytes:
-            self.workspace = self.gpu_device.create_empty_buffer(max(nbytes, 16))
+    def ensure_workspace(self, beams: int, vocab: int) -> DeviceBuffer:
+        """The workspace for rows of `vocab` logits, `beams` a request."""
+        if self._workspace_of != (beams, vocab):
+            nbytes = capi.select_beams_workspace(self.batch, beams, vocab, self.k)
+            if self.workspace is None or self.workspace.nbytes < nbytes:
+                self.workspace = self.gpu_device.create_empty_buffer(max(nbytes, 16))
+            self._workspace_of = (beams, vocab)
         return self.workspace
 
     def values(self):

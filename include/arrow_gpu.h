@@ -592,7 +592,8 @@ typedef struct agpu_state {
 /* dst row i = src row idx[i], i < n, of every state (n_states <= 64): the reordering of the states by a selection's parents, whatever the bytes
  * are.  lengths (may be NULL): only the first lengths[i] positions of row i's pieces are copied (all, if they are more than a piece holds), what
  * lies behind them is left as it was.  idx[i] >= n_src: a row of zeros (of that length), reported by the next sync; AGPU_NO_ROW: the row is left as
- * it was.  No dst may overlap a src (AGPU_ERR_ARG): rows are not reordered in place. */
+ * it was.  No dst may overlap a src (AGPU_ERR_ARG): rows are not reordered in place.  A row holds less than 2^31 bytes, a length less than 2^32
+ * positions. */
 agpu_status agpu_take_rows(agpu_pipeline* p, int32_t n_states, const agpu_state* states, uint64_t n_src, const uint32_t* idx,
                            const uint32_t* lengths, uint64_t n);
 

@@ -15,6 +15,34 @@ ROOT = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
 NO_PIPELINE = (capi.ERR_ARG, "null pipeline")
 
 
+# the ABI's structs, field by field (the Python host packs them as bytes)
+class RowsStruct(C.Structure):  # agpu_rows
+    _fields_ = [("data", C.c_void_p), ("row_stride", C.c_uint64), ("head_stride", C.c_uint64), ("type", C.c_int32)]
+
+
+class QuantisedRowsStruct(C.Structure):  # agpu_quantised_rows
+    _fields_ = [("codes", C.c_void_p), ("scales", C.c_void_p), ("n_slots", C.c_uint64), ("heads", C.c_uint32), ("dim", C.c_uint32),
+                ("group", C.c_uint32), ("code", C.c_int32)]
+
+
+class PageMapStruct(C.Structure):  # agpu_page_map
+    _fields_ = [("tables", C.c_void_p), ("table_stride", C.c_uint64), ("offsets", C.c_void_p), ("first", C.c_void_p), ("n_seqs", C.c_uint32),
+                ("max_pages", C.c_uint32), ("page_rows", C.c_uint32)]
+
+
+class StateStruct(C.Structure):  # agpu_state
+    _fields_ = [("src", C.c_void_p), ("dst", C.c_void_p), ("src_row_stride", C.c_uint64), ("src_piece_stride", C.c_uint64),
+                ("dst_row_stride", C.c_uint64), ("dst_piece_stride", C.c_uint64), ("n_pieces", C.c_uint64), ("piece_bytes", C.c_uint64),
+                ("position_bytes", C.c_uint64)]
+
+
+class BeamsStruct(C.Structure):  # agpu_beams
+    _fields_ = [("logits", C.c_void_p), ("row_stride", C.c_uint64), ("type", C.c_int32), ("batch", C.c_uint32), ("beams", C.c_uint32),
+                ("vocab", C.c_uint32), ("k", C.c_uint32), ("end_token", C.c_uint32), ("scores", C.c_void_p), ("allowed", C.c_void_p),
+                ("allowed_stride", C.c_uint64), ("finished", C.c_void_p), ("out_scores", C.c_void_p), ("out_parents", C.c_void_p),
+                ("out_tokens", C.c_void_p), ("workspace", C.c_void_p), ("workspace_bytes", C.c_uint64)]
+
+
 def status(name, *args):
     st = getattr(capi.lib(), name)(*args)
     return st, capi.last_error()
@@ -23,13 +51,13 @@ def status(name, *args):
 def store(**kw):
     a = dict(codes=1 << 20, scales=1 << 21, n_slots=8, heads=2, dim=64, group=32, code=capi.CODE_I8)
     a.update(kw)
-    return capi.QuantisedRowsStruct(**a)
+    return QuantisedRowsStruct(**a)
 
 
 def rows(**kw):
     a = dict(data=1 << 22, row_stride=128, head_stride=64, type=capi.ROW_BF16)
     a.update(kw)
-    return capi.RowsStruct(**a)
+    return RowsStruct(**a)
 
 
 @pytest.mark.parametrize("name", ["agpu_put_quantised", "agpu_take_quantised"])
@@ -70,7 +98,7 @@ def test_page_arguments():
     def pages(**kw):
         a = dict(tables=1 << 24, table_stride=4, offsets=1 << 25, first=None, n_seqs=3, max_pages=4, page_rows=16)
         a.update(kw)
-        return capi.PageMapStruct(**a)
+        return PageMapStruct(**a)
 
     s, r = store(), rows()
     for name in ("agpu_put_quantised_pages", "agpu_take_quantised_pages"):
@@ -88,10 +116,10 @@ def test_take_rows_arguments():
     def state(**kw):
         a = dict(src=1 << 30, dst=1 << 40, src_row_stride=4096, src_piece_stride=1024, dst_row_stride=4096, dst_piece_stride=1024, n_pieces=4, piece_bytes=1024, position_bytes=64)
         a.update(kw)
-        return capi.StateStruct(**a)
+        return StateStruct(**a)
 
     def call(*states, n_src=8, idx=1 << 20, lengths=None, n=8):
-        v = (capi.StateStruct * max(len(states), 1))(*states)
+        v = (StateStruct * max(len(states), 1))(*states)
         return status("agpu_take_rows", None, len(states), v, n_src, idx, lengths, n)
 
     assert NO_PIPELINE[1] in call(state())[1] and NO_PIPELINE[1] in call()[1] and NO_PIPELINE[1] in call(state(), n=0)[1]
@@ -106,6 +134,7 @@ def test_take_rows_arguments():
     assert NO_PIPELINE[1] in call(state(position_bytes=0))[1]
     assert "address space" in call(state(src_row_stride=1 << 62))[1] and "address space" in call(state(n_pieces=1 << 40, piece_bytes=1 << 30, dst_piece_stride=1 << 30))[1]
     assert "address space" in call(state(piece_bytes=(1 << 64) - 1, dst_piece_stride=(1 << 64) - 1, dst_row_stride=(1 << 64) - 1))[1]
+    assert "2^31" in call(state(n_pieces=1, piece_bytes=1 << 31, src=1 << 43, dst=1 << 42, src_row_stride=1 << 31, dst_row_stride=1 << 31))[1]
     # in place, by one byte, and one state's dst on another's src
     assert call(state(dst=1 << 30))[0] == capi.ERR_ARG
     assert call(state(dst=(1 << 30) + 8 * 4096 - 1))[0] == capi.ERR_ARG and NO_PIPELINE[1] in call(state(dst=(1 << 30) + 8 * 4096))[1]
@@ -118,7 +147,7 @@ def test_select_beams_arguments():
         a = dict(logits=1 << 20, row_stride=1000, type=capi.ROW_F16, batch=2, beams=4, vocab=1000, k=8, end_token=0, scores=1 << 21, allowed=1 << 22, allowed_stride=128,
                  finished=1 << 23, out_scores=1 << 24, out_parents=1 << 25, out_tokens=1 << 26, workspace=1 << 27, workspace_bytes=1 << 30)
         a.update(kw)
-        return status("agpu_select_beams", None, C.byref(capi.BeamsStruct(**a)))
+        return status("agpu_select_beams", None, C.byref(BeamsStruct(**a)))
 
     assert NO_PIPELINE[1] in beams()[1] and NO_PIPELINE[1] in beams(batch=0, logits=0)[1]
     assert NO_PIPELINE[1] in beams(scores=0, allowed=0, finished=0, allowed_stride=0)[1]
@@ -149,6 +178,27 @@ def _host():
     buf = lambda n: ag.DeviceBuffer(dev, 4096, n, owned=False)  # noqa: E731
     pipe = types.SimpleNamespace(device=dev, _handle=None, keep=lambda *a: None)
     return ag, dev, buf, pipe
+
+
+def test_the_python_host_packs_the_structs_as_the_header_has_them():
+    ag, dev, buf, _ = _host()
+    import arrow_gpu_amd.kernels.rows as K
+
+    r = ag.RowsGPU(buf(1), dev, (3, 2, 8), "bf16", (40, 16, 1), 4100)
+    assert bytes(RowsStruct(4100, 40, 16, capi.ROW_BF16)) == r.as_rows()
+    c = ag.QuantisedRowsGPU(buf(1), ag.DeviceBuffer(dev, 8192, 1, owned=False), dev, 5, 2, 8, 4, "i4")
+    assert bytes(QuantisedRowsStruct(4096, 8192, 5, 2, 8, 4, capi.CODE_I4)) == c.packed
+    idx = ag.UInt32ArrayGPU(buf(16), dev, 4, None)
+    m = ag.PageMap(ag.RowsGPU(buf(1), dev, (3, 2), "u32", (7, 1)), 16, idx)
+    assert bytes(PageMapStruct(4096, 7, 4096, None, 3, 2, 16)) == m.packed
+    assert C.sizeof(StateStruct) == K._PACK_STATE.size and C.sizeof(BeamsStruct) == K._PACK_BEAMS.size
+    v = tuple(range(1, 18))
+    assert bytes(BeamsStruct(*v)) == K._PACK_BEAMS.pack(*v) and bytes(StateStruct(*v[:9])) == K._PACK_STATE.pack(*v[:9])
+    state = ag.RowsGPU(buf(1), dev, (3, 2, 5, 4), "f16", (100, 30, 4, 1))
+    assert state.as_pieces() == (200, 60, 2, 40, 8)                                       # pieces of 5 positions of 8 bytes
+    assert ag.RowsGPU(buf(1), dev, (3, 5, 4), "f16").as_pieces() == (40, 0, 1, 40, 8)     # one piece
+    assert ag.RowsGPU(buf(1), dev, (3, 5, 4), "f16", (50, 8, 1)).as_pieces() == (100, 16, 5, 8, 0)
+    assert ag.RowsGPU(buf(1), dev, (3, 7), "u8").as_pieces() == (7, 0, 1, 7, 0)
 
 
 def test_python_refusals():
