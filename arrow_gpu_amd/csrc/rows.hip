@@ -49,7 +49,7 @@ struct QuantShape {
 // ---------------------------------------------------------------- eight values a lane
 // Both ways stream: 16-byte accesses (32 of f32) on the rows' side, 8 or 4 on the codes'.  A group is `lanes` neighbouring lanes (a power of two, those
 // past the group's end idle), its span found with data-parallel moves inside the wave.  A block takes whole rows, looks their slots up once and
-// keeps them in LDS: a search of the sequence through memory costs microseconds, so it is shared by up to 16 passes of the block.
+// keeps them in LDS: a search of the sequence through memory costs microseconds, so it is shared by up to 8 passes of the block.
 constexpr int MAX_COLS = 8, MAX_ROWS = 256;
 struct QuantCols {
   QuantCol c[MAX_COLS];
@@ -65,7 +65,8 @@ Divide divide_by(uint32_t d) {
   return {d, (uint32_t)(((1ull << (31 + s)) + d - 1) / d), s};
 }
 struct FastShape {
-  uint32_t group, dim, groups_per_row, lanes, log_lanes, rows;  // rows of a block
+  uint32_t group, groups_per_row, lanes, log_lanes, rows;  // rows of a block
+  bool dense;                                                  // a row's heads follow each other
   Divide by_row, by_head;                                      // groups a row, groups a head
 };
 
@@ -97,34 +98,50 @@ __device__ __forceinline__ float over_group(float x, uint32_t lanes, F f) {
   return x;
 }
 
-// the block's rows' slots; false: nothing to do in this block
-__device__ __forceinline__ uint32_t block_slots(const RowAddr& addr, uint64_t row0, uint64_t n, uint32_t rows, uint64_t n_slots, uint64_t* slots, uint32_t* flags) {
-  const uint32_t mine = (uint32_t)(n - row0 < rows ? n - row0 : rows);
-  if (threadIdx.x < mine) {
-    const uint64_t s = row_slot(addr, row0 + threadIdx.x, n_slots);
-    slots[threadIdx.x] = s;
+// a row of the block: the number of its first group in the cache (ROW_NONE, ROW_BAD), and its values
+template <typename T>
+struct BlockRow {
+  uint64_t at;
+  T* x;
+};
+template <typename T>
+__device__ __forceinline__ uint32_t block_rows(const QuantCol& c, const FastShape& q, const RowAddr& addr, uint64_t n, BlockRow<T>* held, uint32_t* flags) {
+  const uint64_t row0 = (uint64_t)blockIdx.x * q.rows;
+  const uint32_t rows = (uint32_t)(n - row0 < q.rows ? n - row0 : q.rows);
+  if (threadIdx.x < rows) {
+    const uint64_t row = row0 + threadIdx.x, s = row_slot(addr, row, c.n_slots);
+    held[threadIdx.x] = {s < ROW_BAD ? s * q.groups_per_row : s, static_cast<T*>(c.x) + row * c.row_stride};
     if (s == ROW_BAD) *reinterpret_cast<volatile uint32_t*>(flags) = AGPU_FLAG_INDEX_RANGE;
   }
   __syncthreads();
-  return mine;
+  return rows;
+}
+// what a lane has at a time: eight values of one group, from value sub * 8 on
+struct Unit {
+  uint32_t row, in_row, sub;
+};
+__device__ __forceinline__ Unit unit_of(uint32_t i, const FastShape& q) {
+  const uint32_t g = i >> q.log_lanes, row = g / q.by_row;
+  return {row, g - row * q.groups_per_row, i & (q.lanes - 1)};
+}
+__device__ __forceinline__ uint64_t value_offset(const Unit& u, const QuantCol& c, const FastShape& q) {
+  if (q.dense) return u.in_row * q.group + u.sub * 8;
+  const uint32_t head = u.in_row / q.by_head;
+  return head * c.head_stride + (u.in_row - head * q.by_head.d) * q.group + u.sub * 8;
 }
 
 template <typename T, int CODE>
 __global__ __launch_bounds__(AGPU_BLOCK) void put_eight_kernel(QuantCols cols, FastShape q, RowAddr addr, uint64_t n, uint32_t* flags) {
-  __shared__ uint64_t slots[MAX_ROWS];
+  __shared__ BlockRow<const T> held[MAX_ROWS];
   const QuantCol& c = cols.c[blockIdx.y];
-  const uint64_t row0 = (uint64_t)blockIdx.x * q.rows;
-  const uint32_t rows = block_slots(addr, row0, n, q.rows, c.n_slots, slots, flags);
-  const uint32_t total = (rows * q.groups_per_row) << q.log_lanes;
+  const uint32_t total = (block_rows<const T>(c, q, addr, n, held, flags) * q.groups_per_row) << q.log_lanes;
   for (uint32_t i = threadIdx.x; i < total; i += AGPU_BLOCK) {
-    const uint32_t g = i >> q.log_lanes, sub = i & (q.lanes - 1), row = g / q.by_row, in_row = g - row * q.groups_per_row, head = in_row / q.by_head;
-    const uint64_t slot = slots[row];
-    const uint32_t off = (in_row - head * q.by_head.d) * q.group + sub * 8;
-    const bool live = sub * 8 < q.group && slot < ROW_BAD;
+    const Unit t = unit_of(i, q);
+    const BlockRow<const T> row = held[t.row];
+    const bool live = t.sub * 8 < q.group && row.at < ROW_BAD;
     float v[8] = {};
     if (live) {
-      const T* x = static_cast<const T*>(c.x) + (row0 + row) * c.row_stride + head * c.head_stride + off;
-      const typename Eight<T>::type w = *reinterpret_cast<const typename Eight<T>::type*>(x);
+      const typename Eight<T>::type w = *reinterpret_cast<const typename Eight<T>::type*>(row.x + value_offset(t, c, q));
 #pragma unroll
       for (int j = 0; j < 8; j++) v[j] = (float)w[j];
     }
@@ -151,7 +168,8 @@ __global__ __launch_bounds__(AGPU_BLOCK) void put_eight_kernel(QuantCols cols, F
     }
     const Factors f = factors<CODE>(span, lo, bad);
     if (!live) continue;
-    const uint64_t at = slot * q.groups_per_row + in_row;
+    const uint64_t at = row.at + t.in_row;
+    const uint32_t sub = t.sub;
     if (CODE == AGPU_CODE_I4) {
       if (sub == 0) reinterpret_cast<float2*>(c.scales)[at] = {f.scale, f.lo};
       uint32_t w = 0;
@@ -176,46 +194,65 @@ __global__ __launch_bounds__(AGPU_BLOCK) void put_eight_kernel(QuantCols cols, F
   }
 }
 
+constexpr int TAKE_UNROLL = 4;
+
 template <typename T, int CODE>
 __global__ __launch_bounds__(AGPU_BLOCK) void take_eight_kernel(QuantCols cols, FastShape q, RowAddr addr, uint64_t n, uint32_t* flags) {
-  __shared__ uint64_t slots[MAX_ROWS];
+  __shared__ BlockRow<T> held[MAX_ROWS];
   const QuantCol& c = cols.c[blockIdx.y];
-  const uint64_t row0 = (uint64_t)blockIdx.x * q.rows;
-  const uint32_t rows = block_slots(addr, row0, n, q.rows, c.n_slots, slots, flags);
-  const uint32_t total = (rows * q.groups_per_row) << q.log_lanes;
-  for (uint32_t i = threadIdx.x; i < total; i += AGPU_BLOCK) {
-    const uint32_t g = i >> q.log_lanes, sub = i & (q.lanes - 1), row = g / q.by_row, in_row = g - row * q.groups_per_row, head = in_row / q.by_head;
-    const uint64_t slot = slots[row];
-    if (sub * 8 >= q.group || slot == ROW_NONE) continue;
-    const uint64_t at = slot * q.groups_per_row + in_row;
-    float v[8] = {};
-    if (slot != ROW_BAD) {
-      if (CODE == AGPU_CODE_I4) {
-        const float2 f = reinterpret_cast<const float2*>(c.scales)[at];
-        const uint32_t w = *reinterpret_cast<const uint32_t*>(c.codes + at * (q.group / 2) + sub * 4);
+  const uint32_t total = (block_rows<T>(c, q, addr, n, held, flags) * q.groups_per_row) << q.log_lanes;
+  for (uint32_t i0 = threadIdx.x; i0 < total; i0 += AGPU_BLOCK * TAKE_UNROLL) {
+    T* to[TAKE_UNROLL];
+    u32x2 w[TAKE_UNROLL];
+    float2 f[TAKE_UNROLL];
 #pragma unroll
-        for (int j = 0; j < 8; j++) v[j] = __builtin_fmaf((float)(w >> 4 * j & 15), f.x, f.y);
+    for (int u = 0; u < TAKE_UNROLL; u++) {
+      const uint32_t i = i0 + u * AGPU_BLOCK;
+      to[u] = nullptr;
+      w[u] = u32x2{0, 0}, f[u] = float2{0.0f, 0.0f};  // out of range: zeros
+      const Unit t = unit_of(i, q);
+      if (i >= total || t.sub * 8 >= q.group) continue;
+      const BlockRow<T> row = held[t.row];
+      if (row.at == ROW_NONE) continue;
+      to[u] = row.x + value_offset(t, c, q);
+      if (row.at == ROW_BAD) continue;
+      const uint64_t at = row.at + t.in_row;
+      const uint32_t sub = t.sub;
+      if (CODE == AGPU_CODE_I4) {
+        f[u] = reinterpret_cast<const float2*>(c.scales)[at];
+        w[u].x = *reinterpret_cast<const uint32_t*>(c.codes + at * (q.group / 2) + sub * 4);
       } else {
-        const float scale = c.scales[at];
-        const u32x2 w = *reinterpret_cast<const u32x2*>(c.codes + at * q.group + sub * 8);
+        f[u].x = c.scales[at];
+        w[u] = *reinterpret_cast<const u32x2*>(c.codes + at * q.group + sub * 8);
+      }
+    }
+#pragma unroll
+    for (int u = 0; u < TAKE_UNROLL; u++) {
+      if (!to[u]) continue;
+      typename Eight<T>::type o;
+      if (CODE == AGPU_CODE_I4) {
+        const uint32_t even = w[u].x & 0x0F0F0F0Fu, odd = w[u].x >> 4 & 0x0F0F0F0Fu;  // a byte each: the conversion takes them from where they are
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+          o[2 * j] = (T)__builtin_fmaf((float)(even >> 8 * j & 255), f[u].x, f[u].y);
+          o[2 * j + 1] = (T)__builtin_fmaf((float)(odd >> 8 * j & 255), f[u].x, f[u].y);
+        }
+      } else {
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-          const uint32_t b = w[h];
-          if (CODE == AGPU_CODE_I8) {
-#pragma unroll
-            for (int j = 0; j < 4; j++) v[4 * h + j] = (float)(int8_t)(b >> 8 * j) * scale;
-          } else {
+          const uint32_t b = w[u][h];
+          if (CODE == AGPU_CODE_E4M3) {
             const auto low = __builtin_amdgcn_cvt_pk_f32_fp8(b, false), high = __builtin_amdgcn_cvt_pk_f32_fp8(b, true);
-            v[4 * h] = low[0] * scale, v[4 * h + 1] = low[1] * scale, v[4 * h + 2] = high[0] * scale, v[4 * h + 3] = high[1] * scale;
+            o[4 * h] = (T)(low[0] * f[u].x), o[4 * h + 1] = (T)(low[1] * f[u].x), o[4 * h + 2] = (T)(high[0] * f[u].x), o[4 * h + 3] = (T)(high[1] * f[u].x);
+          } else {
+#pragma unroll
+            for (int j = 0; j < 4; j++) o[4 * h + j] = (T)((float)(int8_t)(b >> 8 * j) * f[u].x);
           }
         }
       }
+      // past the caches: nobody reads the rows in this call
+      __builtin_nontemporal_store(o, reinterpret_cast<typename Eight<T>::type*>(to[u]));
     }
-    typename Eight<T>::type o;
-#pragma unroll
-    for (int j = 0; j < 8; j++) o[j] = (T)v[j];
-    T* x = static_cast<T*>(c.x) + (row0 + row) * c.row_stride + head * c.head_stride + (in_row - head * q.by_head.d) * q.group + sub * 8;
-    *reinterpret_cast<typename Eight<T>::type*>(x) = o;
   }
 }
 
@@ -315,14 +352,14 @@ bool by_eights(const QuantCol& c, const QuantShape& q, int type, int code) {
          aligned_to(c.scales, code == AGPU_CODE_I4 ? 8 : 4);
 }
 
-// Rows of a block: 16 passes of its lanes, fewer where that would leave less than 2048 blocks (8 a CU)
+// Rows of a block: 8 passes of its lanes, fewer where that would leave less than 2048 blocks (8 a CU)
 FastShape fast_shape(const QuantShape& q, uint64_t n, uint32_t n_cols) {
   FastShape f = {};
-  f.group = q.group, f.dim = q.dim, f.groups_per_row = q.groups_per_row;
+  f.group = q.group, f.groups_per_row = q.groups_per_row;
   while (8u << f.log_lanes < q.group) f.log_lanes++;
   f.lanes = 1u << f.log_lanes;
   const uint64_t row_lanes = (uint64_t)q.groups_per_row << f.log_lanes;
-  uint64_t rows = 16 * AGPU_BLOCK / row_lanes;
+  uint64_t rows = 8 * AGPU_BLOCK / row_lanes;
   if (rows * 2048 > n * n_cols) rows = n * n_cols / 2048;
   if (rows * row_lanes < AGPU_BLOCK) rows = AGPU_BLOCK / row_lanes;
   f.rows = (uint32_t)(rows < 1 ? 1 : rows > MAX_ROWS ? MAX_ROWS : rows);
@@ -333,7 +370,9 @@ FastShape fast_shape(const QuantShape& q, uint64_t n, uint32_t n_cols) {
 template <typename T, int CODE>
 void launch_code(agpu_pipeline* p, bool put, bool eights, const QuantCols& cols, uint32_t n_cols, const QuantShape& q, const RowAddr& addr, uint64_t n) {
   if (eights) {
-    const FastShape f = fast_shape(q, n, n_cols);
+    FastShape f = fast_shape(q, n, n_cols);
+    f.dense = true;
+    for (uint32_t k = 0; k < n_cols; k++) f.dense = f.dense && (q.heads == 1 || cols.c[k].head_stride == q.dim);
     const dim3 grid((uint32_t)((n + f.rows - 1) / f.rows), n_cols);
     if (put) hipLaunchKernelGGL((put_eight_kernel<T, CODE>), grid, dim3(AGPU_BLOCK), 0, p->stream, cols, f, addr, n, p->flags);
     else hipLaunchKernelGGL((take_eight_kernel<T, CODE>), grid, dim3(AGPU_BLOCK), 0, p->stream, cols, f, addr, n, p->flags);
@@ -412,9 +451,9 @@ agpu_status quantised_pages(agpu_pipeline* p, bool put, int32_t n_cols, const ag
 }
 
 // ---------------------------------------------------------------- take_rows
-// A copy with one indirection: lanes run over the states' accesses of V bytes in the order of the destination, four of a lane in flight, all states in
+// A copy with one indirection: lanes run over the states' accesses of V bytes in the order of the destination, two of a lane in flight, all states in
 // one launch (blockIdx.y).
-constexpr int MAX_STATES = 8, ROWS_UNROLL = 4;
+constexpr int MAX_STATES = 8, ROWS_UNROLL = 2;
 struct State {
   const char* src;
   char* dst;
@@ -448,7 +487,7 @@ __global__ __launch_bounds__(AGPU_BLOCK) void take_rows_kernel(States states, ui
   }
 #pragma unroll
   for (int u = 0; u < ROWS_UNROLL; u++)
-    if (to[u]) *reinterpret_cast<V*>(to[u]) = w[u];
+    if (to[u]) __builtin_nontemporal_store(w[u], reinterpret_cast<V*>(to[u]));
 }
 
 // bytes from the first to behind the last of n rows; 0: none.  false: past 2^63
