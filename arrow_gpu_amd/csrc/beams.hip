@@ -2,7 +2,7 @@
 //
 // One pass over the logits.  A row is cut into segments of one WAVE each; the wave streams its segment, adding up exp(x) and keeping the tokens that
 // can be among its k best, and leaves (sum, k best) in the workspace.  A block a request joins the sums and selects among the segments' bests.
-// No wave waits for another before the join, and none needs the maximum first: exp is taken relative to the first tile's, and f32 holds it as long as
+// No wave needs the maximum first: exp is taken relative to the first tile's, and f32 holds it as long as
 // a segment's maximum is within 60 of that; a segment of another kind is read again.
 //
 // Precision.  The result is whole numbers, and rows that compete differ by their log-sums only: a log-sum 1e-7 off swaps tokens of two beams.  The tokens that
@@ -98,6 +98,7 @@ template <> struct Raw<bf16_t> {
 
 constexpr int TILE = 1024;  // logits a wave takes at a time: 16 a lane
 constexpr int HITS = 2048; // and may look at twice
+constexpr uint32_t EXACT = 16;  // at least so many of the largest terms are taken in f64
 constexpr int RANKED = 8;
 constexpr int LIST = 512;   // tokens it can keep; logits in no order: about 3 k + 10
 
@@ -160,7 +161,11 @@ struct Segment {
 };
 
 // the larger, without the instruction that would quiet a NaN first (of a NaN either: rows that hold one are found by themselves)
-__device__ __forceinline__ float max_of(float a, float b) { return __builtin_amdgcn_fmed3f(a, b, __builtin_inff()); }
+__device__ __forceinline__ float max_of(float a, float b) {
+  float r;
+  asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+  return r;
+}
 __device__ __forceinline__ float max_of(float a, float b, float c) {
   float r;
   asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
@@ -172,11 +177,11 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
   typedef Segment<T, MASK> S;
   constexpr int VE = S::VE, U = S::U, EPT = U * VE;
   __shared__ uint64_t lists[AGPU_BLOCK / 64][LIST + RANKED];
-  const uint32_t id = __builtin_amdgcn_readfirstlane(blockIdx.x * (AGPU_BLOCK / 64) + (threadIdx.x >> 6)), lane = threadIdx.x & 63;
-  if (id >= n_segs) return;
-  const uint32_t row = id / a.segs, seg = id - row * a.segs;
-  if (is_finished(a, row)) return;
-  uint64_t* list = lists[threadIdx.x >> 6];
+  __shared__ float tops[AGPU_BLOCK / 64][2][64];
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), id = blockIdx.x * (AGPU_BLOCK / 64) + wave, lane = threadIdx.x & 63;
+  const uint32_t row = (id < n_segs ? id : n_segs - 1) / a.segs, seg = id - row * a.segs;
+  const bool idle = id >= n_segs || is_finished(a, row);  // (it keeps the others company at the barriers)
+  uint64_t* list = lists[wave];
 
   S s;
   s.x = static_cast<const T*>(a.logits) + row * a.row_stride;
@@ -184,7 +189,7 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
   s.vocab = a.vocab;
   s.lead = (uint32_t)(reinterpret_cast<uintptr_t>(s.x) & 15) / sizeof(T);
   s.lane = lane;
-  const uint32_t t0 = seg * tiles, row_tiles = (uint32_t)(((uint64_t)a.vocab + s.lead + TILE - 1) / TILE), t1 = t0 + tiles < row_tiles ? t0 + tiles : row_tiles;
+  const uint32_t t0 = seg * tiles, row_tiles = (uint32_t)(((uint64_t)a.vocab + s.lead + TILE - 1) / TILE), t1 = idle ? t0 : t0 + tiles < row_tiles ? t0 + tiles : row_tiles;
 
   float top[2] = {LOWEST, LOWEST};  // the largest of the lane's first and second eight logits of every tile
   float floor_v = LOWEST, ref_v = 0.0f, k = MAGIC, least = 0.0f;
@@ -194,25 +199,46 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
   u32x4 w[U], next[U];
   uint32_t m[U], next_m[U];
   if (t0 < t1) s.load(t0, w, m);
-  for (uint32_t t = t0; t < t1; t++) {
-    if (t + 1 < t1) s.load(t + 1, next, next_m);
-    float v[EPT];
-    s.values(t, w, m, v);
-    float tm[2] = {v[0], v[EPT / 2]};
+  for (uint32_t step = 0; step < tiles; step++) {
+    const uint32_t t = t0 + step;
+    float v[EPT], tm[2];
+    if (t < t1) {
+      if (t + 1 < t1) s.load(t + 1, next, next_m);
+      s.values(t, w, m, v);
+      tm[0] = v[0], tm[1] = v[EPT / 2];
 #pragma unroll
-    for (int i = 1; i < EPT / 2 - 1; i += 2) tm[0] = max_of(tm[0], v[i], v[i + 1]), tm[1] = max_of(tm[1], v[EPT / 2 + i], v[EPT / 2 + i + 1]);
-    tm[0] = max_of(tm[0], v[EPT / 2 - 1]), tm[1] = max_of(tm[1], v[EPT - 1]);
+      for (int i = 1; i < EPT / 2 - 1; i += 2) tm[0] = max_of(tm[0], v[i], v[i + 1]), tm[1] = max_of(tm[1], v[EPT / 2 + i], v[EPT / 2 + i + 1]);
+      tm[0] = max_of(tm[0], v[EPT / 2 - 1]), tm[1] = max_of(tm[1], v[EPT - 1]);
 #pragma unroll
-    for (int i = 0; i < EPT; i += 2) nan |= __ballot(__builtin_isunordered(v[i], v[i + 1]));
-    top[0] = fmaxf(top[0], tm[0]), top[1] = fmaxf(top[1], tm[1]);
-    if (t == t0) {  // the reference: the tile's maximum, as far as it is an ordinary number
-      float f = fmaxf(tm[0], tm[1]);
-      for (int d = 32; d; d >>= 1) f = fmaxf(f, __shfl_xor(f, d));
-      ref_v = __builtin_fabsf(f) <= REF_MOST ? f : 0.0f;
-      k = MAGIC - __builtin_rintf(ref_v * LOG2E);
-      least = ref_v - 80.0f;
+      for (int i = 0; i < EPT; i += 2) nan |= __ballot(__builtin_isunordered(v[i], v[i + 1]));
+      top[0] = fmaxf(top[0], tm[0]), top[1] = fmaxf(top[1], tm[1]);
+      if (t == t0) {  // the reference: the tile's maximum, as far as it is an ordinary number
+        float f = fmaxf(tm[0], tm[1]);
+        for (int d = 32; d; d >>= 1) f = fmaxf(f, __shfl_xor(f, d));
+        ref_v = __builtin_fabsf(f) <= REF_MOST ? f : 0.0f;
+        k = MAGIC - __builtin_rintf(ref_v * LOG2E);
+        least = ref_v - 80.0f;
+      }
     }
-    if (((t - t0) & (t - t0 + 1)) == 0) floor_v = wave_kth(top, a.k, Raw<T>::low);  // tiles 0, 1, 3, 7
+    // The floor, after tiles 0 and 2: a value that k logits of the row reach, among the maxima of all the waves that share it
+    if (step == 0 || step == 2) {
+      tops[wave][0][lane] = top[0], tops[wave][1][lane] = top[1];
+      __syncthreads();
+      float two[2] = {top[0], top[1]};  // the lane's largest two of them
+      if (two[1] > two[0]) two[0] = top[1], two[1] = top[0];
+      for (uint32_t o = 1; o < AGPU_BLOCK / 64; o++) {
+        const uint32_t other = (wave + o) % (AGPU_BLOCK / 64);
+        if ((blockIdx.x * (AGPU_BLOCK / 64) + other) / a.segs != row) continue;
+#pragma unroll
+        for (int h = 0; h < 2; h++) {
+          const float x = tops[other][h][lane], low = fminf(x, two[0]);
+          two[0] = fmaxf(x, two[0]), two[1] = fmaxf(two[1], low);
+        }
+      }
+      floor_v = wave_kth(two, a.k > EXACT ? a.k : EXACT, Raw<T>::low);
+      if (step == 0) __syncthreads();  // (before they are written again)
+    }
+    if (t >= t1) continue;
     const float above = fmaxf(floor_v, -0x1.fffffep127f);
     hits[3] = hits[3] << EPT | hits[2] >> (32 - EPT), hits[2] = hits[2] << EPT | hits[1] >> (32 - EPT), hits[1] = hits[1] << EPT | hits[0] >> (32 - EPT);
     hits[0] <<= EPT;
@@ -239,6 +265,7 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
   double ref = (double)(MAGIC - k) * LN2;
   // the logits that reached a floor, one of each lane at a time (read again: the lane's registers cannot be indexed): their terms, and into the list
   // what reaches the last floor
+  if (idle) return;
   uint32_t count = 0, all = 0;
 #pragma unroll
   for (int i = 0; i < 4; i++) all += (uint32_t)__builtin_popcount(hits[i]);
