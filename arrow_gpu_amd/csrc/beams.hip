@@ -242,16 +242,19 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
     const float above = fmaxf(floor_v, -0x1.fffffep127f);
     hits[3] = hits[3] << EPT | hits[2] >> (32 - EPT), hits[2] = hits[2] << EPT | hits[1] >> (32 - EPT), hits[1] = hits[1] << EPT | hits[0] >> (32 - EPT);
     hits[0] <<= EPT;
-    if (__any(max_of(tm[0], tm[1]) >= above)) {
-      uint32_t h = 0;
 #pragma unroll
-      for (int i = EPT - 1; i >= 0; i--) {
-        const bool hit = v[i] >= above;
-        h = h + h + hit;
-        v[i] = hit ? LOWEST : v[i];  // its term is taken in f64
+    for (int half = 0; half < 2; half++)
+      if (__any(tm[half] >= above)) {
+        uint32_t h = 0;
+#pragma unroll
+        for (int i = EPT / 2 - 1; i >= 0; i--) {
+          float& x = v[half * (EPT / 2) + i];
+          const bool hit = x >= above;
+          h = h + h + hit;
+          x = hit ? LOWEST : x;  // its term is taken in f64
+        }
+        hits[0] |= h << half * (EPT / 2);
       }
-      hits[0] |= h;
-    }
     float part = 0.0f;
 #pragma unroll
     for (int i = 0; i < EPT; i++) part += exp_term(max_of(v[i], least), k);  // (e^-80 for what is less, −infinity too: nothing beside the largest)

@@ -71,12 +71,11 @@ def tensor_type(tensor) -> str:
 
 
 def borrow_tensor(tensor, device: "GpuDevice", nbytes: int) -> BorrowedBuffer:
-    """The memory of a tensor on `device` (anything with data_ptr() and device: torch is not needed here).  The rules of torch's own streams hold:
+    """The memory of a tensor on `device` (anything with data_ptr() and get_device(): torch is not needed here).  The rules of torch's own streams hold:
     the tensor's memory may be given back to its allocator when no work on ANOTHER stream than the tensor's still uses it.  A program that uses
     torch on the GPU imports it before this library's first call: then both run on the one GPU runtime that torch has loaded."""
-    where = tensor.device
-    if where.type != "cuda" or (where.index or 0) != device.ordinal:
-        raise capi.ArrowErrorGPU("ArgumentError", f"a tensor on {where} for a buffer on GPU {device.ordinal}", capi.ERR_ARG)
+    if tensor.get_device() != device.ordinal:  # (of host memory: −1)
+        raise capi.ArrowErrorGPU("ArgumentError", f"a tensor on {tensor.device} for a buffer on GPU {device.ordinal}", capi.ERR_ARG)
     return BorrowedBuffer(device, tensor.data_ptr(), nbytes, tensor)
 
 

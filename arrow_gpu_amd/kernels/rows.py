@@ -40,12 +40,15 @@ def _u32(array, what: str):
 def _quantised(name: str, stores, rows, where, n: int, pipeline) -> None:
     if len(stores) > _MAX_COLUMNS:
         raise shape_error(f"{len(stores)} caches in one call: at most {_MAX_COLUMNS}")
+    packed_stores, packed_rows = [], []
     for store, x in zip(stores, rows):
         shape = x.shape
         if shape[0] != n or (shape[1:] != store.shape and (store.heads != 1 or shape[1:] != store.shape[1:])):
-            raise shape_error(f"rows {tuple(shape)} for {n} rows of {store.heads} x {store.dim}")
+            raise shape_error(f"rows {shape} for {n} rows of {store.heads} x {store.dim}")
         _on(pipeline, store, x)
-    s, r = b"".join([store.packed for store in stores]), b"".join([x.as_rows() for x in rows])
+        packed_stores.append(store.packed)
+        packed_rows.append(x._rows or x.as_rows())
+    s, r = b"".join(packed_stores), b"".join(packed_rows)
     if isinstance(where, PageMap):
         held = [where.tables, where.offsets] if where.first is None else [where.tables, where.offsets, where.first]
         _on(pipeline, *held)

@@ -45,16 +45,16 @@ class RowsGPU:
     def __init__(self, data: DeviceBuffer, gpu_device: GpuDevice, shape, type_: str, strides=None, ptr: Optional[int] = None):
         if type_ not in ITEM_SIZE:
             raise capi.OperationNotSupported(f"rows of {type_}")
-        self.data, self.gpu_device, self.type = data, gpu_device, type_
-        self.shape = tuple(shape)
-        self.strides = _dense(self.shape)[0] if strides is None else tuple(strides)
+        shape = tuple(shape)
+        strides = _dense(shape)[0] if strides is None else tuple(strides)
+        if not 2 <= len(shape) <= 4 or len(strides) != len(shape):
+            raise shape_error(f"rows have 2 to 4 axes: got {shape}")
+        if min(strides) < 0 or (strides[-1] != 1 and shape[-1] > 1):
+            raise shape_error(f"the values of a row's last axis lie next to each other: got strides {strides}")
+        self.data, self.gpu_device, self.type, self.shape, self.strides = data, gpu_device, type_, shape, strides
         self.item_size = ITEM_SIZE[type_]
         self.ptr = data.ptr if ptr is None else ptr
         self._rows = self._pieces = None
-        if not 2 <= len(self.shape) <= 4 or len(self.strides) != len(self.shape):
-            raise shape_error(f"rows have 2 to 4 axes: got {self.shape}")
-        if min(self.strides) < 0 or (self.strides[-1] != 1 and self.shape[-1] > 1):
-            raise shape_error(f"the values of a row's last axis lie next to each other: got strides {self.strides}")
 
     # -- construction
     @classmethod
