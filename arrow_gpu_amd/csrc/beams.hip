@@ -5,10 +5,11 @@
 // No wave needs the maximum first: exp is taken relative to the first tile's, and f32 holds it as long as
 // a segment's maximum is within 60 of that; a segment of another kind is read again.
 //
-// Precision.  The result is whole numbers, and rows that compete differ by their log-sums only: a log-sum 1e-7 off swaps tokens of two beams.  The tokens that
-// are kept (about the 3 k largest of a segment) hold the largest terms: theirs are taken in f64, from the list, and left out of the f32 ones.  Those are
-// many and small, each 1e-7 off at random: 1e-8 and less in the sum.  A term is 2^f · 2^n with x log2 e = n + f, |f| <= 1/2: one fma rounds x log2 e to n, the
-// next gives f exactly, a third adds x times what log2 e has beyond f32; n goes into the exponent.
+// Precision.  The result is whole numbers, and rows that compete differ by their log-sums only: a log-sum 1e-7 off swaps tokens of two beams.  Scores are
+// compared in f64.  Of the sum, the terms of the tokens that reach the floor — at least the 16 largest of a row, the bulk where it is sharp — are taken in
+// f64 and left out of the f32 ones.  An f32 term is 2^f · 2^n with x log2 e = n + f, |f| <= 1/2: one fma rounds x log2 e to n, the next gives f, a third adds x
+// times what log2 e has beyond f32 (2^-26 of error each), the instruction for 2^f is within 2^-23; 16 are added with 4 roundings, the rest in f64.
+// That bounds a log-sum's error by 2^-23 + ln 2 · 2^-25 + 4 · 2^-24 < 3.8e-7; many different terms are off at random, and it is about 1e-9.
 #include "common.hpp"
 
 namespace {
@@ -61,8 +62,8 @@ __device__ __forceinline__ uint32_t order_of(float x) {
 }
 __device__ __forceinline__ float value_of(uint32_t o) { return __builtin_bit_cast(float, o ^ ((o >> 31) ? 0x80000000u : 0xFFFFFFFFu)); }
 
-// a value that at least k of the wave's 64 (x[0], … x[N − 1] of every lane) reach, −infinity if there are none: the k-th largest, its bits below
-// `low` cleared — found bit by bit, by how many reach the prefix
+// the k-th largest of the wave's x[0] … x[N − 1] (−infinity if there are fewer above it), found bit by bit, by how many reach the prefix.  Orders have
+// `low` bits that are the same in all values of one sign: clear, of negative values set
 template <int N>
 __device__ __forceinline__ float wave_kth(const float (&x)[N], uint32_t k, int low) {
   uint32_t o[N], t = 0;
@@ -75,8 +76,11 @@ __device__ __forceinline__ float wave_kth(const float (&x)[N], uint32_t k, int l
     for (int i = 0; i < N; i++) n += (uint32_t)__popcll(__ballot(o[i] >= up));
     t = n >= k ? up : t;
   }
+  if (!(t >> 31)) t |= (1u << low) - 1;
   return t > order_of(LOWEST) ? value_of(t) : LOWEST;
 }
+
+__device__ __forceinline__ uint32_t lanes_below(uint64_t who) { return __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0)); }
 
 // ---------------------------------------------------------------- a segment
 template <typename T> struct Raw;  // low: bits of an order that are equal in all values of the type of one sign
@@ -192,7 +196,7 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
   const uint32_t t0 = seg * tiles, row_tiles = (uint32_t)(((uint64_t)a.vocab + s.lead + TILE - 1) / TILE), t1 = idle ? t0 : t0 + tiles < row_tiles ? t0 + tiles : row_tiles;
 
   float top[2] = {LOWEST, LOWEST};  // the largest of the lane's first and second eight logits of every tile
-  float floor_v = LOWEST, ref_v = 0.0f, k = MAGIC, least = 0.0f;
+  float floor_v = LOWEST, above = -0x1.fffffep127f, ref_v = 0.0f, k = MAGIC, least = 0.0f;
   double sum = 0.0;
   uint64_t nan = 0;
   uint32_t hits[4] = {0, 0, 0, 0};  // a bit a logit of the lane's: it reached the floor; the last tile's first in the lowest
@@ -201,16 +205,21 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
   if (t0 < t1) s.load(t0, w, m);
   for (uint32_t step = 0; step < tiles; step++) {
     const uint32_t t = t0 + step;
-    float v[EPT], tm[2];
+    float v[EPT], vm[U];
     if (t < t1) {
       if (t + 1 < t1) s.load(t + 1, next, next_m);
       s.values(t, w, m, v);
-      tm[0] = v[0], tm[1] = v[EPT / 2];
 #pragma unroll
-      for (int i = 1; i < EPT / 2 - 1; i += 2) tm[0] = max_of(tm[0], v[i], v[i + 1]), tm[1] = max_of(tm[1], v[EPT / 2 + i], v[EPT / 2 + i + 1]);
-      tm[0] = max_of(tm[0], v[EPT / 2 - 1]), tm[1] = max_of(tm[1], v[EPT - 1]);
+      for (int u = 0; u < U; u++) {
+        vm[u] = max_of(v[u * VE], v[u * VE + 1]);
+#pragma unroll
+        for (int i = 2; i < VE; i += 2) vm[u] = max_of(vm[u], v[u * VE + i], v[u * VE + i + 1]);
+      }
 #pragma unroll
       for (int i = 0; i < EPT; i += 2) nan |= __ballot(__builtin_isunordered(v[i], v[i + 1]));
+      float tm[2] = {vm[0], vm[U / 2]};
+#pragma unroll
+      for (int u = 1; u < U / 2; u++) tm[0] = fmaxf(tm[0], vm[u]), tm[1] = fmaxf(tm[1], vm[U / 2 + u]);
       top[0] = fmaxf(top[0], tm[0]), top[1] = fmaxf(top[1], tm[1]);
       if (t == t0) {  // the reference: the tile's maximum, as far as it is an ordinary number
         float f = fmaxf(tm[0], tm[1]);
@@ -235,30 +244,44 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
           two[0] = fmaxf(x, two[0]), two[1] = fmaxf(two[1], low);
         }
       }
-      floor_v = wave_kth(two, a.k > EXACT ? a.k : EXACT, Raw<T>::low);
+      const float f = wave_kth(two, a.k > EXACT ? a.k : EXACT, Raw<T>::low);
+      if (f > floor_v) floor_v = f, above = f;
       if (step == 0) __syncthreads();  // (before they are written again)
     }
     if (t >= t1) continue;
-    const float above = fmaxf(floor_v, -0x1.fffffep127f);
     hits[3] = hits[3] << EPT | hits[2] >> (32 - EPT), hits[2] = hits[2] << EPT | hits[1] >> (32 - EPT), hits[1] = hits[1] << EPT | hits[0] >> (32 - EPT);
     hits[0] <<= EPT;
 #pragma unroll
-    for (int half = 0; half < 2; half++)
-      if (__any(tm[half] >= above)) {
+    for (int u = 0; u < U; u++)
+      if (__any(vm[u] >= above)) {
         uint32_t h = 0;
 #pragma unroll
-        for (int i = EPT / 2 - 1; i >= 0; i--) {
-          float& x = v[half * (EPT / 2) + i];
+        for (int i = VE - 1; i >= 0; i--) {
+          float& x = v[u * VE + i];
           const bool hit = x >= above;
           h = h + h + hit;
           x = hit ? LOWEST : x;  // its term is taken in f64
         }
-        hits[0] |= h << half * (EPT / 2);
-      }
-    float part = 0.0f;
+        // Very many at the floor (all that a mask has set to the lowest number): of equal ones the lower tokens come first.  Tokens rise with the lanes
+        // of a vector and from vector to vector, so behind k lanes with a hit only what is above the floor counts, here and from now on
+        const uint64_t who = __ballot(h != 0);
+        if ((uint32_t)__popcll(who) >= a.k) {
+          const bool late = lanes_below(who) >= a.k;
 #pragma unroll
-    for (int i = 0; i < EPT; i++) part += exp_term(max_of(v[i], least), k);  // (e^-80 for what is less, −infinity too: nothing beside the largest)
-    sum += (double)part;
+          for (int i = 0; i < VE; i++)
+            if (late && (h >> i & 1) && Raw<T>::at(w[u], i) == floor_v) h &= ~(1u << i), v[u * VE + i] = floor_v;
+          above = value_of(order_of(floor_v) + 1);
+        }
+        hits[0] |= h << u * VE;
+      }
+    // the terms (at least e^-80, −infinity too: nothing beside the largest), added in pairs of pairs: four roundings on every way
+#pragma unroll
+    for (int i = 0; i < EPT; i++) v[i] = exp_term(max_of(v[i], least), k);
+#pragma unroll
+    for (int d = 1; d < EPT; d *= 2)
+#pragma unroll
+      for (int i = 0; i < EPT; i += 2 * d) v[i] += v[i + d];
+    sum += (double)v[0];
 #pragma unroll
     for (int u = 0; u < U; u++) w[u] = next[u], m[u] = next_m[u];
   }
@@ -273,8 +296,21 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
 #pragma unroll
   for (int i = 0; i < 4; i++) all += (uint32_t)__builtin_popcount(hits[i]);
   for (int d = 32; d; d >>= 1) all += __shfl_xor(all, d);
-  const bool again = most > LOWEST && most < __builtin_inff() && (all > HITS || __builtin_fabsf(most - ref_v) > APART);
-  if (!again) {
+  const bool many = all > HITS, again = most > LOWEST && most < __builtin_inff() && (many || __builtin_fabsf(most - ref_v) > APART);
+  if (again) {  // in f64, below the maximum that is now known
+    ref = most;
+    sum = 0.0;
+    for (uint32_t t = t0; t < t1; t++) {
+      float v[EPT];
+      s.load(t, w, m);
+      s.values(t, w, m, v);
+#pragma unroll 1
+      for (int i = 0; i < EPT; i++) sum += exp((double)v[i] - ref);
+    }
+  }
+  if (many) {
+    count = LIST + 1;
+  } else {
     while (__any((hits[0] | hits[1] | hits[2] | hits[3]) != 0)) {
       const int word = hits[0] ? 0 : hits[1] ? 1 : hits[2] ? 2 : 3;
       const uint32_t h = word == 0 ? hits[0] : word == 1 ? hits[1] : word == 2 ? hits[2] : hits[3];
@@ -284,26 +320,15 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
         const uint32_t bit = word * 32 + __builtin_ctz(h), t = t1 - 1 - bit / EPT, i = bit % EPT;
         token = t * TILE + i / VE * (64 * VE) + lane * VE + i % VE - s.lead;
         y = (float)s.x[token];
-        sum += exp((double)y - ref);
+        if (!again) sum += exp((double)y - ref);
       }
       const uint32_t rest = h & (h - 1);
       hits[0] = word == 0 ? rest : hits[0], hits[1] = word == 1 ? rest : hits[1], hits[2] = word == 2 ? rest : hits[2], hits[3] = word == 3 ? rest : hits[3];
       const bool keep = y >= floor_v && y > LOWEST;
       const uint64_t who = __ballot(keep);
-      const uint32_t at = count + __builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0));
+      const uint32_t at = count + lanes_below(who);
       if (keep && at < LIST) list[at] = (uint64_t)order_of(y) << 32 | ~token;
       count += (uint32_t)__popcll(who);
-    }
-  } else {  // in f64, below the maximum that is now known
-    ref = most;
-    sum = 0.0;
-    count = LIST + 1;
-    for (uint32_t t = t0; t < t1; t++) {
-      float v[EPT];
-      s.load(t, w, m);
-      s.values(t, w, m, v);
-#pragma unroll 1
-      for (int i = 0; i < EPT; i++) sum += exp((double)v[i] - ref);
     }
   }
   for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
@@ -327,7 +352,7 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
       }
       if (rank < a.k) out[rank] = {value_of((uint32_t)(e >> 32)), ~(uint32_t)e};
     }
-  } else {  // very many equal logits, or ascending ones: the best, then the best behind it, k times
+  } else {  // ascending logits: the best, then the best behind it, k times
     uint64_t before = ~0ull;
     for (uint32_t r = 0; r < a.k; r++) {
       uint64_t best = 0;
@@ -509,7 +534,7 @@ __global__ __launch_bounds__(MERGE_BLOCK) void beam_merge_kernel(BeamArgs a, con
       bool taken = false;
       for (uint32_t j = 0; j < found; j++) taken |= chosen[j] == f;
       const uint64_t free = __ballot(!taken);
-      const uint32_t mine = at + __builtin_amdgcn_mbcnt_hi((uint32_t)(free >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)free, 0));
+      const uint32_t mine = at + lanes_below(free);
       if (!taken && mine < a.k) {
         const uint64_t o = (uint64_t)blockIdx.x * a.k + mine;
         a.out_scores[o] = LOWEST;
@@ -577,7 +602,6 @@ agpu_status agpu_select_beams(agpu_pipeline* p, const agpu_beams* args) {
   AGPU_REQUIRE(b.logits && b.out_scores && b.out_parents && b.out_tokens && b.workspace, AGPU_ERR_ARG, "null pointer");
   AGPU_REQUIRE(b.workspace_bytes >= need, AGPU_ERR_SHAPE, "workspace too small");
   AGPU_REQUIRE(b.end_token < b.vocab, AGPU_ERR_SHAPE, "end_token < vocab");
-  AGPU_REQUIRE(b.batch * b.beams == 1 || b.row_stride >= b.vocab, AGPU_ERR_SHAPE, "row_stride >= vocab");
   AGPU_REQUIRE(b.allowed_stride % 8 == 0 && (b.allowed_stride == 0 || b.allowed_stride >= agpu_bitmap_bytes(b.vocab)), AGPU_ERR_SHAPE,
                "allowed_stride: 0, or a multiple of 8 that holds vocab bits");
   AGPU_REQUIRE(aligned_to(b.logits, b.type == AGPU_ROW_F32 ? 4 : 2) && aligned_to(b.scores, 4) && aligned_to(b.allowed, 8) && aligned_to(b.finished, 8) &&

@@ -9,6 +9,29 @@
 #define AGPU_ROW_FN inline
 #endif
 
+// x / d by a product, x < 2^31: m = ⌈2^(31 + s) / d⌉ is off by less than d <= 2^s in 2^(31 + s), so the quotient by less than 1 / d
+struct Divide {
+  uint32_t d, m, s;
+};
+AGPU_ROW_FN uint32_t operator/(uint32_t x, Divide d) { return (uint32_t)((uint64_t)(x << 1) * d.m >> 32) >> d.s; }
+inline Divide divide_by(uint32_t d) {
+  uint32_t s = 0;
+  while ((1ull << s) < d) s++;
+  return {d, (uint32_t)(((1ull << (31 + s)) + d - 1) / d), s};
+}
+
+// whether n rows of m parts of `part` values each, rows and parts so far apart, lie beside each other: one of the two encloses the other
+inline bool disjoint(uint64_t n, uint64_t row_stride, uint64_t m, uint64_t part_stride, uint64_t part) {
+  const auto within = [&](uint64_t count, uint64_t step, uint64_t size, uint64_t outer) {  // (count − 1) · step + size <= outer, step >= size
+    uint64_t span;
+    if (count <= 1) return size <= outer;
+    return step >= size && !__builtin_mul_overflow(count - 1, step, &span) && !__builtin_add_overflow(span, size, &span) && span <= outer;
+  };
+  if (n <= 1) return within(m, part_stride, part, ~0ull);
+  if (m <= 1) return row_stride >= part;
+  return within(m, part_stride, part, row_stride) || within(n, row_stride, part, part_stride);
+}
+
 constexpr uint64_t ROW_NONE = ~0ull;     // the row is neither stored nor written
 constexpr uint64_t ROW_BAD = ~0ull - 1;  // out of range
 

@@ -54,16 +54,6 @@ constexpr int MAX_COLS = 8, MAX_ROWS = 256;
 struct QuantCols {
   QuantCol c[MAX_COLS];
 };
-// x / d by a product, x < 2^31
-struct Divide {
-  uint32_t d, m, s;
-};
-__device__ __forceinline__ uint32_t operator/(uint32_t x, Divide d) { return __umulhi(x << 1, d.m) >> d.s; }
-Divide divide_by(uint32_t d) {
-  uint32_t s = 0;
-  while ((1ull << s) < d) s++;
-  return {d, (uint32_t)(((1ull << (31 + s)) + d - 1) / d), s};
-}
 struct FastShape {
   uint32_t group, groups_per_row, lanes, log_lanes, rows;  // rows of a block
   bool dense;                                                  // a row's heads follow each other
@@ -73,7 +63,7 @@ struct FastShape {
 typedef uint32_t u32x8 __attribute__((ext_vector_type(8)));
 template <typename T> struct Eight;  // eight values as they lie in memory
 template <> struct Eight<float> {
-  typedef float type __attribute__((ext_vector_type(8)));
+  typedef float type __attribute__((ext_vector_type(8), aligned(16)));
 };
 template <> struct Eight<f16_t> {
   typedef f16_t type __attribute__((ext_vector_type(8)));
@@ -338,8 +328,7 @@ agpu_status check_columns(int32_t n_cols, const agpu_quantised_rows* stores, con
     AGPU_REQUIRE(r.data && s.codes && s.scales, AGPU_ERR_ARG, "null pointer");
     AGPU_REQUIRE(aligned_to(r.data, r.type == AGPU_ROW_F32 ? 4 : 2) && aligned_to(s.scales, 4), AGPU_ERR_SHAPE, "alignment");
     if (writes_rows) {
-      const uint64_t hs = s.heads > 1 ? r.head_stride : s.dim, rs = n > 1 ? r.row_stride : (uint64_t)-1;
-      AGPU_REQUIRE(hs >= s.dim && rs >= s.dim, AGPU_ERR_SHAPE, "rows that are written may not overlap");
+      AGPU_REQUIRE(disjoint(n, r.row_stride, s.heads, r.head_stride, s.dim), AGPU_ERR_SHAPE, "rows that are written may not overlap");
     }
   }
   return AGPU_OK;
@@ -427,7 +416,7 @@ agpu_status quantised_slots(agpu_pipeline* p, bool put, int32_t n_cols, const ag
   RowAddr a = {};
   if (n_cols == 0 || n == 0) return quantised(p, put, 0, stores, rows, a, 0, name);
   AGPU_REQUIRE(stores && rows && slots, AGPU_ERR_ARG, "null pointer");
-  AGPU_REQUIRE(n <= (1ull << 32), AGPU_ERR_SHAPE, "n <= 2^32");
+  AGPU_REQUIRE(n < (1ull << 31), AGPU_ERR_SHAPE, "n < 2^31");
   AGPU_REQUIRE(aligned_to(slots, 4), AGPU_ERR_SHAPE, "alignment");
   const agpu_status st = check_columns(n_cols, stores, rows, n, !put);
   if (st != AGPU_OK) return st;
@@ -440,7 +429,7 @@ agpu_status quantised_pages(agpu_pipeline* p, bool put, int32_t n_cols, const ag
   AGPU_REQUIRE(n_cols >= 0 && n_cols <= 64, AGPU_ERR_ARG, "0 <= n_cols <= 64");
   if (n_cols == 0 || n == 0) return quantised(p, put, 0, stores, rows, RowAddr{}, 0, name);
   AGPU_REQUIRE(stores && rows && m && m->offsets, AGPU_ERR_ARG, "null pointer");
-  AGPU_REQUIRE(n <= (1ull << 32), AGPU_ERR_SHAPE, "n <= 2^32");
+  AGPU_REQUIRE(n < (1ull << 31), AGPU_ERR_SHAPE, "n < 2^31");
   AGPU_REQUIRE(m->n_seqs > 0 && m->n_seqs < (1u << 31) && m->page_rows > 0, AGPU_ERR_SHAPE, "1 <= n_seqs < 2^31, page_rows >= 1");
   AGPU_REQUIRE(m->max_pages == 0 || m->tables, AGPU_ERR_ARG, "null pointer");
   AGPU_REQUIRE(aligned_to(m->tables, 4) && aligned_to(m->offsets, 4) && aligned_to(m->first, 4), AGPU_ERR_SHAPE, "alignment");
@@ -510,8 +499,7 @@ agpu_status check_states(int32_t n_states, const agpu_state* states, uint64_t n_
     AGPU_REQUIRE(!__builtin_mul_overflow(s.n_pieces, s.piece_bytes, &row_bytes) && extent(n_src, s.src_row_stride, s.n_pieces, s.src_piece_stride, s.piece_bytes, &from) &&
                      extent(n, s.dst_row_stride, s.n_pieces, s.dst_piece_stride, s.piece_bytes, &to),
                  AGPU_ERR_SHAPE, "a state past the address space");
-    AGPU_REQUIRE((s.n_pieces == 1 || s.dst_piece_stride >= s.piece_bytes) && (n == 1 || s.dst_row_stride >= s.piece_bytes), AGPU_ERR_SHAPE,
-                 "rows that are written may not overlap");
+    AGPU_REQUIRE(disjoint(n, s.dst_row_stride, s.n_pieces, s.dst_piece_stride, s.piece_bytes), AGPU_ERR_SHAPE, "rows that are written may not overlap");
     AGPU_REQUIRE(row_bytes < (1ull << 31), AGPU_ERR_SHAPE, "a row holds less than 2^31 bytes");
     AGPU_REQUIRE(!lengths || s.position_bytes > 0, AGPU_ERR_SHAPE, "lengths need position_bytes");
     for (int32_t j = 0; j < n_states; j++) {

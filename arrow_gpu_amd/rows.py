@@ -210,7 +210,7 @@ class BeamSelection:
     tokens (UInt32ArrayGPU), best first.  It holds the selection's workspace too: a selection that is passed as `out` again is not in use by two
     calls at one time, and lives as long as a captured graph that writes it."""
 
-    __slots__ = ("scores", "parents", "tokens", "gpu_device", "batch", "k", "workspace", "_workspace_of")
+    __slots__ = ("scores", "parents", "tokens", "gpu_device", "batch", "k", "workspace", "_workspace_of", "_outgrown")
 
     def __init__(self, scores: Float32ArrayGPU, parents: UInt32ArrayGPU, tokens: UInt32ArrayGPU, gpu_device: GpuDevice, batch: int, k: int):
         if not (scores.len == parents.len == tokens.len == batch * k):
@@ -218,6 +218,7 @@ class BeamSelection:
         self.scores, self.parents, self.tokens, self.gpu_device = scores, parents, tokens, gpu_device
         self.batch, self.k = batch, k
         self.workspace = self._workspace_of = None
+        self._outgrown = []
 
     @classmethod
     def empty(cls, batch: int, k: int, gpu_device: GpuDevice) -> "BeamSelection":
@@ -237,6 +238,8 @@ class BeamSelection:
         if self._workspace_of != (beams, vocab):
             nbytes = capi.select_beams_workspace(self.batch, beams, vocab, self.k)
             if self.workspace is None or self.workspace.nbytes < nbytes:
+                if self.workspace is not None:
+                    self._outgrown.append(self.workspace)  # a captured graph may hold it
                 self.workspace = self.gpu_device.create_empty_buffer(max(nbytes, 16))
             self._workspace_of = (beams, vocab)
         return self.workspace

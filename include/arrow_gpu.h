@@ -565,15 +565,17 @@ typedef struct agpu_page_map {
   uint32_t n_seqs, max_pages, page_rows;
 } agpu_page_map;
 
-/* stores[c] row slots[i] = rows[c] row i, quantised, for i < n and c < n_cols <= 64: the columns of one table (keys, values, of one layer or
+/* stores[c] row slots[i] = rows[c] row i, quantised, for i < n < 2^31 and c < n_cols <= 64: the columns of one table (keys, values, of one layer or
  * of all) by one slot column.  A slot >= n_slots is dropped and reported by the next agpu_pipeline_sync (AGPU_ERR_SHAPE), as for put.  The slots of
- * one call are distinct (AGPU_NO_ROW aside): of a slot named twice the codes and scales may come from either row. */
+ * one call are distinct (AGPU_NO_ROW aside): of a slot named twice the codes and scales may come from either row.  The rows may be
+ * the same one many times (stride 0); neither they nor the slots lie in a cache that is written. */
 agpu_status agpu_put_quantised(agpu_pipeline* p, int32_t n_cols, const agpu_quantised_rows* stores, const agpu_rows* rows,
                                const uint32_t* slots, uint64_t n);
 agpu_status agpu_put_quantised_pages(agpu_pipeline* p, int32_t n_cols, const agpu_quantised_rows* stores, const agpu_rows* rows,
                                      const agpu_page_map* pages, uint64_t n);
 /* rows[c] row i = the values of stores[c] row slots[i], rounded once to the rows' type from f32.  A slot >= n_slots gives a row of zeros and is
- * reported; a row whose slot is AGPU_NO_ROW is left as it was. */
+ * reported; a row whose slot is AGPU_NO_ROW is left as it was.  Rows (or heads) that are written lie beside each other: all heads of a row before
+ * the next row's, or all rows of a head before the next head's. */
 agpu_status agpu_take_quantised(agpu_pipeline* p, int32_t n_cols, const agpu_quantised_rows* stores, const agpu_rows* rows,
                                 const uint32_t* slots, uint64_t n);
 agpu_status agpu_take_quantised_pages(agpu_pipeline* p, int32_t n_cols, const agpu_quantised_rows* stores, const agpu_rows* rows,
@@ -597,9 +599,9 @@ typedef struct agpu_state {
 agpu_status agpu_take_rows(agpu_pipeline* p, int32_t n_states, const agpu_state* states, uint64_t n_src, const uint32_t* idx,
                            const uint32_t* lengths, uint64_t n);
 
-/* Beam search's selection.  logits: [batch * beams, vocab] of an agpu_row_type, row_stride elements apart.  For row r of request b
- *   score(r, v) = scores[r] + logits[r, v] - log sum_u exp(logits[r, u]),   u over the row's allowed tokens, in 64 bits,
- * and the k largest of the request's beams * vocab scores go to out_scores / out_parents / out_tokens [batch, k], largest first; parents are
+/* Beam search's selection.  logits: [batch * beams, vocab] of an agpu_row_type, row_stride elements apart (0: one row for all).  For row r of request b
+ *   score(r, v) = scores[r] + logits[r, v] - log sum_u exp(logits[r, u]),   u over the row's allowed tokens,
+ * compared in 64 bits (the log-sum's error is below 4e-7, of a row of many different logits about 1e-9), and the k largest of the request's beams * vocab scores go to out_scores / out_parents / out_tokens [batch, k], largest first; parents are
  * rows r (indices for agpu_take_rows).  Equal scores: the lower row, then the higher logit, then the lower token.  scores NULL: 0.
  * allowed: per row a bitmap of vocab bits, allowed_stride bytes apart (a multiple of 8, 0: one bitmap for all rows), NULL: every token.  What the
  * logits of other tokens hold does not matter.  finished: a bitmap of batch * beams rows; a finished row has one candidate, (end_token,

@@ -426,14 +426,20 @@ def test_take_rows_past_32_bits(dev, p):
 
 
 # ---------------------------------------------------------------------------------------------------------- select_beams
+# The largest relative error of a sum of positive terms is the largest of a term's and its additions' together: a term 2^f, f rounded twice below 1/2
+# (2 · 2^-26, times ln 2), by an instruction within one unit of f32 (2^-23); groups of 16 terms added pair by pair, 4 roundings of 2^-24 each; the groups
+# in f64.  The logarithm's error is that.
+LOG_SUM = 2.0**-23 + np.log(2) * 2.0**-25 + 4 * 2.0**-24 + 1e-12
+
+
 def assert_selection(sel, want, tol=None):
-    """parents and tokens are whole numbers; a score is rounded to f32 once (its log-sum is far below that)"""
+    """parents and tokens are whole numbers; a score is rounded to f32 once, and its log-sum is off by less than LOG_SUM"""
     s, r, t = sel.values()
     ws, wr, wt = want
     assert np.array_equal(r, wr) and np.array_equal(t, wt), (np.argwhere((r != wr) | (t != wt))[:4], s[(r != wr) | (t != wt)][:4], ws[(r != wr) | (t != wt)][:4])
     assert np.array_equal(np.isfinite(s), np.isfinite(ws)) and np.array_equal(s[~np.isfinite(ws)], ws[~np.isfinite(ws)])
     fine = np.isfinite(ws)
-    assert (np.abs(s[fine] - ws[fine]) <= np.abs(ws[fine]) * R.HALF_STEP["f32"] * (1 + 2.0**-10) + 1e-9).all()
+    assert (np.abs(s[fine] - ws[fine]) <= np.abs(ws[fine]) * R.HALF_STEP["f32"] * (1 + 2.0**-10) + LOG_SUM).all()
 
 
 def logits(rng, rows, vocab, kind):
@@ -508,6 +514,45 @@ def test_select_ties_and_rows_without_a_distribution(dev, p):
         want = R.select(x.astype(np.float64), beams, k)
         assert want[2][0].tolist() == list(range(k)) and set(want[1][2][:5]) == {11} and want[2][2][5:].tolist() == list(range(7))
         assert_selection(sel, want)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+@pytest.mark.parametrize("k", [1, 5, 16, 64])
+@pytest.mark.parametrize("low", [0.0, -1e4, -3e38, -2.5])
+def test_select_very_many_equal_logits(dev, p, kind, k, low):
+    """rows in which all but a few logits hold one value (a mask's lowest number), the few anywhere; and rows of a few values many times"""
+    import arrow_gpu_amd as ag
+
+    rng = np.random.default_rng(k)
+    low = max(low, -6e4) if kind == "f16" else low
+    beams, vocab = 2, 40009
+    x = np.full((10, vocab), low, np.float32)
+    for r in range(6):
+        at = rng.integers(0, vocab, r * 4)
+        x[r, at] = np.maximum(low, 0) + 3 * rng.random(len(at))
+    x[4, ::2] = low + 0.5
+    x[6] = rng.integers(0, 3, vocab) - 1.0
+    x[7, vocab - 20:] = rng.random(20) * 5 + np.maximum(low, 0)
+    x[8] = np.where(rng.random(vocab) < 0.999, low, low + 1)
+    x[9] = np.minimum(np.arange(vocab) // 64, 500)       # rising
+    x = R.rounded(x, kind)
+    sel = ag.select_beams_op(up(x, kind, dev), beams, k, p)
+    p.sync()
+    assert_selection(sel, R.select(x.astype(np.float64), beams, k))
+
+
+def test_select_rows_of_one_row(dev, p):
+    """one row of logits for all beams (stride 0), as at a request's first step"""
+    import arrow_gpu_amd as ag
+
+    rng = np.random.default_rng(8)
+    x = logits(rng, 1, 5001, "bf16")
+    flat = up(x, "bf16", dev)
+    view = ag.RowsGPU(flat.data, dev, (6, 5001), "bf16", (0, 1))
+    cum = -3 * rng.random(6).astype(np.float32)
+    sel = ag.select_beams_op(view, 3, 9, p, scores=ag.Float32ArrayGPU.from_slice(cum, dev))
+    p.sync()
+    assert_selection(sel, R.select(np.repeat(x, 6, 0).astype(np.float64), 3, 9, cum))
 
 
 def test_select_scores_at_the_ends(dev, p):

@@ -85,11 +85,14 @@ def test_quantised_calls():
         assert "null pointer" in status(name, None, 1, C.byref(s), C.byref(r), None, 4)[1]
         assert "null pointer" in status(name, None, 1, None, C.byref(r), 1 << 23, 4)[1]
         assert "alignment" in status(name, None, 1, C.byref(s), C.byref(r), (1 << 23) + 1, 4)[1]
-        assert status(name, None, 1, C.byref(s), C.byref(r), 1 << 23, (1 << 32) + 1)[0] == capi.ERR_SHAPE
+        assert status(name, None, 1, C.byref(s), C.byref(r), 1 << 23, 1 << 31)[0] == capi.ERR_SHAPE
         assert NO_PIPELINE[1] in status(name, None, 0, None, None, None, 4)[1]  # nothing to do, but still a pipeline's call
         assert NO_PIPELINE[1] in status(name, None, 1, None, None, None, 0)[1]
     # rows that are written may not lie on each other; read ones may (a broadcast row)
-    for kw in (dict(head_stride=63), dict(row_stride=63), dict(head_stride=0)):
+    assert NO_PIPELINE[1] in status("agpu_take_quantised", None, 1, C.byref(s), C.byref(rows(row_stride=64, head_stride=256)), 1 << 23, 4)[1]  # heads, then rows
+    assert NO_PIPELINE[1] in status("agpu_take_quantised", None, 1, C.byref(s), C.byref(rows(row_stride=0, head_stride=64)), 1 << 23, 1)[1]     # one row
+    for kw in (dict(head_stride=63), dict(row_stride=63), dict(head_stride=0), dict(row_stride=64, head_stride=64), dict(row_stride=127), dict(row_stride=64, head_stride=255),
+               dict(row_stride=(1 << 64) - 1, head_stride=1)):
         assert "overlap" in status("agpu_take_quantised", None, 1, C.byref(s), C.byref(rows(**kw)), 1 << 23, 4)[1]
         assert NO_PIPELINE[1] in status("agpu_put_quantised", None, 1, C.byref(s), C.byref(rows(**kw)), 1 << 23, 4)[1]
 
@@ -129,6 +132,7 @@ def test_take_rows_arguments():
     assert call(state(src=None))[0] == capi.ERR_ARG and call(state(dst=None))[0] == capi.ERR_ARG
     assert NO_PIPELINE[1] in call(state(src=None), n_src=0)[1]  # no rows to take from: every index is out of range
     assert call(state(), idx=(1 << 20) + 2)[0] == capi.ERR_SHAPE and call(state(), lengths=(1 << 20) + 2)[0] == capi.ERR_SHAPE
+    assert "overlap" in call(state(dst_row_stride=1024))[1] and NO_PIPELINE[1] in call(state(dst_row_stride=1024, dst_piece_stride=8192))[1]
     assert "overlap" in call(state(dst_piece_stride=1023))[1] and "overlap" in call(state(dst_row_stride=100))[1]
     assert "position_bytes" in call(state(position_bytes=0), lengths=1 << 21)[1]
     assert NO_PIPELINE[1] in call(state(position_bytes=0))[1]
@@ -150,12 +154,13 @@ def test_select_beams_arguments():
         return status("agpu_select_beams", None, C.byref(BeamsStruct(**a)))
 
     assert NO_PIPELINE[1] in beams()[1] and NO_PIPELINE[1] in beams(batch=0, logits=0)[1]
+    assert NO_PIPELINE[1] in beams(row_stride=0)[1]
     assert NO_PIPELINE[1] in beams(scores=0, allowed=0, finished=0, allowed_stride=0)[1]
     assert status("agpu_select_beams", None, None)[0] == capi.ERR_ARG
     for kw in (dict(type=3), dict(logits=0), dict(out_scores=0), dict(out_parents=0), dict(out_tokens=0), dict(workspace=0)):
         assert beams(**kw)[0] == capi.ERR_ARG, kw
     for kw in (dict(k=0), dict(k=65), dict(beams=0), dict(beams=1025), dict(vocab=0), dict(vocab=1 << 31), dict(k=9, beams=1, vocab=8), dict(batch=1 << 22),
-               dict(workspace_bytes=8), dict(end_token=1000), dict(row_stride=999), dict(allowed_stride=120), dict(allowed_stride=132), dict(logits=(1 << 20) + 1),
+               dict(workspace_bytes=8), dict(end_token=1000), dict(allowed_stride=120), dict(allowed_stride=132), dict(logits=(1 << 20) + 1),
                dict(scores=(1 << 21) + 1), dict(allowed=(1 << 22) + 4), dict(finished=(1 << 23) + 4), dict(out_scores=(1 << 24) + 2), dict(out_tokens=(1 << 26) + 2),
                dict(workspace=(1 << 27) + 8)):
         assert beams(**kw)[0] == capi.ERR_SHAPE, kw
@@ -251,10 +256,27 @@ extern "C" void slots(const uint32_t* slot_column, const uint32_t* tables, uint6
 """
 
 
+DIVIDE = r"""
+extern "C" uint32_t divide(uint32_t d) {  // the first x from 0, or around the multiples of d and 2^31, whose quotient is wrong; 0xFFFFFFFF: none
+  const Divide by = divide_by(d);
+  const auto wrong = [&](uint64_t x) { return x < (1ull << 31) && (uint32_t)x / by != (uint32_t)x / d; };
+  for (uint32_t x = 0; x < 5000; x++)
+    if (wrong(x)) return x;
+  for (uint64_t k = 1; k < 4000; k++)
+    for (int64_t o = -2; o <= 2; o++) {
+      const uint64_t near = (uint64_t)((int64_t)(k * d) + o), far = (((1ull << 31) - 1) / d - k + 1) * d + o;
+      if (wrong(near)) return (uint32_t)near;
+      if (k <= ((1ull << 31) - 1) / d && wrong(far)) return (uint32_t)far;
+    }
+  return 0xFFFFFFFFu;
+}
+"""
+
+
 @pytest.fixture(scope="module")
 def slots_lib(tmp_path_factory):
     d = tmp_path_factory.mktemp("rows")
-    (d / "s.cpp").write_text(SRC % ROOT)
+    (d / "s.cpp").write_text(SRC % ROOT + DIVIDE)
     subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-shared", "-fPIC", "-o", str(d / "s.so"), str(d / "s.cpp")], check=True, timeout=120)
     return C.CDLL(str(d / "s.so"))
 
@@ -265,6 +287,13 @@ def _slots(lib, n, n_slots, column=None, tables=None, offsets=None, first=None, 
     lib.slots(ptr(column), ptr(tables), C.c_uint64(tables.shape[1] if tables is not None else 0), ptr(offsets), ptr(first), C.c_uint32(len(offsets) - 1 if offsets is not None else 0),
               C.c_uint32(tables.shape[1] if tables is not None else 0), C.c_uint32(page_rows), C.c_uint64(n), C.c_uint64(n_slots), ptr(got))
     return got
+
+
+def test_quotients_by_products(slots_lib):
+    slots_lib.divide.restype = C.c_uint32
+    rng = np.random.default_rng(0)
+    for d in [*range(1, 300), *(1 << np.arange(31)).tolist(), *((1 << np.arange(2, 31)) - 1).tolist(), *((1 << np.arange(30)) + 1).tolist(), *rng.integers(1, 1 << 31, 200).tolist(), (1 << 31) - 1]:
+        assert slots_lib.divide(C.c_uint32(int(d))) == 0xFFFFFFFF, d
 
 
 def test_slots_of_a_column(slots_lib):
