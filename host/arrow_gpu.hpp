@@ -1018,6 +1018,178 @@ std::vector<PrimitiveArrayGpu<T>> take_columns(const std::vector<PrimitiveArrayG
   p.sync();
   return out;
 }
+// ------------------------------------------------------------------ rows (include/arrow_gpu.h "rows"; no counterpart in the reference)
+// Rows of values in HBM: (rows, heads, dim), strides in elements, the values of the last axis next to each other.  `type` AGPU_ROW_*.
+struct RowsGPU {
+  BufferPtr data;
+  DevicePtr gpu_device;
+  uint64_t rows = 0, heads = 1, dim = 0, row_stride = 0, head_stride = 0, offset = 0;  // offset: of the first value, in elements
+  agpu_row_type type = AGPU_ROW_F32;
+  static size_t item_size(agpu_row_type t) { return t == AGPU_ROW_F32 ? 4 : 2; }
+  static RowsGPU over(BufferPtr b, const DevicePtr& dev, uint64_t rows, uint64_t heads, uint64_t dim, agpu_row_type type) {
+    return {std::move(b), dev, rows, heads, dim, heads * dim, dim, 0, type};
+  }
+  static RowsGPU empty(uint64_t rows, uint64_t heads, uint64_t dim, agpu_row_type type, const DevicePtr& dev) {
+    const uint64_t bytes = rows * heads * dim * item_size(type);
+    return over(dev->create_empty_buffer(bytes ? bytes : 1), dev, rows, heads, dim, type);
+  }
+  static RowsGPU from_slice(const std::vector<float>& values, uint64_t heads, uint64_t dim, const DevicePtr& dev) {
+    return over(dev->create_gpu_buffer_with_data(values.data(), values.size()), dev, values.size() / (heads * dim), heads, dim, AGPU_ROW_F32);
+  }
+  agpu_rows abi() const {
+    const bool any = rows && heads && dim;
+    if (any && (offset + (rows - 1) * row_stride + (heads - 1) * head_stride + dim) * item_size(type) > data->bytes)
+      throw ArrowErrorGPU(ArrowErrorGPU::Runtime, "rows: behind the end of the buffer");
+    return {static_cast<char*>(data->ptr) + offset * item_size(type), row_stride, head_stride, type};
+  }
+};
+
+// A cache of n_slots rows in 8 or 4 bits, one factor for each group of values.  `code` AGPU_CODE_*; an empty cache's rows read back as zeros.
+struct QuantisedRowsGPU {
+  BufferPtr codes, scales;
+  DevicePtr gpu_device;
+  uint64_t n_slots = 0;
+  uint32_t heads = 1, dim = 0, group = 0;
+  agpu_code_type code = AGPU_CODE_I8;
+  static QuantisedRowsGPU empty(uint64_t n_slots, uint32_t heads, uint32_t dim, uint32_t group, agpu_code_type code, const DevicePtr& dev) {
+    if (heads == 0 || dim == 0 || group == 0 || dim % group != 0) throw ArrowErrorGPU(ArrowErrorGPU::Runtime, "quantised rows: group divides dim");
+    const uint64_t values = n_slots * heads * dim, half = code == AGPU_CODE_I4;
+    const auto zeroed = [&](uint64_t bytes) {
+      auto b = dev->create_empty_buffer(bytes ? bytes : 1);
+      std::lock_guard<std::mutex> lock(dev->io_mu);
+      check(agpu_memset(dev->io, b->ptr, 0, b->bytes), "agpu_memset");
+      check(agpu_pipeline_finish(dev->io), "agpu_pipeline_finish");
+      return b;
+    };
+    return {zeroed(half ? values / 2 : values), zeroed(values / group * (half ? 8 : 4)), dev, n_slots, heads, dim, group, code};
+  }
+  agpu_quantised_rows abi() const { return {codes->ptr, static_cast<float*>(scales->ptr), n_slots, heads, dim, group, code}; }
+};
+
+// Where the rows of ragged sequences lie in a paged cache (agpu_page_map): tables (sequences x max_pages, flat), offsets of sequences + 1
+struct PageMap {
+  UInt32ArrayGPU tables, offsets;
+  uint32_t max_pages, page_rows;
+  std::optional<UInt32ArrayGPU> first = std::nullopt;
+  agpu_page_map abi() const {
+    const uint64_t n = offsets.len ? offsets.len - 1 : 0;
+    if (tables.len != n * max_pages || (first && first->len != n)) throw ArrowErrorGPU(ArrowErrorGPU::Runtime, "page map: tables and first of every sequence");
+    return {static_cast<const uint32_t*>(tables.data->ptr), max_pages, static_cast<const uint32_t*>(offsets.data->ptr),
+            first ? static_cast<const uint32_t*>(first->data->ptr) : nullptr, (uint32_t)n, max_pages, page_rows};
+  }
+};
+
+namespace detail {
+struct QuantisedCall {
+  std::vector<agpu_quantised_rows> stores;
+  std::vector<agpu_rows> rows;
+  QuantisedCall(const std::vector<QuantisedRowsGPU>& s, const std::vector<RowsGPU>& r, uint64_t n) {
+    if (s.size() != r.size()) throw ArrowErrorGPU(ArrowErrorGPU::Runtime, "quantised rows: rows of every cache");
+    for (size_t i = 0; i < s.size(); i++) {
+      if (r[i].rows != n || r[i].heads != s[i].heads || r[i].dim != s[i].dim) throw ArrowErrorGPU(ArrowErrorGPU::Runtime, "quantised rows: rows of the cache's shape, one for each slot");
+      stores.push_back(s[i].abi());
+      rows.push_back(r[i].abi());
+    }
+  }
+};
+inline void keep_quantised(ArrowComputePipeline& p, const std::vector<QuantisedRowsGPU>& s, const std::vector<RowsGPU>& r) {
+  for (size_t i = 0; i < s.size(); i++) p.keep.insert(p.keep.end(), {s[i].codes, s[i].scales, r[i].data});
+}
+inline void keep_pages(ArrowComputePipeline& p, const PageMap& m) {
+  p.keep.insert(p.keep.end(), {m.tables.data, m.offsets.data});
+  if (m.first) p.keep.push_back(m.first->data);
+}
+}  // namespace detail
+
+// stores[c] row slots[i] = rows[c] row i, quantised; a slot out of range is reported by the next sync()
+inline void put_quantised_op(const std::vector<QuantisedRowsGPU>& stores, const std::vector<RowsGPU>& rows, const UInt32ArrayGPU& slots, ArrowComputePipeline& p) {
+  const detail::QuantisedCall c(stores, rows, slots.len);
+  check(agpu_put_quantised(p.h(), (int32_t)stores.size(), c.stores.data(), c.rows.data(), static_cast<const uint32_t*>(slots.data->ptr), slots.len), "agpu_put_quantised");
+  p.keep.push_back(slots.data);
+  detail::keep_quantised(p, stores, rows);
+}
+inline void put_quantised_op(const std::vector<QuantisedRowsGPU>& stores, const std::vector<RowsGPU>& rows, const PageMap& pages, ArrowComputePipeline& p) {
+  const uint64_t n = rows.empty() ? 0 : rows[0].rows;
+  const detail::QuantisedCall c(stores, rows, n);
+  const agpu_page_map m = pages.abi();
+  check(agpu_put_quantised_pages(p.h(), (int32_t)stores.size(), c.stores.data(), c.rows.data(), &m, n), "agpu_put_quantised_pages");
+  detail::keep_pages(p, pages);
+  detail::keep_quantised(p, stores, rows);
+}
+// out[c] row i = the values of stores[c] row slots[i]
+inline void take_quantised_op(const std::vector<QuantisedRowsGPU>& stores, const UInt32ArrayGPU& slots, const std::vector<RowsGPU>& out, ArrowComputePipeline& p) {
+  const detail::QuantisedCall c(stores, out, slots.len);
+  check(agpu_take_quantised(p.h(), (int32_t)stores.size(), c.stores.data(), c.rows.data(), static_cast<const uint32_t*>(slots.data->ptr), slots.len), "agpu_take_quantised");
+  p.keep.push_back(slots.data);
+  detail::keep_quantised(p, stores, out);
+}
+inline void take_quantised_op(const std::vector<QuantisedRowsGPU>& stores, const PageMap& pages, const std::vector<RowsGPU>& out, ArrowComputePipeline& p) {
+  const uint64_t n = out.empty() ? 0 : out[0].rows;
+  const detail::QuantisedCall c(stores, out, n);
+  const agpu_page_map m = pages.abi();
+  check(agpu_take_quantised_pages(p.h(), (int32_t)stores.size(), c.stores.data(), c.rows.data(), &m, n), "agpu_take_quantised_pages");
+  detail::keep_pages(p, pages);
+  detail::keep_quantised(p, stores, out);
+}
+
+// Rows of any bytes: n rows of `pieces` pieces of piece_bytes (agpu_state); position_bytes: of one position inside a piece
+struct StateGPU {
+  BufferPtr data;
+  uint64_t rows = 0, pieces = 1, piece_bytes = 0, position_bytes = 0;
+};
+// out[k] row i = states[k] row indexes[i] (lengths: only the first lengths[i] positions of its pieces)
+inline void take_rows_op(const std::vector<StateGPU>& states, const UInt32ArrayGPU& indexes, const std::vector<StateGPU>& out, ArrowComputePipeline& p,
+                         const std::optional<UInt32ArrayGPU>& lengths = std::nullopt) {
+  if (states.size() != out.size() || (lengths && lengths->len != indexes.len)) throw ArrowErrorGPU(ArrowErrorGPU::Runtime, "take_rows: an output for every state, a length for every row");
+  std::vector<agpu_state> v;
+  for (size_t i = 0; i < states.size(); i++) {
+    const StateGPU &s = states[i], &o = out[i];
+    if (s.rows != states[0].rows || o.rows != indexes.len || o.pieces != s.pieces || o.piece_bytes != s.piece_bytes)
+      throw ArrowErrorGPU(ArrowErrorGPU::Runtime, "take_rows: rows of one kind");
+    const uint64_t row = s.pieces * s.piece_bytes;
+    if (s.rows * row > s.data->bytes || o.rows * row > o.data->bytes) throw ArrowErrorGPU(ArrowErrorGPU::Runtime, "take_rows: behind the end of a buffer");
+    v.push_back({s.data->ptr, o.data->ptr, row, s.piece_bytes, row, s.piece_bytes, s.pieces, s.piece_bytes, s.position_bytes});
+  }
+  check(agpu_take_rows(p.h(), (int32_t)v.size(), v.data(), states.empty() ? 0 : states[0].rows, static_cast<const uint32_t*>(indexes.data->ptr),
+                       lengths ? static_cast<const uint32_t*>(lengths->data->ptr) : nullptr, indexes.len), "agpu_take_rows");
+  p.keep.push_back(indexes.data);
+  if (lengths) p.keep.push_back(lengths->data);
+  for (size_t i = 0; i < states.size(); i++) p.keep.insert(p.keep.end(), {states[i].data, out[i].data});
+}
+
+// What select_beams found, [batch, k] flat, best first: scores, parents (rows of the logits: indexes for take_rows), tokens
+struct BeamSelection {
+  Float32ArrayGPU scores;
+  UInt32ArrayGPU parents, tokens;
+  BufferPtr workspace;
+};
+// Per request the k best of its beams x tokens by scores[row] + log_softmax(logits[row])[token]; logits: rows of 1 x vocab.  allowed: a bitmap of every
+// row's vocab bits, each row's on a multiple of 64 bits; finished: a bitmap of the rows, a finished row's one candidate is (end_token, its score)
+inline BeamSelection select_beams_op(const RowsGPU& logits, uint32_t beams, uint32_t k, ArrowComputePipeline& p, const std::optional<Float32ArrayGPU>& scores = std::nullopt,
+                                     const std::optional<BooleanArrayGPU>& allowed = std::nullopt, const std::optional<BooleanArrayGPU>& finished = std::nullopt,
+                                     uint32_t end_token = 0) {
+  const uint64_t pitch = agpu_bitmap_bytes(logits.dim);
+  if (beams == 0 || logits.heads != 1 || logits.dim >> 31 || logits.rows >> 31 || logits.rows % beams != 0 || (scores && scores->len != logits.rows) || (allowed && allowed->len != logits.rows * pitch * 8) ||
+      (finished && finished->len != logits.rows))
+    throw ArrowErrorGPU(ArrowErrorGPU::Runtime, "select_beams: logits of whole requests, a score, a bitmap, a bit for every row");
+  const auto& dev = logits.gpu_device;
+  const uint32_t batch = (uint32_t)(logits.rows / beams);
+  uint64_t need = 0;
+  check(agpu_select_beams_workspace(batch, beams, (uint32_t)logits.dim, k, &need), "agpu_select_beams_workspace");
+  const uint64_t n = (uint64_t)batch * k, bytes = n ? 4 * n : 4;
+  const BufferPtr s = dev->create_empty_buffer(bytes), r = dev->create_empty_buffer(bytes), t = dev->create_empty_buffer(bytes), w = dev->create_empty_buffer(need ? need : 16);
+  const agpu_rows x = logits.abi();
+  const agpu_beams a = {x.data, x.row_stride, x.type, batch, beams, (uint32_t)logits.dim, k, end_token, scores ? static_cast<const float*>(scores->data->ptr) : nullptr,
+                        allowed ? allowed->data->ptr : nullptr, allowed ? pitch : 0, finished ? finished->data->ptr : nullptr, static_cast<float*>(s->ptr),
+                        static_cast<uint32_t*>(r->ptr), static_cast<uint32_t*>(t->ptr), w->ptr, w->bytes};
+  check(agpu_select_beams(p.h(), &a), "agpu_select_beams");
+  p.keep.insert(p.keep.end(), {logits.data, s, r, t, w});
+  if (scores) p.keep.push_back(scores->data);
+  if (allowed) p.keep.push_back(allowed->data);
+  if (finished) p.keep.push_back(finished->data);
+  return {Float32ArrayGPU(s, dev, n, std::nullopt), UInt32ArrayGPU(r, dev, n, std::nullopt), UInt32ArrayGPU(t, dev, n, std::nullopt), w};
+}
+
 // validity of merge: ((v1 & m) | (v2 & ~m)) & v_mask in one kernel [crates/routines/src/merge.rs:17-86]
 inline std::optional<NullBitBufferGpu> merge_null_buffers_op(const std::optional<NullBitBufferGpu>& a,
                                                              const std::optional<NullBitBufferGpu>& b,
