@@ -241,12 +241,12 @@ struct UnPopc {  // countOneBits per element [logical/compute_shaders/u32/countb
 // ---- transcendental f32 functions.  log / sinh / pow below are evaluated in f64 and rounded ONCE to f32 (≤ 0.5 ULP + 2^-30);
 // the f32 device-library versions measure 2 ULP for sin / cos / log on gfx950 (profiles/r01_probe_first_contact.json).
 //
-// sin / cos (round 6): ALL in f32, TWO ROWS per instruction.  Rounds 1–5 evaluated the Cody–Waite reduction and the outer
+// sin / cos: ALL in f32, two rows side by side (independent chains).  Rounds 1–5 evaluated the Cody–Waite reduction and the outer
 // polynomial step in f64 — 8 f64 operations + 4 conversions + 5 selects per row, ≈ 27 VALU instructions, which an 8 B/row
 // stream hides and a 5–6 B/row cast-headed chain does not (`cast i16 → f32 → sin` in one launch 0.65 of the roof, `cast(u16)·s
-// → sin` 0.54).  gfx950 issues v_pk_fma_f32 / v_pk_mul_f32 / v_pk_add_f32 — two IEEE f32 operations per
-// lane — at ≈ 1.45× the cost of ONE (profiles/r02_valu_rate.json), so the same function written as double-float f32 arithmetic
-// over a PAIR of rows costs ≈ 11 packed + 6 scalar instructions per row:
+// → sin` 0.54).  The same function written as double-float f32 arithmetic over a PAIR of rows has no f64
+// operation and no conversion; the pair's two chains hide each other's latency.  (Packed f32 instructions are switched off in the build; with
+// them sin / cos took 1.18 / 1.20 ms for 1e9 rows, without 1.15 / 1.16, cast i16 → sin 0.976 and 0.922.)
 //   k  = round(x · 2/π) by the 1.5·2^23 trick (one fma; the low bits of the sum ARE k, no conversion), |k| < 2^20 for |x| < 1e6
 //   r1 = fma(−k, P1, x)                      EXACT: P1 = f32(π/2), k·P1 and x are multiples of 2^-24 and |r1| < 1
 //   ph + pl = k·P2 exactly (fma residual), (rh, e) = Fast2Sum(r1, −ph) — valid although |r1| may be < |ph|: r1 is a multiple
@@ -382,7 +382,8 @@ __device__ __attribute__((noinline)) float log_f32_general(float x) {  // any op
 //   tools/probe/log_f32_proto.c prints the fit); ln x = fma(e, LN2_HI, fma(e, LN2_LO, log m)) with LN2_HI of 15 bits, so e · LN2_HI is exact.
 // Every positive normal f32 is within 1 ULP of f64 libm rounded once — 12 408 324 of 2 122 317 824 inputs differ, all by one; largest error against
 // the true value 0.874 ULP — checked on the CPU with this operation sequence (tools/probe/log_f32_proto.c, 15 s) and on the device
-// (tests/tools/exhaustive_vs_oracle.py log).  7.5 packed + 5 scalar instructions per row, no table, no LDS: the generic f32 tile kernel runs it.
+// (tests/tools/exhaustive_vs_oracle.py log).  No table, no LDS: the generic f32 tile kernel runs it (1e9 rows in 1.21 ms; 1.157 with packed f32 instructions, which the build
+// switches off).
 __device__ __forceinline__ bool log_ordinary(float x) {
   return __builtin_amdgcn_classf(x, 0x100);  // +normal: one v_cmp_class_f32
 }
@@ -512,7 +513,7 @@ struct UnCos {
   __device__ static __forceinline__ float ap(float x, float) { return sincos_f32_dev<1>(x); }
   template <int N> __device__ static __forceinline__ void ap_rows(const float (&x)[N], float (&r)[N]) { sincos_f32_rows<1, N>(x, r); }
 };
-// functors with a several-rows-at-a-time form (sin / cos: packed f32 arithmetic over row pairs); everything else goes row by row
+// functors with a several-rows-at-a-time form (sin / cos: row pairs); everything else goes row by row
 template <typename Op> struct EwRowsOp { static constexpr bool value = false; };
 template <> struct EwRowsOp<UnSin> { static constexpr bool value = true; };
 template <> struct EwRowsOp<UnCos> { static constexpr bool value = true; };
@@ -655,7 +656,7 @@ template <> struct EwWaveLds<UnCos> { static constexpr unsigned value = AGPU_WAV
 template <> struct EwPrefetch<UnSin> { static constexpr bool value = true; static constexpr int tiles = 1; };
 template <> struct EwPrefetch<UnCos> { static constexpr bool value = true; static constexpr int tiles = 1; };
 template <> struct EwPrefetch<UnSinh> { static constexpr bool value = true; static constexpr int tiles = 1; };
-// log (round 6: packed f32, no table — the generic tile kernel instead of a kernel of its own).  One tile per block like the others: two were level
+// log (round 6: f32, no table — the generic tile kernel instead of a kernel of its own).  One tile per block like the others: two were level
 // or 1 % ahead in one process and 5 % behind in the next (0.84 / 0.79 — the by-process effect of R4.1 / R5.4), one tile is 0.83 everywhere
 template <> struct EwPrefetch<UnLog> { static constexpr bool value = true; static constexpr int tiles = 1; };
 template <> struct EwWaveLds<UnLog> { static constexpr unsigned value = AGPU_WAVE_LDS_24; };  // (tools/probe/r06_sincos_sweep.py: ≈ 24 waves 0.83–0.84, ≈ 16 0.77–0.78, no cap 0.79–0.83)
@@ -1366,7 +1367,7 @@ static agpu_status launch_cvt(agpu_pipeline* p, const void* in, void* out, uint6
         const uint64_t blocks = (nchunks + AGPU_CVTW_BLOCK / AGPU_WAVE - 1) / (AGPU_CVTW_BLOCK / AGPU_WAVE);
         const int grid = stream_grid_for(p, (blocks + k - 1) / k);
         // occupancy cap (common.hpp): ×2 casts to 32 bits ≈ 24 waves per CU, ×4 ≈ 16; u8 → u16 none (not measured to gain)
-        // (round 6: none for cast → sin / cos of a 16-bit column — with sin / cos in packed f32 the kernel wants all its waves: 0.79–0.80 against 0.75)
+        // (round 6: none for cast → sin / cos of a 16-bit column — with sin / cos in f32 the kernel wants all its waves: 0.79–0.80 against 0.75)
         constexpr unsigned cap = ConvHasRows<Conv>::value ? 0u : sizeof(TO) == 4 ? (sizeof(TI) == 2 ? AGPU_WAVE_LDS_24 : AGPU_WAVE_LDS_16) : 0u;
         const unsigned lds = cap ? wave_lds_for(p, cap, AGPU_CVTW_BLOCK / AGPU_WAVE) : 0u;
         // ×2 casts walk the chunks as two lock-step streams (common.hpp two_streams: u16 → f32 0.836 → 0.857, u8 → u16 0.80 → 0.83, sin_u16 0.78 → 0.79);
@@ -1461,7 +1462,7 @@ struct CvtThenF32 {  // fused sin_u8-style kernels [trigonometry/compute_shaders
     else if constexpr (sizeof(TI) <= 2 && std::is_same<F, UnCos>::value) return sincos_f32_fast<1>((float)x);
     else return F::ap((float)x, 0.0f);
   }
-  // several rows at a time: sin / cos evaluate row PAIRS in packed f32 (sincos_f32_pair); same bits as ap()
+  // several rows at a time: sin / cos evaluate row PAIRS (sincos_f32_pair); same bits as ap()
   static constexpr bool has_rows = sizeof(TI) <= 2 && (std::is_same<F, UnSin>::value || std::is_same<F, UnCos>::value || std::is_same<F, UnLog>::value);
   template <int N> __device__ static __forceinline__ void ap_rows(const TI (&x)[N], float (&r)[N]) {
     static_assert(N % 2 == 0, "rows come in pairs");
