@@ -216,6 +216,9 @@ class ArrowArrayGPU:
         return self.len
 
 
+_FITS = set()  # (array class, tensor dtype) that go together
+
+
 class PrimitiveArrayGpu(ArrowArrayGPU):
     """Arrow primitive array in HBM.  [ref: crates/array/src/array/primitive_array_gpu.rs:12-117]"""
 
@@ -252,9 +255,11 @@ class PrimitiveArrayGpu(ArrowArrayGPU):
     def of_tensor(cls, tensor, gpu_device: GpuDevice):
         """The array over a contiguous tensor's memory, without a copy (integers of one width may change their sign: an int32 tensor is a
         UInt32ArrayGPU's memory too).  `values()` and the ops see what the tensor holds when they run."""
-        t = tensor_type(tensor)
-        if (t[0] == "f") != (cls.NP_DTYPE is np.float32) or tensor.element_size() != cls.ITEM_SIZE or t == "bf16":
-            raise capi.ArrowErrorGPU("ArgumentError", f"{cls.__name__} over a tensor of {tensor.dtype}", capi.ERR_ARG)
+        if (cls, tensor.dtype) not in _FITS:
+            t = tensor_type(tensor)
+            if (t[0] == "f") != (cls.NP_DTYPE is np.float32) or tensor.element_size() != cls.ITEM_SIZE or t == "bf16":
+                raise capi.ArrowErrorGPU("ArgumentError", f"{cls.__name__} over a tensor of {tensor.dtype}", capi.ERR_ARG)
+            _FITS.add((cls, tensor.dtype))
         if not tensor.is_contiguous():
             raise capi.ArrowErrorGPU("ShapeError", f"{cls.__name__} over a tensor that is not contiguous", capi.ERR_SHAPE)
         n = tensor.numel()

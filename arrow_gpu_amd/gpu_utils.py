@@ -41,17 +41,21 @@ class DeviceBuffer:
             self.ptr = 0
 
 
-class BorrowedBuffer(DeviceBuffer):
-    """Device memory of somebody else's (a torch tensor's, …).  `owner` is held as long as the buffer is, never freed here."""
+class BorrowedBuffer:
+    """Device memory of somebody else's (a torch tensor's, …), where a DeviceBuffer is taken.  `owner` is held as long as the buffer is; nothing is freed
+    here, and there is no destructor to run (a serving loop makes one for every tensor of a call)."""
 
-    __slots__ = ("owner",)
+    __slots__ = ("device", "ptr", "nbytes", "owner", "__weakref__")
+    _owned = False
 
     def __init__(self, device: "GpuDevice", ptr: int, nbytes: int, owner=None):
         self.device = device
         self.ptr = ptr
         self.nbytes = nbytes
-        self._owned = False
         self.owner = owner
+
+    def size(self) -> int:
+        return self.nbytes
 
 
 _TENSOR_TYPES = {"float32": "f32", "float16": "f16", "bfloat16": "bf16", "int8": "i8", "uint8": "u8", "int16": "i16", "uint16": "u16", "int32": "i32",

@@ -40,26 +40,29 @@ def _u32(array, what: str):
 def _quantised(name: str, stores, rows, where, n: int, pipeline) -> None:
     if len(stores) > _MAX_COLUMNS:
         raise shape_error(f"{len(stores)} caches in one call: at most {_MAX_COLUMNS}")
-    packed_stores, packed_rows = [], []
+    dev, s, r = pipeline.device, b"", b""
     for store, x in zip(stores, rows):
         shape = x.shape
         if shape[0] != n or (shape[1:] != store.shape and (store.heads != 1 or shape[1:] != store.shape[1:])):
             raise shape_error(f"rows {shape} for {n} rows of {store.heads} x {store.dim}")
-        _on(pipeline, store, x)
-        packed_stores.append(store.packed)
-        packed_rows.append(x._rows or x.as_rows())
-    s, r = b"".join(packed_stores), b"".join(packed_rows)
+        if x.gpu_device is not dev or store.gpu_device is not dev:
+            _on(pipeline, store, x)
+        s += store.packed
+        r += x._rows or x.as_rows()
     if isinstance(where, PageMap):
-        held = [where.tables, where.offsets] if where.first is None else [where.tables, where.offsets, where.first]
+        held = (where.tables, where.offsets) if where.first is None else (where.tables, where.offsets, where.first)
         _on(pipeline, *held)
         capi.call(name + "_pages", pipeline._handle, len(stores), s, r, where.packed, n)
         _keep(pipeline, *[x.data for x in held])
     else:
-        _on(pipeline, where)
+        if where.gpu_device is not dev:
+            _on(pipeline, where)
         capi.call(name, pipeline._handle, len(stores), s, r, where.data.ptr, n)
-        _keep(pipeline, where.data)
+        if where.data._owned:
+            pipeline.keep(where.data)
     for store, x in zip(stores, rows):
-        _keep(pipeline, store.codes, store.scales, x.data)
+        if store.codes._owned or store.scales._owned or x.data._owned:
+            _keep(pipeline, store.codes, store.scales, x.data)
 
 
 def put_quantised_op(stores, rows, where, pipeline: ArrowComputePipeline) -> None:
@@ -123,27 +126,28 @@ def take_rows_op(states, indexes: UInt32ArrayGPU, pipeline: ArrowComputePipeline
         out = [RowsGPU.empty((n,) + tuple(s.shape[1:]), s.type, s.gpu_device) for s in states]
     if len(out) != len(states):
         raise shape_error(f"{len(out)} outputs for {len(states)} states")
-    n_src = len(states[0])
-    packed = []
+    n_src, dev, packed = states[0].shape[0], pipeline.device, b""
     for s, o in zip(states, out):
         if s.shape[0] != n_src or o.shape[1:] != s.shape[1:] or o.shape[0] != n or o.item_size != s.item_size:
             raise shape_error(f"rows {tuple(o.shape)} from a state {tuple(s.shape)} by {n} indexes, in a call over {n_src} rows")
-        row, step, pieces, size, position = s.as_pieces()
-        out_row, out_step, out_pieces, out_size, _ = o.as_pieces()
+        row, step, pieces, size, position = s._pieces or s.as_pieces()
+        out_row, out_step, out_pieces, out_size, _ = o._pieces or o.as_pieces()
         if (pieces, size) != (out_pieces, out_size):
             raise shape_error(f"the pieces of {tuple(s.shape)}: strides {s.strides} and {o.strides}")
         if lengths is not None and not position:
             raise shape_error("lengths count positions, the axis before the last: they lie next to each other")
-        packed.append(_PACK_STATE.pack(s.ptr, o.ptr, row, step, out_row, out_step, pieces, size, position))
-        _on(pipeline, s, o)
+        packed += _PACK_STATE.pack(s.ptr, o.ptr, row, step, out_row, out_step, pieces, size, position)
+        if s.gpu_device is not dev or o.gpu_device is not dev:
+            _on(pipeline, s, o)
     _on(pipeline, indexes)
     if lengths is not None:
         _on(pipeline, lengths)
         _keep(pipeline, lengths.data)
-    capi.call("agpu_take_rows", pipeline._handle, len(states), b"".join(packed), n_src, indexes.data.ptr, lengths.data.ptr if lengths is not None else None, n)
+    capi.call("agpu_take_rows", pipeline._handle, len(states), packed, n_src, indexes.data.ptr, lengths.data.ptr if lengths is not None else None, n)
     _keep(pipeline, indexes.data)
     for s, o in zip(states, out):
-        _keep(pipeline, s.data, o.data)
+        if s.data._owned or o.data._owned:
+            _keep(pipeline, s.data, o.data)
     return out
 
 

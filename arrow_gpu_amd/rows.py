@@ -61,7 +61,14 @@ class RowsGPU:
     def of_tensor(cls, tensor, gpu_device: GpuDevice) -> "RowsGPU":
         """The rows over a tensor's memory, without a copy (a slice of a bigger tensor keeps its strides)."""
         t = tensor_type(tensor)
-        return cls(borrow_tensor(tensor, gpu_device, tensor.numel() * ITEM_SIZE[t]), gpu_device, tensor.shape, t, tensor.stride())
+        shape, strides, item = tuple(tensor.shape), tensor.stride(), ITEM_SIZE[t]
+        if not 2 <= len(shape) <= 4 or (strides[-1] != 1 and shape[-1] > 1):
+            return cls(None, gpu_device, shape, t, strides, 0)  # raises
+        self = cls.__new__(cls)
+        self.data = data = borrow_tensor(tensor, gpu_device, tensor.numel() * item)
+        self.ptr, self.gpu_device, self.type, self.shape, self.strides, self.item_size = data.ptr, gpu_device, t, shape, strides, item
+        self._rows = self._pieces = None
+        return self
 
     # -- what the ABI's calls take
     def as_rows(self) -> bytes:
