@@ -101,6 +101,7 @@ template <> struct Raw<bf16_t> {
 };
 
 constexpr int TILE = 1024;  // logits a wave takes at a time: 16 a lane
+constexpr uint32_t MOST_TILES = 8;  // of a segment
 constexpr int HITS = 2048; // and may look at twice
 constexpr uint32_t EXACT = 16;  // at least so many of the largest terms are taken in f64
 constexpr int RANKED = 8;
@@ -124,16 +125,25 @@ struct Segment {
       const u32x4* at = reinterpret_cast<const u32x4*>(x - lead) + (uint64_t)t * (TILE / VE) + lane;
 #pragma unroll
       for (int u = 0; u < U; u++) w[u] = at[u * 64];
-    } else {  // the row's ends
+    } else {  // the row's ends: whole vectors, and the two that the row does not fill value by value, all on their way at once
 #pragma unroll
       for (int u = 0; u < U; u++) {
         const int64_t at = token(t, u);
-        T e[VE] = {};
         m[u] = 0;
+        w[u] = u32x4{0, 0, 0, 0};
+        if (at >= 0 && at + VE <= vocab) w[u] = *reinterpret_cast<const u32x4*>(x + at), m[u] = (1u << VE) - 1;
+      }
 #pragma unroll
-        for (int i = 0; i < VE; i++)
-          if (at + i >= 0 && at + i < vocab) e[i] = x[at + i], m[u] |= 1u << i;
-        w[u] = __builtin_bit_cast(u32x4, e);
+      for (int u = 0; u < U; u++) {
+        const int64_t at = token(t, u);
+        if (m[u] == 0 && at + VE > 0 && at < vocab) {
+          T e[VE];
+#pragma unroll
+          for (int i = 0; i < VE; i++) e[i] = x[at + i < 0 ? 0 : at + i < vocab ? at + i : vocab - 1];
+#pragma unroll
+          for (int i = 0; i < VE; i++) m[u] |= (uint32_t)(at + i >= 0 && at + i < vocab) << i;
+          w[u] = __builtin_bit_cast(u32x4, e);
+        }
       }
     }
     if (MASK) {
@@ -170,9 +180,10 @@ __device__ __forceinline__ float max_of(float a, float b) {
   asm("v_max_f32 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
   return r;
 }
-__device__ __forceinline__ float max_of(float a, float b, float c) {
+// the largest, a NaN if there is one
+__device__ __forceinline__ float maximum_of(float a, float b, float c) {
   float r;
-  asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  asm("v_maximum3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
   return r;
 }
 
@@ -199,24 +210,28 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
   float floor_v = LOWEST, above = -0x1.fffffep127f, ref_v = 0.0f, k = MAGIC, least = 0.0f;
   double sum = 0.0;
   uint64_t nan = 0;
-  uint32_t hits[4] = {0, 0, 0, 0};  // a bit a logit of the lane's: it reached the floor; the last tile's first in the lowest
-  u32x4 w[U], next[U];
-  uint32_t m[U], next_m[U];
-  if (t0 < t1) s.load(t0, w, m);
-  for (uint32_t step = 0; step < tiles; step++) {
+  uint32_t hits[4] = {0, 0, 0, 0};  // a bit a logit of the lane's, tile by tile: it reached the floor
+  u32x4 two_w[2][U];  // the tile at hand and the next, on its way
+  uint32_t two_m[2][U];
+  if (t0 < t1) s.load(t0, two_w[0], two_m[0]);
+#pragma unroll  // (the buffers and the bits' places are then fixed: 4 % of the time)
+  for (uint32_t step = 0; step < MOST_TILES; step++) {
+    if (step >= tiles) break;
     const uint32_t t = t0 + step;
+    u32x4 (&w)[U] = two_w[step % 2];
+    uint32_t (&m)[U] = two_m[step % 2];
     float v[EPT], vm[U];
     if (t < t1) {
-      if (t + 1 < t1) s.load(t + 1, next, next_m);
+      if (t + 1 < t1) s.load(t + 1, two_w[(step + 1) % 2], two_m[(step + 1) % 2]);
       s.values(t, w, m, v);
 #pragma unroll
       for (int u = 0; u < U; u++) {
-        vm[u] = max_of(v[u * VE], v[u * VE + 1]);
+        vm[u] = maximum_of(v[u * VE], v[u * VE + 1], v[u * VE + 2]);
 #pragma unroll
-        for (int i = 2; i < VE; i += 2) vm[u] = max_of(vm[u], v[u * VE + i], v[u * VE + i + 1]);
+        for (int i = 3; i < VE; i += 2) vm[u] = maximum_of(vm[u], v[u * VE + i], v[u * VE + (i + 1 < VE ? i + 1 : i)]);
       }
 #pragma unroll
-      for (int i = 0; i < EPT; i += 2) nan |= __ballot(__builtin_isunordered(v[i], v[i + 1]));
+      for (int u = 0; u < U; u += 2) nan |= __ballot(__builtin_isunordered(vm[u], vm[u + 1]));
       float tm[2] = {vm[0], vm[U / 2]};
 #pragma unroll
       for (int u = 1; u < U / 2; u++) tm[0] = fmaxf(tm[0], vm[u]), tm[1] = fmaxf(tm[1], vm[U / 2 + u]);
@@ -249,8 +264,6 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
       if (step == 0) __syncthreads();  // (before they are written again)
     }
     if (t >= t1) continue;
-    hits[3] = hits[3] << EPT | hits[2] >> (32 - EPT), hits[2] = hits[2] << EPT | hits[1] >> (32 - EPT), hits[1] = hits[1] << EPT | hits[0] >> (32 - EPT);
-    hits[0] <<= EPT;
 #pragma unroll
     for (int u = 0; u < U; u++)
       if (__any(vm[u] >= above)) {
@@ -272,7 +285,7 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
             if (late && (h >> i & 1) && Raw<T>::at(w[u], i) == floor_v) h &= ~(1u << i), v[u * VE + i] = floor_v;
           above = value_of(order_of(floor_v) + 1);
         }
-        hits[0] |= h << u * VE;
+        hits[step / 2] |= h << (step % 2 * EPT + u * VE);
       }
     // the terms (at least e^-80, −infinity too: nothing beside the largest), added in pairs of pairs: four roundings on every way
 #pragma unroll
@@ -282,8 +295,6 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
 #pragma unroll
       for (int i = 0; i < EPT; i += 2 * d) v[i] += v[i + d];
     sum += (double)v[0];
-#pragma unroll
-    for (int u = 0; u < U; u++) w[u] = next[u], m[u] = next_m[u];
   }
 
   float most = fmaxf(top[0], top[1]);
@@ -297,6 +308,8 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
   for (int i = 0; i < 4; i++) all += (uint32_t)__builtin_popcount(hits[i]);
   for (int d = 32; d; d >>= 1) all += __shfl_xor(all, d);
   const bool many = all > HITS, again = most > LOWEST && most < __builtin_inff() && (many || __builtin_fabsf(most - ref_v) > APART);
+  u32x4 w[U];
+  uint32_t m[U];
   if (again) {  // in f64, below the maximum that is now known
     ref = most;
     sum = 0.0;
@@ -317,7 +330,7 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
       float y = LOWEST;
       uint32_t token = 0;
       if (h) {
-        const uint32_t bit = word * 32 + __builtin_ctz(h), t = t1 - 1 - bit / EPT, i = bit % EPT;
+        const uint32_t bit = word * 32 + __builtin_ctz(h), t = t0 + bit / EPT, i = bit % EPT;
         token = t * TILE + i / VE * (64 * VE) + lane * VE + i % VE - s.lead;
         y = (float)s.x[token];
         if (!again) sum += exp((double)y - ref);
@@ -550,7 +563,7 @@ __global__ __launch_bounds__(MERGE_BLOCK) void beam_merge_kernel(BeamArgs a, con
 // Tiles of a segment: the fewer, the more waves share the work; the more, the fewer lists there are to join.  As many as leave 4096 waves (16 a
 // CU), at most 8.  (The type does not enter: the workspace does not depend on it.)
 uint32_t segment_tiles(uint64_t rows, uint64_t vocab) {
-  uint32_t t = 8;
+  uint32_t t = MOST_TILES;
   while (t > 1 && rows * ((vocab + 7 + t * TILE - 1) / (t * TILE)) < 4096) t /= 2;
   return t;
 }
