@@ -11,6 +11,7 @@
 // times what log2 e has beyond f32 (2^-26 of error each), the instruction for 2^f is within 2^-23; 16 are added with 4 roundings, the rest in f64.
 // That bounds a log-sum's error by 2^-23 + ln 2 · 2^-25 + 4 · 2^-24 < 3.8e-7; many different terms are off at random, and it is about 1e-9.
 #include "common.hpp"
+#include "row_address.hpp"
 
 namespace {
 
@@ -403,33 +404,28 @@ __device__ __forceinline__ bool before_equal(const Candidate& x, const Candidate
 __device__ __forceinline__ bool better(const Candidate& x, const Candidate& y) { return x.score > y.score || (x.score == y.score && before_equal(x, y)); }
 
 constexpr int MERGE_BLOCK = 512, MERGE_WAVES = MERGE_BLOCK / 64, MERGE_LIST = 512, HELD = 4, PARTS = 4;
+constexpr uint32_t TURN = 37;  // a thread's entries are of different ranks in their segments
 
-// A wave a beam: its log-sum, its entries' scores, and a bound that k of them reach.  What reaches the best of the beams' bounds goes to LDS and is
-// ranked there by counting.
-__global__ __launch_bounds__(MERGE_BLOCK) void beam_merge_kernel(BeamArgs a, const SegSum* sums, const Entry* entries) {
+// The rows' log-sums, a wave a beam; then all threads over all entries of the request, for a bound that k of them reach: the k-th of each lane's two
+// largest among the threads' bests.  What reaches it goes to LDS and is ranked there by counting.
+__global__ __launch_bounds__(MERGE_BLOCK) void beam_merge_kernel(BeamArgs a, Divide by_row, const SegSum* sums, const Entry* entries) {
   __shared__ double lse[1024];  // per beam: its log-sum, NaN for a row whose scores are −infinity
-  __shared__ float cum[1024], wave_floor[MERGE_WAVES];
+  __shared__ float cum[1024], bests[MERGE_BLOCK];
   __shared__ double scores[MERGE_LIST + PARTS * RANKED];
   __shared__ Candidate list[MERGE_LIST];
   __shared__ uint64_t chosen[64];
   __shared__ uint32_t count;
-  const uint32_t r0 = blockIdx.x * a.beams, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), per_row = a.segs * a.k;
+  const uint32_t r0 = blockIdx.x * a.beams, lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), total = a.beams * by_row.d;
   const double none = -__builtin_inf();
+  const Entry* mine = entries + (uint64_t)r0 * by_row.d;  // (a finished row's are what an earlier call left: its log-sum, NaN, keeps them out)
+  const auto place = [](uint32_t j) { return j * MERGE_BLOCK + (threadIdx.x + j * TURN) % MERGE_BLOCK; };
   if (threadIdx.x == 0) count = 0;
+  Entry held[HELD];  // the thread's first
+#pragma unroll
+  for (uint32_t j = 0; j < HELD; j++) held[j] = place(j) < total ? mine[place(j)] : Entry{LOWEST, 0};
 
-  const auto score = [&](Entry x, double c, double l) {
-    const double s = c + ((double)x.logit - l);
-    return x.logit > LOWEST && s > none ? s : none;  // (NaN: none)
-  };
-  float floor_v = LOWEST;
-  Entry held[HELD];  // of the wave's first beam
   for (uint32_t b = wave; b < a.beams; b += MERGE_WAVES) {
     const uint32_t row = r0 + b;
-    const Entry* mine = entries + (uint64_t)row * per_row;
-    if (b == wave) {  // (a finished row's are what an earlier call left: its log-sum, NaN, keeps them out)
-#pragma unroll
-      for (int i = 0; i < HELD; i++) held[i] = lane + i * 64 < per_row ? mine[lane + i * 64] : Entry{LOWEST, 0};
-    }
     const SegSum* parts = sums + (uint64_t)row * a.segs;
     const SegSum first = lane < a.segs ? parts[lane] : SegSum{0.0, none};
     const float c = a.scores ? a.scores[row] : 0.0f;
@@ -443,20 +439,40 @@ __global__ __launch_bounds__(MERGE_BLOCK) void beam_merge_kernel(BeamArgs a, con
       if (g.sum != 0.0) s += g.sum * exp(g.ref - top);
     }
     for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
-    const double l = done ? __builtin_nan("") : top + log(s);
-    if (lane == 0) lse[b] = l, cum[b] = c;
-    float best[1] = {LOWEST};  // rounding to f32 keeps the order, but for ties
-    if (b == wave) {
-#pragma unroll
-      for (int i = 0; i < HELD; i++) best[0] = fmaxf(best[0], (float)score(held[i], c, l));
-    }
-    for (uint32_t e = lane + (b == wave ? HELD * 64 : 0); e < per_row && !done; e += 64) best[0] = fmaxf(best[0], (float)score(mine[e], c, l));
-    floor_v = fmaxf(floor_v, wave_kth(best, a.k, 0));
+    if (lane == 0) lse[b] = done ? __builtin_nan("") : top + log(s), cum[b] = c;
   }
-  if (lane == 0) wave_floor[wave] = floor_v;
   __syncthreads();
+
+  const auto score = [&](Entry x, uint32_t b) {
+    const double s = cum[b] + ((double)x.logit - lse[b]);
+    return x.logit > LOWEST && s > none ? s : none;  // (NaN: none)
+  };
+  // all entries, and a finished beam's only candidate: f(score, beam, entry)
+  const auto each = [&](uint32_t from, const auto& f) {  // from: so many of the thread's are left out
+    for (uint32_t j = from; j * MERGE_BLOCK < total; j++) {
+      const uint32_t i = place(j);
+      if (i >= total) continue;
+      const Entry x = mine[i];
+      const uint32_t b = i / by_row;
+      f(score(x, b), b, x);
+    }
+    for (uint32_t b = threadIdx.x; b < a.beams; b += MERGE_BLOCK)
+      if (is_finished(a, r0 + b) && cum[b] == cum[b]) f((double)cum[b], b, Entry{0.0f, a.end_token});
+  };
+  float best = LOWEST;  // rounding to f32 keeps the order, but for ties
 #pragma unroll
-  for (int w = 0; w < MERGE_WAVES; w++) floor_v = fmaxf(floor_v, wave_floor[w]);
+  for (uint32_t j = 0; j < HELD; j++)
+    if (place(j) < total) best = fmaxf(best, (float)score(held[j], place(j) / by_row));
+  each(HELD, [&](double s, uint32_t, Entry) { best = fmaxf(best, (float)s); });
+  bests[threadIdx.x] = best;
+  __syncthreads();
+  float two[2] = {LOWEST, LOWEST};
+#pragma unroll
+  for (int i = 0; i < MERGE_WAVES; i++) {
+    const float x = bests[i * 64 + lane], low = fminf(x, two[0]);
+    two[0] = fmaxf(x, two[0]), two[1] = fmaxf(two[1], low);
+  }
+  float floor_v = wave_kth(two, a.k, 0);
 
   const auto offer = [&](double s, uint32_t b, Entry x) {
     if (s > none && (float)s >= floor_v) {
@@ -464,27 +480,38 @@ __global__ __launch_bounds__(MERGE_BLOCK) void beam_merge_kernel(BeamArgs a, con
       if (at < MERGE_LIST) scores[at] = s, list[at] = candidate_of(s, b, x);
     }
   };
-  // every beam's entries, and a finished one's only candidate: f(score, beam, entry)
-  const auto each = [&](uint32_t from, const auto& f) {  // from: entries of the wave's first beam that f has had
-    for (uint32_t b = wave; b < a.beams; b += MERGE_WAVES) {
-      if (is_finished(a, r0 + b)) {
-        if (lane == 0 && cum[b] == cum[b]) f((double)cum[b], b, Entry{0.0f, a.end_token});
-        continue;
-      }
-      const double l = lse[b], c = cum[b];
-      for (uint32_t e = lane + (b == wave ? from : 0); e < per_row; e += 64) {
-        const Entry x = entries[(uint64_t)(r0 + b) * per_row + e];
-        f(score(x, c, l), b, x);
-      }
-    }
-  };
-  if (wave < a.beams) {
 #pragma unroll
-    for (int i = 0; i < HELD; i++) offer(score(held[i], cum[wave], lse[wave]), wave, held[i]);
-  }
-  each(HELD * 64, offer);
+  for (uint32_t j = 0; j < HELD; j++)
+    if (place(j) < total) offer(score(held[j], place(j) / by_row), place(j) / by_row, held[j]);
+  each(HELD, offer);
   __syncthreads();
-  const uint32_t n = count, found = n < a.k ? n : a.k;
+  uint32_t n = count;
+  if (n > MERGE_LIST) {  // the bound is too low for the list (k is large): any that k and at most MERGE_LIST reach, found by halving
+    uint32_t low = order_of(floor_v), high = order_of(-LOWEST) + 1;
+    while (n > MERGE_LIST && high - low > 1) {
+      const uint32_t mid = low + (high - low) / 2;
+      uint32_t reach = 0;
+      each(0, [&](double s, uint32_t, Entry) { reach += s > none && order_of((float)s) >= mid; });
+      for (int d = 32; d; d >>= 1) reach += __shfl_xor(reach, d);
+      __syncthreads();
+      if (threadIdx.x == 0) count = 0;
+      __syncthreads();
+      if (lane == 0) atomicAdd(&count, reach);
+      __syncthreads();
+      const uint32_t c = count;
+      if (c > MERGE_LIST) low = mid;
+      else if (c < a.k) high = mid;
+      else n = c, floor_v = value_of(mid);
+    }
+    if (n <= MERGE_LIST) {
+      __syncthreads();
+      if (threadIdx.x == 0) count = 0;
+      __syncthreads();
+      each(0, offer);
+      __syncthreads();
+    }
+  }
+  const uint32_t found = n < a.k ? n : a.k;
   const auto put = [&](uint32_t rank, const Candidate& c) {
     const uint64_t o = (uint64_t)blockIdx.x * a.k + rank;
     const uint32_t beam = (uint32_t)(c.tie >> 32);
@@ -517,7 +544,7 @@ __global__ __launch_bounds__(MERGE_BLOCK) void beam_merge_kernel(BeamArgs a, con
       for (int d = 1; d < PARTS; d *= 2) rank += __shfl_xor(rank, d);
       if (part == 0 && rank < a.k) put(rank, c);
     }
-  } else {  // very many equal scores: the best, then the best behind it, k times
+  } else {  // very many scores equal in f32: the best, then the best behind it, k times
     Candidate before = {__builtin_inf(), 0, 0};
     for (uint32_t r = 0; r < a.k; r++) {
       Candidate top = {none, ~0ull, 0};
@@ -575,7 +602,7 @@ uint32_t segments(uint64_t rows, uint64_t vocab) {
 bool workspace_bytes(uint64_t batch, uint64_t beams, uint64_t vocab, uint64_t k, uint64_t* out) {
   if (batch == 0 || beams == 0 || vocab == 0 || k == 0 || k > 64 || beams > 1024 || k > beams * vocab || batch * beams >= (1u << 24) || vocab >= (1ull << 31)) return false;
   const uint64_t segs = segments(batch * beams, vocab);
-  if (beams * segs * k >= (1ull << 32) || batch * beams * segs >= (1ull << 31)) return false;  // a request's entries, the blocks
+  if (beams * segs * k >= (1ull << 31) || batch * beams * segs >= (1ull << 31)) return false;  // a request's entries, the blocks
   *out = batch * beams * segs * (sizeof(SegSum) + k * sizeof(Entry));
   return true;
 }
@@ -629,7 +656,7 @@ agpu_status agpu_select_beams(agpu_pipeline* p, const agpu_beams* args) {
   else if (b.type == AGPU_ROW_F16) launch_segments<f16_t>(p, a, sums, entries);
   else launch_segments<bf16_t>(p, a, sums, entries);
   AGPU_LAUNCH_CHECK();
-  hipLaunchKernelGGL(beam_merge_kernel, dim3(b.batch), dim3(MERGE_BLOCK), 0, p->stream, a, sums, entries);
+  hipLaunchKernelGGL(beam_merge_kernel, dim3(b.batch), dim3(MERGE_BLOCK), 0, p->stream, a, divide_by(a.segs * a.k), sums, entries);
   AGPU_LAUNCH_CHECK();
   return AGPU_OK;
 }

@@ -546,6 +546,38 @@ def test_select_very_many_equal_logits(dev, p, kind, k, low):
     assert_selection(sel, R.select(x.astype(np.float64), beams, k))
 
 
+@pytest.mark.parametrize("batch,beams,vocab,k", [(1, 32, 5000, 64), (2, 64, 777, 64), (1, 1, 150001, 64), (3, 4, 12345, 33), (2, 9, 33000, 50), (1, 1024, 40, 64)])
+@pytest.mark.parametrize("kind", KINDS)
+def test_select_many_beams_and_a_large_k(dev, p, kind, batch, beams, vocab, k):
+    """thousands of entries to join for a request"""
+    import arrow_gpu_amd as ag
+
+    rng = np.random.default_rng(beams + k)
+    x = logits(rng, batch * beams, vocab, kind)
+    cum = -np.float32(3) * rng.random(batch * beams).astype(np.float32)
+    cum[:beams] = 0.0
+    sel = ag.select_beams_op(up(x, kind, dev), beams, k, p, scores=ag.Float32ArrayGPU.from_slice(cum, dev))
+    p.sync()
+    assert_selection(sel, R.select(x.astype(np.float64), beams, k, cum))
+
+
+def test_select_candidates_beside_each_other(dev, p):
+    """640 tokens of a row are all that is above -infinity, 16 in each of some stretches of 1024: no bound is known before they are joined"""
+    import arrow_gpu_amd as ag
+
+    rng = np.random.default_rng(3)
+    x = np.full((2, 262144), -np.inf, np.float32)
+    for j in (0, 12, 19, 24, 31):
+        for seg in range(8 * j, 8 * j + 8):
+            at = seg * 1024 + rng.choice(1024, 16, replace=False)
+            x[0, at] = 5 * rng.random(16)
+            x[1, at] = rng.integers(0, 40, 16)           # and many equal ones
+    for k in (16, 40, 64):
+        sel = ag.select_beams_op(up(x, "f32", dev), 1, k, p)
+        p.sync()
+        assert_selection(sel, R.select(x.astype(np.float64), 1, k))
+
+
 def test_select_rows_of_one_row(dev, p):
     """one row of logits for all beams (stride 0), as at a request's first step"""
     import arrow_gpu_amd as ag
