@@ -49,7 +49,11 @@ struct QuantShape {
 // ---------------------------------------------------------------- eight values a lane
 // Both ways stream: 16-byte accesses (32 of f32) on the rows' side, 8 or 4 on the codes'.  A group is `lanes` neighbouring lanes (a power of two, those
 // past the group's end idle), its span found with data-parallel moves inside the wave.  A block takes whole rows, looks their slots up once and
-// keeps them in LDS: a search of the sequence through memory costs microseconds, so it is shared by up to 8 passes of the block.
+// keeps them in LDS: a search of the sequence through memory costs microseconds, so it is shared by up to 8 passes of the block (16 passes: 131072
+// rows of 4 bits in 138 us instead of 127).
+// What bounds it is memory: two columns of 16384 rows of 8 x 128 bf16 go to e4m3 in 18 us and come back in 16.6 (102 MB each: 5.7 and 6.1 TB/s; a copy
+// of as many bytes takes 17), ragged e4m3 rows of 4 x 96 come back as f16 in 30.5 us (181 MB, 5.9 TB/s), two columns of 131072 rows of 4 bits as bf16
+// in 127 us (705 MB, 5.6 TB/s; a u8 -> f32 cast of as many bytes 109).  A token's rows take 2.5 us a call, that is one launch.
 constexpr int MAX_COLS = 8, MAX_ROWS = 256;
 struct QuantCols {
   QuantCol c[MAX_COLS];
@@ -123,7 +127,7 @@ __device__ __forceinline__ uint64_t value_offset(const Unit& u, const QuantCol& 
 template <typename T, int CODE>
 __global__ __launch_bounds__(AGPU_BLOCK) void put_eight_kernel(QuantCols cols, FastShape q, RowAddr addr, uint64_t n, uint32_t* flags) {
   __shared__ BlockRow<const T> held[MAX_ROWS];
-  const QuantCol& c = cols.c[blockIdx.y];
+  const QuantCol& c = cols.c[blockIdx.y];  // (one load of a lane in flight: two or four do not pay, 18.2 -> 18.9 us)
   const uint32_t total = (block_rows<const T>(c, q, addr, n, held, flags) * q.groups_per_row) << q.log_lanes;
   for (uint32_t i = threadIdx.x; i < total; i += AGPU_BLOCK) {
     const Unit t = unit_of(i, q);
@@ -240,13 +244,16 @@ __global__ __launch_bounds__(AGPU_BLOCK) void take_eight_kernel(QuantCols cols, 
           }
         }
       }
-      // past the caches: nobody reads the rows in this call
+      // past the caches: nobody reads the rows in this call (ragged e4m3 rows 30.5 us, through the caches 42)
       __builtin_nontemporal_store(o, reinterpret_cast<typename Eight<T>::type*>(to[u]));
     }
   }
 }
 
 // ---------------------------------------------------------------- one wave a group: any group, stride and alignment
+// What the lanes of the form above cannot share: groups that are no multiple of 8 or above 512, rows off their vectors' alignment.  Bound by its
+// instructions, narrow accesses and a slot's look-up for each group: 2^24 bf16 values in groups of 100 to 8 bits in 64 us, back in 42; groups of 20 in 233
+// and 147, of 1024 in 26 and 20 (a group of 128 in the form above: 13 and 11).
 template <typename T, int CODE>
 __global__ __launch_bounds__(AGPU_BLOCK) void put_group_kernel(QuantCol c, QuantShape q, RowAddr addr, uint64_t n_groups, uint32_t* flags) {
   const uint32_t lane = threadIdx.x & 63;
@@ -325,6 +332,7 @@ agpu_status check_columns(int32_t n_cols, const agpu_quantised_rows* stores, con
     AGPU_REQUIRE(s.group > 0 && s.group <= 65536 && s.dim % s.group == 0, AGPU_ERR_SHAPE, "group divides dim, 1 <= group <= 65536");
     AGPU_REQUIRE(s.code != AGPU_CODE_I4 || s.group % 2 == 0, AGPU_ERR_SHAPE, "4-bit codes: an even group");
     AGPU_REQUIRE(s.n_slots <= (1ull << 32), AGPU_ERR_SHAPE, "n_slots <= 2^32");
+    AGPU_REQUIRE(n * s.heads * s.dim < (1ull << 48), AGPU_ERR_SHAPE, "less than 2^48 values a column");
     AGPU_REQUIRE(r.data && s.codes && s.scales, AGPU_ERR_ARG, "null pointer");
     AGPU_REQUIRE(aligned_to(r.data, r.type == AGPU_ROW_F32 ? 4 : 2) && aligned_to(s.scales, 4), AGPU_ERR_SHAPE, "alignment");
     if (writes_rows) {
@@ -351,6 +359,7 @@ FastShape fast_shape(const QuantShape& q, uint64_t n, uint32_t n_cols) {
   uint64_t rows = 8 * AGPU_BLOCK / row_lanes;
   if (rows * 2048 > n * n_cols) rows = n * n_cols / 2048;
   if (rows * row_lanes < AGPU_BLOCK) rows = AGPU_BLOCK / row_lanes;
+  if (rows < n >> 23) rows = (n + (1u << 23) - 1) >> 23;  // a launch has less than 2^32 threads
   f.rows = (uint32_t)(rows < 1 ? 1 : rows > MAX_ROWS ? MAX_ROWS : rows);
   f.by_row = divide_by(q.groups_per_row), f.by_head = divide_by(q.groups_per_head);
   return f;
@@ -441,7 +450,7 @@ agpu_status quantised_pages(agpu_pipeline* p, bool put, int32_t n_cols, const ag
 
 // ---------------------------------------------------------------- take_rows
 // A copy with one indirection: lanes run over the states' accesses of V bytes in the order of the destination, two of a lane in flight, all states in
-// one launch (blockIdx.y).
+// one launch (blockIdx.y).  Bound by memory where V is 16 bytes: 904 MB in 144 us, 6.3 TB/s, a copy's rate; 4 bytes 3.1 TB/s, single bytes 1.2.
 constexpr int MAX_STATES = 8, ROWS_UNROLL = 2;
 struct State {
   const char* src;

@@ -54,6 +54,9 @@ class RowsGPU:
         self.data, self.gpu_device, self.type, self.shape, self.strides = data, gpu_device, type_, shape, strides
         self.item_size = ITEM_SIZE[type_]
         self.ptr = data.ptr if ptr is None else ptr
+        end = (self.ptr - data.ptr) + (1 + sum((n - 1) * s for n, s in zip(shape, strides))) * self.item_size if 0 not in shape else 0
+        if data._owned and (self.ptr < data.ptr or end > data.nbytes):  # (of memory that is not the library's, the caller knows the extent)
+            raise shape_error(f"rows {shape} with strides {strides} in a buffer of {data.nbytes} bytes")
         self._rows = self._pieces = None
 
     # -- construction
@@ -151,6 +154,9 @@ class QuantisedRowsGPU:
             raise capi.OperationNotSupported(f"codes of {code}")
         if heads < 1 or dim < 1 or group < 1 or dim % group or (code == "i4" and group % 2):
             raise shape_error(f"group {group} of {code} codes in rows of {heads} x {dim}")
+        need = self.bytes_of(n_slots, heads, dim, group, code)
+        if (codes._owned and codes.nbytes < need[0]) or (scales._owned and scales.nbytes < need[1]):
+            raise shape_error(f"{n_slots} rows of {heads} x {dim} need {need} bytes, not {codes.nbytes, scales.nbytes}")
         self.codes, self.scales, self.gpu_device = codes, scales, gpu_device
         self.n_slots, self.heads, self.dim, self.group, self.code = n_slots, heads, dim, group, code
         self.shape = (heads, dim)  # of a row

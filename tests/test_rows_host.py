@@ -170,6 +170,21 @@ def test_select_beams_arguments():
     assert status("agpu_select_beams_workspace", 2, 4, 1000, 8, None)[0] == capi.ERR_ARG
 
 
+def test_the_largest_calls():
+    """what a launch's threads and 31-bit counts bound is refused, what the documentation allows is not"""
+    n = C.c_uint64(0)
+    workspace = lambda batch, beams, vocab, k: status("agpu_select_beams_workspace", batch, beams, vocab, k, C.byref(n))[0]  # noqa: E731
+    for batch, beams, vocab, k in ((1, 1, (1 << 31) - 1, 64), (127, 1, (1 << 31) - 1, 1), (1, 64, (1 << 31) - 1, 64), (1 << 14, 1023, 8191, 64), (1, 1024, 1 << 26, 64),
+                                   (1 << 14, 1023, 1, 1), ((1 << 24) - 1, 1, 1 << 14, 64)):
+        assert batch * beams * vocab < 1 << 38 and beams * k * vocab < 1 << 43
+        assert workspace(batch, beams, vocab, k) == 0 and n.value > 0, (batch, beams, vocab, k)
+    for batch, beams, vocab, k in ((1, 1024, (1 << 31) - 1, 64), (1 << 13, 1, (1 << 31) - 1, 1), (1 << 23, 1, 1 << 20, 1)):
+        assert workspace(batch, beams, vocab, k) == capi.ERR_SHAPE, (batch, beams, vocab, k)
+    s, r = store(heads=1 << 13, dim=1 << 6, group=64), rows(row_stride=1 << 19)
+    assert NO_PIPELINE[1] in status("agpu_put_quantised", None, 1, C.byref(s), C.byref(r), 1 << 23, 1 << 28)[1]
+    assert "2^48" in status("agpu_put_quantised", None, 1, C.byref(s), C.byref(r), 1 << 23, 1 << 29)[1]
+
+
 # ---------------------------------------------------------------------------------------------------------- the Python host
 class _Device:
     ordinal = 0
@@ -204,6 +219,21 @@ def test_the_python_host_packs_the_structs_as_the_header_has_them():
     assert ag.RowsGPU(buf(1), dev, (3, 5, 4), "f16").as_pieces() == (40, 0, 1, 40, 8)     # one piece
     assert ag.RowsGPU(buf(1), dev, (3, 5, 4), "f16", (50, 8, 1)).as_pieces() == (100, 16, 5, 8, 0)
     assert ag.RowsGPU(buf(1), dev, (3, 7), "u8").as_pieces() == (7, 0, 1, 7, 0)
+
+
+def test_rows_past_their_buffer_are_refused():
+    ag, dev, _, _ = _host()
+    dev._handle = None
+    own = lambda n: ag.DeviceBuffer(dev, 4096, n)  # noqa: E731
+    for make in (lambda n: ag.RowsGPU(own(n), dev, (3, 2, 8), "bf16", (40, 16, 1), 4100), lambda n: ag.QuantisedRowsGPU(own(n - 132), own(80), dev, 5, 2, 8, 4, "i8"),
+                 lambda n: ag.QuantisedRowsGPU(own(80), own(n - 132), dev, 5, 2, 8, 4, "i8")):
+        make(4 + 2 * (2 * 40 + 16 + 8))
+        with pytest.raises(ag.ArrowErrorGPU) as e:
+            make(4 + 2 * (2 * 40 + 16 + 8) - 1)
+        assert e.value.status == capi.ERR_SHAPE
+    with pytest.raises(ag.ArrowErrorGPU):
+        ag.RowsGPU(own(4096), dev, (3, 8), "f32", None, 4092)
+    ag.RowsGPU(own(1), dev, (0, 8), "f32")
 
 
 def test_python_refusals():
