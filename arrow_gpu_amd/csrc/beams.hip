@@ -35,7 +35,7 @@ struct BeamArgs {
   uint32_t* out_tokens;
   uint32_t segs;
 };
-// a segment's part of its row: sum = Σ exp(x − ref), NaN where it holds a NaN or +infinity, 0 where nothing is above −infinity
+// a segment's part of its row: sum = Σ exp(x − ref), ref its maximum; NaN where it holds a NaN or +infinity, 0 where nothing is above −infinity
 struct SegSum {
   double sum, ref;
 };
@@ -89,7 +89,10 @@ __device__ __forceinline__ uint32_t lanes_below(uint64_t who) { return __builtin
 
 // ---------------------------------------------------------------- a segment
 template <typename T> struct Raw;  // low: bits of an order that are equal in all values of the type of one sign
+typedef uint32_t u32x4_at_4 __attribute__((ext_vector_type(4), aligned(4)));
+typedef uint32_t u32x4_at_2 __attribute__((ext_vector_type(4), aligned(2)));
 template <> struct Raw<float> {
+  typedef u32x4_at_4 Vector;  // 16 bytes from any element on
   static constexpr int low = 0;
   static __device__ __forceinline__ float at(u32x4 w, int i) {
     const uint32_t b = w[i];  // (a bit cast of w[i] itself takes element 0)
@@ -97,10 +100,12 @@ template <> struct Raw<float> {
   }
 };
 template <> struct Raw<f16_t> {
+  typedef u32x4_at_2 Vector;
   static constexpr int low = 13;
   static __device__ __forceinline__ float at(u32x4 w, int i) { return (float)__builtin_bit_cast(f16_t, (uint16_t)(w[i / 2] >> (i & 1) * 16)); }
 };
 template <> struct Raw<bf16_t> {
+  typedef u32x4_at_2 Vector;
   static constexpr int low = 16;
   static __device__ __forceinline__ float at(u32x4 w, int i) { return __builtin_bit_cast(float, (i & 1) ? w[i / 2] & 0xFFFF0000u : w[i / 2] << 16); }
 };
@@ -115,38 +120,39 @@ constexpr int LIST = 512;   // tokens it can keep; of logits in no order about 3
 template <typename T, bool MASK>
 struct Segment {
   static constexpr int VE = 16 / sizeof(T), U = TILE / 64 / VE;
+  typedef typename Raw<T>::Vector Vector;
   const T* x;           // the row
   const uint8_t* bits;  // its allowed tokens
-  uint32_t vocab, lead, lane;
+  uint32_t vocab, lane;
 
-  // first token of vector u of tile t: vectors lie on 16 bytes, the row starts `lead` elements into its first
-  __device__ __forceinline__ int64_t token(uint32_t t, int u) const { return (int64_t)t * TILE + u * (64 * VE) + lane * VE - lead; }
+  // first token of vector u of tile t: counted from the row's start, wherever in memory that is — so a row's sum depends on its logits only, and equal
+  // rows have equal scores (the loads may start at any element)
+  __device__ __forceinline__ uint32_t token(uint32_t t, int u) const { return t * TILE + u * (64 * VE) + lane * VE; }
   // whether all of a tile are the row's (the same in all lanes)
-  __device__ __forceinline__ bool whole(uint32_t t) const { return (uint64_t)t * TILE >= lead && (uint64_t)(t + 1) * TILE <= (uint64_t)vocab + lead; }
+  __device__ __forceinline__ bool whole(uint32_t t) const { return (t + 1) * TILE <= vocab; }
 
   // m: bit i: element i of the vector counts
   __device__ __forceinline__ void load(uint32_t t, u32x4 (&w)[U], uint32_t (&m)[U]) const {
     if (whole(t)) {
-      const u32x4* at = reinterpret_cast<const u32x4*>(x - lead) + (uint64_t)t * (TILE / VE) + lane;
+      const T* at = x + (uint64_t)t * TILE + lane * VE;
 #pragma unroll
-      for (int u = 0; u < U; u++) w[u] = at[u * 64];
-    } else {  // the row's ends: whole vectors, and the two that the row does not fill value by value, all on their way at once
+      for (int u = 0; u < U; u++) w[u] = *reinterpret_cast<const Vector*>(at + u * (64 * VE));
+    } else {  // the row's end: whole vectors, and the one that it does not fill value by value, all on their way at once
 #pragma unroll
       for (int u = 0; u < U; u++) {
-        const int64_t at = token(t, u);
+        const uint32_t at = token(t, u);
         m[u] = 0;
         w[u] = u32x4{0, 0, 0, 0};
-        if (at >= 0 && at + VE <= vocab) w[u] = *reinterpret_cast<const u32x4*>(x + at), m[u] = (1u << VE) - 1;
+        if (at + VE <= vocab) w[u] = *reinterpret_cast<const Vector*>(x + at), m[u] = (1u << VE) - 1;
       }
 #pragma unroll
       for (int u = 0; u < U; u++) {
-        const int64_t at = token(t, u);
-        if (m[u] == 0 && at + VE > 0 && at < vocab) {
+        const uint32_t at = token(t, u);
+        if (at < vocab && at + VE > vocab) {
           T e[VE];
 #pragma unroll
-          for (int i = 0; i < VE; i++) e[i] = x[at + i < 0 ? 0 : at + i < vocab ? at + i : vocab - 1];
-#pragma unroll
-          for (int i = 0; i < VE; i++) m[u] |= (uint32_t)(at + i >= 0 && at + i < vocab) << i;
+          for (int i = 0; i < VE; i++) e[i] = x[at + i < vocab ? at + i : vocab - 1];
+          m[u] = (1u << (vocab - at)) - 1;
           w[u] = __builtin_bit_cast(u32x4, e);
         }
       }
@@ -154,12 +160,7 @@ struct Segment {
     if (MASK) {
 #pragma unroll
       for (int u = 0; u < U; u++) {
-        const int64_t at = token(t, u);
-        uint32_t b = 0;
-        if (at + VE > 0 && at < vocab) {
-          const uint32_t first = at < 0 ? 0u : (uint32_t)at, byte = first >> 3, last = (vocab - 1) >> 3;
-          b = (bits[byte] | (uint32_t)bits[byte < last ? byte + 1 : last] << 8) >> (first & 7) << (at < 0 ? -at : 0);
-        }
+        const uint32_t at = token(t, u), b = at < vocab ? bits[at >> 3] >> (at & 7) : 0u;
         m[u] = whole(t) ? b : m[u] & b;
       }
     }
@@ -193,23 +194,22 @@ __device__ __forceinline__ float maximum_of(float a, float b, float c) {
 }
 
 template <typename T, bool MASK>
-__global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, uint32_t tiles, uint32_t n_segs, SegSum* sums, Entry* entries) {
+__global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, uint32_t tiles, uint32_t row_blocks, SegSum* sums, Entry* entries) {
   typedef Segment<T, MASK> S;
   constexpr int VE = S::VE, U = S::U, EPT = U * VE;
   __shared__ uint64_t lists[AGPU_BLOCK / 64][LIST + RANKED];
   __shared__ float tops[AGPU_BLOCK / 64][2][64];
-  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), id = blockIdx.x * (AGPU_BLOCK / 64) + wave, lane = threadIdx.x & 63;
-  const uint32_t row = (id < n_segs ? id : n_segs - 1) / a.segs, seg = id - row * a.segs;
-  const bool idle = id >= n_segs || is_finished(a, row);  // (it keeps the others company at the barriers)
+  const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6, lane = threadIdx.x & 63;
+  const uint32_t row = blockIdx.x / row_blocks, seg = (blockIdx.x - row * row_blocks) * waves + wave, id = row * a.segs + seg;
+  const bool idle = seg >= a.segs || is_finished(a, row);  // (it keeps the others company at the barriers)
   uint64_t* list = lists[wave];
 
   S s;
   s.x = static_cast<const T*>(a.logits) + row * a.row_stride;
   s.bits = MASK ? a.allowed + row * a.allowed_stride : nullptr;
   s.vocab = a.vocab;
-  s.lead = (uint32_t)(reinterpret_cast<uintptr_t>(s.x) & 15) / sizeof(T);
   s.lane = lane;
-  const uint32_t t0 = seg * tiles, row_tiles = (uint32_t)(((uint64_t)a.vocab + s.lead + TILE - 1) / TILE), t1 = idle ? t0 : t0 + tiles < row_tiles ? t0 + tiles : row_tiles;
+  const uint32_t t0 = seg * tiles, row_tiles = (a.vocab + TILE - 1) / TILE, t1 = idle ? t0 : t0 + tiles < row_tiles ? t0 + tiles : row_tiles;
 
   float top[2] = {LOWEST, LOWEST};  // the largest of the lane's first and second eight logits of every tile
   float floor_v = LOWEST, above = -0x1.fffffep127f, ref_v = 0.0f, k = MAGIC, least = 0.0f;
@@ -249,18 +249,17 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
         least = ref_v - 80.0f;
       }
     }
-    // The floor, after tiles 0 and 2: a value that k logits of the row reach, among the maxima of all the waves that share it
+    // The floor, after tiles 0 and 2: a value that k logits of the row reach, among the maxima of the block's waves, all of one row
     if (step == 0 || step == 2) {
       tops[wave][0][lane] = top[0], tops[wave][1][lane] = top[1];
       __syncthreads();
       float two[2] = {top[0], top[1]};  // the lane's largest two of them
       if (two[1] > two[0]) two[0] = top[1], two[1] = top[0];
-      for (uint32_t o = 1; o < AGPU_BLOCK / 64; o++) {
-        const uint32_t other = (wave + o) % (AGPU_BLOCK / 64);
-        if ((blockIdx.x * (AGPU_BLOCK / 64) + other) / a.segs != row) continue;
+      for (uint32_t o = 0; o < waves; o++) {  // (an idle wave's are −infinity)
+        if (o == wave) continue;
 #pragma unroll
         for (int h = 0; h < 2; h++) {
-          const float x = tops[other][h][lane], low = fminf(x, two[0]);
+          const float x = tops[o][h][lane], low = fminf(x, two[0]);
           two[0] = fmaxf(x, two[0]), two[1] = fmaxf(two[1], low);
         }
       }
@@ -304,7 +303,6 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
 
   float most = fmaxf(top[0], top[1]);
   for (int d = 32; d; d >>= 1) most = fmaxf(most, __shfl_xor(most, d));
-  double ref = (double)(MAGIC - k) * LN2;
   // the logits that reached a floor, one of each lane at a time (read again: the lane's registers cannot be indexed): their terms, and into the list
   // what reaches the last floor
   if (idle) return;
@@ -315,8 +313,9 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
   const bool many = all > HITS, again = most > LOWEST && most < __builtin_inff() && (many || __builtin_fabsf(most - ref_v) > APART);
   u32x4 w[U];
   uint32_t m[U];
-  if (again) {  // in f64, below the maximum that is now known
-    ref = most;
+  const double ref = most;  // (a lone token's term is then exactly 1, its log-sum the logit)
+  if (most > LOWEST && !again) sum *= exp((double)(MAGIC - k) * LN2 - ref);
+  if (again) {  // in f64
     sum = 0.0;
     for (uint32_t t = t0; t < t1; t++) {
       float v[EPT];
@@ -336,7 +335,7 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
       uint32_t token = 0;
       if (h) {
         const uint32_t bit = word * 32 + __builtin_ctz(h), t = t0 + bit / EPT, i = bit % EPT;
-        token = t * TILE + i / VE * (64 * VE) + lane * VE + i % VE - s.lead;
+        token = t * TILE + i / VE * (64 * VE) + lane * VE + i % VE;
         y = (float)s.x[token];
         if (!again) sum += exp((double)y - ref);
       }
@@ -596,28 +595,32 @@ __global__ __launch_bounds__(MERGE_BLOCK) void beam_merge_kernel(BeamArgs a, Div
 // not depend on it.)
 uint32_t segment_tiles(uint64_t rows, uint64_t vocab) {
   uint32_t t = MOST_TILES;
-  while (t > 1 && rows * ((vocab + 7 + t * TILE - 1) / (t * TILE)) < 4096) t /= 2;
+  while (t > 1 && rows * ((vocab + t * TILE - 1) / (t * TILE)) < 4096) t /= 2;
   return t;
 }
 uint32_t segments(uint64_t rows, uint64_t vocab) {
   const uint64_t e = (uint64_t)segment_tiles(rows, vocab) * TILE;
-  return (uint32_t)((vocab + 7 + e - 1) / e);  // + 7: a row may start anywhere in a vector
+  return (uint32_t)((vocab + e - 1) / e);
 }
+// a block's waves are a row's
+uint32_t block_waves(uint32_t segs) { return segs < AGPU_BLOCK / 64 ? segs : AGPU_BLOCK / 64; }
+uint32_t row_blocks(uint32_t segs) { return (segs + block_waves(segs) - 1) / block_waves(segs); }
 
 bool workspace_bytes(uint64_t batch, uint64_t beams, uint64_t vocab, uint64_t k, uint64_t* out) {
   if (batch == 0 || beams == 0 || vocab == 0 || k == 0 || k > 64 || beams > 1024 || k > beams * vocab || batch * beams >= (1u << 24) || vocab >= (1ull << 31)) return false;
   const uint64_t segs = segments(batch * beams, vocab);
-  if (beams * segs * k >= (1ull << 31) || batch * beams * segs > (1ull << 26) - 4) return false;  // a request's entries; the grid's threads, 2^32
+  if (beams * segs * k >= (1ull << 31)) return false;                                                                            // a request's entries
+  if (batch * beams * row_blocks((uint32_t)segs) * block_waves((uint32_t)segs) >= (1ull << 26)) return false;  // the grid's threads, 2^32
   *out = batch * beams * segs * (sizeof(SegSum) + k * sizeof(Entry));
   return true;
 }
 
 template <typename T>
 void launch_segments(agpu_pipeline* p, const BeamArgs& a, SegSum* sums, Entry* entries) {
-  const uint32_t rows = a.batch * a.beams, n = rows * a.segs, tiles = segment_tiles(rows, a.vocab);
-  const dim3 grid((n + AGPU_BLOCK / 64 - 1) / (AGPU_BLOCK / 64));
-  if (a.allowed) hipLaunchKernelGGL((beam_segment_kernel<T, true>), grid, dim3(AGPU_BLOCK), 0, p->stream, a, tiles, n, sums, entries);
-  else hipLaunchKernelGGL((beam_segment_kernel<T, false>), grid, dim3(AGPU_BLOCK), 0, p->stream, a, tiles, n, sums, entries);
+  const uint32_t rows = a.batch * a.beams, tiles = segment_tiles(rows, a.vocab), blocks = row_blocks(a.segs);
+  const dim3 grid(rows * blocks), block(64 * block_waves(a.segs));
+  if (a.allowed) hipLaunchKernelGGL((beam_segment_kernel<T, true>), grid, block, 0, p->stream, a, tiles, blocks, sums, entries);
+  else hipLaunchKernelGGL((beam_segment_kernel<T, false>), grid, block, 0, p->stream, a, tiles, blocks, sums, entries);
 }
 
 }  // namespace

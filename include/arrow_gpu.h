@@ -601,8 +601,10 @@ agpu_status agpu_take_rows(agpu_pipeline* p, int32_t n_states, const agpu_state*
 
 /* Beam search's selection.  logits: [batch * beams, vocab] of an agpu_row_type, row_stride elements apart (0: one row for all).  For row r of request b
  *   score(r, v) = scores[r] + logits[r, v] - log sum_u exp(logits[r, u]),   u over the row's allowed tokens,
- * compared in 64 bits (the log-sum's error is below 4e-7, of a row of many different logits about 1e-9), and the k largest of the request's beams * vocab scores go to out_scores / out_parents / out_tokens [batch, k], largest first; parents are
- * rows r (indices for agpu_take_rows).  Equal scores: the lower row, then the higher logit, then the lower token.  scores NULL: 0.
+ * compared in 64 bits (the log-sum's error is below 4e-7, of a row of many different logits about 1e-9; it depends on the row's
+ * allowed logits only: equal rows have equal scores, and a row with one live token keeps scores[r]), and the k largest of the request's beams * vocab
+ * scores go to out_scores / out_parents / out_tokens [batch, k], largest first; parents are rows r (indices for agpu_take_rows).  Equal scores: the
+ * lower row, then the higher logit, then the lower token.  scores NULL: 0.
  * allowed: per row a bitmap of vocab bits, allowed_stride bytes apart (a multiple of 8, 0: one bitmap for all rows), NULL: every token.  What the
  * logits of other tokens hold does not matter.  finished: a bitmap of batch * beams rows; a finished row has one candidate, (end_token,
  * scores[r]), its logits are not read.  A row with a NaN or +infinity among its allowed logits, or with none above -infinity, and a row whose

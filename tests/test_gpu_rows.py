@@ -592,6 +592,52 @@ def test_select_rows_of_one_row(dev, p):
     assert_selection(sel, R.select(np.repeat(x, 6, 0).astype(np.float64), 3, 9, cum))
 
 
+@pytest.mark.parametrize("vocab,pitch", [(5001, 5003), (999, 1000), (50257, 50257), (13, 17), (70001, 70016)])
+@pytest.mark.parametrize("kind", KINDS)
+def test_select_equal_rows_have_equal_scores(dev, p, kind, vocab, pitch):
+    """wherever in memory the rows begin: of equal scores the lower row's comes first"""
+    import arrow_gpu_amd as ag
+
+    rng = np.random.default_rng(vocab)
+    beams, k = 7, 12
+    x = np.repeat(logits(rng, 2, vocab, kind), beams, 0)
+    wide = np.zeros((2 * beams, pitch), np.float32)
+    wide[:, :vocab] = x
+    base = up(wide, kind, dev)
+    view = ag.RowsGPU(base.data, dev, (2 * beams, vocab), kind, (pitch, 1))
+    allowed = np.tile(rng.random((1, (vocab + 63) // 64 * 64)) < 0.6, (2 * beams, 1))
+    for mask in (None, allowed):
+        sel = ag.select_beams_op(view, beams, k, p, allowed=bits(mask, dev) if mask is not None else None)
+        p.sync()
+        want = R.select(x.astype(np.float64), beams, k, allowed=mask[:, :vocab] if mask is not None else None)
+        assert want[1][0, :beams].tolist() == list(range(beams))
+        assert_selection(sel, want)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_select_forced_tokens_keep_the_scores(dev, p, kind):
+    """rows whose mask leaves one token: its log-softmax is 0, the running score stays what it was"""
+    import arrow_gpu_amd as ag
+
+    rng = np.random.default_rng(4)
+    beams, vocab, k = 6, 30011, 6
+    x = logits(rng, 2 * beams, vocab, kind)
+    allowed = np.zeros((2 * beams, (vocab + 63) // 64 * 64), bool)
+    only = rng.integers(0, vocab, 2 * beams)
+    allowed[np.arange(2 * beams), only] = True
+    cum = np.repeat(-np.float32(3) * rng.random(4).astype(np.float32), 3)
+    sel = ag.select_beams_op(up(x, kind, dev), beams, k, p, scores=ag.Float32ArrayGPU.from_slice(cum, dev), allowed=bits(allowed, dev))
+    x[~allowed[:, :vocab]] = -np.inf
+    bare = ag.select_beams_op(up(x, kind, dev), beams, k, p)
+    p.sync()
+    s, r, t = sel.values()
+    for b in range(2):
+        order = np.argsort(-cum[b * beams:(b + 1) * beams], kind="stable") + b * beams
+        assert np.array_equal(s[b], cum[order]) and np.array_equal(r[b], order) and np.array_equal(t[b], only[order])
+    s, r, t = bare.values()
+    assert not s.any() and np.array_equal(r.reshape(-1), np.arange(2 * beams)) and np.array_equal(t.reshape(-1), only)
+
+
 def test_select_scores_at_the_ends(dev, p):
     """the first step (one live beam), NaN and infinite running scores, also of finished rows"""
     import arrow_gpu_amd as ag
