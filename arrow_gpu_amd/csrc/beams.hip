@@ -5,9 +5,9 @@
 // No wave needs the maximum first: exp is taken relative to the first tile's, and f32 holds it as long as
 // a segment's maximum is within 60 of that; a segment of another kind is read again.
 //
-// 256 rows x 128256 bf16, 8 beams, k 16: segments 22.5 us (66 MB: 2.9 TB/s), join 6.0.  The segments are bound by their instructions, not by memory — the
+// 256 rows x 128256 bf16, 8 beams, k 16: segments 21.7 us (66 MB: 3.0 TB/s), join 5.8.  The segments are bound by their instructions, not by memory — the
 // loads alone take 12.6 us: about 12 a logit, of which the term's exp are 6 and the pair sums, the clamp, the unpacking and the maxima 3.5; the floors
-// and the hits' exact terms are the rest.  One request (4 x 32000): 5.8 + 5.0 us, launches and latency.
+// and the hits' exact terms are the rest.  One request (4 x 32000): 5.8 + 4.7 us, launches and latency.
 //
 // Precision.  The result is whole numbers, and rows that compete differ by their log-sums only: a log-sum 1e-7 off swaps tokens of two beams.  Scores are
 // compared in f64.  Of the sum, the terms of the tokens that reach the floor — at least the 16 largest of a row, the bulk where it is sharp — are taken in
