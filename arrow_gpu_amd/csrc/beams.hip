@@ -656,6 +656,13 @@ agpu_status agpu_select_beams(agpu_pipeline* p, const agpu_beams* args) {
   AGPU_REQUIRE(aligned_to(b.logits, b.type == AGPU_ROW_F32 ? 4 : 2) && aligned_to(b.scores, 4) && aligned_to(b.allowed, 8) && aligned_to(b.finished, 8) &&
                    aligned_to(b.out_scores, 4) && aligned_to(b.out_parents, 4) && aligned_to(b.out_tokens, 4) && aligned16(b.workspace),
                AGPU_ERR_SHAPE, "alignment");
+  // a request's block writes while another's still reads: results do not go where scores come from
+  const uint64_t found = 4ull * b.batch * b.k, rows = (uint64_t)b.batch * b.beams;
+  for (const void* out : {(const void*)b.out_scores, (const void*)b.out_parents, (const void*)b.out_tokens}) {
+    const uintptr_t o = reinterpret_cast<uintptr_t>(out), s = reinterpret_cast<uintptr_t>(b.scores), w = reinterpret_cast<uintptr_t>(b.workspace);
+    AGPU_REQUIRE(!b.scores || o + found <= s || s + 4 * rows <= o, AGPU_ERR_ARG, "an output overlaps the scores");
+    AGPU_REQUIRE(o + found <= w || w + need <= o, AGPU_ERR_ARG, "an output overlaps the workspace");
+  }
   AGPU_BIND(p);
   const BeamArgs a = {b.logits, b.row_stride, b.batch, b.beams, b.vocab, b.k, b.end_token, b.scores, static_cast<const uint8_t*>(b.allowed), b.allowed_stride,
                       static_cast<const uint64_t*>(b.finished), b.out_scores, b.out_parents, b.out_tokens, segments((uint64_t)b.batch * b.beams, b.vocab)};

@@ -272,6 +272,29 @@ def test_pages(dev, p, code, dim, group, page):
     assert_values(again.values()[some], R.values(want_codes, want_scales, code, group), "f32")
 
 
+@pytest.mark.parametrize("code,dim,group", [("i8", 64, 32), ("i4", 96, 96), ("e4m3", 12, 6)])
+def test_a_slot_named_twice(dev, p, code, dim, group):
+    """what the slot holds then may come from either row, group by group or mixed; the other slots are right"""
+    import arrow_gpu_amd as ag
+
+    rng = np.random.default_rng(31)
+    n, heads = 300, 3
+    x = activations(rng, (n, heads, dim), "f32")
+    slots = rng.permutation(n + 20)[:n]
+    slots[200:260] = slots[7]
+    store = ag.QuantisedRowsGPU.empty(n + 20, heads, dim, dev, code=code, group=group)
+    ag.put_quantised_op(store, up(x, "f32", dev), u32(slots, dev), p)
+    p.sync()
+    codes, scales = stored(store, dev)
+    want_codes, want_scales = R.quantise(x, code, group)
+    once = np.array([s != slots[7] for s in slots])
+    assert np.array_equal(scales[slots[once]].view(np.uint32), want_scales[once].view(np.uint32))
+    assert_codes(codes[slots[once]], want_codes[once], code, want_scales[once])
+    left = np.setdiff1d(np.arange(n + 20), slots)
+    assert not codes[left].any() and not scales[left].any()
+    assert np.isin(scales[slots[7]].reshape(heads, -1), want_scales[~once].reshape(61, heads, -1)).all()
+
+
 def test_pages_out_of_range(dev, p):
     import arrow_gpu_amd as ag
 

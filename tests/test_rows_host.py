@@ -164,6 +164,14 @@ def test_select_beams_arguments():
                dict(scores=(1 << 21) + 1), dict(allowed=(1 << 22) + 4), dict(finished=(1 << 23) + 4), dict(out_scores=(1 << 24) + 2), dict(out_tokens=(1 << 26) + 2),
                dict(workspace=(1 << 27) + 8)):
         assert beams(**kw)[0] == capi.ERR_SHAPE, kw
+    # 2 x 8 results of 4 bytes, 8 scores: where the last step's scores are, on the workspace, and just beside both
+    for out in ("out_scores", "out_parents", "out_tokens"):
+        for at in ((1 << 21), (1 << 21) + 28, (1 << 21) - 60):
+            assert "scores" in beams(**{out: at})[1]
+        assert "workspace" in beams(**{out: (1 << 27) + 64})[1] and "workspace" in beams(**{out: (1 << 27) - 60})[1]
+        for at in ((1 << 21) + 32, (1 << 21) - 64, (1 << 27) - 64):
+            assert NO_PIPELINE[1] in beams(**{out: at})[1]
+        assert NO_PIPELINE[1] in beams(**{out: 1 << 21, "scores": 0})[1]
     n = C.c_uint64(1)
     assert status("agpu_select_beams_workspace", 0, 0, 0, 0, C.byref(n))[0] == 0 and n.value == 0
     assert status("agpu_select_beams_workspace", 2, 4, 1000, 8, C.byref(n))[0] == 0 and n.value > 0
