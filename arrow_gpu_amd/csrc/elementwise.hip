@@ -241,10 +241,10 @@ struct UnPopc {  // countOneBits per element [logical/compute_shaders/u32/countb
 // ---- transcendental f32 functions.  log / sinh / pow below are evaluated in f64 and rounded ONCE to f32 (≤ 0.5 ULP + 2^-30);
 // the f32 device-library versions measure 2 ULP for sin / cos / log on gfx950 (profiles/r01_probe_first_contact.json).
 //
-// sin / cos: ALL in f32, two rows side by side (independent chains).  Rounds 1–5 evaluated the Cody–Waite reduction and the outer
-// polynomial step in f64 — 8 f64 operations + 4 conversions + 5 selects per row, ≈ 27 VALU instructions, which an 8 B/row
+// sin / cos: ALL in f32, two rows side by side (independent chains).  With the Cody–Waite reduction and the outer polynomial step in
+// f64 it was 8 f64 operations + 4 conversions + 5 selects per row, ≈ 27 VALU instructions, which an 8 B/row
 // stream hides and a 5–6 B/row cast-headed chain does not (`cast i16 → f32 → sin` in one launch 0.65 of the roof, `cast(u16)·s
-// → sin` 0.54: VERDICT r5 weak #3).  The same function written as double-float f32 arithmetic over a PAIR of rows has no f64
+// → sin` 0.54).  The same function written as double-float f32 arithmetic over a PAIR of rows has no f64
 // operation and no conversion; the pair's two chains hide each other's latency.  (Packed f32 instructions are switched off in the build; with
 // them sin / cos took 1.18 / 1.20 ms for 1e9 rows, without 1.15 / 1.16, cast i16 → sin 0.976 and 0.922.)
 //   k  = round(x · 2/π) by the 1.5·2^23 trick (one fma; the low bits of the sum ARE k, no conversion), |k| < 2^20 for |x| < 1e6
@@ -656,7 +656,7 @@ template <> struct EwWaveLds<UnCos> { static constexpr unsigned value = AGPU_WAV
 template <> struct EwPrefetch<UnSin> { static constexpr bool value = true; static constexpr int tiles = 1; };
 template <> struct EwPrefetch<UnCos> { static constexpr bool value = true; static constexpr int tiles = 1; };
 template <> struct EwPrefetch<UnSinh> { static constexpr bool value = true; static constexpr int tiles = 1; };
-// log (round 6: f32, no table — the generic tile kernel instead of a kernel of its own).  One tile per block like the others: two were level
+// log (f32, no table — the generic tile kernel instead of a kernel of its own).  One tile per block like the others: two were level
 // or 1 % ahead in one process and 5 % behind in the next (0.84 / 0.79 — the by-process effect of R4.1 / R5.4), one tile is 0.83 everywhere
 template <> struct EwPrefetch<UnLog> { static constexpr bool value = true; static constexpr int tiles = 1; };
 template <> struct EwWaveLds<UnLog> { static constexpr unsigned value = AGPU_WAVE_LDS_24; };  // (tools/probe/r06_sincos_sweep.py: ≈ 24 waves 0.83–0.84, ≈ 16 0.77–0.78, no cap 0.79–0.83)
@@ -1367,7 +1367,7 @@ static agpu_status launch_cvt(agpu_pipeline* p, const void* in, void* out, uint6
         const uint64_t blocks = (nchunks + AGPU_CVTW_BLOCK / AGPU_WAVE - 1) / (AGPU_CVTW_BLOCK / AGPU_WAVE);
         const int grid = stream_grid_for(p, (blocks + k - 1) / k);
         // occupancy cap (common.hpp): ×2 casts to 32 bits ≈ 24 waves per CU, ×4 ≈ 16; u8 → u16 none (not measured to gain)
-        // (round 6: none for cast → sin / cos of a 16-bit column — with sin / cos in f32 the kernel wants all its waves: 0.79–0.80 against 0.75)
+        // (none for cast → sin / cos of a 16-bit column — with sin / cos in f32 the kernel wants all its waves: 0.79–0.80 against 0.75)
         constexpr unsigned cap = ConvHasRows<Conv>::value ? 0u : sizeof(TO) == 4 ? (sizeof(TI) == 2 ? AGPU_WAVE_LDS_24 : AGPU_WAVE_LDS_16) : 0u;
         const unsigned lds = cap ? wave_lds_for(p, cap, AGPU_CVTW_BLOCK / AGPU_WAVE) : 0u;
         // ×2 casts walk the chunks as two lock-step streams (common.hpp two_streams: u16 → f32 0.836 → 0.857, u8 → u16 0.80 → 0.83, sin_u16 0.78 → 0.79);
