@@ -64,17 +64,20 @@ struct FastShape {
   Divide by_row, by_head;                                      // groups a row, groups a head
 };
 
-typedef uint32_t u32x8 __attribute__((ext_vector_type(8)));
-template <typename T> struct Eight;  // eight values as they lie in memory
+// Vectors from any element (any byte of the codes) on
+template <typename T> struct Eight;
 template <> struct Eight<float> {
-  typedef float type __attribute__((ext_vector_type(8), aligned(16)));
+  typedef float type __attribute__((ext_vector_type(8), aligned(4)));
 };
 template <> struct Eight<f16_t> {
-  typedef f16_t type __attribute__((ext_vector_type(8)));
+  typedef f16_t type __attribute__((ext_vector_type(8), aligned(2)));
 };
 template <> struct Eight<bf16_t> {
-  typedef bf16_t type __attribute__((ext_vector_type(8)));
+  typedef bf16_t type __attribute__((ext_vector_type(8), aligned(2)));
 };
+typedef uint32_t u32_at_1 __attribute__((aligned(1)));
+typedef uint32_t u32x2_at_1 __attribute__((ext_vector_type(2), aligned(1)));
+typedef float f32x2_at_4 __attribute__((ext_vector_type(2), aligned(4)));
 
 template <int CTRL>
 __device__ __forceinline__ float moved(float x) {  // another lane's of the row of 16
@@ -92,50 +95,50 @@ __device__ __forceinline__ float over_group(float x, uint32_t lanes, F f) {
   return x;
 }
 
-// a row of the block: the number of its first group in the cache (ROW_NONE, ROW_BAD), and its values
-template <typename T>
+// a row of the block: the number of its first group in the cache (ROW_NONE, ROW_BAD), and where its values begin (from the column's: a pointer out of LDS
+// would be one into any memory, and its accesses the slower ones)
 struct BlockRow {
-  uint64_t at;
-  T* x;
+  uint64_t at, x;
 };
-template <typename T>
-__device__ __forceinline__ uint32_t block_rows(const QuantCol& c, const FastShape& q, const RowAddr& addr, uint64_t n, BlockRow<T>* held, uint32_t* flags) {
+__device__ __forceinline__ uint32_t block_rows(const QuantCol& c, const FastShape& q, const RowAddr& addr, uint64_t n, BlockRow* held, uint32_t* flags) {
   const uint64_t row0 = (uint64_t)blockIdx.x * q.rows;
   const uint32_t rows = (uint32_t)(n - row0 < q.rows ? n - row0 : q.rows);
   if (threadIdx.x < rows) {
     const uint64_t row = row0 + threadIdx.x, s = row_slot(addr, row, c.n_slots);
-    held[threadIdx.x] = {s < ROW_BAD ? s * q.groups_per_row : s, static_cast<T*>(c.x) + row * c.row_stride};
+    held[threadIdx.x] = {s < ROW_BAD ? s * q.groups_per_row : s, row * c.row_stride};
     if (s == ROW_BAD) *reinterpret_cast<volatile uint32_t*>(flags) = AGPU_FLAG_INDEX_RANGE;
   }
   __syncthreads();
   return rows;
 }
-// what a lane has at a time: eight values of one group, from value sub * 8 on
+// what a lane has at a time: eight values of one group, from value `from` on; the last lane of a group that is no multiple of 8 has the group's last eight
+// (some of its neighbour's too: they get the same codes)
 struct Unit {
-  uint32_t row, in_row, sub;
+  uint32_t row, in_row, from;
+  bool idle;  // past the group's end
 };
 __device__ __forceinline__ Unit unit_of(uint32_t i, const FastShape& q) {
-  const uint32_t g = i >> q.log_lanes, row = g / q.by_row;
-  return {row, g - row * q.groups_per_row, i & (q.lanes - 1)};
+  const uint32_t g = i >> q.log_lanes, row = g / q.by_row, from = (i & (q.lanes - 1)) * 8;
+  return {row, g - row * q.groups_per_row, from + 8 <= q.group ? from : q.group - 8, from >= q.group};
 }
 __device__ __forceinline__ uint64_t value_offset(const Unit& u, const QuantCol& c, const FastShape& q) {
-  if (q.dense) return u.in_row * q.group + u.sub * 8;
+  if (q.dense) return u.in_row * q.group + u.from;
   const uint32_t head = u.in_row / q.by_head;
-  return head * c.head_stride + (u.in_row - head * q.by_head.d) * q.group + u.sub * 8;
+  return head * c.head_stride + (u.in_row - head * q.by_head.d) * q.group + u.from;
 }
 
 template <typename T, int CODE>
 __global__ __launch_bounds__(AGPU_BLOCK) void put_eight_kernel(QuantCols cols, FastShape q, RowAddr addr, uint64_t n, uint32_t* flags) {
-  __shared__ BlockRow<const T> held[MAX_ROWS];
+  __shared__ BlockRow held[MAX_ROWS];
   const QuantCol& c = cols.c[blockIdx.y];  // (one load of a lane in flight: two or four do not pay, 18.2 -> 18.9 us)
-  const uint32_t total = (block_rows<const T>(c, q, addr, n, held, flags) * q.groups_per_row) << q.log_lanes;
+  const uint32_t total = (block_rows(c, q, addr, n, held, flags) * q.groups_per_row) << q.log_lanes;
   for (uint32_t i = threadIdx.x; i < total; i += AGPU_BLOCK) {
     const Unit t = unit_of(i, q);
-    const BlockRow<const T> row = held[t.row];
-    const bool live = t.sub * 8 < q.group && row.at < ROW_BAD;
+    const BlockRow row = held[t.row];
+    const bool live = !t.idle && row.at < ROW_BAD;
     float v[8] = {};
     if (live) {
-      const typename Eight<T>::type w = *reinterpret_cast<const typename Eight<T>::type*>(row.x + value_offset(t, c, q));
+      const typename Eight<T>::type w = *reinterpret_cast<const typename Eight<T>::type*>(static_cast<const T*>(c.x) + row.x + value_offset(t, c, q));
 #pragma unroll
       for (int j = 0; j < 8; j++) v[j] = (float)w[j];
     }
@@ -163,16 +166,15 @@ __global__ __launch_bounds__(AGPU_BLOCK) void put_eight_kernel(QuantCols cols, F
     const Factors f = factors<CODE>(span, lo, bad);
     if (!live) continue;
     const uint64_t at = row.at + t.in_row;
-    const uint32_t sub = t.sub;
     if (CODE == AGPU_CODE_I4) {
-      if (sub == 0) reinterpret_cast<float2*>(c.scales)[at] = {f.scale, f.lo};
+      if (t.from == 0) reinterpret_cast<f32x2_at_4*>(c.scales)[at] = f32x2_at_4{f.scale, f.lo};
       uint32_t w = 0;
 #pragma unroll
       for (int j = 0; j < 8; j++) w |= (whole(v[j] - f.lo, f.inv) & 15) << 4 * j;
-      *reinterpret_cast<uint32_t*>(c.codes + at * (q.group / 2) + sub * 4) = w;
+      *reinterpret_cast<u32_at_1*>(c.codes + at * (q.group / 2) + t.from / 2) = w;
     } else {
-      if (sub == 0) c.scales[at] = f.scale;
-      u32x2 w;
+      if (t.from == 0) c.scales[at] = f.scale;
+      u32x2_at_1 w;
 #pragma unroll
       for (int h = 0; h < 2; h++) {
         if (CODE == AGPU_CODE_I8) {
@@ -183,7 +185,7 @@ __global__ __launch_bounds__(AGPU_BLOCK) void put_eight_kernel(QuantCols cols, F
           w[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[4 * h + 2] * f.inv, v[4 * h + 3] * f.inv, low, true);
         }
       }
-      *reinterpret_cast<u32x2*>(c.codes + at * q.group + sub * 8) = w;
+      *reinterpret_cast<u32x2_at_1*>(c.codes + at * q.group + t.from) = w;
     }
   }
 }
@@ -192,37 +194,36 @@ constexpr int TAKE_UNROLL = 8;  // all of a block's passes in flight: 131072 row
 
 template <typename T, int CODE>
 __global__ __launch_bounds__(AGPU_BLOCK) void take_eight_kernel(QuantCols cols, FastShape q, RowAddr addr, uint64_t n, uint32_t* flags) {
-  __shared__ BlockRow<T> held[MAX_ROWS];
+  __shared__ BlockRow held[MAX_ROWS];
   const QuantCol& c = cols.c[blockIdx.y];
-  const uint32_t total = (block_rows<T>(c, q, addr, n, held, flags) * q.groups_per_row) << q.log_lanes;
+  const uint32_t total = (block_rows(c, q, addr, n, held, flags) * q.groups_per_row) << q.log_lanes;
   for (uint32_t i0 = threadIdx.x; i0 < total; i0 += AGPU_BLOCK * TAKE_UNROLL) {
-    T* to[TAKE_UNROLL];
+    uint64_t to[TAKE_UNROLL];  // from the column's first value
     u32x2 w[TAKE_UNROLL];
-    float2 f[TAKE_UNROLL];
+    f32x2_at_4 f[TAKE_UNROLL];
 #pragma unroll
     for (int u = 0; u < TAKE_UNROLL; u++) {
       const uint32_t i = i0 + u * AGPU_BLOCK;
-      to[u] = nullptr;
-      w[u] = u32x2{0, 0}, f[u] = float2{0.0f, 0.0f};  // out of range: zeros
+      to[u] = ROW_NONE;
+      w[u] = u32x2{0, 0}, f[u] = f32x2_at_4{0.0f, 0.0f};  // out of range: zeros
       const Unit t = unit_of(i, q);
-      if (i >= total || t.sub * 8 >= q.group) continue;
-      const BlockRow<T> row = held[t.row];
+      if (i >= total || t.idle) continue;
+      const BlockRow row = held[t.row];
       if (row.at == ROW_NONE) continue;
       to[u] = row.x + value_offset(t, c, q);
       if (row.at == ROW_BAD) continue;
       const uint64_t at = row.at + t.in_row;
-      const uint32_t sub = t.sub;
       if (CODE == AGPU_CODE_I4) {
-        f[u] = reinterpret_cast<const float2*>(c.scales)[at];
-        w[u].x = *reinterpret_cast<const uint32_t*>(c.codes + at * (q.group / 2) + sub * 4);
+        f[u] = reinterpret_cast<const f32x2_at_4*>(c.scales)[at];
+        w[u].x = *reinterpret_cast<const u32_at_1*>(c.codes + at * (q.group / 2) + t.from / 2);
       } else {
         f[u].x = c.scales[at];
-        w[u] = *reinterpret_cast<const u32x2*>(c.codes + at * q.group + sub * 8);
+        w[u] = *reinterpret_cast<const u32x2_at_1*>(c.codes + at * q.group + t.from);
       }
     }
 #pragma unroll
     for (int u = 0; u < TAKE_UNROLL; u++) {
-      if (!to[u]) continue;
+      if (to[u] == ROW_NONE) continue;
       typename Eight<T>::type o;
       if (CODE == AGPU_CODE_I4) {
         const uint32_t even = w[u].x & 0x0F0F0F0Fu, odd = w[u].x >> 4 & 0x0F0F0F0Fu;  // a byte each: the conversion takes them from where they are
@@ -245,20 +246,19 @@ __global__ __launch_bounds__(AGPU_BLOCK) void take_eight_kernel(QuantCols cols, 
         }
       }
       // past the caches: nobody reads the rows in this call (ragged e4m3 rows 30.5 us, through the caches 42)
-      __builtin_nontemporal_store(o, reinterpret_cast<typename Eight<T>::type*>(to[u]));
+      __builtin_nontemporal_store(o, reinterpret_cast<typename Eight<T>::type*>(static_cast<T*>(c.x) + to[u]));
     }
   }
 }
 
-// ---------------------------------------------------------------- one wave a group: any group, stride and alignment
-// What the lanes of the form above cannot share: groups that are no multiple of 8 or above 512, rows off their vectors' alignment.  Bound by its
-// instructions, narrow accesses and a slot's look-up for each group: 2^24 bf16 values in groups of 100 to 8 bits in 64 us, back in 42; groups of 20 in 233
-// and 147, of 1024 in 26 and 20 (a group of 128 in the form above: 13 and 11).
+// ---------------------------------------------------------------- a value a lane at a time: groups below 8 and above 512
+// A group is `lanes` neighbouring lanes, at most a wave.  Bound by its narrow accesses and a slot's look-up for each group: 2^24 bf16 values in groups of
+// 1024 go to 8 bits in 28 us and come back in 20 (of 512, in the form above: 13 and 11).
 template <typename T, int CODE>
-__global__ __launch_bounds__(AGPU_BLOCK) void put_group_kernel(QuantCol c, QuantShape q, RowAddr addr, uint64_t n_groups, uint32_t* flags) {
-  const uint32_t lane = threadIdx.x & 63;
-  const uint64_t waves = (uint64_t)gridDim.x * (AGPU_BLOCK / 64);
-  for (uint64_t g = (uint64_t)blockIdx.x * (AGPU_BLOCK / 64) + (threadIdx.x >> 6); g < n_groups; g += waves) {
+__global__ __launch_bounds__(AGPU_BLOCK) void put_group_kernel(QuantCol c, QuantShape q, RowAddr addr, uint64_t n_groups, uint32_t lanes, uint32_t* flags) {
+  const uint32_t lane = threadIdx.x % lanes, held = AGPU_BLOCK / lanes;
+  const uint64_t step = (uint64_t)gridDim.x * held;
+  for (uint64_t g = (uint64_t)blockIdx.x * held + threadIdx.x / lanes; g < n_groups; g += step) {  // (the lanes of a group go together)
     const uint64_t row = g / q.groups_per_row;
     const uint32_t in_row = (uint32_t)(g - row * q.groups_per_row), head = in_row / q.groups_per_head;
     const uint64_t slot = row_slot(addr, row, c.n_slots);
@@ -268,27 +268,27 @@ __global__ __launch_bounds__(AGPU_BLOCK) void put_group_kernel(QuantCol c, Quant
     }
     const T* x = static_cast<const T*>(c.x) + row * c.row_stride + head * c.head_stride + (in_row - head * q.groups_per_head) * q.group;
     float lo = __builtin_inff(), hi = -__builtin_inff();
-    bool bad = false;
-    for (uint32_t i = lane; i < q.group; i += 64) {
+    uint32_t bad = 0;
+    for (uint32_t i = lane; i < q.group; i += lanes) {
       const float v = (float)x[i];
       bad |= !(__builtin_fabsf(v) < __builtin_inff());
       lo = fminf(lo, v);
       hi = fmaxf(hi, v);
     }
-    for (int s = 32; s; s >>= 1) {
-      lo = fminf(lo, __shfl_xor(lo, s));
-      hi = fmaxf(hi, __shfl_xor(hi, s));
+    for (uint32_t d = lanes / 2; d; d >>= 1) {
+      lo = fminf(lo, __shfl_xor(lo, d));
+      hi = fmaxf(hi, __shfl_xor(hi, d));
+      bad |= __shfl_xor(bad, d);
     }
-    bad = __any(bad);
-    const Factors f = factors<CODE>(CODE == AGPU_CODE_I4 ? hi - lo : fmaxf(hi, -lo), lo, bad);
+    const Factors f = factors<CODE>(CODE == AGPU_CODE_I4 ? hi - lo : fmaxf(hi, -lo), lo, bad != 0);
     const uint64_t at = slot * q.groups_per_row + in_row;
     if (CODE == AGPU_CODE_I4) {
       if (lane == 0) c.scales[2 * at] = f.scale, c.scales[2 * at + 1] = f.lo;
-      for (uint32_t i = lane; i < q.group / 2; i += 64)
+      for (uint32_t i = lane; i < q.group / 2; i += lanes)
         c.codes[at * (q.group / 2) + i] = (uint8_t)((whole((float)x[2 * i] - f.lo, f.inv) & 15) | (whole((float)x[2 * i + 1] - f.lo, f.inv) & 15) << 4);
     } else {
       if (lane == 0) c.scales[at] = f.scale;
-      for (uint32_t i = lane; i < q.group; i += 64) {
+      for (uint32_t i = lane; i < q.group; i += lanes) {
         const float v = (float)x[i];
         c.codes[at * q.group + i] = CODE == AGPU_CODE_I8 ? (uint8_t)whole(v, f.inv)
                                                          : (uint8_t)__builtin_amdgcn_cvt_pk_fp8_f32(v * f.inv, 0.0f, 0, false);
@@ -298,10 +298,10 @@ __global__ __launch_bounds__(AGPU_BLOCK) void put_group_kernel(QuantCol c, Quant
 }
 
 template <typename T, int CODE>
-__global__ __launch_bounds__(AGPU_BLOCK) void take_group_kernel(QuantCol c, QuantShape q, RowAddr addr, uint64_t n_groups, uint32_t* flags) {
-  const uint32_t lane = threadIdx.x & 63;
-  const uint64_t waves = (uint64_t)gridDim.x * (AGPU_BLOCK / 64);
-  for (uint64_t g = (uint64_t)blockIdx.x * (AGPU_BLOCK / 64) + (threadIdx.x >> 6); g < n_groups; g += waves) {
+__global__ __launch_bounds__(AGPU_BLOCK) void take_group_kernel(QuantCol c, QuantShape q, RowAddr addr, uint64_t n_groups, uint32_t lanes, uint32_t* flags) {
+  const uint32_t lane = threadIdx.x % lanes, held = AGPU_BLOCK / lanes;
+  const uint64_t step = (uint64_t)gridDim.x * held;
+  for (uint64_t g = (uint64_t)blockIdx.x * held + threadIdx.x / lanes; g < n_groups; g += step) {
     const uint64_t row = g / q.groups_per_row;
     const uint32_t in_row = (uint32_t)(g - row * q.groups_per_row), head = in_row / q.groups_per_head;
     const uint64_t slot = row_slot(addr, row, c.n_slots);
@@ -311,7 +311,7 @@ __global__ __launch_bounds__(AGPU_BLOCK) void take_group_kernel(QuantCol c, Quan
     T* x = static_cast<T*>(c.x) + row * c.row_stride + head * c.head_stride + (in_row - head * q.groups_per_head) * q.group;
     const uint64_t at = slot * q.groups_per_row + in_row;
     const float scale = !ok ? 0.0f : c.scales[CODE == AGPU_CODE_I4 ? 2 * at : at], lo = ok && CODE == AGPU_CODE_I4 ? c.scales[2 * at + 1] : 0.0f;
-    for (uint32_t i = lane; i < q.group; i += 64) {
+    for (uint32_t i = lane; i < q.group; i += lanes) {
       float v = 0.0f;
       if (ok && CODE == AGPU_CODE_I4) v = __builtin_fmaf((float)((c.codes[(at * q.group + i) / 2] >> (4 * (i & 1))) & 15), scale, lo);
       else if (ok && CODE == AGPU_CODE_I8) v = (float)(int8_t)c.codes[at * q.group + i] * scale;
@@ -342,12 +342,8 @@ agpu_status check_columns(int32_t n_cols, const agpu_quantised_rows* stores, con
   return AGPU_OK;
 }
 
-// Eight values a lane: a group of whole eights in one wave, everything on its vectors' alignment
-bool by_eights(const QuantCol& c, const QuantShape& q, int type, int code) {
-  const uint64_t item = type == AGPU_ROW_F32 ? 4 : 2, strides = (c.row_stride | (q.heads > 1 ? c.head_stride : 0)) * item;
-  return q.group % 8 == 0 && q.group <= 512 && strides % 16 == 0 && aligned16(c.x) && aligned_to(c.codes, code == AGPU_CODE_I4 ? 4 : 8) &&
-         aligned_to(c.scales, code == AGPU_CODE_I4 ? 8 : 4);
-}
+// Eight values a lane: a group that has them and fits a wave
+bool by_eights(const QuantShape& q) { return q.group >= 8 && q.group <= 512; }
 
 // Rows of a block: 8 passes of its lanes, fewer where that would leave less than 2048 blocks (8 a CU)
 FastShape fast_shape(const QuantShape& q, uint64_t n, uint32_t n_cols) {
@@ -377,10 +373,12 @@ void launch_code(agpu_pipeline* p, bool put, bool eights, const QuantCols& cols,
     return;
   }
   for (uint32_t k = 0; k < n_cols; k++) {
-    const uint64_t n_groups = n * q.groups_per_row, blocks = (n_groups + 3) / 4;
+    uint32_t lanes = 1;
+    while (lanes < 64 && lanes < q.group) lanes *= 2;
+    const uint64_t n_groups = n * q.groups_per_row, blocks = (n_groups + AGPU_BLOCK / lanes - 1) / (AGPU_BLOCK / lanes);
     const int grid = (int)(blocks > (1u << 20) ? (1u << 20) : blocks);
-    if (put) hipLaunchKernelGGL((put_group_kernel<T, CODE>), dim3(grid), dim3(AGPU_BLOCK), 0, p->stream, cols.c[k], q, addr, n_groups, p->flags);
-    else hipLaunchKernelGGL((take_group_kernel<T, CODE>), dim3(grid), dim3(AGPU_BLOCK), 0, p->stream, cols.c[k], q, addr, n_groups, p->flags);
+    if (put) hipLaunchKernelGGL((put_group_kernel<T, CODE>), dim3(grid), dim3(AGPU_BLOCK), 0, p->stream, cols.c[k], q, addr, n_groups, lanes, p->flags);
+    else hipLaunchKernelGGL((take_group_kernel<T, CODE>), dim3(grid), dim3(AGPU_BLOCK), 0, p->stream, cols.c[k], q, addr, n_groups, lanes, p->flags);
   }
 }
 template <typename T>
@@ -403,13 +401,12 @@ agpu_status quantised(agpu_pipeline* p, bool put, int32_t n_cols, const agpu_qua
     const QuantShape q = {s.heads, s.dim, s.group, s.dim / s.group, s.heads * (s.dim / s.group)};
     QuantCols cols;
     uint32_t m = 0;
-    bool eights = true;
+    const bool eights = by_eights(q);
     for (; k < n_cols && m < MAX_COLS; k++, m++) {
       const agpu_quantised_rows& o = stores[k];
       const agpu_rows& r = rows[k];
       if (o.heads != s.heads || o.dim != s.dim || o.group != s.group || o.code != s.code || r.type != type) break;
       cols.c[m] = {r.data, r.row_stride, r.head_stride, static_cast<uint8_t*>(o.codes), o.scales, o.n_slots};
-      eights = eights && by_eights(cols.c[m], q, type, s.code);
     }
     if (type == AGPU_ROW_F32) launch_type<float>(p, put, eights, s.code, cols, m, q, addr, n);
     else if (type == AGPU_ROW_F16) launch_type<f16_t>(p, put, eights, s.code, cols, m, q, addr, n);
@@ -449,43 +446,67 @@ agpu_status quantised_pages(agpu_pipeline* p, bool put, int32_t n_cols, const ag
 }
 
 // ---------------------------------------------------------------- take_rows
-// A copy with one indirection: lanes run over the states' accesses of V bytes in the order of the destination, two of a lane in flight, all states in
-// one launch (blockIdx.y).  Bound by memory where V is 16 bytes: 904 MB in 144 us, 6.3 TB/s, a copy's rate; 4 bytes 3.1 TB/s, single bytes 1.2.
+// A copy with one indirection: lanes run over the states' accesses of 16 bytes in the order of the destination, two of a lane in flight, all states in
+// one launch (blockIdx.y).  Accesses begin at any byte; the last of a piece that is no multiple of 16 (or of what a length leaves) is the 16 bytes before
+// its end, some of them its neighbour's too, the same.  Bound by memory: 904 MB in 147 us, 6.1 TB/s, where a copy of as many bytes reaches 6.6; 64 rows of
+// 4000001 bytes UNALIGNEDFIGURES.
 constexpr int MAX_STATES = 8, ROWS_UNROLL = 2;
 struct State {
   const char* src;
   char* dst;
   uint64_t src_row_stride, src_piece_stride, dst_row_stride, dst_piece_stride, position_bytes;
-  uint32_t n_vecs, vecs_per_row;
+  uint32_t n_vecs, vecs_per_row, piece_bytes;
   Divide by_row, by_piece;
 };
 struct States {
   State s[MAX_STATES];
 };
+typedef uint32_t u32x4_at_1 __attribute__((ext_vector_type(4), aligned(1)));
 
-template <typename V>
+// less than 16 bytes, in one access of each size that they hold; src NULL: zeros
+__device__ __forceinline__ void copy_few(char* dst, const char* src, uint32_t n) {
+  typedef uint64_t u64_at_1 __attribute__((aligned(1)));
+  typedef uint16_t u16_at_1 __attribute__((aligned(1)));
+  uint32_t at = 0;
+  if (n & 8) *reinterpret_cast<u64_at_1*>(dst) = src ? *reinterpret_cast<const u64_at_1*>(src) : 0, at = 8;
+  if (n & 4) *reinterpret_cast<u32_at_1*>(dst + at) = src ? *reinterpret_cast<const u32_at_1*>(src + at) : 0, at += 4;
+  if (n & 2) *reinterpret_cast<u16_at_1*>(dst + at) = src ? *reinterpret_cast<const u16_at_1*>(src + at) : 0, at += 2;
+  if (n & 1) dst[at] = src ? src[at] : 0;
+}
+
 __global__ __launch_bounds__(AGPU_BLOCK) void take_rows_kernel(States states, uint64_t n_src, const uint32_t* idx, const uint32_t* lengths, uint32_t* flags) {
   const State& s = states.s[blockIdx.y];
   const uint32_t v0 = blockIdx.x * (AGPU_BLOCK * ROWS_UNROLL) + threadIdx.x;
-  V w[ROWS_UNROLL];
-  char* to[ROWS_UNROLL];
+  u32x4_at_1 w[ROWS_UNROLL];
+  uint64_t to[ROWS_UNROLL];
 #pragma unroll
   for (int u = 0; u < ROWS_UNROLL; u++) {
     const uint32_t v = v0 + u * AGPU_BLOCK;
-    to[u] = nullptr;
-    w[u] = V{};
+    to[u] = ROW_NONE;
+    w[u] = u32x4_at_1{0, 0, 0, 0};
     if (v >= s.n_vecs) continue;
-    const uint32_t row = v / s.by_row, in_row = v - row * s.vecs_per_row, piece = in_row / s.by_piece, off = (in_row - piece * s.by_piece.d) * (uint32_t)sizeof(V);
-    if (lengths && off >= lengths[row] * s.position_bytes) continue;
+    const uint32_t row = v / s.by_row, in_row = v - row * s.vecs_per_row, piece = in_row / s.by_piece;
+    uint32_t off = (in_row - piece * s.by_piece.d) * 16, end = s.piece_bytes;
+    if (lengths) {
+      const uint64_t held = lengths[row] * s.position_bytes;
+      end = held < end ? (uint32_t)held : end;
+    }
+    if (off >= end) continue;
     const uint32_t from = idx[row];
     if (from == AGPU_NO_ROW) continue;
-    to[u] = s.dst + row * s.dst_row_stride + piece * s.dst_piece_stride + off;
-    if (from < n_src) w[u] = *reinterpret_cast<const V*>(s.src + from * s.src_row_stride + piece * s.src_piece_stride + off);
-    else *reinterpret_cast<volatile uint32_t*>(flags) = AGPU_FLAG_INDEX_RANGE;
+    if (from >= n_src) *reinterpret_cast<volatile uint32_t*>(flags) = AGPU_FLAG_INDEX_RANGE;
+    const uint64_t source = from * s.src_row_stride + piece * s.src_piece_stride, target = row * s.dst_row_stride + piece * s.dst_piece_stride;
+    if (end < 16) {
+      copy_few(s.dst + target, from < n_src ? s.src + source : nullptr, end);
+      continue;
+    }
+    if (off + 16 > end) off = end - 16;
+    to[u] = target + off;
+    if (from < n_src) w[u] = *reinterpret_cast<const u32x4_at_1*>(s.src + source + off);
   }
 #pragma unroll
   for (int u = 0; u < ROWS_UNROLL; u++)
-    if (to[u]) __builtin_nontemporal_store(w[u], reinterpret_cast<V*>(to[u]));
+    if (to[u] != ROW_NONE) __builtin_nontemporal_store(w[u], reinterpret_cast<u32x4_at_1*>(s.dst + to[u]));
 }
 
 // bytes from the first to behind the last of n rows; 0: none.  false: past 2^63
@@ -551,19 +572,13 @@ agpu_status agpu_take_rows(agpu_pipeline* p, int32_t n_states, const agpu_state*
   }
   AGPU_BIND(p);
   if (!any) return AGPU_OK;
-  // the widest access that everything is a multiple of, the same for the states of one launch
-  uint64_t all = 0, longest = 0;
-  for (int32_t k = 0; k < n_states; k++) {
-    const agpu_state& s = states[k];
-    if (s.n_pieces == 0 || s.piece_bytes == 0) continue;
-    all |= reinterpret_cast<uintptr_t>(s.src) | reinterpret_cast<uintptr_t>(s.dst) | s.src_row_stride | s.src_piece_stride | s.dst_row_stride | s.dst_piece_stride |
-           s.piece_bytes | (lengths ? s.position_bytes : 0);
-    if (s.n_pieces * s.piece_bytes > longest) longest = s.n_pieces * s.piece_bytes;
-  }
+  const auto accesses = [](const agpu_state& s) { return s.n_pieces * ((s.piece_bytes + 15) / 16); };  // of a row
+  uint64_t longest = 0;
+  for (int32_t k = 0; k < n_states; k++)
+    if (accesses(states[k]) > longest) longest = accesses(states[k]);
   if (longest == 0) return AGPU_OK;
-  const uint32_t width = (all & 15) == 0 ? 16 : (all & 3) == 0 ? 4 : 1;
   // accesses are counted in 31 bits: as many rows at a time as that holds
-  const uint64_t at_once = ((1ull << 31) - 1) / (longest / width);
+  const uint64_t at_once = ((1ull << 31) - 1) / longest;
   for (uint64_t r0 = 0; r0 < n; r0 += at_once) {
     const uint64_t rows = n - r0 < at_once ? n - r0 : at_once;
     for (int32_t k = 0; k < n_states;) {
@@ -572,18 +587,16 @@ agpu_status agpu_take_rows(agpu_pipeline* p, int32_t n_states, const agpu_state*
       for (; k < n_states && m < MAX_STATES; k++) {
         const agpu_state& s = states[k];
         if (s.n_pieces == 0 || s.piece_bytes == 0) continue;
-        const uint32_t per_piece = (uint32_t)(s.piece_bytes / width), per_row = (uint32_t)s.n_pieces * per_piece, n_vecs = (uint32_t)rows * per_row;
+        const uint32_t per_row = (uint32_t)accesses(s), per_piece = per_row / (uint32_t)s.n_pieces, n_vecs = (uint32_t)rows * per_row;
         held.s[m++] = {static_cast<const char*>(s.src), static_cast<char*>(s.dst) + r0 * s.dst_row_stride, s.src_row_stride, s.src_piece_stride, s.dst_row_stride,
-                       s.dst_piece_stride, s.position_bytes, n_vecs, per_row, divide_by(per_row), divide_by(per_piece)};
+                       s.dst_piece_stride, s.position_bytes, n_vecs, per_row, (uint32_t)s.piece_bytes, divide_by(per_row), divide_by(per_piece)};
         most = n_vecs > most ? n_vecs : most;
       }
       if (m == 0) break;
       const dim3 grid((most + AGPU_BLOCK * ROWS_UNROLL - 1) / (AGPU_BLOCK * ROWS_UNROLL), m);
       const uint32_t* at = idx + r0;
       const uint32_t* len = lengths ? lengths + r0 : nullptr;
-      if (width == 16) hipLaunchKernelGGL((take_rows_kernel<u32x4>), grid, dim3(AGPU_BLOCK), 0, p->stream, held, n_src, at, len, p->flags);
-      else if (width == 4) hipLaunchKernelGGL((take_rows_kernel<uint32_t>), grid, dim3(AGPU_BLOCK), 0, p->stream, held, n_src, at, len, p->flags);
-      else hipLaunchKernelGGL((take_rows_kernel<uint8_t>), grid, dim3(AGPU_BLOCK), 0, p->stream, held, n_src, at, len, p->flags);
+      hipLaunchKernelGGL(take_rows_kernel, grid, dim3(AGPU_BLOCK), 0, p->stream, held, n_src, at, len, p->flags);
       AGPU_LAUNCH_CHECK();
     }
   }
