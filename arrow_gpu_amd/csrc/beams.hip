@@ -491,8 +491,7 @@ __global__ __launch_bounds__(MERGE_BLOCK) void beam_merge_kernel(BeamArgs a, Div
   uint32_t n = count;
   if (n > MERGE_LIST) {  // the bound is too low for the list (k is large): any that k and at most MERGE_LIST reach, found by halving
     uint32_t low = order_of(floor_v), high = order_of(-LOWEST) + 1;
-    while (n > MERGE_LIST && high - low > 1) {
-      const uint32_t mid = low + (high - low) / 2;
+    for (uint32_t mid = low + 1; n > MERGE_LIST && high - low > 1; mid = low + (high - low) / 2) {  // (first whether the bound itself is what so many hold)
       uint32_t reach = 0;
       each(0, [&](double s, uint32_t, Entry) { reach += s > none && order_of((float)s) >= mid; });
       for (int d = 32; d; d >>= 1) reach += __shfl_xor(reach, d);

@@ -448,8 +448,8 @@ agpu_status quantised_pages(agpu_pipeline* p, bool put, int32_t n_cols, const ag
 // ---------------------------------------------------------------- take_rows
 // A copy with one indirection: lanes run over the states' accesses of 16 bytes in the order of the destination, two of a lane in flight, all states in
 // one launch (blockIdx.y).  Accesses begin at any byte; the last of a piece that is no multiple of 16 (or of what a length leaves) is the 16 bytes before
-// its end, some of them its neighbour's too, the same.  Bound by memory: 904 MB in 147 us, 6.1 TB/s, where a copy of as many bytes reaches 6.6; 64 rows of
-// 4000001 bytes UNALIGNEDFIGURES.
+// its end, some of them its neighbour's too, the same.  Bound by memory: 904 MB in 147 us, 6.1 TB/s, where a copy of as many bytes reaches 6.6 (one or four
+// of a lane in flight: 151 and 147, of a short row's 3.6 and 4.8 instead of 3.5); 64 rows of 4000001 f32, no row on 16 bytes, in 349 us, 5.9 TB/s.
 constexpr int MAX_STATES = 8, ROWS_UNROLL = 2;
 struct State {
   const char* src;
@@ -479,30 +479,37 @@ __global__ __launch_bounds__(AGPU_BLOCK) void take_rows_kernel(States states, ui
   const uint32_t v0 = blockIdx.x * (AGPU_BLOCK * ROWS_UNROLL) + threadIdx.x;
   u32x4_at_1 w[ROWS_UNROLL];
   uint64_t to[ROWS_UNROLL];
+  uint32_t row[ROWS_UNROLL], from[ROWS_UNROLL], held[ROWS_UNROLL];
+  // what the addresses depend on first: a wait for it behind a row's load would be one for the row
+#pragma unroll
+  for (int u = 0; u < ROWS_UNROLL; u++) {
+    const uint32_t v = v0 + u * AGPU_BLOCK, at = v < s.n_vecs ? v : 0;
+    row[u] = at / s.by_row;
+    from[u] = idx[row[u]];
+    held[u] = lengths ? lengths[row[u]] : 0;
+  }
 #pragma unroll
   for (int u = 0; u < ROWS_UNROLL; u++) {
     const uint32_t v = v0 + u * AGPU_BLOCK;
     to[u] = ROW_NONE;
     w[u] = u32x4_at_1{0, 0, 0, 0};
-    if (v >= s.n_vecs) continue;
-    const uint32_t row = v / s.by_row, in_row = v - row * s.vecs_per_row, piece = in_row / s.by_piece;
+    if (v >= s.n_vecs || from[u] == AGPU_NO_ROW) continue;
+    const uint32_t in_row = v - row[u] * s.vecs_per_row, piece = in_row / s.by_piece;
     uint32_t off = (in_row - piece * s.by_piece.d) * 16, end = s.piece_bytes;
     if (lengths) {
-      const uint64_t held = lengths[row] * s.position_bytes;
-      end = held < end ? (uint32_t)held : end;
+      const uint64_t most = held[u] * s.position_bytes;
+      end = most < end ? (uint32_t)most : end;
     }
     if (off >= end) continue;
-    const uint32_t from = idx[row];
-    if (from == AGPU_NO_ROW) continue;
-    if (from >= n_src) *reinterpret_cast<volatile uint32_t*>(flags) = AGPU_FLAG_INDEX_RANGE;
-    const uint64_t source = from * s.src_row_stride + piece * s.src_piece_stride, target = row * s.dst_row_stride + piece * s.dst_piece_stride;
+    if (from[u] >= n_src) *reinterpret_cast<volatile uint32_t*>(flags) = AGPU_FLAG_INDEX_RANGE;
+    const uint64_t source = from[u] * s.src_row_stride + piece * s.src_piece_stride, target = row[u] * s.dst_row_stride + piece * s.dst_piece_stride;
     if (end < 16) {
-      copy_few(s.dst + target, from < n_src ? s.src + source : nullptr, end);
+      copy_few(s.dst + target, from[u] < n_src ? s.src + source : nullptr, end);
       continue;
     }
     if (off + 16 > end) off = end - 16;
     to[u] = target + off;
-    if (from < n_src) w[u] = *reinterpret_cast<const u32x4_at_1*>(s.src + source + off);
+    if (from[u] < n_src) w[u] = *reinterpret_cast<const u32x4_at_1*>(s.src + source + off);
   }
 #pragma unroll
   for (int u = 0; u < ROWS_UNROLL; u++)
