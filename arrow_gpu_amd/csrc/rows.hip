@@ -46,8 +46,9 @@ struct QuantShape {
   uint32_t heads, dim, group, groups_per_head, groups_per_row;
 };
 
-// ---------------------------------------------------------------- eight values a lane
-// Both ways stream: 16-byte accesses (32 of f32) on the rows' side, 8 or 4 on the codes'.  A group is `lanes` neighbouring lanes (a power of two, those
+// ---------------------------------------------------------------- 16 bytes of values a lane
+// Both ways stream: 16-byte accesses on the rows' side (two of f32 a lane, 32 bytes apart, would write parts of lines: 468 us instead of 201 for two
+// columns of 131072 rows of 4 bits as f32), 2 to 8 bytes on the codes'.  A group is `lanes` neighbouring lanes (a power of two, those
 // past the group's end idle), its span found with data-parallel moves inside the wave.  A block takes whole rows, looks their slots up once and
 // keeps them in LDS: a search of the sequence through memory costs microseconds, so it is shared by up to 8 passes of the block (16 passes: 131072
 // rows of 4 bits in 138 us instead of 127).
@@ -64,17 +65,21 @@ struct FastShape {
   Divide by_row, by_head;                                      // groups a row, groups a head
 };
 
-// Vectors from any element (any byte of the codes) on
-template <typename T> struct Eight;
-template <> struct Eight<float> {
-  typedef float type __attribute__((ext_vector_type(8), aligned(4)));
+// Vectors of `many` values, from any element (any byte of the codes) on
+template <typename T> struct Wide;
+template <> struct Wide<float> {
+  static constexpr int many = 4;
+  typedef float type __attribute__((ext_vector_type(4), aligned(4)));
 };
-template <> struct Eight<f16_t> {
+template <> struct Wide<f16_t> {
+  static constexpr int many = 8;
   typedef f16_t type __attribute__((ext_vector_type(8), aligned(2)));
 };
-template <> struct Eight<bf16_t> {
+template <> struct Wide<bf16_t> {
+  static constexpr int many = 8;
   typedef bf16_t type __attribute__((ext_vector_type(8), aligned(2)));
 };
+typedef uint16_t u16_at_1 __attribute__((aligned(1)));
 typedef uint32_t u32_at_1 __attribute__((aligned(1)));
 typedef uint32_t u32x2_at_1 __attribute__((ext_vector_type(2), aligned(1)));
 typedef float f32x2_at_4 __attribute__((ext_vector_type(2), aligned(4)));
@@ -111,15 +116,16 @@ __device__ __forceinline__ uint32_t block_rows(const QuantCol& c, const FastShap
   __syncthreads();
   return rows;
 }
-// what a lane has at a time: eight values of one group, from value `from` on; the last lane of a group that is no multiple of 8 has the group's last eight
-// (some of its neighbour's too: they get the same codes)
+// what a lane has at a time: W values of one group, from value `from` on; the last lane of a group that is no multiple of W has the group's last W (some of
+// its neighbour's too: they get the same codes)
 struct Unit {
   uint32_t row, in_row, from;
   bool idle;  // past the group's end
 };
+template <int W>
 __device__ __forceinline__ Unit unit_of(uint32_t i, const FastShape& q) {
-  const uint32_t g = i >> q.log_lanes, row = g / q.by_row, from = (i & (q.lanes - 1)) * 8;
-  return {row, g - row * q.groups_per_row, from + 8 <= q.group ? from : q.group - 8, from >= q.group};
+  const uint32_t g = i >> q.log_lanes, row = g / q.by_row, from = (i & (q.lanes - 1)) * W;
+  return {row, g - row * q.groups_per_row, from + W <= q.group ? from : q.group - W, from >= q.group};
 }
 __device__ __forceinline__ uint64_t value_offset(const Unit& u, const QuantCol& c, const FastShape& q) {
   if (q.dense) return u.in_row * q.group + u.from;
@@ -128,24 +134,26 @@ __device__ __forceinline__ uint64_t value_offset(const Unit& u, const QuantCol& 
 }
 
 template <typename T, int CODE>
-__global__ __launch_bounds__(AGPU_BLOCK) void put_eight_kernel(QuantCols cols, FastShape q, RowAddr addr, uint64_t n, uint32_t* flags) {
+__global__ __launch_bounds__(AGPU_BLOCK) void put_wide_kernel(QuantCols cols, FastShape q, RowAddr addr, uint64_t n, uint32_t* flags) {
+  typedef typename Wide<T>::type Vector;
+  constexpr int W = Wide<T>::many;
   __shared__ BlockRow held[MAX_ROWS];
   const QuantCol& c = cols.c[blockIdx.y];  // (one load of a lane in flight: two or four do not pay, 18.2 -> 18.9 us)
   const uint32_t total = (block_rows(c, q, addr, n, held, flags) * q.groups_per_row) << q.log_lanes;
   for (uint32_t i = threadIdx.x; i < total; i += AGPU_BLOCK) {
-    const Unit t = unit_of(i, q);
+    const Unit t = unit_of<W>(i, q);
     const BlockRow row = held[t.row];
     const bool live = !t.idle && row.at < ROW_BAD;
-    float v[8] = {};
+    float v[W] = {};
     if (live) {
-      const typename Eight<T>::type w = *reinterpret_cast<const typename Eight<T>::type*>(static_cast<const T*>(c.x) + row.x + value_offset(t, c, q));
+      const Vector w = *reinterpret_cast<const Vector*>(static_cast<const T*>(c.x) + row.x + value_offset(t, c, q));
 #pragma unroll
-      for (int j = 0; j < 8; j++) v[j] = (float)w[j];
+      for (int j = 0; j < W; j++) v[j] = (float)w[j];
     }
     // the largest magnitude by its bits: a NaN's lie above infinity's, and stay
     uint32_t most = 0;
 #pragma unroll
-    for (int j = 0; j < 8; j++) {
+    for (int j = 0; j < W; j++) {
       const uint32_t b = __builtin_bit_cast(uint32_t, v[j]) & 0x7FFFFFFFu;
       most = b > most ? b : most;
     }
@@ -159,7 +167,7 @@ __global__ __launch_bounds__(AGPU_BLOCK) void put_eight_kernel(QuantCols cols, F
     if (CODE == AGPU_CODE_I4) {
       float l = live ? v[0] : __builtin_inff(), h = live ? v[0] : -__builtin_inff();
 #pragma unroll
-      for (int j = 1; j < 8; j++) l = live ? fminf(l, v[j]) : l, h = live ? fmaxf(h, v[j]) : h;
+      for (int j = 1; j < W; j++) l = live ? fminf(l, v[j]) : l, h = live ? fmaxf(h, v[j]) : h;
       lo = over_group(l, q.lanes, [](float a, float b) { return fminf(a, b); });
       span = over_group(h, q.lanes, [](float a, float b) { return fmaxf(a, b); }) - lo;
     }
@@ -170,13 +178,15 @@ __global__ __launch_bounds__(AGPU_BLOCK) void put_eight_kernel(QuantCols cols, F
       if (t.from == 0) reinterpret_cast<f32x2_at_4*>(c.scales)[at] = f32x2_at_4{f.scale, f.lo};
       uint32_t w = 0;
 #pragma unroll
-      for (int j = 0; j < 8; j++) w |= (whole(v[j] - f.lo, f.inv) & 15) << 4 * j;
-      *reinterpret_cast<u32_at_1*>(c.codes + at * (q.group / 2) + t.from / 2) = w;
+      for (int j = 0; j < W; j++) w |= (whole(v[j] - f.lo, f.inv) & 15) << 4 * j;
+      uint8_t* to = c.codes + at * (q.group / 2) + t.from / 2;
+      if constexpr (W == 8) *reinterpret_cast<u32_at_1*>(to) = w;
+      else *reinterpret_cast<u16_at_1*>(to) = (uint16_t)w;
     } else {
       if (t.from == 0) c.scales[at] = f.scale;
       u32x2_at_1 w;
 #pragma unroll
-      for (int h = 0; h < 2; h++) {
+      for (int h = 0; h < W / 4; h++) {
         if (CODE == AGPU_CODE_I8) {
           w[h] = __builtin_amdgcn_perm(__builtin_amdgcn_perm(whole(v[4 * h + 3], f.inv), whole(v[4 * h + 2], f.inv), 0x0C0C0400u),
                                        __builtin_amdgcn_perm(whole(v[4 * h + 1], f.inv), whole(v[4 * h], f.inv), 0x0C0C0400u), 0x05040100u);
@@ -185,7 +195,9 @@ __global__ __launch_bounds__(AGPU_BLOCK) void put_eight_kernel(QuantCols cols, F
           w[h] = (uint32_t)__builtin_amdgcn_cvt_pk_fp8_f32(v[4 * h + 2] * f.inv, v[4 * h + 3] * f.inv, low, true);
         }
       }
-      *reinterpret_cast<u32x2_at_1*>(c.codes + at * q.group + t.from) = w;
+      uint8_t* to = c.codes + at * q.group + t.from;
+      if constexpr (W == 8) *reinterpret_cast<u32x2_at_1*>(to) = w;
+      else *reinterpret_cast<u32_at_1*>(to) = w.x;
     }
   }
 }
@@ -193,7 +205,9 @@ __global__ __launch_bounds__(AGPU_BLOCK) void put_eight_kernel(QuantCols cols, F
 constexpr int TAKE_UNROLL = 8;  // all of a block's passes in flight: 131072 rows of 4 bits 127 us, of four at a time 132
 
 template <typename T, int CODE>
-__global__ __launch_bounds__(AGPU_BLOCK) void take_eight_kernel(QuantCols cols, FastShape q, RowAddr addr, uint64_t n, uint32_t* flags) {
+__global__ __launch_bounds__(AGPU_BLOCK) void take_wide_kernel(QuantCols cols, FastShape q, RowAddr addr, uint64_t n, uint32_t* flags) {
+  typedef typename Wide<T>::type Vector;
+  constexpr int W = Wide<T>::many;
   __shared__ BlockRow held[MAX_ROWS];
   const QuantCol& c = cols.c[blockIdx.y];
   const uint32_t total = (block_rows(c, q, addr, n, held, flags) * q.groups_per_row) << q.log_lanes;
@@ -206,7 +220,7 @@ __global__ __launch_bounds__(AGPU_BLOCK) void take_eight_kernel(QuantCols cols, 
       const uint32_t i = i0 + u * AGPU_BLOCK;
       to[u] = ROW_NONE;
       w[u] = u32x2{0, 0}, f[u] = f32x2_at_4{0.0f, 0.0f};  // out of range: zeros
-      const Unit t = unit_of(i, q);
+      const Unit t = unit_of<W>(i, q);
       if (i >= total || t.idle) continue;
       const BlockRow row = held[t.row];
       if (row.at == ROW_NONE) continue;
@@ -215,26 +229,30 @@ __global__ __launch_bounds__(AGPU_BLOCK) void take_eight_kernel(QuantCols cols, 
       const uint64_t at = row.at + t.in_row;
       if (CODE == AGPU_CODE_I4) {
         f[u] = reinterpret_cast<const f32x2_at_4*>(c.scales)[at];
-        w[u].x = *reinterpret_cast<const u32_at_1*>(c.codes + at * (q.group / 2) + t.from / 2);
+        const uint8_t* from = c.codes + at * (q.group / 2) + t.from / 2;
+        if constexpr (W == 8) w[u].x = *reinterpret_cast<const u32_at_1*>(from);
+        else w[u].x = *reinterpret_cast<const u16_at_1*>(from);
       } else {
         f[u].x = c.scales[at];
-        w[u] = *reinterpret_cast<const u32x2_at_1*>(c.codes + at * q.group + t.from);
+        const uint8_t* from = c.codes + at * q.group + t.from;
+        if constexpr (W == 8) w[u] = *reinterpret_cast<const u32x2_at_1*>(from);
+        else w[u].x = *reinterpret_cast<const u32_at_1*>(from);
       }
     }
 #pragma unroll
     for (int u = 0; u < TAKE_UNROLL; u++) {
       if (to[u] == ROW_NONE) continue;
-      typename Eight<T>::type o;
+      Vector o;
       if (CODE == AGPU_CODE_I4) {
         const uint32_t even = w[u].x & 0x0F0F0F0Fu, odd = w[u].x >> 4 & 0x0F0F0F0Fu;  // a byte each: the conversion takes them from where they are
 #pragma unroll
-        for (int j = 0; j < 4; j++) {
+        for (int j = 0; j < W / 2; j++) {
           o[2 * j] = (T)__builtin_fmaf((float)(even >> 8 * j & 255), f[u].x, f[u].y);
           o[2 * j + 1] = (T)__builtin_fmaf((float)(odd >> 8 * j & 255), f[u].x, f[u].y);
         }
       } else {
 #pragma unroll
-        for (int h = 0; h < 2; h++) {
+        for (int h = 0; h < W / 4; h++) {
           const uint32_t b = w[u][h];
           if (CODE == AGPU_CODE_E4M3) {
             const auto low = __builtin_amdgcn_cvt_pk_f32_fp8(b, false), high = __builtin_amdgcn_cvt_pk_f32_fp8(b, true);
@@ -246,12 +264,12 @@ __global__ __launch_bounds__(AGPU_BLOCK) void take_eight_kernel(QuantCols cols, 
         }
       }
       // past the caches: nobody reads the rows in this call (ragged e4m3 rows 30.5 us, through the caches 42)
-      __builtin_nontemporal_store(o, reinterpret_cast<typename Eight<T>::type*>(static_cast<T*>(c.x) + to[u]));
+      __builtin_nontemporal_store(o, reinterpret_cast<Vector*>(static_cast<T*>(c.x) + to[u]));
     }
   }
 }
 
-// ---------------------------------------------------------------- a value a lane at a time: groups below 8 and above 512
+// ---------------------------------------------------------------- a value a lane at a time: groups below 16 bytes and above 64 times that
 // A group is `lanes` neighbouring lanes, at most a wave.  Bound by its narrow accesses and a slot's look-up for each group: 2^24 bf16 values in groups of
 // 1024 go to 8 bits in 28 us and come back in 20 (of 512, in the form above: 13 and 11).
 template <typename T, int CODE>
@@ -342,14 +360,14 @@ agpu_status check_columns(int32_t n_cols, const agpu_quantised_rows* stores, con
   return AGPU_OK;
 }
 
-// Eight values a lane: a group that has them and fits a wave (2^24 values in groups of 100 to 8 bits: 16 us, a value a lane at a time 64)
-bool by_eights(const QuantShape& q) { return q.group >= 8 && q.group <= 512; }
+// 16 bytes of values a lane: a group that has them and fits a wave (2^24 bf16 values in groups of 100 to 8 bits: 16 us, a value a lane at a time 64)
+bool is_wide(uint32_t group, uint32_t many) { return group >= many && group <= 64 * many; }
 
 // Rows of a block: 8 passes of its lanes, fewer where that would leave less than 2048 blocks (8 a CU)
-FastShape fast_shape(const QuantShape& q, uint64_t n, uint32_t n_cols) {
+FastShape fast_shape(const QuantShape& q, uint32_t many, uint64_t n, uint32_t n_cols) {
   FastShape f = {};
   f.group = q.group, f.groups_per_row = q.groups_per_row;
-  while (8u << f.log_lanes < q.group) f.log_lanes++;
+  while (many << f.log_lanes < q.group) f.log_lanes++;
   f.lanes = 1u << f.log_lanes;
   const uint64_t row_lanes = (uint64_t)q.groups_per_row << f.log_lanes;
   uint64_t rows = 8 * AGPU_BLOCK / row_lanes;
@@ -362,14 +380,14 @@ FastShape fast_shape(const QuantShape& q, uint64_t n, uint32_t n_cols) {
 }
 
 template <typename T, int CODE>
-void launch_code(agpu_pipeline* p, bool put, bool eights, const QuantCols& cols, uint32_t n_cols, const QuantShape& q, const RowAddr& addr, uint64_t n) {
-  if (eights) {
-    FastShape f = fast_shape(q, n, n_cols);
+void launch_code(agpu_pipeline* p, bool put, const QuantCols& cols, uint32_t n_cols, const QuantShape& q, const RowAddr& addr, uint64_t n) {
+  if (is_wide(q.group, Wide<T>::many)) {
+    FastShape f = fast_shape(q, Wide<T>::many, n, n_cols);
     f.dense = true;
     for (uint32_t k = 0; k < n_cols; k++) f.dense = f.dense && (q.heads == 1 || cols.c[k].head_stride == q.dim);
     const dim3 grid((uint32_t)((n + f.rows - 1) / f.rows), n_cols);
-    if (put) hipLaunchKernelGGL((put_eight_kernel<T, CODE>), grid, dim3(AGPU_BLOCK), 0, p->stream, cols, f, addr, n, p->flags);
-    else hipLaunchKernelGGL((take_eight_kernel<T, CODE>), grid, dim3(AGPU_BLOCK), 0, p->stream, cols, f, addr, n, p->flags);
+    if (put) hipLaunchKernelGGL((put_wide_kernel<T, CODE>), grid, dim3(AGPU_BLOCK), 0, p->stream, cols, f, addr, n, p->flags);
+    else hipLaunchKernelGGL((take_wide_kernel<T, CODE>), grid, dim3(AGPU_BLOCK), 0, p->stream, cols, f, addr, n, p->flags);
     return;
   }
   for (uint32_t k = 0; k < n_cols; k++) {
@@ -382,11 +400,11 @@ void launch_code(agpu_pipeline* p, bool put, bool eights, const QuantCols& cols,
   }
 }
 template <typename T>
-void launch_type(agpu_pipeline* p, bool put, bool eights, int code, const QuantCols& cols, uint32_t n_cols, const QuantShape& q, const RowAddr& addr, uint64_t n) {
+void launch_type(agpu_pipeline* p, bool put, int code, const QuantCols& cols, uint32_t n_cols, const QuantShape& q, const RowAddr& addr, uint64_t n) {
   switch (code) {
-    case AGPU_CODE_I8: return launch_code<T, AGPU_CODE_I8>(p, put, eights, cols, n_cols, q, addr, n);
-    case AGPU_CODE_I4: return launch_code<T, AGPU_CODE_I4>(p, put, eights, cols, n_cols, q, addr, n);
-    default: return launch_code<T, AGPU_CODE_E4M3>(p, put, eights, cols, n_cols, q, addr, n);
+    case AGPU_CODE_I8: return launch_code<T, AGPU_CODE_I8>(p, put, cols, n_cols, q, addr, n);
+    case AGPU_CODE_I4: return launch_code<T, AGPU_CODE_I4>(p, put, cols, n_cols, q, addr, n);
+    default: return launch_code<T, AGPU_CODE_E4M3>(p, put, cols, n_cols, q, addr, n);
   }
 }
 
@@ -401,16 +419,15 @@ agpu_status quantised(agpu_pipeline* p, bool put, int32_t n_cols, const agpu_qua
     const QuantShape q = {s.heads, s.dim, s.group, s.dim / s.group, s.heads * (s.dim / s.group)};
     QuantCols cols;
     uint32_t m = 0;
-    const bool eights = by_eights(q);
     for (; k < n_cols && m < MAX_COLS; k++, m++) {
       const agpu_quantised_rows& o = stores[k];
       const agpu_rows& r = rows[k];
       if (o.heads != s.heads || o.dim != s.dim || o.group != s.group || o.code != s.code || r.type != type) break;
       cols.c[m] = {r.data, r.row_stride, r.head_stride, static_cast<uint8_t*>(o.codes), o.scales, o.n_slots};
     }
-    if (type == AGPU_ROW_F32) launch_type<float>(p, put, eights, s.code, cols, m, q, addr, n);
-    else if (type == AGPU_ROW_F16) launch_type<f16_t>(p, put, eights, s.code, cols, m, q, addr, n);
-    else launch_type<bf16_t>(p, put, eights, s.code, cols, m, q, addr, n);
+    if (type == AGPU_ROW_F32) launch_type<float>(p, put, s.code, cols, m, q, addr, n);
+    else if (type == AGPU_ROW_F16) launch_type<f16_t>(p, put, s.code, cols, m, q, addr, n);
+    else launch_type<bf16_t>(p, put, s.code, cols, m, q, addr, n);
     AGPU_LAUNCH_CHECK();
   }
   return AGPU_OK;
@@ -466,7 +483,6 @@ typedef uint32_t u32x4_at_1 __attribute__((ext_vector_type(4), aligned(1)));
 // less than 16 bytes, in one access of each size that they hold; src NULL: zeros
 __device__ __forceinline__ void copy_few(char* dst, const char* src, uint32_t n) {
   typedef uint64_t u64_at_1 __attribute__((aligned(1)));
-  typedef uint16_t u16_at_1 __attribute__((aligned(1)));
   uint32_t at = 0;
   if (n & 8) *reinterpret_cast<u64_at_1*>(dst) = src ? *reinterpret_cast<const u64_at_1*>(src) : 0, at = 8;
   if (n & 4) *reinterpret_cast<u32_at_1*>(dst + at) = src ? *reinterpret_cast<const u32_at_1*>(src + at) : 0, at += 4;
