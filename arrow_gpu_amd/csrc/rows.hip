@@ -20,11 +20,11 @@ template <> struct Top<AGPU_CODE_E4M3> { static constexpr float v = 448.0f; };
 struct Factors {
   float scale, inv, lo;
 };
-// span: max |x| or max − min; bad: the group holds a NaN or an infinity
+// span: max |x| or max − min, not finite where the group holds a NaN or an infinity
 template <int CODE>
-__device__ __forceinline__ Factors factors(float span, float lo, bool bad) {
+__device__ __forceinline__ Factors factors(float span, float lo) {
   constexpr float top = Top<CODE>::v;
-  if (bad || !(span < __builtin_inff())) return {__builtin_nanf(""), 0.0f, lo};
+  if (!(span < __builtin_inff())) return {__builtin_nanf(""), 0.0f, lo};
   if (span < top * 0x1p-126f) return {0.0f, 0.0f, lo};  // span / top would be subnormal and top / span could overflow
   // span / top, rounded once: the remainder of span · (1 / top) is exact and corrects it (compared with the division for all 2^23 mantissas)
   constexpr float r = 1.0f / top;
@@ -33,6 +33,23 @@ __device__ __forceinline__ Factors factors(float span, float lo, bool bad) {
 }
 __device__ __forceinline__ uint32_t whole(float x, float inv) {  // low byte: the code in two's complement
   return __builtin_bit_cast(uint32_t, __builtin_fmaf(x, inv, 0x1.8p23f));
+}
+
+// of three, a NaN if there is one
+__device__ __forceinline__ float maximum_of(float a, float b, float c) {
+  float r;
+  asm("v_maximum3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+__device__ __forceinline__ float maximum_of_abs(float a, float b, float c) {
+  float r;
+  asm("v_maximum3_f32 %0, |%1|, |%2|, |%3|" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
+}
+__device__ __forceinline__ float minimum_of(float a, float b, float c) {
+  float r;
+  asm("v_minimum3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+  return r;
 }
 
 struct QuantCol {
@@ -150,28 +167,23 @@ __global__ __launch_bounds__(AGPU_BLOCK) void put_wide_kernel(QuantCols cols, Fa
 #pragma unroll
       for (int j = 0; j < W; j++) v[j] = (float)w[j];
     }
-    // the largest magnitude by its bits: a NaN's lie above infinity's, and stay
-    uint32_t most = 0;
-#pragma unroll
-    for (int j = 0; j < W; j++) {
-      const uint32_t b = __builtin_bit_cast(uint32_t, v[j]) & 0x7FFFFFFFu;
-      most = b > most ? b : most;
-    }
-    const auto higher = [](float a, float b) {
-      const uint32_t x = __builtin_bit_cast(uint32_t, a), y = __builtin_bit_cast(uint32_t, b);
-      return __builtin_bit_cast(float, x > y ? x : y);
-    };
-    const float mag = over_group(__builtin_bit_cast(float, most), q.lanes, higher);
-    const bool bad = __builtin_bit_cast(uint32_t, mag) >= 0x7F800000u;
-    float span = mag, lo = 0.0f;
+    // the largest magnitude, or the lowest and the highest value; a NaN stays
+    float span, lo = 0.0f;
     if (CODE == AGPU_CODE_I4) {
       float l = live ? v[0] : __builtin_inff(), h = live ? v[0] : -__builtin_inff();
+      if (live) {
 #pragma unroll
-      for (int j = 1; j < W; j++) l = live ? fminf(l, v[j]) : l, h = live ? fmaxf(h, v[j]) : h;
-      lo = over_group(l, q.lanes, [](float a, float b) { return fminf(a, b); });
-      span = over_group(h, q.lanes, [](float a, float b) { return fmaxf(a, b); }) - lo;
+        for (int j = 1; j < W; j += 2) l = minimum_of(l, v[j], v[j + 1 < W ? j + 1 : j]), h = maximum_of(h, v[j], v[j + 1 < W ? j + 1 : j]);
+      }
+      lo = over_group(l, q.lanes, [](float a, float b) { return minimum_of(a, b, b); });
+      span = over_group(h, q.lanes, [](float a, float b) { return maximum_of(a, b, b); }) - lo;
+    } else {
+      float most = 0.0f;
+#pragma unroll
+      for (int j = 0; j < W; j += 2) most = maximum_of_abs(most, v[j], v[j + 1]);
+      span = over_group(most, q.lanes, [](float a, float b) { return maximum_of(a, b, b); });
     }
-    const Factors f = factors<CODE>(span, lo, bad);
+    const Factors f = factors<CODE>(span, lo);
     if (!live) continue;
     const uint64_t at = row.at + t.in_row;
     if (CODE == AGPU_CODE_I4) {
@@ -298,7 +310,7 @@ __global__ __launch_bounds__(AGPU_BLOCK) void put_group_kernel(QuantCol c, Quant
       hi = fmaxf(hi, __shfl_xor(hi, d));
       bad |= __shfl_xor(bad, d);
     }
-    const Factors f = factors<CODE>(CODE == AGPU_CODE_I4 ? hi - lo : fmaxf(hi, -lo), lo, bad != 0);
+    const Factors f = factors<CODE>(bad ? __builtin_nanf("") : CODE == AGPU_CODE_I4 ? hi - lo : fmaxf(hi, -lo), lo);
     const uint64_t at = slot * q.groups_per_row + in_row;
     if (CODE == AGPU_CODE_I4) {
       if (lane == 0) c.scales[2 * at] = f.scale, c.scales[2 * at + 1] = f.lo;
