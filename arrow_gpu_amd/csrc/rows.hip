@@ -69,7 +69,7 @@ struct QuantShape {
 // past the group's end idle), its span found with data-parallel moves inside the wave.  A block takes whole rows, looks their slots up once and
 // keeps them in LDS: a search of the sequence through memory costs microseconds, so it is shared by up to 8 passes of the block (16 passes: 131072
 // rows of 4 bits in 138 us instead of 127).
-// What bounds it is memory: two columns of 16384 rows of 8 x 128 bf16 go to e4m3 in 18 us and come back in 16.6 (102 MB each: 5.7 and 6.1 TB/s; a copy
+// What bounds it is memory: two columns of 16384 rows of 8 x 128 bf16 go to e4m3 in 17 us and come back in 17 (102 MB each: 6.0 TB/s; a copy
 // of as many bytes takes 17), ragged e4m3 rows of 4 x 96 come back as f16 in 30.5 us (181 MB, 5.9 TB/s), two columns of 131072 rows of 4 bits as bf16
 // in 127 us (705 MB, 5.6 TB/s; a u8 -> f32 cast of as many bytes 109).  A token's rows take 2.5 us a call, that is one launch.
 constexpr int MAX_COLS = 8, MAX_ROWS = 256;
@@ -155,7 +155,7 @@ __global__ __launch_bounds__(AGPU_BLOCK) void put_wide_kernel(QuantCols cols, Fa
   typedef typename Wide<T>::type Vector;
   constexpr int W = Wide<T>::many;
   __shared__ BlockRow held[MAX_ROWS];
-  const QuantCol& c = cols.c[blockIdx.y];  // (one load of a lane in flight: two or four do not pay, 18.2 -> 18.9 us)
+  const QuantCol& c = cols.c[blockIdx.y];  // (one load of a lane in flight: two or four do not pay, 18.2 -> 18.9 us of 2 x 16384 rows)
   const uint32_t total = (block_rows(c, q, addr, n, held, flags) * q.groups_per_row) << q.log_lanes;
   for (uint32_t i = threadIdx.x; i < total; i += AGPU_BLOCK) {
     const Unit t = unit_of<W>(i, q);

@@ -128,8 +128,9 @@ def take_rows_op(states, indexes: UInt32ArrayGPU, pipeline: ArrowComputePipeline
         raise shape_error(f"{len(out)} outputs for {len(states)} states")
     n_src, dev, packed = states[0].shape[0], pipeline.device, b""
     for s, o in zip(states, out):
-        if s.shape[0] != n_src or o.shape[1:] != s.shape[1:] or o.shape[0] != n or o.item_size != s.item_size:
-            raise shape_error(f"rows {tuple(o.shape)} from a state {tuple(s.shape)} by {n} indexes, in a call over {n_src} rows")
+        here, there = s.shape, o.shape
+        if here[0] != n_src or there[0] != n or o.item_size != s.item_size or (here != there and here[1:] != there[1:]):
+            raise shape_error(f"rows {there} from a state {here} by {n} indexes, in a call over {n_src} rows")
         row, step, pieces, size, position = s._pieces or s.as_pieces()
         out_row, out_step, out_pieces, out_size, _ = o._pieces or o.as_pieces()
         if (pieces, size) != (out_pieces, out_size):
@@ -139,12 +140,14 @@ def take_rows_op(states, indexes: UInt32ArrayGPU, pipeline: ArrowComputePipeline
         packed += _PACK_STATE.pack(s.ptr, o.ptr, row, step, out_row, out_step, pieces, size, position)
         if s.gpu_device is not dev or o.gpu_device is not dev:
             _on(pipeline, s, o)
-    _on(pipeline, indexes)
-    if lengths is not None:
-        _on(pipeline, lengths)
-        _keep(pipeline, lengths.data)
+    given = (indexes,) if lengths is None else (indexes, lengths)
+    for x in given:
+        if x.gpu_device is not dev:
+            _on(pipeline, x)
     capi.call("agpu_take_rows", pipeline._handle, len(states), packed, n_src, indexes.data.ptr, lengths.data.ptr if lengths is not None else None, n)
-    _keep(pipeline, indexes.data)
+    for x in given:
+        if x.data._owned:
+            pipeline.keep(x.data)
     for s, o in zip(states, out):
         if s.data._owned or o.data._owned:
             _keep(pipeline, s.data, o.data)
@@ -181,17 +184,24 @@ def select_beams_op(logits: RowsGPU, beams: int, k: int, pipeline: ArrowComputeP
         out = BeamSelection.empty(batch, k, pipeline.device)
     elif (out.batch, out.k) != (batch, k):
         raise shape_error(f"a selection of {out.batch} x {out.k} for {batch} x {k}")
-    given = [x for x in (scores, allowed, finished) if x is not None]
-    _on(pipeline, logits, out, *given)
+    dev, given = pipeline.device, [x for x in (logits, scores, allowed, finished) if x is not None]
+    if out.gpu_device is not dev:
+        _on(pipeline, out)
+    for x in given:
+        if x.gpu_device is not dev:
+            _on(pipeline, x)
     if batch == 0:
         return out
-    work = out.ensure_workspace(beams, vocab)
+    work = out.workspace if out._workspace_of == (beams, vocab) else out.ensure_workspace(beams, vocab)
     args = _PACK_BEAMS.pack(logits.ptr, logits.strides[0], ROW_TYPE[logits.type], batch, beams, vocab, k, end_token,
                             scores.data.ptr if scores is not None else 0, allowed.data.ptr if allowed is not None else 0, stride,
                             finished.data.ptr if finished is not None else 0, out.scores.data.ptr, out.parents.data.ptr, out.tokens.data.ptr,
                             work.ptr, work.nbytes)
     capi.call("agpu_select_beams", pipeline._handle, args)
-    _keep(pipeline, logits.data, out.scores.data, out.parents.data, out.tokens.data, work, *[x.data for x in given])
+    for x in given:
+        if x.data._owned:
+            pipeline.keep(x.data)
+    _keep(pipeline, out.scores.data, out.parents.data, out.tokens.data, work)
     return out
 
 
