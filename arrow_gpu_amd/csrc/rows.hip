@@ -70,8 +70,8 @@ struct QuantShape {
 // keeps them in LDS: a search of the sequence through memory costs microseconds, so it is shared by up to 8 passes of the block (16 passes: 131072
 // rows of 4 bits in 138 us instead of 127).
 // What bounds it is memory: two columns of 16384 rows of 8 x 128 bf16 go to e4m3 in 17 us and come back in 17 (102 MB each: 6.0 TB/s; a copy
-// of as many bytes takes 17), ragged e4m3 rows of 4 x 96 come back as f16 in 30.5 us (181 MB, 5.9 TB/s), two columns of 131072 rows of 4 bits as bf16
-// in 127 us (705 MB, 5.6 TB/s; a u8 -> f32 cast of as many bytes 109).  A token's rows take 2.5 us a call, that is one launch.
+// of as many bytes takes 19), ragged e4m3 rows of 4 x 96 come back as f16 in 30.5 us (181 MB, 5.9 TB/s), two columns of 131072 rows of 4 bits as bf16
+// in 127 us (705 MB, 5.6 TB/s; a u8 -> f32 cast of as many bytes 112).  A token's rows take 2.5 us a call, that is one launch.
 constexpr int MAX_COLS = 8, MAX_ROWS = 256;
 struct QuantCols {
   QuantCol c[MAX_COLS];
