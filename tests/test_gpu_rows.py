@@ -700,6 +700,26 @@ def test_select_from_slices(dev, p, kind, at, pitch):
     assert_selection(sel, R.select(x.astype(np.float64), beams, k))
 
 
+def test_select_past_32_bits(dev, p):
+    """rows whose logits lie more than 4 GiB behind the first; nearly all of them equal"""
+    import arrow_gpu_amd as ag
+
+    vocab, beams, k = 800_000_011, 3, 5
+    x = ag.RowsGPU.empty((beams, vocab), "bf16", dev)
+    capi.call("agpu_memset", p._handle, C.c_void_p(x.ptr), 0, 2 * beams * vocab)
+    places = [(2, vocab - 1, 9.0), (1, vocab // 2, 6.0), (0, 7, 3.0)]
+    for r, t, v in places:
+        bits16 = np.array([v], np.float32).view(np.uint32) >> 16
+        half = np.ascontiguousarray(bits16.astype(np.uint16))
+        capi.call("agpu_upload", p._handle, C.c_void_p(x.ptr + 2 * (r * vocab + t)), C.c_void_p(half.ctypes.data), 2)
+    cum = np.array([0.0, -1.0, -2.0], np.float32)
+    sel = ag.select_beams_op(x, beams, k, p, scores=ag.Float32ArrayGPU.from_slice(cum, dev))
+    p.sync()
+    lse = {r: np.log(vocab - 1 + np.exp(v)) for r, _, v in places}
+    want = [cum[r] + (v - lse[r]) for r, _, v in places] + [-lse[0], -lse[0]]
+    assert_selection(sel, (np.array([want]), np.array([[2, 1, 0, 0, 0]]), np.array([[vocab - 1, vocab // 2, 7, 0, 1]])))
+
+
 def test_select_far_apart_logits(dev, p):
     """logits over the whole range of f32: the sum's terms vanish, one by one"""
     import arrow_gpu_amd as ag
@@ -801,6 +821,25 @@ def test_a_step_captured_and_replayed(dev, p):
         eager = ag.select_beams(dl, state["beams"], state["beams"], scores=state["scores"])  # on a pipeline of its own
         assert_selection(eager, R.select(lg.astype(np.float64), state["beams"], state["beams"], state["scores_np"]))
     capi.call("agpu_graph_destroy", g)
+
+
+def test_rows_of_columns_that_a_fusing_pipeline_has_only_recorded(dev):
+    import arrow_gpu_amd as ag
+
+    rng = np.random.default_rng(41)
+    a = rng.standard_normal(64 * 96).astype(np.float32)
+    pipe = ag.ArrowComputePipeline(dev, "fusing", fuse=True)
+    two, three = (ag.Float32ArrayGPU.from_slice([v], dev) for v in (2.0, 3.0))
+    x = ag.add_scalar_op_dyn(ag.mul_scalar_op_dyn(ag.Float32ArrayGPU.from_slice(a, dev), two, pipe), three, pipe)
+    store = ag.QuantisedRowsGPU.empty(64, 1, 96, dev)
+    slots = u32(rng.permutation(64), dev)
+    ag.put_quantised_op(store, ag.RowsGPU.of_array(x, (64, 1, 96)), slots, pipe)
+    got = ag.take_quantised_op(store, slots, pipe)[0]
+    pipe.finish()
+    pipe.sync()
+    want = (a * np.float32(2) + np.float32(3)).reshape(64, 1, 96)
+    codes, scales = R.quantise(want, "i8", 96)
+    assert_values(got.values(), R.values(codes, scales, "i8", 96), "f32")
 
 
 def test_two_pipelines_at_once(dev):
