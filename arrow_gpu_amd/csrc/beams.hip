@@ -639,7 +639,7 @@ agpu_status agpu_select_beams_workspace(uint32_t batch, uint32_t beams, uint32_t
 agpu_status agpu_select_beams(agpu_pipeline* p, const agpu_beams* args) {
   AGPU_REQUIRE(args, AGPU_ERR_ARG, "null argument");
   const agpu_beams& b = *args;
-  AGPU_REQUIRE(b.type >= AGPU_ROW_F32 && b.type <= AGPU_ROW_BF16, AGPU_ERR_ARG, "row type");
+  AGPU_REQUIRE(b.row_type >= AGPU_ROW_F32 && b.row_type <= AGPU_ROW_BF16, AGPU_ERR_ARG, "row type");
   if (b.batch == 0) {
     AGPU_BIND(p);
     return AGPU_OK;
@@ -652,7 +652,7 @@ agpu_status agpu_select_beams(agpu_pipeline* p, const agpu_beams* args) {
   AGPU_REQUIRE(b.end_token < b.vocab, AGPU_ERR_SHAPE, "end_token < vocab");
   AGPU_REQUIRE(b.allowed_stride % 8 == 0 && (b.allowed_stride == 0 || b.allowed_stride >= agpu_bitmap_bytes(b.vocab)), AGPU_ERR_SHAPE,
                "allowed_stride: 0, or a multiple of 8 that holds vocab bits");
-  AGPU_REQUIRE(aligned_to(b.logits, b.type == AGPU_ROW_F32 ? 4 : 2) && aligned_to(b.scores, 4) && aligned_to(b.allowed, 8) && aligned_to(b.finished, 8) &&
+  AGPU_REQUIRE(aligned_to(b.logits, b.row_type == AGPU_ROW_F32 ? 4 : 2) && aligned_to(b.scores, 4) && aligned_to(b.allowed, 8) && aligned_to(b.finished, 8) &&
                    aligned_to(b.out_scores, 4) && aligned_to(b.out_parents, 4) && aligned_to(b.out_tokens, 4) && aligned16(b.workspace),
                AGPU_ERR_SHAPE, "alignment");
   // a request's block writes while another's still reads: results do not go where scores come from
@@ -667,8 +667,8 @@ agpu_status agpu_select_beams(agpu_pipeline* p, const agpu_beams* args) {
                       static_cast<const uint64_t*>(b.finished), b.out_scores, b.out_parents, b.out_tokens, segments((uint64_t)b.batch * b.beams, b.vocab)};
   SegSum* sums = static_cast<SegSum*>(b.workspace);
   Entry* entries = reinterpret_cast<Entry*>(sums + (uint64_t)b.batch * b.beams * a.segs);
-  if (b.type == AGPU_ROW_F32) launch_segments<float>(p, a, sums, entries);
-  else if (b.type == AGPU_ROW_F16) launch_segments<f16_t>(p, a, sums, entries);
+  if (b.row_type == AGPU_ROW_F32) launch_segments<float>(p, a, sums, entries);
+  else if (b.row_type == AGPU_ROW_F16) launch_segments<f16_t>(p, a, sums, entries);
   else launch_segments<bf16_t>(p, a, sums, entries);
   AGPU_LAUNCH_CHECK();
   hipLaunchKernelGGL(beam_merge_kernel, dim3(b.batch), dim3(MERGE_BLOCK), 0, p->stream, a, divide_by(a.segs * a.k), sums, entries);

@@ -356,7 +356,7 @@ agpu_status check_columns(int32_t n_cols, const agpu_quantised_rows* stores, con
   for (int32_t k = 0; k < n_cols; k++) {
     const agpu_quantised_rows& s = stores[k];
     const agpu_rows& r = rows[k];
-    AGPU_REQUIRE(r.type >= AGPU_ROW_F32 && r.type <= AGPU_ROW_BF16, AGPU_ERR_ARG, "row type");
+    AGPU_REQUIRE(r.row_type >= AGPU_ROW_F32 && r.row_type <= AGPU_ROW_BF16, AGPU_ERR_ARG, "row type");
     AGPU_REQUIRE(s.code >= AGPU_CODE_I8 && s.code <= AGPU_CODE_E4M3, AGPU_ERR_ARG, "code type");
     AGPU_REQUIRE(s.heads > 0 && s.dim > 0 && (uint64_t)s.heads * s.dim <= (1u << 30), AGPU_ERR_SHAPE, "1 <= heads * dim <= 2^30");
     AGPU_REQUIRE(s.group > 0 && s.group <= 65536 && s.dim % s.group == 0, AGPU_ERR_SHAPE, "group divides dim, 1 <= group <= 65536");
@@ -364,7 +364,7 @@ agpu_status check_columns(int32_t n_cols, const agpu_quantised_rows* stores, con
     AGPU_REQUIRE(s.n_slots <= (1ull << 32), AGPU_ERR_SHAPE, "n_slots <= 2^32");
     AGPU_REQUIRE(n * s.heads * s.dim < (1ull << 48), AGPU_ERR_SHAPE, "less than 2^48 values a column");
     AGPU_REQUIRE(r.data && s.codes && s.scales, AGPU_ERR_ARG, "null pointer");
-    AGPU_REQUIRE(aligned_to(r.data, r.type == AGPU_ROW_F32 ? 4 : 2) && aligned_to(s.scales, 4), AGPU_ERR_SHAPE, "alignment");
+    AGPU_REQUIRE(aligned_to(r.data, r.row_type == AGPU_ROW_F32 ? 4 : 2) && aligned_to(s.scales, 4), AGPU_ERR_SHAPE, "alignment");
     if (writes_rows) {
       AGPU_REQUIRE(disjoint(n, r.row_stride, s.heads, r.head_stride, s.dim), AGPU_ERR_SHAPE, "rows that are written may not overlap");
     }
@@ -427,14 +427,14 @@ agpu_status quantised(agpu_pipeline* p, bool put, int32_t n_cols, const agpu_qua
   // neighbouring columns of one kind go into one launch
   for (int32_t k = 0; k < n_cols;) {
     const agpu_quantised_rows& s = stores[k];
-    const int type = rows[k].type;
+    const int type = rows[k].row_type;
     const QuantShape q = {s.heads, s.dim, s.group, s.dim / s.group, s.heads * (s.dim / s.group)};
     QuantCols cols;
     uint32_t m = 0;
     for (; k < n_cols && m < MAX_COLS; k++, m++) {
       const agpu_quantised_rows& o = stores[k];
       const agpu_rows& r = rows[k];
-      if (o.heads != s.heads || o.dim != s.dim || o.group != s.group || o.code != s.code || r.type != type) break;
+      if (o.heads != s.heads || o.dim != s.dim || o.group != s.group || o.code != s.code || r.row_type != type) break;
       cols.c[m] = {r.data, r.row_stride, r.head_stride, static_cast<uint8_t*>(o.codes), o.scales, o.n_slots};
     }
     if (type == AGPU_ROW_F32) launch_type<float>(p, put, s.code, cols, m, q, addr, n);

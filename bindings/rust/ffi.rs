@@ -117,7 +117,7 @@ pub struct agpu_rows {
     pub data: *mut c_void,
     pub row_stride: u64,
     pub head_stride: u64,
-    pub type: i32,
+    pub row_type: i32,
 }
 #[repr(C)]
 pub struct agpu_quantised_rows {
@@ -155,7 +155,7 @@ pub struct agpu_state {
 pub struct agpu_beams {
     pub logits: *const c_void,
     pub row_stride: u64,
-    pub type: i32,
+    pub row_type: i32,
     pub batch: u32,
     pub beams: u32,
     pub vocab: u32,

@@ -1179,7 +1179,7 @@ inline BeamSelection select_beams_op(const RowsGPU& logits, uint32_t beams, uint
   const uint64_t n = (uint64_t)batch * k, bytes = n ? 4 * n : 4;
   const BufferPtr s = dev->create_empty_buffer(bytes), r = dev->create_empty_buffer(bytes), t = dev->create_empty_buffer(bytes), w = dev->create_empty_buffer(need ? need : 16);
   const agpu_rows x = logits.abi();
-  const agpu_beams a = {x.data, x.row_stride, x.type, batch, beams, (uint32_t)logits.dim, k, end_token, scores ? static_cast<const float*>(scores->data->ptr) : nullptr,
+  const agpu_beams a = {x.data, x.row_stride, x.row_type, batch, beams, (uint32_t)logits.dim, k, end_token, scores ? static_cast<const float*>(scores->data->ptr) : nullptr,
                         allowed ? allowed->data->ptr : nullptr, allowed ? pitch : 0, finished ? finished->data->ptr : nullptr, static_cast<float*>(s->ptr),
                         static_cast<uint32_t*>(r->ptr), static_cast<uint32_t*>(t->ptr), w->ptr, w->bytes};
   check(agpu_select_beams(p.h(), &a), "agpu_select_beams");

@@ -533,7 +533,7 @@ typedef struct agpu_rows {
   void* data;
   uint64_t row_stride;
   uint64_t head_stride;
-  int32_t type; /* agpu_row_type */
+  int32_t row_type; /* agpu_row_type */
 } agpu_rows;
 
 /* A cache of n_slots rows in 8 or 4 bits.  codes: [n_slots, heads, dim], contiguous, one byte a value; AGPU_CODE_I4: two values a byte, the
@@ -617,7 +617,7 @@ agpu_status agpu_take_rows(agpu_pipeline* p, int32_t n_states, const agpu_state*
 typedef struct agpu_beams {
   const void* logits;
   uint64_t row_stride;
-  int32_t type; /* agpu_row_type */
+  int32_t row_type; /* agpu_row_type */
   uint32_t batch, beams, vocab, k, end_token;
   const float* scores;
   const void* allowed;

@@ -232,6 +232,27 @@ def test_rust_structs_mirror_the_headers_fields_in_order():
         assert re.search(r"pub const %s: \w+ = \d+;" % const, rust), const
 
 
+# the Rust reference, "Keywords": strict ones, those of later editions, reserved ones
+_RUST_KEYWORDS = set("""as break const continue crate else enum extern false fn for if impl in let loop match mod move mut pub ref return self Self static
+struct super trait true type unsafe use where while async await dyn abstract become box do final macro override priv typeof unsized virtual yield try
+gen""".split())
+
+
+def test_rust_ffi_names_no_keyword():
+    """a keyword in the place of a name ends the parse of the whole file: fields, arguments, functions, types and constants"""
+    text = re.sub(r"//[^\n]*", "", open(os.path.join(RUST_DIR, "ffi.rs")).read())
+    names = []
+    for body in re.findall(r"pub struct \w+ \{(.*?)\}", text, flags=re.S):
+        names += re.findall(r"(?:^|[,{]|\n)\s*(?:pub\s+)?([\w#]+)\s*:", body)
+    for args in re.findall(r"pub fn \w+\((.*?)\)(?: ->|;)", text):
+        names += [a.split(":", 1)[0].strip() for a in _split_args(args)]
+    names += re.findall(r"pub (?:fn|type|const|struct) ([\w#]+)", text)
+    assert len(names) > 500 and "r#in" in names and "row_type" in names
+    assert not [n for n in names if n in _RUST_KEYWORDS], sorted(set(names) & _RUST_KEYWORDS)
+    raw = {n[2:] for n in names if n.startswith("r#")}
+    assert raw <= _RUST_KEYWORDS - {"crate", "self", "Self", "super"}  # those have no raw form
+
+
 def test_rust_host_modules_call_only_existing_ffi_functions_with_the_right_arity():
     rs = _rust_signatures()
     seen = set()

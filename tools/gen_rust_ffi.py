@@ -164,6 +164,20 @@ def width_class(rust: str) -> str:
     return WIDTH.get(rust, "i4")  # enums and agpu_status are 32-bit integers
 
 
+# Rust's keywords, strict and reserved [the Rust reference, "Keywords"]; those of the second row have no raw form
+RAW_KEYWORDS = set("as break const continue else enum extern false fn for if impl in let loop match mod move mut pub ref return static struct trait true type "
+                   "unsafe use where while async await dyn abstract become box do final macro override priv typeof unsized virtual yield try gen".split())
+BARE_KEYWORDS = {"crate", "self", "Self", "super", "_"}
+
+
+def rust_name(name: str, raw: bool) -> str:
+    """A C name as Rust can spell it.  raw: whether `r#name` will do — a struct's field is compared with the header's name by name, so that one
+    is to be renamed in the header instead."""
+    if name in BARE_KEYWORDS or (name in RAW_KEYWORDS and not raw):
+        raise ValueError(f"{name!r} is a keyword of Rust: give it another name in the header")
+    return "r#" + name if name in RAW_KEYWORDS else name
+
+
 def generate_ffi(h: Header) -> str:
     known = {n for n, _ in h.enums} | set(h.opaque) | {n for n, _ in h.structs} | {n for n, _ in h.aliases}
     o = []
@@ -201,17 +215,17 @@ def generate_ffi(h: Header) -> str:
                 _, fname, ret, args = f
                 rargs = ", ".join(rust_type(a, known) for a in args)
                 rret = "" if ret == "void" else f" -> {rust_type(ret, known)}"
-                w(f"    pub {fname}: Option<unsafe extern \"C\" fn({rargs}){rret}>,")
+                w(f"    pub {rust_name(fname, False)}: Option<unsafe extern \"C\" fn({rargs}){rret}>,")
             else:
                 ctype, fname, arr = f
                 rt = rust_type(ctype, known)
-                w(f"    pub {fname}: {'[%s; %d]' % (rt, arr) if arr else rt},")
+                w(f"    pub {rust_name(fname, False)}: {'[%s; %d]' % (rt, arr) if arr else rt},")
         w("}")
     w("")
     w('#[link(name = "arrow_gpu_hip")]')
     w('extern "C" {')
     for name, ret, args in h.functions:
-        rargs = ", ".join(f"{('r#' + an) if an in ('in', 'type', 'ref', 'box', 'move') else an}: {rust_type(ct, known)}" for ct, an in args)
+        rargs = ", ".join(f"{rust_name(an, True)}: {rust_type(ct, known)}" for ct, an in args)
         rret = "" if ret == "void" else f" -> {rust_type(ret, known)}"
         w(f"    pub fn {name}({rargs}){rret};")
     w("}")
