@@ -3,7 +3,7 @@
 // One pass over the logits.  A row is cut into segments of one WAVE each; the wave streams its segment, adding up exp(x) and keeping the tokens that
 // can be among its k best, and leaves (sum, k best) in the workspace.  A block a request joins the sums and selects among the segments' bests.
 // No wave needs the maximum first: exp is taken relative to the first tile's, and f32 holds it as long as
-// a segment's maximum is within 60 of that; a segment of another kind is read again.
+// a segment's maximum is at most 60 above that, or 30 below a reference that is no tile's maximum; a segment of another kind is read again.
 //
 // 256 rows x 128256 bf16, 8 beams, k 16: segments 21.7 us (66 MB: 3.0 TB/s), join 5.8.  The segments are bound by their instructions, not by memory — the
 // loads alone take 12.6 us: about 12 a logit, of which the term's exp are 6 and the pair sums, the clamp, the unpacking and the maxima 3.5; the floors
@@ -14,6 +14,8 @@
 // f64 and left out of the f32 ones.  An f32 term is 2^f · 2^n with x log2 e = n + f, |f| <= 1/2: one fma rounds x log2 e to n, the next gives f, a third adds x
 // times what log2 e has beyond f32 (2^-26 of error each), the instruction for 2^f is within 2^-23; 16 are added with 4 roundings, the rest in f64.
 // That bounds a log-sum's error by 2^-23 + ln 2 · 2^-25 + 4 · 2^-24 < 3.8e-7; many different terms are off at random, and it is about 1e-9.
+// What does not count (a masked logit, −infinity, one that a f64 term stands for) is e^-80 of the reference in the f32 sum: at most 8192 of them beside a
+// segment's largest term, which is e^-30 of it or more: 8192 e^-50 < 2e-18, nothing in a f64 sum — a lone token's is exactly 1.
 #include "common.hpp"
 #include "row_address.hpp"
 
@@ -50,7 +52,9 @@ __device__ __forceinline__ bool is_finished(const BeamArgs& a, uint32_t row) { r
 constexpr float LOG2E = 0x1.715476p+0f, LOG2E_LOW = 0x1.4ae0cp-26f, MAGIC = 0x1.8p23f;
 constexpr double LN2 = 0.69314718055994530942;
 constexpr float REF_MOST = 16384.0f;  // of a reference: MAGIC − k holds its steps
-constexpr float APART = 60.0f;        // of a segment's maximum from its reference
+constexpr float APART = 60.0f;        // of a segment's maximum above its reference
+constexpr float BELOW = 30.0f;        // of it below the reference (0, where the first tile's maximum is no ordinary number)
+constexpr float LEAST = 80.0f;        // of a term below the reference
 // exp(x) / 2^N, k = MAGIC − N; x log2 e − N within 2^±126
 __device__ __forceinline__ float exp_term(float x, float k) {
   const float z = __builtin_fmaf(x, LOG2E, k);  // its low bits: n − N
@@ -246,7 +250,7 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
         for (int d = 32; d; d >>= 1) f = fmaxf(f, __shfl_xor(f, d));
         ref_v = __builtin_fabsf(f) <= REF_MOST ? f : 0.0f;
         k = MAGIC - __builtin_rintf(ref_v * LOG2E);
-        least = ref_v - 80.0f;
+        least = ref_v - LEAST;
       }
     }
     // The floor, after tiles 0 and 2: a value that k logits of the row reach, among the maxima of the block's waves, all of one row
@@ -291,7 +295,7 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
         }
         hits[step / 2] |= h << (step % 2 * EPT + u * VE);
       }
-    // the terms (at least e^-80, −infinity too: nothing beside the largest), added in pairs of pairs: four roundings on every way
+    // the terms (at least e^-80 of the reference, −infinity too), added in pairs of pairs: four roundings on every way
 #pragma unroll
     for (int i = 0; i < EPT; i++) v[i] = exp_term(max_of(v[i], least), k);
 #pragma unroll
@@ -310,7 +314,7 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
 #pragma unroll
   for (int i = 0; i < 4; i++) all += (uint32_t)__builtin_popcount(hits[i]);
   for (int d = 32; d; d >>= 1) all += __shfl_xor(all, d);
-  const bool many = all > HITS, again = most > LOWEST && most < __builtin_inff() && (many || __builtin_fabsf(most - ref_v) > APART);
+  const bool many = all > HITS, again = most > LOWEST && most < __builtin_inff() && (many || most - ref_v > APART || ref_v - most > BELOW);
   u32x4 w[U];
   uint32_t m[U];
   const double ref = most;  // (a lone token's term is then exactly 1, its log-sum the logit)

@@ -122,3 +122,44 @@ def select(x, beams, k, scores=None, allowed=None, finished=None, end_token=0):
             at += 1
         out_s.append(s), out_p.append(r), out_t.append(t)
     return np.array(out_s), np.array(out_p, np.int64), np.array(out_t, np.int64)
+
+
+def select_many(x, beams, k, scores=None, allowed=None, finished=None, end_token=0):
+    """select() for large inputs: of every row only the k tokens that can be chosen are sorted, a block of rows at a time.  x [rows, vocab] of any float type."""
+    rows, vocab = x.shape
+    out = [[], [], []]
+    block = max(1, (1 << 23) // (beams * vocab)) * beams
+    for r0 in range(0, rows, block):
+        v = x[r0:r0 + block].astype(np.float64)
+        n, each = v.shape[0], min(k, vocab)
+        if allowed is not None:
+            v = np.where(allowed if allowed.ndim == 1 else allowed[r0:r0 + block], v, -np.inf)
+        done = np.zeros(n, bool) if finished is None else np.asarray(finished[r0:r0 + block], bool)
+        cum = np.zeros(n) if scores is None else scores[r0:r0 + block].astype(np.float64)
+        with np.errstate(all="ignore"):
+            m = v.max(-1, keepdims=True)
+            lse = (m + np.log(np.exp(v - m).sum(-1, keepdims=True)))[:, 0]
+            lse[~np.isfinite(m[:, 0])] = np.nan  # a NaN, +infinity or nothing
+            border = np.partition(v, vocab - each, -1)[:, vocab - each, None]
+            above, equal = v > border, v == border
+            take = above | (equal & (np.cumsum(equal, -1) <= each - above.sum(-1, keepdims=True)))
+            row, token = np.nonzero(take)
+            logit = v[row, token]
+            score = cum[row] + (logit - lse[row])
+        live = (score > -np.inf) & ~done[row]
+        ends = np.nonzero(done & (cum > -np.inf))[0]
+        row, token = np.concatenate([row[live], ends]), np.concatenate([token[live], np.full(len(ends), end_token)])
+        logit, score = np.concatenate([logit[live], np.zeros(len(ends))]), np.concatenate([score[live], cum[ends]])
+        order = np.lexsort((token, -logit, row, -score, row // beams))
+        row, token, score = row[order], token[order], score[order]
+        first = np.searchsorted(row // beams, np.arange(n // beams + 1))
+        for b in range(n // beams):
+            at = slice(first[b], min(first[b] + k, first[b + 1]))
+            s, r, t = score[at].tolist(), (row[at] + r0).tolist(), token[at].tolist()
+            have, f = {(p - r0 - b * beams) * vocab + q for p, q in zip(r, t)}, 0
+            while len(s) < k:
+                if f not in have:
+                    s.append(-np.inf), r.append(r0 + b * beams + f // vocab), t.append(f % vocab)
+                f += 1
+            out[0].append(s), out[1].append(r), out[2].append(t)
+    return np.array(out[0]), np.array(out[1], np.int64), np.array(out[2], np.int64)
