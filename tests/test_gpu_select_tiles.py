@@ -29,6 +29,27 @@ def f32(values, dev):  # noqa: F811
     return ag.Float32ArrayGPU.from_slice(np.asarray(values, np.float32), dev)
 
 
+def assert_near(sel, want, x, cum):
+    """assert_selection() where rows compete whose log-sums are equal, or nearly so, in exact arithmetic (an ascending row and a descending one).  A row's
+    scores are all off by one error, at most LOG_SUM: the i-th of the scores so moved is at most LOG_SUM from the i-th of the exact ones, and the exact score of
+    the token that stands there at most LOG_SUM from its moved one.  So the token's exact score is at most 2 LOG_SUM from the i-th exact score; and the
+    tokens of one row, all moved alike, stand in the exact order."""
+    s, r, t = sel.values()
+    ws, wr, wt = want
+    fine = np.isfinite(ws)
+    assert np.array_equal(np.isfinite(s), fine)
+    assert (np.abs(s[fine] - ws[fine]) <= np.abs(ws[fine]) * R.HALF_STEP["f32"] * (1 + 2.0**-10) + LOG_SUM).all()
+    for b in np.nonzero(((r != wr) | (t != wt)).any(-1))[0]:
+        lse = {}
+        for row in set(r[b].tolist()):
+            v = x[row].astype(np.float64)
+            lse[row] = v.max() + np.log(np.exp(v - v.max()).sum())
+            mine = t[b][r[b] == row]
+            assert np.array_equal(mine, np.lexsort((np.arange(len(v)), -v))[:len(mine)])
+        score = np.array([float(cum[p]) + (float(x[p, q]) - lse[p]) for p, q in zip(r[b].tolist(), t[b].tolist())])
+        assert fine[b].all() and (np.abs(score - ws[b]) <= 2 * LOG_SUM).all()
+
+
 LOWEST = {"f32": -3.4028235e38, "f16": -65504.0, "bf16": -3.3895314e38}
 
 
@@ -63,4 +84,92 @@ def test_low_logits_behind_a_first_tile_that_holds_none(dev, p, kind, hole):  # 
     assert np.array_equal(s[lone][:, :beams], np.sort(cum.reshape(-1, beams)[lone])[:, ::-1])  # exactly
     fine = np.isfinite(want[0])
     assert (np.abs(s[fine] - want[0][fine]) <= np.abs(want[0][fine]) * R.HALF_STEP["f32"] * (1 + 2.0**-10) + LOG_SUM).all(), np.abs(s[fine] - want[0][fine]).max()
+    assert_selection(sel, want)
+
+
+@pytest.mark.parametrize("rows,vocab,beams,k,of", [(2100, 4001, 7, 14, 2), (1040, 16001, 8, 16, 4), (820, 40003, 4, 64, 8), (4100, 8190, 1, 1, 8), (256, 128256, 8, 16, 8)])
+@pytest.mark.parametrize("kind", KINDS)
+def test_a_batch(dev, p, kind, rows, vocab, beams, k, of):  # noqa: F811
+    """ordinary logits; then with masks that leave much, little, one token and nothing, and whole tiles out, NaN and infinities under them, rows finished"""
+    import arrow_gpu_amd as ag
+
+    rng = np.random.default_rng(rows + vocab)
+    assert tiles(rows, vocab) == of
+    x = logits(rng, rows, vocab, kind)
+    cum = -np.float32(15) * rng.random(rows).astype(np.float32)
+    sel = ag.select_beams_op(up(x, kind, dev), beams, k, p, scores=f32(cum, dev))
+    p.sync()
+    assert_selection(sel, R.select_many(x, beams, k, cum))
+
+    pitch = (vocab + 63) // 64 * 64
+    allowed = np.zeros((rows, pitch), bool)
+    for r in range(rows):
+        allowed[r, :vocab] = rng.random(vocab, dtype=np.float32) < (0.001, 0.02, 0.5, 0.97)[r % 4]
+    for r in range(0, rows, 3):  # whole tiles, the segment's first among them
+        allowed[r, :vocab] &= np.repeat((np.arange(-(-vocab // 1024)) > 0) & (rng.random(-(-vocab // 1024)) < 0.5), 1024)[:vocab]
+    allowed[1] = False
+    allowed[2] = False
+    allowed[2, vocab - 1] = True
+    allowed[beams * 5:beams * 6] = False
+    some = rng.integers(0, rows * vocab, rows * 40)
+    some = some[~allowed[some // vocab, some % vocab]]
+    x[some // vocab, some % vocab] = R.rounded(rng.choice(np.array([np.nan, np.inf, -np.inf, 6e4, -6e4], np.float32), len(some)), kind)
+    allowed[:, vocab:] = True
+    finished = rng.random(rows) < 0.2
+    sel = ag.select_beams_op(up(x, kind, dev), beams, k, p, scores=f32(cum, dev), allowed=bits(allowed, dev), finished=bits(finished, dev), end_token=vocab // 2)
+    p.sync()
+    assert_selection(sel, R.select_many(x, beams, k, cum, allowed[:, :vocab], finished, vocab // 2))
+
+
+@pytest.mark.parametrize("k", [1, 16, 64])
+@pytest.mark.parametrize("kind", KINDS)
+def test_rows_of_other_kinds(dev, p, kind, k):  # noqa: F811
+    """ascending and descending rows, equal logits, ties that begin in a late tile, spans past a segment's range, rows without a distribution"""
+    import arrow_gpu_amd as ag
+
+    rng = np.random.default_rng(k)
+    rows, vocab, beams = 820, 40003, 2
+    assert tiles(rows, vocab) == 8
+    at = np.arange(vocab)
+
+    def late(n, value, other):
+        row = np.full(vocab, other, np.float32)
+        row[rng.integers(vocab // 2, vocab, n)] = value
+        return row
+
+    def with_one(value, where):
+        row = rng.standard_normal(vocab).astype(np.float32)
+        row[where] = value
+        return row
+
+    make = [lambda: at / 2048.0, lambda: -at / 2048.0, lambda: np.zeros(vocab), lambda: np.full(vocab, LOWEST[kind]), lambda: late(2000, 3.0, 1.0), lambda: late(30, 3.0, LOWEST[kind]),
+            lambda: rng.standard_normal(vocab) * 100, lambda: with_one(np.nan, vocab - 1), lambda: with_one(np.inf, vocab - 3000), lambda: np.where(at // 1024 % 8 == 3, rng.random(vocab) * 5 - 60, -np.inf),
+            lambda: (at % 509) / 64.0, lambda: np.where(at // 1024 % 2 == 1, 0.5, -0.5), lambda: np.where(at < 9000, -500.0, rng.standard_normal(vocab)), lambda: np.full(vocab, -np.inf),
+            lambda: np.where(at // 1024 % 8 == 5, 80.0, 0.0) + rng.random(vocab), lambda: np.floor(rng.random(vocab) * 4) - 2, lambda: np.minimum(at // 1024, 37) * 1.0]
+    one = [R.rounded(np.asarray(m(), np.float32), kind) for m in make]
+    x = np.stack([one[r // 2 % len(one)] if r // 2 < 2 * len(one) else one[rng.integers(len(one))] for r in range(rows)])
+    cum = -np.float32(3) * rng.random(rows).astype(np.float32)
+    cum[:rows // 2] = 0  # pairs of equal rows first: of equal scores the lower row's, then its lower tokens
+    sel = ag.select_beams_op(up(x, kind, dev), beams, k, p, scores=f32(cum, dev))
+    p.sync()
+    assert_near(sel, R.select_many(x, beams, k, cum), x, cum)
+
+
+@pytest.mark.parametrize("kind", KINDS)
+def test_equal_rows_wherever_they_begin(dev, p, kind):  # noqa: F811
+    """rows on every alignment, NaN beside them: equal rows have equal scores, the lower row's come first"""
+    import arrow_gpu_amd as ag
+
+    rng = np.random.default_rng(6)
+    rows, vocab, pitch, beams, k = 2100, 5001, 5003, 5, 12
+    assert tiles(rows, vocab) == 4
+    x = np.repeat(logits(rng, rows // beams, vocab, kind), beams, 0)
+    wide = np.full((rows, pitch), np.nan, np.float32)
+    wide[:, :vocab] = x
+    base = up(wide, kind, dev)
+    view = ag.RowsGPU(base.data, dev, (rows, vocab), kind, (pitch, 1))
+    sel = ag.select_beams_op(view, beams, k, p)
+    p.sync()
+    want = R.select_many(x, beams, k)
+    assert want[1][0, :beams].tolist() == list(range(beams))
     assert_selection(sel, want)
