@@ -173,3 +173,24 @@ def test_equal_rows_wherever_they_begin(dev, p, kind):  # noqa: F811
     want = R.select_many(x, beams, k)
     assert want[1][0, :beams].tolist() == list(range(beams))
     assert_selection(sel, want)
+
+
+@pytest.mark.parametrize("rows,vocab", [(12, 999), (12, 4099), (2100, 4001)])
+@pytest.mark.parametrize("kind", KINDS)
+def test_one_mask_for_all_rows(dev, p, kind, rows, vocab):  # noqa: F811
+    """a bitmap of one row's tokens: log-sums, scores, parents, order — a vocabulary that is no multiple of 64, and the bitmap's length that or a multiple"""
+    import arrow_gpu_amd as ag
+
+    rng = np.random.default_rng(vocab)
+    beams, k = 6, 10
+    x = logits(rng, rows, vocab, kind)
+    allowed = np.zeros((vocab + 63) // 64 * 64, bool)
+    allowed[:vocab] = rng.random(vocab) < 0.3
+    x[:, ~allowed[:vocab]] = np.inf
+    cum = -np.float32(5) * rng.random(rows).astype(np.float32)
+    want = R.select_many(x, beams, k, cum, allowed[:vocab])
+    assert np.isfinite(want[0]).all()
+    for mask in (allowed, allowed[:vocab]):
+        sel = ag.select_beams_op(up(x, kind, dev), beams, k, p, scores=f32(cum, dev), allowed=bits(mask, dev))
+        p.sync()
+        assert_selection(sel, want)
