@@ -190,6 +190,7 @@ class ArrowArrayGPU:
 
     ARROW_TYPE: ArrowType
     DTYPE: int
+    PARTS = ("data",)  # where a tensor's memory may lie (gpu_utils.pipeline_for); a null buffer is this library's
 
     def get_gpu_device(self) -> GpuDevice:
         return self.gpu_device

@@ -74,13 +74,57 @@ def tensor_type(tensor) -> str:
     return t
 
 
+_lent = False  # whether any tensor's memory was ever borrowed
+
+
 def borrow_tensor(tensor, device: "GpuDevice", nbytes: int) -> BorrowedBuffer:
-    """The memory of a tensor on `device` (anything with data_ptr() and get_device(): torch is not needed here).  The rules of torch's own streams hold:
-    the tensor's memory may be given back to its allocator when no work on ANOTHER stream than the tensor's still uses it.  A program that uses
-    torch on the GPU imports it before this library's first call: then both run on the one GPU runtime that torch has loaded."""
+    """The memory of a tensor on `device` (anything with data_ptr() and get_device(): torch is not needed here).  A program that uses
+    torch on the GPU imports it before this library's first call: then both run on the one GPU runtime that torch has loaded.
+
+    Order.  Calls that take no pipeline run on torch's current stream where any of their arguments is a tensor's memory, and are over when they return;
+    reading values back waits for that stream first.  A `*_op` call runs on its pipeline: over torch's current stream
+    (`ArrowComputePipeline(device, hip_stream=torch.cuda.current_stream().cuda_stream)`) it stands in torch's order; a pipeline of its own is not ordered
+    with torch's streams, there the program waits, before and after.  Work of other libraries on tensors of theirs is over before any call.
+
+    Memory.  The rules of torch's own streams hold: the tensor's memory may be given back to its allocator when no work on ANOTHER stream than the
+    tensor's still uses it."""
+    global _lent
     if tensor.get_device() != device.ordinal:  # (of host memory: −1)
         raise capi.ArrowErrorGPU("ArgumentError", f"a tensor on {tensor.device} for a buffer on GPU {device.ordinal}", capi.ERR_ARG)
+    _lent = True
     return BorrowedBuffer(device, tensor.data_ptr(), nbytes, tensor)
+
+
+def _is_lent(x) -> bool:
+    """Whether x — a buffer, an array, rows, a list of them — lies, with any of its PARTS, in a tensor's memory."""
+    if isinstance(x, BorrowedBuffer):
+        return True
+    if isinstance(x, (list, tuple)):
+        return any(map(_is_lent, x))
+    return any(_is_lent(getattr(x, part)) for part in getattr(x, "PARTS", ()))
+
+
+def _torch_stream(device: "GpuDevice"):
+    torch = sys.modules.get("torch")  # (not there: the tensors are another library's)
+    return torch.cuda.current_stream(device.ordinal) if torch is not None else None
+
+
+def pipeline_for(device: "GpuDevice", label: str, *things) -> "ArrowComputePipeline":
+    """The pipeline of a call that takes none: one of its own, or one over torch's current stream where any of `things` is a tensor's memory (what torch
+    has enqueued there is then over before, and the call's work before what torch enqueues next)."""
+    if _lent and _is_lent(things):
+        stream = _torch_stream(device)
+        if stream is not None:
+            return ArrowComputePipeline(device, label, hip_stream=stream.cuda_stream)
+    return ArrowComputePipeline(device, label)
+
+
+def settle(device: "GpuDevice", *things) -> None:
+    """Waits for torch's current stream where any of `things` is a tensor's memory."""
+    if _lent and _is_lent(things):
+        stream = _torch_stream(device)
+        if stream is not None:
+            stream.synchronize()
 
 
 class GpuDevice:
@@ -150,6 +194,7 @@ class GpuDevice:
     def retrive_data(self, buf: DeviceBuffer, nbytes: int | None = None, pipeline=None) -> np.ndarray:
         """Blocking read-back as bytes.  [ref: retrive_data gpu_device.rs:232-265]"""
         nbytes = buf.nbytes if nbytes is None else nbytes
+        settle(self, buf)
         out = np.empty(nbytes, dtype=np.uint8)
         if nbytes <= capi.MAILBOX_MAX_BYTES:  # (with or without `pipeline`: the device-level wait covers its stream too)
             # a scalar, a small array: the device-level wait delivers it on the way — one wait instead of two
@@ -166,7 +211,7 @@ class GpuDevice:
             return pipeline.clone_buffer(buf)
         # immediate form = record + submit, like the reference's queue.submit inside GpuDevice::clone_buffer: `finish`
         # publishes the copy so pipelines that consume the clone are ordered behind it (and this one behind its producer)
-        p = self._default_pipeline()
+        p = pipeline_for(self, "clone_buffer", buf) if isinstance(buf, BorrowedBuffer) else self._default_pipeline()
         out = p.clone_buffer(buf)
         p.finish()
         return out

@@ -23,7 +23,7 @@ from . import _capi as capi
 from .array import (ArrowArrayGPU, BooleanArrayGPU, Date32ArrayGPU, Float32ArrayGPU, Int8ArrayGPU, Int16ArrayGPU,
                     Int32ArrayGPU, NullBitBufferGpu, PrimitiveArrayGpu, UInt8ArrayGPU, UInt16ArrayGPU, UInt32ArrayGPU,
                     bitmap_bytes)
-from .gpu_utils import ArrowComputePipeline, DeviceBuffer, GpuDevice
+from .gpu_utils import ArrowComputePipeline, DeviceBuffer, GpuDevice, settle
 
 
 def _pa():
@@ -205,6 +205,7 @@ def to_arrow(gpu_array: ArrowArrayGPU, pipeline: ArrowComputePipeline | None = N
     else:
         col.null_count = 0
     p = pipeline or ArrowComputePipeline(dev, "to_arrow")
+    settle(dev, gpu_array)
     dev.sync()  # other pipelines may still be writing the array (the reference's read-back polls the whole queue)
     if gpu_array.null_buffer is not None and gpu_array.null_buffer.null_count_known():
         col.null_count = gpu_array.null_buffer.null_count()  # left behind by the kernel that made the bitmap: an 8-byte read, no pass

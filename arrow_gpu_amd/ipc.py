@@ -17,7 +17,7 @@ import numpy as np
 
 from . import _capi as capi
 from .array import ArrowArrayGPU, NullBitBufferGpu
-from .gpu_utils import ArrowComputePipeline, DeviceBuffer, GpuDevice
+from .gpu_utils import ArrowComputePipeline, DeviceBuffer, GpuDevice, settle
 
 
 def _classes():
@@ -233,6 +233,7 @@ class IpcWriter:
         if dev is None:
             raise capi.ArrowErrorGPU("ArgumentError", "write_batch needs at least one column")
         p = pipeline or ArrowComputePipeline(dev, "ipc.write_batch")
+        settle(dev, list(arrays))
         dev.sync()  # other pipelines may still be writing the arrays (same rule as interop.to_arrow)
         capi.call("agpu_ipc_writer_write_device_batch", self._handle, p._handle, cols)
 

@@ -14,7 +14,7 @@ import weakref
 from .. import _capi as capi
 from .._capi import OperationNotSupported
 from ..array import (ArrowArrayGPU, BooleanArrayGPU, NullBitBufferGpu, PrimitiveArrayGpu, bitmap_bytes)
-from ..gpu_utils import ArrowComputePipeline
+from ..gpu_utils import ArrowComputePipeline, pipeline_for
 
 
 def vp(buf):
@@ -25,7 +25,7 @@ def default_impl(op_name: str):
     """`fn x(&self, ..) { let mut pipeline = new(); let r = self.x_op(.., &mut pipeline); pipeline.finish(); r }`"""
 
     def method(self, *args):
-        pipeline = ArrowComputePipeline(self.get_gpu_device(), op_name)
+        pipeline = pipeline_for(self.get_gpu_device(), op_name, self, args)
         out = getattr(self, op_name + "_op")(*args, pipeline)
         pipeline.finish()
         return out
@@ -149,7 +149,7 @@ def dyn_binary(name: str, op_attr: str, same_type, mixed=()):
             f"Operation {name} not supported for type {data_1.get_dtype().name} {data_2.get_dtype().name}")
 
     def fn(data_1, data_2):
-        pipeline = ArrowComputePipeline(data_1.get_gpu_device(), name)
+        pipeline = pipeline_for(data_1.get_gpu_device(), name, data_1, data_2)
         out = fn_op(data_1, data_2, pipeline)
         pipeline.finish()
         return out
@@ -168,7 +168,7 @@ def dyn_unary(name: str, op_attr: str, types):
         raise OperationNotSupported(f"Operation {name} not supported for type {data.get_dtype().name}")
 
     def fn(data):
-        pipeline = ArrowComputePipeline(data.get_gpu_device(), name)
+        pipeline = pipeline_for(data.get_gpu_device(), name, data)
         out = fn_op(data, pipeline)
         pipeline.finish()
         return out

@@ -9,7 +9,7 @@ from __future__ import annotations
 
 from .. import _capi as capi
 from ..array import (Date32ArrayGPU, Float32ArrayGPU, Int32ArrayGPU, UInt16ArrayGPU, UInt32ArrayGPU)
-from ..gpu_utils import ArrowComputePipeline
+from ..gpu_utils import ArrowComputePipeline, pipeline_for
 from ._ops import array_op, dyn_binary, dyn_unary, impl, scalar_op, unary_op, vp
 
 _F32 = (Float32ArrayGPU,)
@@ -109,7 +109,7 @@ def _len_dispatch(name, array_op_dyn, scalar_op_dyn):
         return scalar_op_dyn(input2, input1, pipeline)
 
     def fn(input1, input2):
-        pipeline = ArrowComputePipeline(input1.get_gpu_device(), name)
+        pipeline = pipeline_for(input1.get_gpu_device(), name, input1, input2)
         out = fn_op(input1, input2, pipeline)
         pipeline.finish()
         return out

@@ -10,7 +10,7 @@ from .. import _capi as capi
 from .._capi import CastingNotSupported
 from ..array import (ARRAY_OF_TYPE, ArrowArrayGPU, ArrowType, BooleanArrayGPU, Float32ArrayGPU, Int8ArrayGPU,
                      Int16ArrayGPU, Int32ArrayGPU, NullBitBufferGpu, UInt8ArrayGPU, UInt16ArrayGPU, UInt32ArrayGPU)
-from ..gpu_utils import ArrowComputePipeline
+from ..gpu_utils import ArrowComputePipeline, pipeline_for
 from ._ops import _finish_record, vp
 
 # cast_dyn's table [crates/cast/src/lib.rs:135-161]
@@ -64,7 +64,7 @@ def apply_boolean_unary_function(gpu_device, original_values, new_buffer_size: i
 
 
 def _cast(self, into):
-    p = ArrowComputePipeline(self.get_gpu_device(), "cast")
+    p = pipeline_for(self.get_gpu_device(), "cast", self)
     out = _cast_op(self, into, p)
     p.finish()
     return out
@@ -79,7 +79,7 @@ def _bitcast_op(self, into, pipeline: ArrowComputePipeline):
 
 
 def _bitcast(self, into):
-    p = ArrowComputePipeline(self.get_gpu_device(), "bitcast")
+    p = pipeline_for(self.get_gpu_device(), "bitcast", self)
     out = _bitcast_op(self, into, p)
     p.finish()
     return out
@@ -101,7 +101,7 @@ def cast_op_dyn(from_: ArrowArrayGPU, into: ArrowType, pipeline: ArrowComputePip
 
 
 def cast_dyn(from_: ArrowArrayGPU, into: ArrowType) -> ArrowArrayGPU:
-    p = ArrowComputePipeline(from_.get_gpu_device(), "cast_dyn")
+    p = pipeline_for(from_.get_gpu_device(), "cast_dyn", from_)
     out = cast_op_dyn(from_, into, p)
     p.finish()
     return out
@@ -115,7 +115,7 @@ def bitcast_op_dyn(from_: ArrowArrayGPU, into: ArrowType, pipeline: ArrowCompute
 
 
 def bitcast_dyn(from_: ArrowArrayGPU, into: ArrowType) -> ArrowArrayGPU:
-    p = ArrowComputePipeline(from_.get_gpu_device(), "bitcast_dyn")
+    p = pipeline_for(from_.get_gpu_device(), "bitcast_dyn", from_)
     out = bitcast_op_dyn(from_, into, p)
     p.finish()
     return out

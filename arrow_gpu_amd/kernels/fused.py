@@ -23,7 +23,7 @@ from .. import _capi as capi
 from .._capi import ArrowErrorGPU, OperationNotSupported
 from ..array import (Date32ArrayGPU, Float32ArrayGPU, Int8ArrayGPU, Int16ArrayGPU, Int32ArrayGPU, NullBitBufferGpu, UInt8ArrayGPU,
                      UInt16ArrayGPU, UInt32ArrayGPU)
-from ..gpu_utils import ArrowComputePipeline
+from ..gpu_utils import ArrowComputePipeline, pipeline_for
 from ._ops import vp
 
 MAX_STEPS = 8
@@ -93,7 +93,7 @@ class FusedChain:
         return self.acc_cls(out, dev, a.len, nulls)
 
     def finish(self):
-        p = ArrowComputePipeline(self.src.get_gpu_device(), "fused_chain")
+        p = pipeline_for(self.src.get_gpu_device(), "fused_chain", self.src, [operand for _, _, operand in self.steps])
         out = self.finish_op(p)
         p.finish()
         return out
@@ -131,7 +131,7 @@ class FusedChain:
         return BooleanArrayGPU(out, dev, a.len, nulls)
 
     def _compare(self, name: str, op: int, other):
-        p = ArrowComputePipeline(self.src.get_gpu_device(), "fused_chain_compare")
+        p = pipeline_for(self.src.get_gpu_device(), "fused_chain_compare", self.src, other, [operand for _, _, operand in self.steps])
         out = self._compare_op(name, op, other, p)
         p.finish()
         return out

@@ -14,7 +14,7 @@ import numpy as np
 from .. import _capi as capi
 from ..array import (BooleanArrayGPU, Int8ArrayGPU, Int16ArrayGPU, Int32ArrayGPU, NullBitBufferGpu, UInt8ArrayGPU,
                      UInt16ArrayGPU, UInt32ArrayGPU, bitmap_bytes)
-from ..gpu_utils import ArrowComputePipeline
+from ..gpu_utils import ArrowComputePipeline, pipeline_for
 from ._ops import array_op, check_same_len, dyn_binary, dyn_unary, impl, unary_op, vp
 
 _INTS = (Int32ArrayGPU, UInt32ArrayGPU, UInt16ArrayGPU, Int16ArrayGPU, UInt8ArrayGPU, Int8ArrayGPU)
@@ -57,7 +57,7 @@ impl((BooleanArrayGPU,), "bitwise_not", _bool_not)
 # ---- LogicalContains  [boolean.rs:106-147]  (blocking: they return a host bool, like the reference)
 def _any(self: BooleanArrayGPU) -> bool:
     dev = self.gpu_device
-    p = ArrowComputePipeline(dev, "any")
+    p = pipeline_for(dev, "any", self)
     out = dev.create_empty_buffer(16)
     capi.call("agpu_bitmap_any", p._handle, vp(self.data), self.len, vp(out))
     res = dev.retrive_data(out, 4, pipeline=p).view(np.uint32)[0]
@@ -68,7 +68,7 @@ def _all(self: BooleanArrayGPU) -> bool:
     """popcount(first len bits) == len.  (The reference counts whole words including padding bits, boolean.rs:120-146;
     padding is unspecified there, so only the first `len` bits are counted here.)"""
     dev = self.gpu_device
-    p = ArrowComputePipeline(dev, "all")
+    p = pipeline_for(dev, "all", self)
     out = dev.create_empty_buffer(16)
     capi.call("agpu_bitmap_popcount", p._handle, vp(self.data), self.len, vp(out))
     res = dev.retrive_data(out, 8, pipeline=p).view(np.uint64)[0]
@@ -77,7 +77,7 @@ def _all(self: BooleanArrayGPU) -> bool:
 
 def _count_set_bits(self: BooleanArrayGPU) -> int:
     dev = self.gpu_device
-    p = ArrowComputePipeline(dev, "popcount")
+    p = pipeline_for(dev, "popcount", self)
     out = dev.create_empty_buffer(16)
     capi.call("agpu_bitmap_popcount", p._handle, vp(self.data), self.len, vp(out))
     return int(dev.retrive_data(out, 8, pipeline=p).view(np.uint64)[0])

@@ -13,7 +13,7 @@ from .._capi import OperationNotSupported
 from ..array import (ArrowArrayGPU, BooleanArrayGPU, Date32ArrayGPU, Float32ArrayGPU, Int8ArrayGPU, Int16ArrayGPU,
                      Int32ArrayGPU, NullBitBufferGpu, PrimitiveArrayGpu, UInt8ArrayGPU, UInt16ArrayGPU, UInt32ArrayGPU,
                      bitmap_bytes)
-from ..gpu_utils import ArrowComputePipeline
+from ..gpu_utils import ArrowComputePipeline, pipeline_for
 from ._ops import check_same_len, impl, vp
 
 _PRIMS = (Date32ArrayGPU, Int32ArrayGPU, Int16ArrayGPU, Int8ArrayGPU, UInt32ArrayGPU, UInt16ArrayGPU, UInt8ArrayGPU,
@@ -111,14 +111,14 @@ def _put_op(self: PrimitiveArrayGpu, src_indexes: UInt32ArrayGPU, dst, dst_index
 # never block; the default forms below synchronise before returning so the error surfaces at the call, as it did when
 # the indices were pre-checked with a separate pass.
 def _put(self, src_indexes, dst, dst_indexes) -> None:
-    p = ArrowComputePipeline(self.get_gpu_device(), "put")
+    p = pipeline_for(self.get_gpu_device(), "put", self, src_indexes, dst, dst_indexes)
     self.put_op(src_indexes, dst, dst_indexes, p)
     p.finish()
     p.sync()
 
 
 def _take(self, indexes):
-    p = ArrowComputePipeline(self.get_gpu_device(), "take")
+    p = pipeline_for(self.get_gpu_device(), "take", self, indexes)
     out = self.take_op(indexes, p)
     p.finish()
     p.sync()
@@ -181,7 +181,7 @@ def merge_op_dyn(operand_1: ArrowArrayGPU, operand_2: ArrowArrayGPU, mask: Boole
 
 
 def merge_dyn(operand_1, operand_2, mask):
-    p = ArrowComputePipeline(operand_1.get_gpu_device(), "merge")
+    p = pipeline_for(operand_1.get_gpu_device(), "merge", operand_1, operand_2, mask)
     out = merge_op_dyn(operand_1, operand_2, mask, p)
     p.finish()
     return out
@@ -194,7 +194,7 @@ def take_op_dyn(operand_1: ArrowArrayGPU, indexes: UInt32ArrayGPU, pipeline):
 
 
 def take_dyn(operand_1, indexes):
-    p = ArrowComputePipeline(operand_1.get_gpu_device(), "take")
+    p = pipeline_for(operand_1.get_gpu_device(), "take", operand_1, indexes)
     out = take_op_dyn(operand_1, indexes, p)
     p.finish()
     p.sync()  # surfaces an out-of-range index here (see _take)
@@ -242,7 +242,7 @@ def take_columns_op(columns, indexes: UInt32ArrayGPU, pipeline: ArrowComputePipe
 def take_columns(columns, indexes: UInt32ArrayGPU) -> list:
     if not columns:
         return []
-    p = ArrowComputePipeline(columns[0].gpu_device)
+    p = pipeline_for(columns[0].gpu_device, "take_columns", columns, indexes)
     out = take_columns_op(columns, indexes, p)
     p.finish()
     return out
@@ -256,7 +256,7 @@ def put_op_dyn(src: ArrowArrayGPU, src_indexes, dst: ArrowArrayGPU, dst_indexes,
 
 
 def put_dyn(src, src_indexes, dst, dst_indexes) -> None:
-    p = ArrowComputePipeline(src.get_gpu_device(), "put")
+    p = pipeline_for(src.get_gpu_device(), "put", src, src_indexes, dst, dst_indexes)
     put_op_dyn(src, src_indexes, dst, dst_indexes, p)
     p.finish()
     p.sync()

@@ -1,15 +1,16 @@
 """Operators on whole rows (include/arrow_gpu.h "rows"): put_quantised / take_quantised — take and put with a cast to 8 or 4 bits between them —
 select_beams, whose parents are an index column, and take_rows, which reorders the states by it.  No counterpart in the reference.
 
-As everywhere here the `*_op` forms enqueue on a pipeline and return without waiting; the plain forms run on a pipeline of their own and wait, so
-that an index out of range is raised by the call.  `out` writes into memory the caller has (a torch tensor's, last step's)."""
+As everywhere here the `*_op` forms enqueue on a pipeline and return without waiting; the plain forms run on a pipeline of their own — over tensors'
+memory on torch's current stream — and wait, so that an index out of range is raised by the call.  `out` writes into memory the caller has (a torch
+tensor's, last step's)."""
 from __future__ import annotations
 
 import struct
 
 from .. import _capi as capi
 from ..array import BooleanArrayGPU, Float32ArrayGPU, UInt32ArrayGPU
-from ..gpu_utils import ArrowComputePipeline
+from ..gpu_utils import ArrowComputePipeline, pipeline_for
 from ..rows import ROW_TYPE, BeamSelection, PageMap, QuantisedRowsGPU, RowsGPU, shape_error
 
 _MAX_COLUMNS = 64
@@ -205,8 +206,8 @@ def select_beams_op(logits: RowsGPU, beams: int, k: int, pipeline: ArrowComputeP
     return out
 
 
-def _waited(device, label: str, op):
-    p = ArrowComputePipeline(device, label)
+def _waited(device, label: str, op, *things):
+    p = pipeline_for(device, label, *things)
     got = op(p)
     p.finish()
     p.sync()  # surfaces an index out of range here
@@ -215,21 +216,22 @@ def _waited(device, label: str, op):
 
 def put_quantised(stores, rows, where) -> None:
     first = stores if isinstance(stores, QuantisedRowsGPU) else stores[0]
-    _waited(first.gpu_device, "put_quantised", lambda p: put_quantised_op(stores, rows, where, p))
+    _waited(first.gpu_device, "put_quantised", lambda p: put_quantised_op(stores, rows, where, p), stores, rows, where)
 
 
 def take_quantised(stores, where, type_: str = "f32", n_rows: int | None = None, out=None) -> list:
     first = stores if isinstance(stores, QuantisedRowsGPU) else stores[0]
-    return _waited(first.gpu_device, "take_quantised", lambda p: take_quantised_op(stores, where, p, type_, n_rows, out))
+    return _waited(first.gpu_device, "take_quantised", lambda p: take_quantised_op(stores, where, p, type_, n_rows, out), stores, where, out)
 
 
 def take_rows(states, indexes: UInt32ArrayGPU, lengths: UInt32ArrayGPU | None = None, out=None) -> list:
-    return _waited(indexes.gpu_device, "take_rows", lambda p: take_rows_op(states, indexes, p, lengths, out))
+    return _waited(indexes.gpu_device, "take_rows", lambda p: take_rows_op(states, indexes, p, lengths, out), states, indexes, lengths, out)
 
 
 def select_beams(logits: RowsGPU, beams: int, k: int, scores: Float32ArrayGPU | None = None, allowed: BooleanArrayGPU | None = None,
                  finished: BooleanArrayGPU | None = None, end_token: int = 0, out: BeamSelection | None = None) -> BeamSelection:
-    return _waited(logits.gpu_device, "select_beams", lambda p: select_beams_op(logits, beams, k, p, scores, allowed, finished, end_token, out))
+    return _waited(logits.gpu_device, "select_beams", lambda p: select_beams_op(logits, beams, k, p, scores, allowed, finished, end_token, out),
+                   logits, scores, allowed, finished, out)
 
 
 __all__ = ["put_quantised", "put_quantised_op", "take_quantised", "take_quantised_op", "take_rows", "take_rows_op", "select_beams", "select_beams_op"]

@@ -10,7 +10,7 @@ import numpy as np
 
 from . import _capi as capi
 from .array import Float32ArrayGPU, UInt32ArrayGPU
-from .gpu_utils import DeviceBuffer, GpuDevice, borrow_tensor, tensor_type
+from .gpu_utils import DeviceBuffer, GpuDevice, borrow_tensor, settle, tensor_type
 
 ITEM_SIZE = {"f32": 4, "f16": 2, "bf16": 2, "i8": 1, "u8": 1, "i16": 2, "u16": 2, "i32": 4, "u32": 4, "i64": 8, "f64": 8}
 ROW_TYPE = {"f32": capi.ROW_F32, "f16": capi.ROW_F16, "bf16": capi.ROW_BF16}
@@ -40,6 +40,7 @@ def _dense(shape):
 class RowsGPU:
     """Rows of values in HBM: shape (n, …) of 2 to 4 axes, strides in elements, the values of the last axis next to each other."""
 
+    PARTS = ("data",)
     __slots__ = ("data", "gpu_device", "shape", "strides", "type", "ptr", "item_size", "_rows", "_pieces")
 
     def __init__(self, data: DeviceBuffer, gpu_device: GpuDevice, shape, type_: str, strides=None, ptr: Optional[int] = None):
@@ -129,6 +130,7 @@ class RowsGPU:
     def values(self) -> np.ndarray:
         """The values on the host (bf16: as float32).  Blocking."""
         span = 1 + sum((n - 1) * s for n, s in zip(self.shape, self.strides)) if 0 not in self.shape else 0
+        settle(self.gpu_device, self)
         view = DeviceBuffer(self.gpu_device, self.ptr, span * self.item_size, owned=False)
         flat = self.gpu_device.retrive_data(view).view(_NUMPY[self.type])
         got = np.lib.stride_tricks.as_strided(flat, self.shape, [s * self.item_size for s in self.strides]).copy() if span else np.zeros(self.shape, _NUMPY[self.type])
@@ -147,6 +149,7 @@ class QuantisedRowsGPU:
     code "i8": whole numbers -127..127, "e4m3": 8-bit floating, "i4": whole numbers 0..15 above the group's lowest value.  An empty cache's rows
     read back as zeros."""
 
+    PARTS = ("codes", "scales")
     __slots__ = ("codes", "scales", "gpu_device", "n_slots", "heads", "dim", "group", "code", "shape", "packed")
 
     def __init__(self, codes: DeviceBuffer, scales: DeviceBuffer, gpu_device: GpuDevice, n_slots: int, heads: int, dim: int, group: int, code: str):
@@ -203,6 +206,7 @@ class PageMap:
 
     tables: RowsGPU of u32 / i32, (sequences, pages); offsets: UInt32ArrayGPU of sequences + 1; first: UInt32ArrayGPU of sequences, or none."""
 
+    PARTS = ("tables", "offsets", "first")
     __slots__ = ("tables", "page_rows", "offsets", "first", "packed")
 
     def __init__(self, tables: RowsGPU, page_rows: int, offsets: UInt32ArrayGPU, first: Optional[UInt32ArrayGPU] = None):
@@ -223,6 +227,7 @@ class BeamSelection:
     tokens (UInt32ArrayGPU), best first.  It holds the selection's workspace too: a selection that is passed as `out` again is not in use by two
     calls at one time, and lives as long as a captured graph that writes it."""
 
+    PARTS = ("scores", "parents", "tokens")
     __slots__ = ("scores", "parents", "tokens", "gpu_device", "batch", "k", "workspace", "_workspace_of", "_outgrown")
 
     def __init__(self, scores: Float32ArrayGPU, parents: UInt32ArrayGPU, tokens: UInt32ArrayGPU, gpu_device: GpuDevice, batch: int, k: int):
