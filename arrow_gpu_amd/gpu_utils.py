@@ -86,8 +86,9 @@ def borrow_tensor(tensor, device: "GpuDevice", nbytes: int) -> BorrowedBuffer:
     (`ArrowComputePipeline(device, hip_stream=torch.cuda.current_stream().cuda_stream)`) it stands in torch's order; a pipeline of its own is not ordered
     with torch's streams, there the program waits, before and after.  Work of other libraries on tensors of theirs is over before any call.
 
-    Memory.  The rules of torch's own streams hold: the tensor's memory may be given back to its allocator when no work on ANOTHER stream than the
-    tensor's still uses it."""
+    Memory.  A pipeline of its own holds the tensors of its calls until its sync().  One over torch's stream holds none, the rules of torch's streams do: a
+    tensor's memory goes back to its allocator when its last owner lets go, and is used again in its stream's order (a tensor of another of torch's
+    streams: record_stream)."""
     global _lent
     if tensor.get_device() != device.ordinal:  # (of host memory: −1)
         raise capi.ArrowErrorGPU("ArgumentError", f"a tensor on {tensor.device} for a buffer on GPU {device.ordinal}", capi.ERR_ARG)
@@ -262,6 +263,7 @@ class ArrowComputePipeline:
     def __init__(self, device: GpuDevice, label: str | None = None, hip_stream: int | None = None, fuse: bool | None = None):
         self.device = device
         self.label = label
+        self.own_stream = hip_stream is None
         h = C.c_void_p()
         if hip_stream is None:
             capi.call("agpu_pipeline_create", device._handle, C.byref(h))

@@ -19,7 +19,10 @@ _PACK_BEAMS = struct.Struct("=QQiIIIIIQQQQQQQQQ")  # agpu_beams
 
 
 def _keep(pipeline, *buffers) -> None:
-    """Buffers of this library's own: a borrowed one's lifetime is its owner's affair."""
+    """The buffers of a call, until the pipeline's sync(); tensors' memory only where torch's stream does not keep its order."""
+    if pipeline.own_stream:
+        pipeline.keep(*buffers)
+        return
     for b in buffers:
         if b._owned:
             pipeline.keep(b)
@@ -59,10 +62,10 @@ def _quantised(name: str, stores, rows, where, n: int, pipeline) -> None:
         if where.gpu_device is not dev:
             _on(pipeline, where)
         capi.call(name, pipeline._handle, len(stores), s, r, where.data.ptr, n)
-        if where.data._owned:
+        if where.data._owned or pipeline.own_stream:
             pipeline.keep(where.data)
     for store, x in zip(stores, rows):
-        if store.codes._owned or store.scales._owned or x.data._owned:
+        if pipeline.own_stream or store.codes._owned or store.scales._owned or x.data._owned:
             _keep(pipeline, store.codes, store.scales, x.data)
 
 
@@ -147,10 +150,10 @@ def take_rows_op(states, indexes: UInt32ArrayGPU, pipeline: ArrowComputePipeline
             _on(pipeline, x)
     capi.call("agpu_take_rows", pipeline._handle, len(states), packed, n_src, indexes.data.ptr, lengths.data.ptr if lengths is not None else None, n)
     for x in given:
-        if x.data._owned:
+        if x.data._owned or pipeline.own_stream:
             pipeline.keep(x.data)
     for s, o in zip(states, out):
-        if s.data._owned or o.data._owned:
+        if pipeline.own_stream or s.data._owned or o.data._owned:
             _keep(pipeline, s.data, o.data)
     return out
 
@@ -200,7 +203,7 @@ def select_beams_op(logits: RowsGPU, beams: int, k: int, pipeline: ArrowComputeP
                             work.ptr, work.nbytes)
     capi.call("agpu_select_beams", pipeline._handle, args)
     for x in given:
-        if x.data._owned:
+        if x.data._owned or pipeline.own_stream:
             pipeline.keep(x.data)
     _keep(pipeline, out.scores.data, out.parents.data, out.tokens.data, work)
     return out

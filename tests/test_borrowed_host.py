@@ -163,3 +163,26 @@ def test_reading_back_waits_for_torchs_stream(monkeypatch):
     with pytest.raises(Made):
         mine.values()
     assert not waited
+
+
+@pytest.mark.parametrize("own_stream", [True, False])
+def test_a_pipeline_of_its_own_holds_the_tensors_of_its_calls(monkeypatch, own_stream):
+    """their memory would otherwise go back to torch while a kernel on a stream that torch does not know still uses it; torch's own stream keeps its order"""
+    import arrow_gpu_amd.kernels.rows as K
+
+    kept = []
+    monkeypatch.setattr(K.capi, "call", lambda *a: None)
+    pipe = types.SimpleNamespace(device=DEV, _handle=None, keep=lambda *b: kept.extend(b), own_stream=own_stream)
+    cache, rows, index, pages = CACHE(True), ROWS((3, 2, 8), True), INDEX(3, True), PAGES(True, True, True)
+    state, out, parents, lengths = ROWS((3, 5, 2), True), ROWS((3, 5, 2), True), INDEX(3, True), INDEX(3, True)
+    logits, scores, mask, sel = ROWS((4, 64), True), FLOATS(4, True), BITS(64, True), SELECTION(True)
+    sel.workspace, sel._workspace_of = ag.DeviceBuffer(DEV, 4096, 1 << 20, owned=False), (2, 64)
+    for call, things in ((lambda: ag.put_quantised_op(cache, rows, index, pipe), (cache.codes, cache.scales, rows.data, index.data)),
+                         (lambda: ag.take_quantised_op(cache, pages, pipe, out=rows), (cache.codes, cache.scales, rows.data, pages.tables.data, pages.offsets.data, pages.first.data)),
+                         (lambda: ag.take_rows_op(state, parents, pipe, lengths=lengths, out=out), (state.data, out.data, parents.data, lengths.data)),
+                         (lambda: ag.select_beams_op(logits, 2, 2, pipe, scores=scores, allowed=mask, out=sel),
+                          (logits.data, scores.data, mask.data, sel.scores.data, sel.parents.data, sel.tokens.data))):
+        call()
+        lent = [b for b in kept if isinstance(b, gpu_utils.BorrowedBuffer)]
+        assert {id(b) for b in lent} == ({id(b) for b in things} if own_stream else set())
+        kept.clear()
