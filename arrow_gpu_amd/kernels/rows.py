@@ -115,8 +115,8 @@ def take_quantised_op(stores, where, pipeline: ArrowComputePipeline, type_: str 
 
 def take_rows_op(states, indexes: UInt32ArrayGPU, pipeline: ArrowComputePipeline, lengths: UInt32ArrayGPU | None = None, out=None) -> list:
     """[row indexes[i] of every state]: the states reordered by a selection's parents (any element type, 2 to 4 axes: rows, (pieces,) (positions,)
-    values).  lengths: per row how many positions (the axis before the last) hold anything; what lies behind them is left as it was in `out` (in
-    memory allocated here: unspecified).  An index out of range gives a row of zeros, and ShapeError at the next sync; 0xFFFFFFFF leaves it."""
+    values; the positions of four axes lie next to each other, of three they may lie apart).  lengths: per row how many positions (the axis before the last,
+    next to each other) hold anything; what lies behind them is left as it was in `out` (in memory allocated here: unspecified).  An index out of range gives a row of zeros, and ShapeError at the next sync; 0xFFFFFFFF leaves it."""
     states = [states] if isinstance(states, RowsGPU) else states
     out = [out] if isinstance(out, RowsGPU) else out
     n = _u32(indexes, "indexes").len
@@ -137,8 +137,9 @@ def take_rows_op(states, indexes: UInt32ArrayGPU, pipeline: ArrowComputePipeline
             raise shape_error(f"rows {there} from a state {here} by {n} indexes, in a call over {n_src} rows")
         row, step, pieces, size, position = s._pieces or s.as_pieces()
         out_row, out_step, out_pieces, out_size, _ = o._pieces or o.as_pieces()
-        if (pieces, size) != (out_pieces, out_size):
-            raise shape_error(f"the pieces of {tuple(s.shape)}: strides {s.strides} and {o.strides}")
+        if (pieces, size) != (out_pieces, out_size):  # of three axes, one of the two dense and the other not
+            row, step, pieces, size, position = s.as_split_pieces()
+            out_row, out_step, *_ = o.as_split_pieces()
         if lengths is not None and not position:
             raise shape_error("lengths count positions, the axis before the last: they lie next to each other")
         packed += _PACK_STATE.pack(s.ptr, o.ptr, row, step, out_row, out_step, pieces, size, position)

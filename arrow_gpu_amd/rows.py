@@ -98,6 +98,11 @@ class RowsGPU:
             self._pieces = (strides[0] * item, strides[1] * item if axis == 2 else 0, shape[1] if axis == 2 else 1, inner * item, counted)
         return self._pieces
 
+    def as_split_pieces(self):
+        """as_pieces() of (n, positions, values) with each position a piece of its own: beside a state whose positions do not lie densely."""
+        item, (_, positions, values) = self.item_size, self.shape
+        return self.strides[0] * item, self.strides[1] * item, positions, values * item, 0
+
     @classmethod
     def empty(cls, shape, type_: str, gpu_device: GpuDevice) -> "RowsGPU":
         if type_ not in ITEM_SIZE:

@@ -434,6 +434,28 @@ def test_take_rows_of_slices(dev, p, at, pitch):
     assert np.array_equal(got, want)
 
 
+@pytest.mark.parametrize("type_,wide", [("u8", np.uint8), ("bf16", np.uint16), ("f32", np.uint32)])
+def test_take_rows_whose_positions_lie_apart(dev, p, type_, wide):
+    """(rows, positions, values) with a gap behind each position: into dense rows that the call allocates, and from dense rows into gaps that stay as they were"""
+    import arrow_gpu_amd as ag
+
+    rng = np.random.default_rng(12)
+    rows, positions, values, pitch = 7, 9, 21, 26
+    whole = rng.integers(0, np.iinfo(wide).max, (rows, positions, pitch), dtype=wide, endpoint=True)
+    raw = lambda b, shape: dev.retrive_data(b).view(wide)[:int(np.prod(shape))].reshape(shape)  # noqa: E731
+    apart = lambda b: ag.RowsGPU(b, dev, (rows, positions, values), type_, (positions * pitch, pitch, 1))  # noqa: E731
+    idx = rng.integers(0, rows, rows)
+    got = ag.take_rows_op(apart(dev.create_gpu_buffer_with_data(whole)), u32(idx, dev), p)[0]
+    p.sync()
+    assert np.array_equal(raw(got.data, (rows, positions, values)), whole[idx][..., :values])
+    into = dev.create_gpu_buffer_with_data(np.full_like(whole, 7))
+    ag.take_rows_op(got, u32(idx, dev), p, out=apart(into))
+    p.sync()
+    want = np.full_like(whole, 7)
+    want[..., :values] = whole[idx][idx][..., :values]
+    assert np.array_equal(raw(into, whole.shape), want)
+
+
 def test_take_rows_past_32_bits(dev, p):
     """a state of more than 4 GiB"""
     import arrow_gpu_amd as ag

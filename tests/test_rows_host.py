@@ -283,6 +283,27 @@ def test_python_refusals():
     assert e.value.status == capi.ERR_ARG
 
 
+def test_positions_that_lie_apart_go_into_dense_rows_and_back(monkeypatch):
+    """(rows, positions, values): each position is a piece, in the state and in the output, whichever of the two is dense"""
+    import arrow_gpu_amd.kernels.rows as K
+
+    ag, dev, buf, _ = _host()
+    pipe = types.SimpleNamespace(device=dev, _handle=None, keep=lambda *a: None, own_stream=True)
+    called = []
+    monkeypatch.setattr(K.capi, "call", lambda *a: called.append(a))
+    idx = ag.UInt32ArrayGPU(buf(12), dev, 3, None)
+    apart = ag.RowsGPU(buf(1), dev, (3, 5, 4), "f16", (100, 8, 1))
+    dense = ag.RowsGPU(ag.DeviceBuffer(dev, 8192, 1, owned=False), dev, (3, 5, 4), "f16")
+    for s, o, want in ((apart, dense, (4096, 8192, 200, 16, 40, 8, 5, 8, 0)), (dense, apart, (8192, 4096, 40, 8, 200, 16, 5, 8, 0)),
+                       (apart, apart, (4096, 4096, 200, 16, 200, 16, 5, 8, 0)), (dense, dense, (8192, 8192, 40, 0, 40, 0, 1, 40, 8))):
+        assert K.take_rows_op(s, idx, pipe, out=o) == [o]
+        assert called.pop()[3] == bytes(StateStruct(*want))
+        if s is not o or s is apart:
+            with pytest.raises(ag.ArrowErrorGPU) as e:
+                K.take_rows_op(s, idx, pipe, lengths=idx, out=o)
+            assert e.value.status == capi.ERR_SHAPE and not called
+
+
 # ------------------------------------------------------------------------------------------------- slots, broken tables too
 SRC = r"""
 #include "%s/arrow_gpu_amd/csrc/row_address.hpp"
