@@ -352,7 +352,13 @@ __global__ __launch_bounds__(AGPU_BLOCK) void take_group_kernel(QuantCol c, Quan
 }
 
 // ---------------------------------------------------------------- host: checks and dispatch
-agpu_status check_columns(int32_t n_cols, const agpu_quantised_rows* stores, const agpu_rows* rows, uint64_t n, bool writes_rows) {
+// where: the slot column, or the page map's three columns
+agpu_status check_columns(int32_t n_cols, const agpu_quantised_rows* stores, const agpu_rows* rows, uint64_t n, bool writes_rows, std::initializer_list<Places> where) {
+  Places places[3 * 64 + 3];
+  uint32_t count = 0;
+  if (writes_rows)
+    for (const Places& w : where)
+      if (w.at && w.size) places[count++] = w;
   for (int32_t k = 0; k < n_cols; k++) {
     const agpu_quantised_rows& s = stores[k];
     const agpu_rows& r = rows[k];
@@ -367,7 +373,22 @@ agpu_status check_columns(int32_t n_cols, const agpu_quantised_rows* stores, con
     AGPU_REQUIRE(aligned_to(r.data, r.row_type == AGPU_ROW_F32 ? 4 : 2) && aligned_to(s.scales, 4), AGPU_ERR_SHAPE, "alignment");
     if (writes_rows) {
       AGPU_REQUIRE(disjoint(n, r.row_stride, s.heads, r.head_stride, s.dim), AGPU_ERR_SHAPE, "rows that are written may not overlap");
+      const uint64_t item = r.row_type == AGPU_ROW_F32 ? 4 : 2;
+      uint64_t bytes;
+      AGPU_REQUIRE(r.row_stride < (1ull << 61) && r.head_stride < (1ull << 61) &&
+                       extent(n, r.row_stride * item, s.heads, r.head_stride * item, s.dim * item, &bytes), AGPU_ERR_SHAPE, "rows past the address space");
+      places[count++] = {reinterpret_cast<uintptr_t>(r.data), n, r.row_stride * item, s.heads, r.head_stride * item, s.dim * item, true, 2 * k};
     }
+    const uint64_t values = s.n_slots * s.heads * s.dim, pair = s.code == AGPU_CODE_I4 ? 2 : 1;
+    if (s.n_slots == 0) continue;
+    places[count++] = {reinterpret_cast<uintptr_t>(s.codes), 1, 0, 1, 0, values / pair, !writes_rows, 2 * k + 1};
+    places[count++] = {reinterpret_cast<uintptr_t>(s.scales), 1, 0, 1, 0, values / s.group * 4 * pair, !writes_rows, 2 * k + 1};
+  }
+  uint32_t x, y;
+  if (overlapping(places, count, &x, &y)) {
+    AGPU_REQUIRE(writes_rows, AGPU_ERR_ARG, "two columns into one cache");
+    AGPU_REQUIRE(places[x].written && places[y].written, AGPU_ERR_ARG, "rows that are written overlap a cache or the slots");
+    AGPU_REQUIRE(false, AGPU_ERR_ARG, "the rows of two columns overlap");
   }
   return AGPU_OK;
 }
@@ -453,7 +474,7 @@ agpu_status quantised_slots(agpu_pipeline* p, bool put, int32_t n_cols, const ag
   AGPU_REQUIRE(stores && rows && slots, AGPU_ERR_ARG, "null pointer");
   AGPU_REQUIRE(n < (1ull << 31), AGPU_ERR_SHAPE, "n < 2^31");
   AGPU_REQUIRE(aligned_to(slots, 4), AGPU_ERR_SHAPE, "alignment");
-  const agpu_status st = check_columns(n_cols, stores, rows, n, !put);
+  const agpu_status st = check_columns(n_cols, stores, rows, n, !put, {{reinterpret_cast<uintptr_t>(slots), 1, 0, 1, 0, 4 * n, false, -1}});
   if (st != AGPU_OK) return st;
   a.slots = slots;
   return quantised(p, put, n_cols, stores, rows, a, n, name);
@@ -468,7 +489,11 @@ agpu_status quantised_pages(agpu_pipeline* p, bool put, int32_t n_cols, const ag
   AGPU_REQUIRE(m->n_seqs > 0 && m->n_seqs < (1u << 31) && m->page_rows > 0, AGPU_ERR_SHAPE, "1 <= n_seqs < 2^31, page_rows >= 1");
   AGPU_REQUIRE(m->max_pages == 0 || m->tables, AGPU_ERR_ARG, "null pointer");
   AGPU_REQUIRE(aligned_to(m->tables, 4) && aligned_to(m->offsets, 4) && aligned_to(m->first, 4), AGPU_ERR_SHAPE, "alignment");
-  const agpu_status st = check_columns(n_cols, stores, rows, n, !put);
+  uint64_t tables;
+  AGPU_REQUIRE(m->table_stride < (1ull << 61) && extent(m->n_seqs, 4 * m->table_stride, 1, 0, 4ull * m->max_pages, &tables), AGPU_ERR_SHAPE, "page tables past the address space");
+  const agpu_status st = check_columns(n_cols, stores, rows, n, !put, {{reinterpret_cast<uintptr_t>(m->tables), m->n_seqs, 4 * m->table_stride, 1, 0, 4ull * m->max_pages, false, -1},
+                                                                       {reinterpret_cast<uintptr_t>(m->offsets), 1, 0, 1, 0, 4ull * m->n_seqs + 4, false, -1},
+                                                                       {reinterpret_cast<uintptr_t>(m->first), 1, 0, 1, 0, 4ull * m->n_seqs, false, -1}});
   if (st != AGPU_OK) return st;
   const RowAddr a = {nullptr, m->tables, m->table_stride, m->offsets, m->first, m->n_seqs, m->max_pages, m->page_rows};
   return quantised(p, put, n_cols, stores, rows, a, n, name);
@@ -544,18 +569,11 @@ __global__ __launch_bounds__(AGPU_BLOCK) void take_rows_kernel(States states, ui
     if (to[u] != ROW_NONE) __builtin_nontemporal_store(w[u], reinterpret_cast<u32x4_at_1*>(s.dst + to[u]));
 }
 
-// bytes from the first to behind the last of n rows; 0: none.  false: past 2^63
-bool extent(uint64_t n, uint64_t row_stride, uint64_t pieces, uint64_t piece_stride, uint64_t piece_bytes, uint64_t* out) {
-  uint64_t a, b;
-  if (n == 0 || pieces == 0 || piece_bytes == 0) {
-    *out = 0;
-    return true;
-  }
-  return !__builtin_mul_overflow(n - 1, row_stride, &a) && !__builtin_mul_overflow(pieces - 1, piece_stride, &b) && !__builtin_add_overflow(a, b, &a) &&
-         !__builtin_add_overflow(a, piece_bytes, out) && *out < (1ull << 63);
-}
-
-agpu_status check_states(int32_t n_states, const agpu_state* states, uint64_t n_src, const uint32_t* lengths, uint64_t n) {
+agpu_status check_states(int32_t n_states, const agpu_state* states, uint64_t n_src, const uint32_t* idx, const uint32_t* lengths, uint64_t n) {
+  Places places[2 * 64 + 2];
+  uint32_t count = 0;
+  for (const uint32_t* column : {idx, lengths})
+    if (column) places[count++] = {reinterpret_cast<uintptr_t>(column), 1, 0, 1, 0, 4 * n, false, -1};
   for (int32_t k = 0; k < n_states; k++) {
     const agpu_state& s = states[k];
     if (s.n_pieces == 0 || s.piece_bytes == 0) continue;
@@ -567,13 +585,15 @@ agpu_status check_states(int32_t n_states, const agpu_state* states, uint64_t n_
     AGPU_REQUIRE(disjoint(n, s.dst_row_stride, s.n_pieces, s.dst_piece_stride, s.piece_bytes), AGPU_ERR_SHAPE, "rows that are written may not overlap");
     AGPU_REQUIRE(row_bytes < (1ull << 31), AGPU_ERR_SHAPE, "a row holds less than 2^31 bytes");
     AGPU_REQUIRE(!lengths || s.position_bytes > 0, AGPU_ERR_SHAPE, "lengths need position_bytes");
-    for (int32_t j = 0; j < n_states; j++) {
-      const agpu_state& o = states[j];
-      uint64_t there;
-      if (!extent(n_src, o.src_row_stride, o.n_pieces, o.src_piece_stride, o.piece_bytes, &there) || there == 0) continue;
-      const uintptr_t d = reinterpret_cast<uintptr_t>(s.dst), f = reinterpret_cast<uintptr_t>(o.src);
-      AGPU_REQUIRE(d + to <= f || f + there <= d, AGPU_ERR_ARG, "a dst overlaps a src");
-    }
+    // (its src and its dst are compared too: rows are not reordered in place)
+    places[count++] = {reinterpret_cast<uintptr_t>(s.dst), n, s.dst_row_stride, s.n_pieces, s.dst_piece_stride, s.piece_bytes, true, 2 * k};
+    if (from) places[count++] = {reinterpret_cast<uintptr_t>(s.src), n_src, s.src_row_stride, s.n_pieces, s.src_piece_stride, s.piece_bytes, false, 2 * k + 1};
+  }
+  uint32_t x, y;
+  if (overlapping(places, count, &x, &y)) {
+    AGPU_REQUIRE(places[x].owner >= 0 && places[y].owner >= 0, AGPU_ERR_ARG, "a dst overlaps the indexes or the lengths");
+    AGPU_REQUIRE(places[x].written && places[y].written, AGPU_ERR_ARG, "a dst overlaps a src");
+    AGPU_REQUIRE(false, AGPU_ERR_ARG, "two dsts overlap");
   }
   return AGPU_OK;
 }
@@ -602,7 +622,7 @@ agpu_status agpu_take_rows(agpu_pipeline* p, int32_t n_states, const agpu_state*
   AGPU_REQUIRE(aligned_to(idx, 4) && aligned_to(lengths, 4), AGPU_ERR_SHAPE, "alignment");
   AGPU_REQUIRE(n <= (1ull << 32) && n_src <= (1ull << 32), AGPU_ERR_SHAPE, "at most 2^32 rows");
   if (any) {
-    const agpu_status st = check_states(n_states, states, n_src, lengths, n);
+    const agpu_status st = check_states(n_states, states, n_src, idx, lengths, n);
     if (st != AGPU_OK) return st;
   }
   AGPU_BIND(p);

@@ -568,14 +568,15 @@ typedef struct agpu_page_map {
 /* stores[c] row slots[i] = rows[c] row i, quantised, for i < n < 2^31 and c < n_cols <= 64: the columns of one table (keys, values, of one layer or
  * of all) by one slot column.  A slot >= n_slots is dropped and reported by the next agpu_pipeline_sync (AGPU_ERR_SHAPE), as for put.  The slots of
  * one call are distinct (AGPU_NO_ROW aside): of a slot named twice the codes and scales may come from either row.  The rows may be
- * the same one many times (stride 0); neither they nor the slots lie in a cache that is written. */
+ * the same one many times (stride 0); neither they nor the slots lie in a cache that is written, and no two columns go into one (AGPU_ERR_ARG). */
 agpu_status agpu_put_quantised(agpu_pipeline* p, int32_t n_cols, const agpu_quantised_rows* stores, const agpu_rows* rows,
                                const uint32_t* slots, uint64_t n);
 agpu_status agpu_put_quantised_pages(agpu_pipeline* p, int32_t n_cols, const agpu_quantised_rows* stores, const agpu_rows* rows,
                                      const agpu_page_map* pages, uint64_t n);
 /* rows[c] row i = the values of stores[c] row slots[i], rounded once to the rows' type from f32.  A slot >= n_slots gives a row of zeros and is
  * reported; a row whose slot is AGPU_NO_ROW is left as it was.  Rows (or heads) that are written lie beside each other: all heads of a row before
- * the next row's, or all rows of a head before the next head's. */
+ * the next row's, or all rows of a head before the next head's.  What is written overlaps neither another column's rows nor what is read (AGPU_ERR_ARG);
+ * columns that lie interleaved, one behind the other within a common stride, are apart. */
 agpu_status agpu_take_quantised(agpu_pipeline* p, int32_t n_cols, const agpu_quantised_rows* stores, const agpu_rows* rows,
                                 const uint32_t* slots, uint64_t n);
 agpu_status agpu_take_quantised_pages(agpu_pipeline* p, int32_t n_cols, const agpu_quantised_rows* stores, const agpu_rows* rows,
@@ -594,8 +595,8 @@ typedef struct agpu_state {
 /* dst row i = src row idx[i], i < n, of every state (n_states <= 64): the reordering of the states by a selection's parents, whatever the bytes
  * are.  lengths (may be NULL): only the first lengths[i] positions of row i's pieces are copied (all, if they are more than a piece holds), what
  * lies behind them is left as it was.  idx[i] >= n_src: a row of zeros (of that length), reported by the next sync; AGPU_NO_ROW: the row is left as
- * it was.  No dst may overlap a src (AGPU_ERR_ARG): rows are not reordered in place.  A row holds less than 2^31 bytes, a length less than 2^32
- * positions. */
+ * it was.  No dst may overlap a src, another dst, idx or lengths (AGPU_ERR_ARG): rows are not reordered in place.  States that lie interleaved, one behind
+ * the other within a common stride, are apart.  A row holds less than 2^31 bytes, a length less than 2^32 positions. */
 agpu_status agpu_take_rows(agpu_pipeline* p, int32_t n_states, const agpu_state* states, uint64_t n_src, const uint32_t* idx,
                            const uint32_t* lengths, uint64_t n);
 

@@ -456,6 +456,27 @@ def test_take_rows_whose_positions_lie_apart(dev, p, type_, wide):
     assert np.array_equal(raw(into, whole.shape), want)
 
 
+def test_states_that_lie_interleaved_in_one_allocation(dev, p):
+    """[rows, (old keys, new keys, old values, new values), heads, values]: taken from their places into those beside them"""
+    import arrow_gpu_amd as ag
+
+    rng = np.random.default_rng(17)
+    rows, heads, values = 9, 3, 21
+    whole = rng.integers(0, 65536, (rows, 4, heads, values), dtype=np.uint16)
+    buf = dev.create_gpu_buffer_with_data(whole)
+    part = lambda i: ag.RowsGPU(buf, dev, (rows, heads, values), "f16", (4 * heads * values, values, 1), buf.ptr + 2 * i * heads * values)  # noqa: E731
+    idx = rng.integers(0, rows, rows)
+    ag.take_rows_op([part(0), part(2)], u32(idx, dev), p, out=[part(1), part(3)])
+    p.sync()
+    want = whole.copy()
+    want[:, 1], want[:, 3] = whole[idx, 0], whole[idx, 2]
+    assert np.array_equal(dev.retrive_data(buf).view(np.uint16)[:whole.size].reshape(whole.shape), want)
+    for states, out in (([part(0)], [part(0)]), ([part(0), part(2)], [part(1), part(1)]), ([part(0), part(1)], [part(2), part(0)])):
+        with pytest.raises(ag.ArrowErrorGPU) as e:
+            ag.take_rows_op(states, u32(idx, dev), p, out=out)
+        assert e.value.status == capi.ERR_ARG
+
+
 def test_take_rows_past_32_bits(dev, p):
     """a state of more than 4 GiB"""
     import arrow_gpu_amd as ag

@@ -193,6 +193,53 @@ def test_the_largest_calls():
     assert "2^48" in status("agpu_put_quantised", None, 1, C.byref(s), C.byref(r), 1 << 23, 1 << 29)[1]
 
 
+def test_what_is_written_lies_apart():
+    """two outputs on each other, an output on an index column or on a cache; and what lies interleaved in one allocation is none of these"""
+    def state(**kw):
+        a = dict(src=1 << 30, dst=1 << 40, src_row_stride=4096, src_piece_stride=1024, dst_row_stride=4096, dst_piece_stride=1024, n_pieces=4, piece_bytes=1024, position_bytes=64)
+        a.update(kw)
+        return StateStruct(**a)
+
+    def call(*states, idx=1 << 20, lengths=None):
+        return status("agpu_take_rows", None, len(states), (StateStruct * len(states))(*states), 8, idx, lengths, 8)
+
+    other = dict(src=1 << 31)
+    for dst in (1 << 40, (1 << 40) + 8 * 4096 - 1, (1 << 40) - 8 * 4096 + 1, (1 << 40) + 1024):
+        assert call(state(), state(**other, dst=dst))[0] == capi.ERR_ARG and "dsts" in capi.last_error()
+    assert NO_PIPELINE[1] in call(state(), state(**other, dst=(1 << 40) + 8 * 4096))[1]
+    # the halves of rows of 8192 bytes, of pieces of 2048; source and destination of one state, and two states
+    row, piece = dict(src_row_stride=8192, dst_row_stride=8192), dict(src_row_stride=8192, dst_row_stride=8192, src_piece_stride=2048, dst_piece_stride=2048)
+    for kw, step in ((row, 4096), (piece, 1024)):
+        for off, ok in ((step, True), (-step, True), (0, False), (step - 1, False), (step + 1, False), (8 * 8192 + step, True), (3 * 8192 - step, True), (3 * 8192, False)):
+            for got in (call(state(**kw, dst=(1 << 30) + off)), call(state(**kw), state(**kw, src=1 << 31, dst=(1 << 40) + off))):
+                assert (NO_PIPELINE[1] in got[1]) == ok and (ok or got[0] == capi.ERR_ARG and "overlap" in got[1]), (kw, off, got)
+    for kw in (dict(idx=(1 << 40) + 64), dict(idx=(1 << 40) - 28), dict(lengths=(1 << 40) + 4096 * 8 - 4)):
+        assert call(state(), **kw)[0] == capi.ERR_ARG and "lengths" in capi.last_error()
+    assert NO_PIPELINE[1] in call(state(), idx=(1 << 40) - 32, lengths=(1 << 40) + 8 * 4096)[1]
+
+    def columns(name, stores, rws, at=1 << 23):
+        return status(name, None, len(stores), (QuantisedRowsStruct * len(stores))(*stores), (RowsStruct * len(rws))(*rws), at, 4)
+
+    two = [store(), store(codes=1 << 26, scales=1 << 27)]
+    take, put = "agpu_take_quantised", "agpu_put_quantised"
+    assert NO_PIPELINE[1] in columns(take, two, [rows(), rows(data=(1 << 22) + 1024)])[1]                # 4 rows of 256 bytes, one behind the other
+    assert NO_PIPELINE[1] in columns(take, two, [rows(row_stride=256), rows(row_stride=256, data=(1 << 22) + 256)])[1]  # beside each other in wider rows
+    assert columns(take, two, [rows(), rows()])[0] == capi.ERR_ARG and "two columns" in capi.last_error()
+    assert columns(take, two, [rows(), rows(data=(1 << 22) + 1022)])[0] == capi.ERR_ARG
+    assert NO_PIPELINE[1] in columns(put, two, [rows(), rows()])[1]                                      # read twice
+    for at in (1 << 20, (1 << 20) + 1022, (1 << 21) + 60, (1 << 23) + 8, (1 << 26)):
+        assert columns(take, two, [rows(), rows(data=at)])[0] == capi.ERR_ARG and "cache or the slots" in capi.last_error(), at
+    assert NO_PIPELINE[1] in columns(take, two, [rows(), rows(data=(1 << 20) + 1024)])[1]
+    assert NO_PIPELINE[1] in columns(take, [store(), store()], [rows(), rows(data=1 << 25)])[1]          # one cache read twice
+    for kw in ({}, dict(codes=(1 << 20) + 1023), dict(codes=(1 << 21) + 32), dict(scales=(1 << 20) + 4, codes=1 << 26)):
+        assert columns(put, [store(), store(**kw)], [rows(), rows()])[0] == capi.ERR_ARG and "one cache" in capi.last_error()
+    pages = PageMapStruct(1 << 24, 4, 1 << 25, 1 << 28, 3, 4, 16)
+    for at, ok in ((1 << 24, False), ((1 << 24) + 44, False), ((1 << 24) + 48, True), ((1 << 25) + 12, False), ((1 << 25) + 16, True), ((1 << 28) + 8, False)):
+        st, msg = status("agpu_take_quantised_pages", None, 1, C.byref(store()), C.byref(rows(data=at)), C.byref(pages), 4)
+        assert (NO_PIPELINE[1] in msg) == ok and (ok or st == capi.ERR_ARG), (at, msg)
+    assert "address space" in status("agpu_take_quantised", None, 1, C.byref(store()), C.byref(rows(row_stride=1 << 62)), 1 << 23, 4)[1]
+
+
 # ---------------------------------------------------------------------------------------------------------- the Python host
 class _Device:
     ordinal = 0
@@ -332,10 +379,19 @@ extern "C" uint32_t divide(uint32_t d) {  // the first x from 0, or around the m
 """
 
 
+APART = r"""
+extern "C" int overlap(const uint64_t* a, const uint64_t* b) {  // at, n, row stride, m, part stride, size
+  Places p[2] = {{a[0], a[1], a[2], a[3], a[4], a[5], true, 0}, {b[0], b[1], b[2], b[3], b[4], b[5], false, 1}};
+  uint32_t x, y;
+  return overlapping(p, 2, &x, &y);
+}
+"""
+
+
 @pytest.fixture(scope="module")
 def slots_lib(tmp_path_factory):
     d = tmp_path_factory.mktemp("rows")
-    (d / "s.cpp").write_text(SRC % ROOT + DIVIDE)
+    (d / "s.cpp").write_text(SRC % ROOT + DIVIDE + APART)
     subprocess.run(["g++", "-std=c++17", "-O1", "-Wall", "-Werror", "-shared", "-fPIC", "-o", str(d / "s.so"), str(d / "s.cpp")], check=True, timeout=120)
     return C.CDLL(str(d / "s.so"))
 
@@ -353,6 +409,42 @@ def test_quotients_by_products(slots_lib):
     rng = np.random.default_rng(0)
     for d in [*range(1, 300), *(1 << np.arange(31)).tolist(), *((1 << np.arange(2, 31)) - 1).tolist(), *((1 << np.arange(30)) + 1).tolist(), *rng.integers(1, 1 << 31, 200).tolist(), (1 << 31) - 1]:
         assert slots_lib.divide(C.c_uint32(int(d))) == 0xFFFFFFFF, d
+
+
+def test_places_that_are_called_apart_share_no_byte(slots_lib):
+    """against the sets of their bytes, for random strides; and rows, parts or both within a common stride are found apart"""
+    rng = np.random.default_rng(0)
+
+    def bytes_of(at, n, row, m, part, size):
+        return {at + i * row + j * part + k for i in range(n) for j in range(m) for k in range(size)}
+
+    def overlap(a, b):
+        return slots_lib.overlap((C.c_uint64 * 6)(*a), (C.c_uint64 * 6)(*b)) != 0
+
+    apart = meet = 0
+    for _ in range(20000):
+        strides = rng.integers(0, 40, 3).tolist()
+        some = lambda: [int(rng.integers(0, 120)), int(rng.integers(1, 5)), int(rng.choice(strides)) * int(rng.integers(1, 4)), int(rng.integers(1, 4)),  # noqa: E731, B023
+                        int(rng.choice(strides)), int(rng.integers(1, 12))]
+        a, b = some(), some()
+        if not overlap(a, b):
+            assert not bytes_of(*a) & bytes_of(*b), (a, b)
+            apart += 1
+        else:
+            meet += bool(bytes_of(*a) & bytes_of(*b))
+    assert apart > 5000 and meet > 2000
+    for _ in range(3000):  # [n, m, 2, size] or [n, 2, m, size] or [m, n, 2, size], gaps behind any
+        size, n, m = (int(v) for v in rng.integers(1, 6, 3))
+        first, gap = int(rng.integers(0, 50)), int(rng.integers(0, 3))
+        part = 2 * size + gap
+        row = m * part + int(rng.integers(0, 3)) * part
+        assert not overlap((first, n, row, m, part, size), (first + size, n, row, m, part, size))
+        row = 2 * m * size + gap
+        assert not overlap((first + m * size, n, row, m, size, size), (first, n, row, m, size, size))
+        assert not overlap((first + size, n, part, m, part * n, size), (first, n + 2, part, m, part * n, size))
+        row = m * part + int(rng.integers(0, 9))  # no multiple of the parts' stride
+        a, b = (first, n, row, m, part, size), (first + size, n, row, m, part, size)
+        assert not overlap(a, b) and not overlap(b, a)
 
 
 def test_slots_of_a_column(slots_lib):
