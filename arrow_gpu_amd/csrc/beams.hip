@@ -659,13 +659,24 @@ agpu_status agpu_select_beams(agpu_pipeline* p, const agpu_beams* args) {
   AGPU_REQUIRE(aligned_to(b.logits, b.row_type == AGPU_ROW_F32 ? 4 : 2) && aligned_to(b.scores, 4) && aligned_to(b.allowed, 8) && aligned_to(b.finished, 8) &&
                    aligned_to(b.out_scores, 4) && aligned_to(b.out_parents, 4) && aligned_to(b.out_tokens, 4) && aligned16(b.workspace),
                AGPU_ERR_SHAPE, "alignment");
-  // a request's block writes while another's still reads: results do not go where scores come from
-  const uint64_t found = 4ull * b.batch * b.k, rows = (uint64_t)b.batch * b.beams;
-  for (const void* out : {(const void*)b.out_scores, (const void*)b.out_parents, (const void*)b.out_tokens}) {
-    const uintptr_t o = reinterpret_cast<uintptr_t>(out), s = reinterpret_cast<uintptr_t>(b.scores), w = reinterpret_cast<uintptr_t>(b.workspace);
-    AGPU_REQUIRE(!b.scores || o + found <= s || s + 4 * rows <= o, AGPU_ERR_ARG, "an output overlaps the scores");
-    AGPU_REQUIRE(o + found <= w || w + need <= o, AGPU_ERR_ARG, "an output overlaps the workspace");
+  // a request's block writes while another's still reads: results do not go where scores and finished rows come from, nor the segments' where logits do
+  const uint64_t found = 4ull * b.batch * b.k, rows = (uint64_t)b.batch * b.beams, item = b.row_type == AGPU_ROW_F32 ? 4 : 2;
+  const auto apart = [](const void* x, uint64_t nx, const void* y, uint64_t ny) {
+    const uintptr_t i = reinterpret_cast<uintptr_t>(x), j = reinterpret_cast<uintptr_t>(y);
+    return !y || (i <= j ? nx <= j - i : ny <= i - j);
+  };
+  const void* outs[] = {b.out_scores, b.out_parents, b.out_tokens};
+  for (int i = 0; i < 3; i++) {
+    AGPU_REQUIRE(apart(outs[i], found, b.scores, 4 * rows), AGPU_ERR_ARG, "an output overlaps the scores");
+    AGPU_REQUIRE(apart(outs[i], found, b.finished, agpu_bitmap_bytes(rows)), AGPU_ERR_ARG, "an output overlaps the finished rows");
+    AGPU_REQUIRE(apart(outs[i], found, b.workspace, need), AGPU_ERR_ARG, "an output overlaps the workspace");
+    for (int j = 0; j < i; j++) AGPU_REQUIRE(apart(outs[i], found, outs[j], found), AGPU_ERR_ARG, "two outputs overlap");
   }
+  uint64_t span;
+  AGPU_REQUIRE(b.row_stride < (1ull << 61) && extent(rows, item * b.row_stride, 1, 0, item * b.vocab, &span), AGPU_ERR_SHAPE, "logits past the address space");
+  const uint64_t masks = (rows - 1) * b.allowed_stride + agpu_bitmap_bytes(b.vocab);
+  AGPU_REQUIRE(apart(b.workspace, need, b.logits, span) && apart(b.workspace, need, b.scores, 4 * rows) && apart(b.workspace, need, b.finished, agpu_bitmap_bytes(rows)) &&
+                   apart(b.workspace, need, b.allowed, masks), AGPU_ERR_ARG, "the workspace overlaps an input");
   AGPU_BIND(p);
   const BeamArgs a = {b.logits, b.row_stride, b.batch, b.beams, b.vocab, b.k, b.end_token, b.scores, static_cast<const uint8_t*>(b.allowed), b.allowed_stride,
                       static_cast<const uint64_t*>(b.finished), b.out_scores, b.out_parents, b.out_tokens, segments((uint64_t)b.batch * b.beams, b.vocab)};

@@ -612,7 +612,7 @@ agpu_status agpu_take_rows(agpu_pipeline* p, int32_t n_states, const agpu_state*
  * score is NaN, has scores of -infinity.  Where fewer than k scores are above -infinity, the rest of the k are the other (row, token) in
  * ascending order with score -infinity.  1 <= k <= 64, k <= beams * vocab, beams <= 1024, batch * beams < 2^24, vocab < 2^31,
  * batch * beams * vocab < 2^38, beams * k * vocab < 2^43.
- * The outputs lie apart from the inputs and the workspace (over scores or workspace: AGPU_ERR_ARG).
+ * The outputs lie apart from each other, the workspace, scores and finished, the workspace from every input (AGPU_ERR_ARG).
  * workspace: agpu_select_beams_workspace bytes, 16-byte aligned, not shared with a call that may run at the same time (two captured graphs that
  * hold the same workspace must not be replayed at the same time); its contents need no preparation and are nothing to keep. */
 typedef struct agpu_beams {

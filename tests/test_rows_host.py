@@ -178,6 +178,32 @@ def test_select_beams_arguments():
     assert status("agpu_select_beams_workspace", 2, 4, 1000, 8, None)[0] == capi.ERR_ARG
 
 
+def test_what_a_selection_writes_lies_apart():
+    """outputs on each other or on the bitmap of finished rows, the workspace on an input: blocks would write what others still read"""
+    def beams(**kw):
+        a = dict(logits=1 << 20, row_stride=1000, type=capi.ROW_F16, batch=2, beams=4, vocab=1000, k=8, end_token=0, scores=1 << 21, allowed=1 << 22, allowed_stride=128,
+                 finished=1 << 23, out_scores=1 << 24, out_parents=1 << 25, out_tokens=1 << 26, workspace=1 << 27, workspace_bytes=1 << 30)
+        a.update(kw)
+        return status("agpu_select_beams", None, C.byref(BeamsStruct(**a)))
+
+    assert "two outputs" in beams(out_parents=1 << 24)[1] and "two outputs" in beams(out_tokens=(1 << 25) + 60)[1] and "two outputs" in beams(out_tokens=(1 << 24) - 60)[1]
+    for at in ((1 << 24) + 64, (1 << 24) - 64):
+        assert NO_PIPELINE[1] in beams(out_parents=at)[1]
+    for out in ("out_scores", "out_parents", "out_tokens"):
+        assert "finished" in beams(**{out: 1 << 23})[1] and "finished" in beams(**{out: (1 << 23) + 4})[1] and "finished" in beams(**{out: (1 << 23) - 60})[1]
+        assert NO_PIPELINE[1] in beams(**{out: (1 << 23) + 8})[1] and NO_PIPELINE[1] in beams(**{out: (1 << 23) - 64})[1]
+        assert NO_PIPELINE[1] in beams(**{out: 1 << 23, "finished": 0})[1]
+    n = C.c_uint64()
+    assert status("agpu_select_beams_workspace", 2, 4, 1000, 8, C.byref(n))[0] == 0
+    for at, size in ((1 << 20, 16000), (1 << 21, 32), (1 << 22, 1024), (1 << 23, 8)):  # logits, scores, masks, finished rows
+        last = (at + size - 1) // 16 * 16
+        assert "workspace" in beams(workspace=at)[1] and "workspace" in beams(workspace=last)[1] and "workspace" in beams(workspace=at - (n.value - 1) // 16 * 16)[1]
+        assert NO_PIPELINE[1] in beams(workspace=last + 16)[1] and NO_PIPELINE[1] in beams(workspace=at - (n.value + 15) // 16 * 16)[1]
+    assert NO_PIPELINE[1] in beams(workspace=(1 << 20) + 2000, row_stride=0)[1]  # one row for all
+    assert "workspace" in beams(workspace=(1 << 22) + 112, allowed_stride=0)[1] and NO_PIPELINE[1] in beams(workspace=(1 << 22) + 128, allowed_stride=0)[1]
+    assert "address space" in beams(row_stride=1 << 62)[1]
+
+
 def test_the_largest_calls():
     """what a launch's threads and 31-bit counts bound is refused, what the documentation allows is not"""
     n = C.c_uint64(0)
