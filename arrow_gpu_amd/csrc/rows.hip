@@ -584,7 +584,8 @@ agpu_status check_states(int32_t n_states, const agpu_state* states, uint64_t n_
                  AGPU_ERR_SHAPE, "a state past the address space");
     AGPU_REQUIRE(disjoint(n, s.dst_row_stride, s.n_pieces, s.dst_piece_stride, s.piece_bytes), AGPU_ERR_SHAPE, "rows that are written may not overlap");
     AGPU_REQUIRE(row_bytes < (1ull << 31), AGPU_ERR_SHAPE, "a row holds less than 2^31 bytes");
-    AGPU_REQUIRE(!lengths || s.position_bytes > 0, AGPU_ERR_SHAPE, "lengths need position_bytes");
+    // (a length times position_bytes then stays below 2^63)
+    AGPU_REQUIRE(!lengths || (s.position_bytes > 0 && s.position_bytes <= s.piece_bytes), AGPU_ERR_SHAPE, "lengths need position_bytes, at most piece_bytes");
     // (its src and its dst are compared too: rows are not reordered in place)
     places[count++] = {reinterpret_cast<uintptr_t>(s.dst), n, s.dst_row_stride, s.n_pieces, s.dst_piece_stride, s.piece_bytes, true, 2 * k};
     if (from) places[count++] = {reinterpret_cast<uintptr_t>(s.src), n_src, s.src_row_stride, s.n_pieces, s.src_piece_stride, s.piece_bytes, false, 2 * k + 1};

@@ -590,7 +590,7 @@ typedef struct agpu_state {
   uint64_t src_row_stride, src_piece_stride;
   uint64_t dst_row_stride, dst_piece_stride;
   uint64_t n_pieces, piece_bytes;
-  uint64_t position_bytes; /* with lengths: bytes of one position inside a piece */
+  uint64_t position_bytes; /* with lengths: bytes of one position inside a piece, at most piece_bytes */
 } agpu_state;
 /* dst row i = src row idx[i], i < n, of every state (n_states <= 64): the reordering of the states by a selection's parents, whatever the bytes
  * are.  lengths (may be NULL): only the first lengths[i] positions of row i's pieces are copied (all, if they are more than a piece holds), what

@@ -219,6 +219,15 @@ def test_the_largest_calls():
     assert "2^48" in status("agpu_put_quantised", None, 1, C.byref(s), C.byref(r), 1 << 23, 1 << 29)[1]
 
 
+def test_positions_larger_than_a_piece():
+    """2^31 positions of 2^33 bytes are 2^64: the kernel's product would wrap, and of a row that is copied whole nothing would be"""
+    for position, ok in ((1, True), (1024, True), (1025, False), (1 << 33, False), ((1 << 64) - 1, False)):
+        s = StateStruct(1 << 30, 1 << 40, 4096, 1024, 4096, 1024, 4, 1024, position)
+        st, msg = status("agpu_take_rows", None, 1, C.byref(s), 8, 1 << 20, 1 << 21, 8)
+        assert (NO_PIPELINE[1] in msg) == ok and (ok or (st == capi.ERR_SHAPE and "position_bytes" in msg)), (position, msg)
+        assert NO_PIPELINE[1] in status("agpu_take_rows", None, 1, C.byref(s), 8, 1 << 20, None, 8)[1]  # no lengths, no positions
+
+
 def test_what_is_written_lies_apart():
     """two outputs on each other, an output on an index column or on a cache; and what lies interleaved in one allocation is none of these"""
     def state(**kw):
