@@ -103,6 +103,8 @@ def take_quantised_op(stores, where, pipeline: ArrowComputePipeline, type_: str 
         if n_rows is None:
             raise shape_error("take_quantised through a page map: how many rows? (n_rows or out)")
         n = int(n_rows)
+        if n < 0:
+            raise shape_error(f"{n} rows")
     else:
         n = _u32(where, "slots").len
     if not isinstance(where, PageMap) and _u32(where, "slots").len != n:
@@ -171,6 +173,8 @@ def select_beams_op(logits: RowsGPU, beams: int, k: int, pipeline: ArrowComputeP
     if len(logits.shape) != 2 or beams < 1 or logits.shape[0] % beams:
         raise shape_error(f"logits {logits.shape} of {beams} beams a request")
     rows, vocab = logits.shape
+    if vocab >= 1 << 31 or rows >= 1 << 24:
+        raise shape_error(f"logits {logits.shape}: less than 2^24 rows of less than 2^31")
     batch, pitch = rows // beams, (vocab + 63) // 64 * 64
     if scores is not None and (not isinstance(scores, Float32ArrayGPU) or scores.null_buffer is not None or scores.len != rows):
         raise shape_error(f"scores: a Float32ArrayGPU of {rows} values without nulls")
@@ -218,14 +222,16 @@ def _waited(device, label: str, op, *things):
     return got
 
 
+def _device_of(where):
+    return where.tables.gpu_device if isinstance(where, PageMap) else _u32(where, "slots").gpu_device
+
+
 def put_quantised(stores, rows, where) -> None:
-    first = stores if isinstance(stores, QuantisedRowsGPU) else stores[0]
-    _waited(first.gpu_device, "put_quantised", lambda p: put_quantised_op(stores, rows, where, p), stores, rows, where)
+    _waited(_device_of(where), "put_quantised", lambda p: put_quantised_op(stores, rows, where, p), stores, rows, where)
 
 
 def take_quantised(stores, where, type_: str = "f32", n_rows: int | None = None, out=None) -> list:
-    first = stores if isinstance(stores, QuantisedRowsGPU) else stores[0]
-    return _waited(first.gpu_device, "take_quantised", lambda p: take_quantised_op(stores, where, p, type_, n_rows, out), stores, where, out)
+    return _waited(_device_of(where), "take_quantised", lambda p: take_quantised_op(stores, where, p, type_, n_rows, out), stores, where, out)
 
 
 def take_rows(states, indexes: UInt32ArrayGPU, lengths: UInt32ArrayGPU | None = None, out=None) -> list:

@@ -48,7 +48,7 @@ class RowsGPU:
             raise capi.OperationNotSupported(f"rows of {type_}")
         shape = tuple(shape)
         strides = _dense(shape)[0] if strides is None else tuple(strides)
-        if not 2 <= len(shape) <= 4 or len(strides) != len(shape):
+        if not 2 <= len(shape) <= 4 or len(strides) != len(shape) or min(shape) < 0:
             raise shape_error(f"rows have 2 to 4 axes: got {shape}")
         if min(strides) < 0 or (strides[-1] != 1 and shape[-1] > 1):
             raise shape_error(f"the values of a row's last axis lie next to each other: got strides {strides}")
@@ -158,10 +158,7 @@ class QuantisedRowsGPU:
     __slots__ = ("codes", "scales", "gpu_device", "n_slots", "heads", "dim", "group", "code", "shape", "packed")
 
     def __init__(self, codes: DeviceBuffer, scales: DeviceBuffer, gpu_device: GpuDevice, n_slots: int, heads: int, dim: int, group: int, code: str):
-        if code not in CODE_TYPE:
-            raise capi.OperationNotSupported(f"codes of {code}")
-        if heads < 1 or dim < 1 or group < 1 or dim % group or (code == "i4" and group % 2):
-            raise shape_error(f"group {group} of {code} codes in rows of {heads} x {dim}")
+        self._check(n_slots, heads, dim, group, code)
         need = self.bytes_of(n_slots, heads, dim, group, code)
         if (codes._owned and codes.nbytes < need[0]) or (scales._owned and scales.nbytes < need[1]):
             raise shape_error(f"{n_slots} rows of {heads} x {dim} need {need} bytes, not {codes.nbytes, scales.nbytes}")
@@ -169,6 +166,15 @@ class QuantisedRowsGPU:
         self.n_slots, self.heads, self.dim, self.group, self.code = n_slots, heads, dim, group, code
         self.shape = (heads, dim)  # of a row
         self.packed = _PACK_STORE(codes.ptr, scales.ptr, n_slots, heads, dim, group, CODE_TYPE[code])
+
+    @staticmethod
+    def _check(n_slots, heads, dim, group, code):
+        if code not in CODE_TYPE:
+            raise capi.OperationNotSupported(f"codes of {code}")
+        if heads < 1 or dim < 1 or heads * dim > 1 << 30 or not 1 <= group <= 65536 or dim % group or (code == "i4" and group % 2):
+            raise shape_error(f"group {group} of {code} codes in rows of {heads} x {dim}")
+        if not 0 <= n_slots <= 1 << 32:
+            raise shape_error(f"a cache of {n_slots} rows")
 
     @staticmethod
     def bytes_of(n_slots: int, heads: int, dim: int, group: int, code: str):
@@ -179,21 +185,19 @@ class QuantisedRowsGPU:
     @classmethod
     def empty(cls, n_slots: int, heads: int, dim: int, gpu_device: GpuDevice, code: str = "i8", group: Optional[int] = None) -> "QuantisedRowsGPU":
         group = dim if group is None else group
-        if code not in CODE_TYPE:
-            raise capi.OperationNotSupported(f"codes of {code}")
-        if group < 1:
-            raise shape_error(f"group {group}")
+        cls._check(n_slots, heads, dim, group, code)
         codes, scales = (gpu_device.create_empty_buffer(max(n, 1), zero_fill=True) for n in cls.bytes_of(n_slots, heads, dim, group, code))
         return cls(codes, scales, gpu_device, n_slots, heads, dim, group, code)
 
     @classmethod
     def of_tensors(cls, codes, scales, gpu_device: GpuDevice, code: str, heads: int, dim: int, group: int) -> "QuantisedRowsGPU":
         """The cache over two contiguous tensors' memory: codes (8-bit), scales (f32)."""
+        cls._check(0, heads, dim, group, code)
         per = heads * dim // 2 if code == "i4" else heads * dim
         if codes.element_size() != 1 or tensor_type(scales) != "f32" or not codes.is_contiguous() or not scales.is_contiguous():
             raise shape_error("codes: a contiguous 8-bit tensor, scales: a contiguous f32 one")
-        n_slots = codes.numel() // max(per, 1)
-        want = cls.bytes_of(n_slots, heads, dim, max(group, 1), code)
+        n_slots = codes.numel() // per
+        want = cls.bytes_of(n_slots, heads, dim, group, code)
         if (codes.numel(), 4 * scales.numel()) != want:
             raise shape_error(f"{codes.numel()} codes and {scales.numel()} scales are no cache of rows of {heads} x {dim} in groups of {group}")
         return cls(borrow_tensor(codes, gpu_device, want[0]), borrow_tensor(scales, gpu_device, want[1]), gpu_device, n_slots, heads, dim, group, code)
@@ -218,9 +222,12 @@ class PageMap:
         if tables.type not in ("u32", "i32") or len(tables.shape) != 2:
             raise shape_error("page tables are rows of 32-bit page numbers")
         n = tables.shape[0]
+        for column in (offsets, first):
+            if column is not None and (not isinstance(column, UInt32ArrayGPU) or column.null_buffer is not None):
+                raise capi.OperationNotSupported("offsets and first positions: UInt32ArrayGPUs without nulls")
         if offsets.len != n + 1 or (first is not None and first.len != n):
             raise shape_error(f"{n} page tables need {n + 1} offsets and {n} first positions")
-        if page_rows < 1:
+        if not 1 <= page_rows < 1 << 32:
             raise shape_error(f"pages of {page_rows} rows")
         self.tables, self.page_rows, self.offsets, self.first = tables, page_rows, offsets, first
         self.packed = _PACK_PAGES(tables.ptr, tables.strides[0], offsets.data.ptr, first.data.ptr if first is not None else 0, n, tables.shape[1],

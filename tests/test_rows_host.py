@@ -365,6 +365,39 @@ def test_python_refusals():
     assert e.value.status == capi.ERR_ARG
 
 
+def test_python_refusals_of_sizes_and_types(monkeypatch):
+    """what no field of a struct holds, and index columns of another type or with nulls: an error of this library's, before anything is packed"""
+    ag, dev, buf, pipe = _host()
+    u32 = lambda n: ag.UInt32ArrayGPU(buf(4 * n), dev, n, None)  # noqa: E731
+    nulls = ag.UInt32ArrayGPU(buf(16), dev, 4, object())
+    view = lambda shape, t="f32", strides=None: ag.RowsGPU(buf(1), dev, shape, t, strides)  # noqa: E731
+    cache = lambda **kw: ag.QuantisedRowsGPU(buf(1), buf(1), dev, **{**dict(n_slots=4, heads=2, dim=8, group=4, code="i8"), **kw})  # noqa: E731
+    tables = view((3, 2), "u32")
+    for bad in (lambda: cache(n_slots=-1), lambda: cache(n_slots=(1 << 32) + 1), lambda: cache(heads=1 << 33, dim=4), lambda: cache(heads=1, dim=1 << 17, group=1 << 17),
+                lambda: ag.QuantisedRowsGPU.empty(-1, 2, 8, dev), lambda: ag.QuantisedRowsGPU.empty(4, 0, 8, dev), lambda: ag.QuantisedRowsGPU.empty(4, 2, 8, dev, group=3),
+                lambda: ag.QuantisedRowsGPU.empty(4, 2, 8, dev, group=0), lambda: view((-1, 4)), lambda: view((3, -4)), lambda: ag.RowsGPU.of_array(u32(4), (-1, -4)),
+                lambda: ag.PageMap(tables, 1 << 32, u32(4)), lambda: ag.PageMap(tables, -1, u32(4)),
+                lambda: ag.take_quantised_op(cache(), ag.PageMap(tables, 4, u32(4)), pipe, n_rows=-1),
+                lambda: ag.select_beams_op(view((1, 1 << 33)), 1, 4, pipe), lambda: ag.select_beams_op(view((1 << 24, 4)), 1, 4, pipe)):
+        with pytest.raises(ag.ArrowErrorGPU) as e:
+            bad()
+        assert e.value.status == capi.ERR_SHAPE, e.value
+    f32 = ag.Float32ArrayGPU(buf(16), dev, 4, None)
+    for bad in (lambda: ag.PageMap(tables, 4, f32), lambda: ag.PageMap(tables, 4, nulls), lambda: ag.PageMap(tables, 4, u32(4), ag.Int32ArrayGPU(buf(12), dev, 3, None)),
+                lambda: ag.put_quantised(cache(), view((4, 2, 8)), f32), lambda: ag.take_quantised(cache(), nulls)):
+        with pytest.raises(ag.OperationNotSupported):
+            bad()
+    ag.PageMap(tables, (1 << 32) - 1, u32(4), u32(3))
+    # no caches at all is a call that does nothing, on the index column's device
+    import arrow_gpu_amd.kernels.rows as K
+
+    asked = []
+    done = types.SimpleNamespace(device=dev, _handle=None, keep=lambda *a: None, own_stream=True, finish=lambda: None, sync=lambda: None)
+    monkeypatch.setattr(K, "pipeline_for", lambda device, *a: asked.append(device) or done)
+    ag.put_quantised([], [], u32(3))
+    assert ag.take_quantised([], u32(3)) == [] and ag.take_quantised([], ag.PageMap(tables, 4, u32(4)), n_rows=3) == [] and asked == [dev] * 3
+
+
 def test_positions_that_lie_apart_go_into_dense_rows_and_back(monkeypatch):
     """(rows, positions, values): each position is a piece, in the state and in the output, whichever of the two is dense"""
     import arrow_gpu_amd.kernels.rows as K
