@@ -86,10 +86,15 @@ def borrow_tensor(tensor, device: "GpuDevice", nbytes: int) -> BorrowedBuffer:
     (`ArrowComputePipeline(device, hip_stream=torch.cuda.current_stream().cuda_stream)`) it stands in torch's order; a pipeline of its own is not ordered
     with torch's streams, there the program waits, before and after.  Work of other libraries on tensors of theirs is over before any call.
 
+    Gradients.  Nothing here has a backward pass: a tensor that requires gradients is refused, as where numpy reads one.  Torch does not see what is written
+    into a tensor (its version counter stays): no tensor that a backward pass still needs is an output.
+
     Memory.  A pipeline of its own holds the tensors of its calls until its sync().  One over torch's stream holds none, the rules of torch's streams do: a
     tensor's memory goes back to its allocator when its last owner lets go, and is used again in its stream's order (a tensor of another of torch's
     streams: record_stream)."""
     global _lent
+    if getattr(tensor, "requires_grad", False):
+        raise capi.ArrowErrorGPU("ArgumentError", "a tensor that requires gradients: detach() it (nothing here has a backward pass)", capi.ERR_ARG)
     if tensor.get_device() != device.ordinal:  # (of host memory: −1)
         raise capi.ArrowErrorGPU("ArgumentError", f"a tensor on {tensor.device} for a buffer on GPU {device.ordinal}", capi.ERR_ARG)
     _lent = True

@@ -186,3 +186,27 @@ def test_a_pipeline_of_its_own_holds_the_tensors_of_its_calls(monkeypatch, own_s
         lent = [b for b in kept if isinstance(b, gpu_utils.BorrowedBuffer)]
         assert {id(b) for b in lent} == ({id(b) for b in things} if own_stream else set())
         kept.clear()
+
+
+def test_a_tensor_that_requires_gradients_is_refused():
+    """its graph would end here without a word"""
+    def made(dtype, shape, item):
+        t = Tensor(dtype, shape, item)
+        t.requires_grad = True
+        return t
+
+    plain = Tensor("torch.float32", (4, 2, 2), 4)
+    for bad in (lambda: ag.RowsGPU.of_tensor(made("torch.float32", (3, 4), 4), DEV), lambda: ag.Float32ArrayGPU.of_tensor(made("torch.float32", (3,), 4), DEV),
+                lambda: ag.QuantisedRowsGPU.of_tensors(Tensor("torch.uint8", (4, 2, 8), 1), made("torch.float32", (4, 2, 2), 4), DEV, code="i8", heads=2, dim=8, group=4)):
+        with pytest.raises(ag.ArrowErrorGPU) as e:
+            bad()
+        assert e.value.status == ag._capi.ERR_ARG and "detach" in str(e.value)
+    ag.QuantisedRowsGPU.of_tensors(Tensor("torch.uint8", (4, 2, 8), 1), plain, DEV, code="i8", heads=2, dim=8, group=4)
+    torch = pytest.importorskip("torch")
+    for t in (torch.ones(3, 4, requires_grad=True), torch.ones(3, 4, requires_grad=True) * 2):
+        with pytest.raises(ag.ArrowErrorGPU) as e:
+            ag.RowsGPU.of_tensor(t, DEV)
+        assert "detach" in str(e.value)
+    with pytest.raises(ag.ArrowErrorGPU) as e:
+        ag.RowsGPU.of_tensor(torch.ones(3, 4, requires_grad=True).detach(), DEV)
+    assert "GPU 3" in str(e.value)  # (a host tensor, the next complaint)
