@@ -1132,10 +1132,21 @@ inline void take_quantised_op(const std::vector<QuantisedRowsGPU>& stores, const
   detail::keep_quantised(p, stores, out);
 }
 
-// Rows of any bytes: n rows of `pieces` pieces of piece_bytes (agpu_state); position_bytes: of one position inside a piece
+// Rows of any bytes: n rows of `pieces` pieces of piece_bytes (agpu_state); position_bytes: of one position inside a piece.  Strides in bytes, 0: one row,
+// one piece behind the other; offset: of the first row
 struct StateGPU {
   BufferPtr data;
-  uint64_t rows = 0, pieces = 1, piece_bytes = 0, position_bytes = 0;
+  uint64_t rows = 0, pieces = 1, piece_bytes = 0, position_bytes = 0, row_stride = 0, piece_stride = 0, offset = 0;
+  uint64_t step() const { return piece_stride ? piece_stride : piece_bytes; }
+  uint64_t row_step() const { return row_stride ? row_stride : pieces * step(); }
+  void* first() const {
+    uint64_t rows_span, pieces_span, end = 0;
+    const bool any = rows && pieces && piece_bytes;
+    if (any && (__builtin_mul_overflow(rows - 1, row_step(), &rows_span) || __builtin_mul_overflow(pieces - 1, step(), &pieces_span) ||
+                __builtin_add_overflow(rows_span, pieces_span, &end) || __builtin_add_overflow(end, piece_bytes, &end) || __builtin_add_overflow(end, offset, &end) || end > data->bytes))
+      throw ArrowErrorGPU(ArrowErrorGPU::Runtime, "take_rows: behind the end of a buffer");
+    return static_cast<char*>(data->ptr) + offset;
+  }
 };
 // out[k] row i = states[k] row indexes[i] (lengths: only the first lengths[i] positions of its pieces)
 inline void take_rows_op(const std::vector<StateGPU>& states, const UInt32ArrayGPU& indexes, const std::vector<StateGPU>& out, ArrowComputePipeline& p,
@@ -1146,9 +1157,7 @@ inline void take_rows_op(const std::vector<StateGPU>& states, const UInt32ArrayG
     const StateGPU &s = states[i], &o = out[i];
     if (s.rows != states[0].rows || o.rows != indexes.len || o.pieces != s.pieces || o.piece_bytes != s.piece_bytes)
       throw ArrowErrorGPU(ArrowErrorGPU::Runtime, "take_rows: rows of one kind");
-    const uint64_t row = s.pieces * s.piece_bytes;
-    if (s.rows * row > s.data->bytes || o.rows * row > o.data->bytes) throw ArrowErrorGPU(ArrowErrorGPU::Runtime, "take_rows: behind the end of a buffer");
-    v.push_back({s.data->ptr, o.data->ptr, row, s.piece_bytes, row, s.piece_bytes, s.pieces, s.piece_bytes, s.position_bytes});
+    v.push_back({s.first(), o.first(), s.row_step(), s.step(), o.row_step(), o.step(), s.pieces, s.piece_bytes, s.position_bytes});
   }
   check(agpu_take_rows(p.h(), (int32_t)v.size(), v.data(), states.empty() ? 0 : states[0].rows, static_cast<const uint32_t*>(indexes.data->ptr),
                        lengths ? static_cast<const uint32_t*>(lengths->data->ptr) : nullptr, indexes.len), "agpu_take_rows");
@@ -1164,12 +1173,14 @@ struct BeamSelection {
   BufferPtr workspace;
 };
 // Per request the k best of its beams x tokens by scores[row] + log_softmax(logits[row])[token]; logits: rows of 1 x vocab.  allowed: a bitmap of every
-// row's vocab bits, each row's on a multiple of 64 bits; finished: a bitmap of the rows, a finished row's one candidate is (end_token, its score)
+// row's vocab bits, each row's on a multiple of 64 bits, or one bitmap for all rows; finished: a bitmap of the rows, a finished row's one candidate is
+// (end_token, its score).  out: an earlier selection of as many requests and k, whose memory the results and the workspace go into again (it is not in use
+// by two calls at one time)
 inline BeamSelection select_beams_op(const RowsGPU& logits, uint32_t beams, uint32_t k, ArrowComputePipeline& p, const std::optional<Float32ArrayGPU>& scores = std::nullopt,
                                      const std::optional<BooleanArrayGPU>& allowed = std::nullopt, const std::optional<BooleanArrayGPU>& finished = std::nullopt,
-                                     uint32_t end_token = 0) {
+                                     uint32_t end_token = 0, const BeamSelection* out = nullptr) {
   const uint64_t pitch = agpu_bitmap_bytes(logits.dim);
-  if (beams == 0 || logits.heads != 1 || logits.dim >> 31 || logits.rows >> 31 || logits.rows % beams != 0 || (scores && scores->len != logits.rows) || (allowed && allowed->len != logits.rows * pitch * 8) ||
+  if (beams == 0 || logits.heads != 1 || logits.dim >> 31 || logits.rows >> 31 || logits.rows % beams != 0 || (scores && scores->len != logits.rows) || (allowed && allowed->len != logits.rows * pitch * 8 && allowed->len != pitch * 8 && allowed->len != logits.dim) ||
       (finished && finished->len != logits.rows))
     throw ArrowErrorGPU(ArrowErrorGPU::Runtime, "select_beams: logits of whole requests, a score, a bitmap, a bit for every row");
   const auto& dev = logits.gpu_device;
@@ -1177,10 +1188,13 @@ inline BeamSelection select_beams_op(const RowsGPU& logits, uint32_t beams, uint
   uint64_t need = 0;
   check(agpu_select_beams_workspace(batch, beams, (uint32_t)logits.dim, k, &need), "agpu_select_beams_workspace");
   const uint64_t n = (uint64_t)batch * k, bytes = n ? 4 * n : 4;
-  const BufferPtr s = dev->create_empty_buffer(bytes), r = dev->create_empty_buffer(bytes), t = dev->create_empty_buffer(bytes), w = dev->create_empty_buffer(need ? need : 16);
+  if (out && (out->scores.len != n || out->parents.len != n || out->tokens.len != n)) throw ArrowErrorGPU(ArrowErrorGPU::Runtime, "select_beams: out of another size");
+  const auto made = [&](const BufferPtr& held, uint64_t size) { return held && held->bytes >= size ? held : dev->create_empty_buffer(size); };
+  const BufferPtr s = made(out ? out->scores.data : nullptr, bytes), r = made(out ? out->parents.data : nullptr, bytes), t = made(out ? out->tokens.data : nullptr, bytes),
+                  w = made(out ? out->workspace : nullptr, need ? need : 16);
   const agpu_rows x = logits.abi();
   const agpu_beams a = {x.data, x.row_stride, x.row_type, batch, beams, (uint32_t)logits.dim, k, end_token, scores ? static_cast<const float*>(scores->data->ptr) : nullptr,
-                        allowed ? allowed->data->ptr : nullptr, allowed ? pitch : 0, finished ? finished->data->ptr : nullptr, static_cast<float*>(s->ptr),
+                        allowed ? allowed->data->ptr : nullptr, allowed && allowed->len == logits.rows * pitch * 8 ? pitch : 0, finished ? finished->data->ptr : nullptr, static_cast<float*>(s->ptr),
                         static_cast<uint32_t*>(r->ptr), static_cast<uint32_t*>(t->ptr), w->ptr, w->bytes};
   check(agpu_select_beams(p.h(), &a), "agpu_select_beams");
   p.keep.insert(p.keep.end(), {logits.data, s, r, t, w});
