@@ -295,6 +295,29 @@ def test_a_slot_named_twice(dev, p, code, dim, group):
     assert np.isin(scales[slots[7]].reshape(heads, -1), want_scales[~once].reshape(61, heads, -1)).all()
 
 
+@pytest.mark.parametrize("kind", KINDS)
+def test_4_bit_values_are_rounded_once_and_the_same_each_time(dev, p, kind):
+    """code * scale + lowest with one rounding to f32 (a rounded product would be off by up to half a step of the product, which can be many of the value's),
+    then one to the rows' type; other rows through the same kernels between two runs change nothing"""
+    import arrow_gpu_amd as ag
+
+    rng = np.random.default_rng(13)
+    n, heads, dim, group = 96, 8, 128, 64
+    x, other = (activations(rng, (n, heads, dim), "bf16") for _ in range(2))
+    slots, back = u32(rng.permutation(4096)[:n], dev), []
+    store = ag.QuantisedRowsGPU.empty(4096, heads, dim, dev, code="i4", group=group)
+    for rows in (x, other, x, other, x):
+        ag.put_quantised_op(store, up(rows, "bf16", dev), slots, p)
+        back.append(ag.take_quantised_op(store, slots, p, kind)[0])
+    p.sync()
+    got = [b.values().astype(np.float32) for b in back]
+    codes, scales = R.quantise(x, "i4", group)
+    # a code of 4 bits times a scale of 24 is exact in 64 bits, the sum is within 2^-53 of it: no f32 border is that near for these rows
+    want = R.values(codes, scales, "i4", group).astype(np.float32)
+    assert np.array_equal(got[0].view(np.uint32), R.rounded(want, kind).view(np.uint32))
+    assert np.array_equal(got[0], got[2]) and np.array_equal(got[0], got[4]) and np.array_equal(got[1], got[3])
+
+
 def test_pages_out_of_range(dev, p):
     import arrow_gpu_amd as ag
 
