@@ -371,10 +371,15 @@ class BooleanArrayGPU(ArrowArrayGPU):
 
     @classmethod
     def of_tensor(cls, tensor, gpu_device: GpuDevice, n_bits: Optional[int] = None):
-        """The bitmap over a contiguous 8-bit tensor's memory, without a copy; n_bits: its length (all bits if left out)."""
+        """The bitmap over a contiguous uint8 / int8 tensor's memory, without a copy; n_bits: its length (all bits if left out).  A tensor of truth values holds
+        one a byte and is no bitmap."""
+        if (cls, tensor.dtype) not in _FITS:
+            if str(tensor.dtype).rsplit(".", 1)[-1] not in ("uint8", "int8"):
+                raise capi.ArrowErrorGPU("ArgumentError", f"a bitmap over a tensor of {tensor.dtype}: bits are packed in uint8", capi.ERR_ARG)
+            _FITS.add((cls, tensor.dtype))
         held = tensor.numel()
         n_bits = 8 * held if n_bits is None else int(n_bits)
-        if tensor.element_size() != 1 or not tensor.is_contiguous() or bitmap_bytes(n_bits) > held:
+        if not tensor.is_contiguous() or n_bits < 0 or bitmap_bytes(n_bits) > held:
             raise capi.ArrowErrorGPU("ShapeError", f"a bitmap of {n_bits} bits needs {bitmap_bytes(n_bits)} contiguous bytes", capi.ERR_SHAPE)
         return cls(borrow_tensor(tensor, gpu_device, held), gpu_device, n_bits, None)
 

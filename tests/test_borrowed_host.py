@@ -210,3 +210,17 @@ def test_a_tensor_that_requires_gradients_is_refused():
     with pytest.raises(ag.ArrowErrorGPU) as e:
         ag.RowsGPU.of_tensor(torch.ones(3, 4, requires_grad=True).detach(), DEV)
     assert "GPU 3" in str(e.value)  # (a host tensor, the next complaint)
+
+
+def test_a_tensor_of_truth_values_is_no_bitmap():
+    """one a byte: read as packed bits it would be a mask of other rows, without an error"""
+    for dtype, item in (("torch.bool", 1), ("torch.float8_e4m3fn", 1), ("torch.int32", 4)):
+        with pytest.raises(ag.ArrowErrorGPU) as e:
+            ag.BooleanArrayGPU.of_tensor(Tensor(dtype, (64,), item), DEV, 64)
+        assert e.value.status == ag._capi.ERR_ARG
+    for dtype in ("torch.uint8", "torch.int8"):
+        assert ag.BooleanArrayGPU.of_tensor(Tensor(dtype, (64,), 1), DEV).len == 512
+        assert ag.BooleanArrayGPU.of_tensor(Tensor(dtype, (64,), 1), DEV, 100).len == 100
+        for bits in (513, -1):
+            with pytest.raises(ag.ArrowErrorGPU):
+                ag.BooleanArrayGPU.of_tensor(Tensor(dtype, (64,), 1), DEV, bits)
