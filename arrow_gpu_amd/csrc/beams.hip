@@ -5,9 +5,10 @@
 // No wave needs the maximum first: exp is taken relative to the first tile's, and f32 holds it as long as
 // a segment's maximum is at most 60 above that, or 30 below a reference that is no tile's maximum; a segment of another kind is read again.
 //
-// 256 rows x 128256 bf16, 8 beams, k 16: segments 21.7 us (66 MB: 3.0 TB/s), join 5.8.  The segments are bound by their instructions, not by memory — the
-// loads alone take 12.6 us: about 12 a logit, of which the term's exp are 6 and the pair sums, the clamp, the unpacking and the maxima 3.5; the floors
-// and the hits' exact terms are the rest.  One request (4 x 32000): 5.8 + 4.7 us, launches and latency.
+// 256 rows x 128256 bf16, 8 beams, k 16 (least and average of 100 launches): segments 22.1 and 23.5 us (66 MB: 3.0 and 2.8 TB/s), join 6.0 and 6.3.  The
+// segments execute 19 vector instructions a logit, 13.3 us of every SIMD — about 12 in the stream, of which the term's exp are 6 and the pair sums, the clamp, the
+// unpacking and the maxima 3.5; the floors and the hits' exact terms are the rest — and the loads alone take 12.6 us; one generation of waves in step
+// overlaps the two in part only.  One request (4 x 32000): 6.0 and 6.5 + 4.8 and 5.3 us, launches and latency.
 //
 // Precision.  The result is whole numbers, and rows that compete differ by their log-sums only: a log-sum 1e-7 off swaps tokens of two beams.  Scores are
 // compared in f64.  Of the sum, the terms of the tokens that reach the floor — at least the 16 largest of a row, the bulk where it is sharp — are taken in
@@ -594,7 +595,7 @@ __global__ __launch_bounds__(MERGE_BLOCK) void beam_merge_kernel(BeamArgs a, Div
 
 // ---------------------------------------------------------------- host
 // Tiles of a segment: the fewer, the more waves share the work; the more, the fewer lists there are to join.  As many as leave 4096 waves (16 a
-// CU), at most 8: 256 rows x 128256 in 8 tiles a segment 22.9 us and 5.8 to join, in 4 tiles 27.5 and 8.7.  (The type does not enter: the workspace does
+// CU), at most 8: 256 rows x 128256 in 4 tiles a segment take 1.2 times as long as in 8 (27.5 us beside 22.9), and 1.5 times to join.  (The type does not enter: the workspace does
 // not depend on it.)
 uint32_t segment_tiles(uint64_t rows, uint64_t vocab) {
   uint32_t t = MOST_TILES;
