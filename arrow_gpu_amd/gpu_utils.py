@@ -84,7 +84,9 @@ def borrow_tensor(tensor, device: "GpuDevice", nbytes: int) -> BorrowedBuffer:
     Order.  Calls that take no pipeline run on torch's current stream where any of their arguments is a tensor's memory, and are over when they return;
     reading values back waits for that stream first.  A `*_op` call runs on its pipeline: over torch's current stream
     (`ArrowComputePipeline(device, hip_stream=torch.cuda.current_stream().cuda_stream)`) it stands in torch's order; a pipeline of its own is not ordered
-    with torch's streams, there the program waits, before and after.  Work of other libraries on tensors of theirs is over before any call.
+    with torch's streams, there the program waits, before and after.  Work of other libraries on tensors of theirs is over before any call.  Where torch
+    captures a graph, `*_op` calls on a pipeline over the captured stream are recorded (the pipeline and what they write live as long as the graph; a selection
+    has its workspace from a call before), and calls that wait are refused.
 
     Gradients.  Nothing here has a backward pass: a tensor that requires gradients is refused, as where numpy reads one.  Torch does not see what is written
     into a tensor (its version counter stays): no tensor that a backward pass still needs is an output.
@@ -107,12 +109,16 @@ def _is_lent(x) -> bool:
         return True
     if isinstance(x, (list, tuple)):
         return any(map(_is_lent, x))
-    return any(_is_lent(getattr(x, part)) for part in getattr(x, "PARTS", ()))
+    return any(_is_lent(getattr(x, part, None)) for part in getattr(x, "PARTS", ()))
 
 
 def _torch_stream(device: "GpuDevice"):
     torch = sys.modules.get("torch")  # (not there: the tensors are another library's)
-    return torch.cuda.current_stream(device.ordinal) if torch is not None else None
+    if torch is None:
+        return None
+    if torch.cuda.is_current_stream_capturing():
+        raise capi.ArrowErrorGPU("ArgumentError", "a call that waits for torch's stream while torch captures it: record the *_op form", capi.ERR_ARG)
+    return torch.cuda.current_stream(device.ordinal)
 
 
 def pipeline_for(device: "GpuDevice", label: str, *things) -> "ArrowComputePipeline":
