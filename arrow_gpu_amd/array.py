@@ -264,7 +264,7 @@ class PrimitiveArrayGpu(ArrowArrayGPU):
         if not tensor.is_contiguous():
             raise capi.ArrowErrorGPU("ShapeError", f"{cls.__name__} over a tensor that is not contiguous", capi.ERR_SHAPE)
         n = tensor.numel()
-        return cls(borrow_tensor(tensor, gpu_device, n * cls.ITEM_SIZE), gpu_device, n, None)
+        return cls(borrow_tensor(tensor, gpu_device, n * cls.ITEM_SIZE, cls.NP_DTYPE is np.float32), gpu_device, n, None)
 
     @classmethod
     def _to_native(cls, v):
@@ -381,7 +381,7 @@ class BooleanArrayGPU(ArrowArrayGPU):
         n_bits = 8 * held if n_bits is None else int(n_bits)
         if not tensor.is_contiguous() or n_bits < 0 or bitmap_bytes(n_bits) > held:
             raise capi.ArrowErrorGPU("ShapeError", f"a bitmap of {n_bits} bits needs {bitmap_bytes(n_bits)} contiguous bytes", capi.ERR_SHAPE)
-        return cls(borrow_tensor(tensor, gpu_device, held), gpu_device, n_bits, None)
+        return cls(borrow_tensor(tensor, gpu_device, held, False), gpu_device, n_bits, None)
 
     def raw_bytes(self) -> np.ndarray:
         return self.gpu_device.retrive_data(self.data, (self.len + 7) // 8)

@@ -77,7 +77,7 @@ def tensor_type(tensor) -> str:
 _lent = False  # whether any tensor's memory was ever borrowed
 
 
-def borrow_tensor(tensor, device: "GpuDevice", nbytes: int) -> BorrowedBuffer:
+def borrow_tensor(tensor, device: "GpuDevice", nbytes: int, floating: bool = True) -> BorrowedBuffer:
     """The memory of a tensor on `device` (anything with data_ptr() and get_device(): torch is not needed here).  A program that uses
     torch on the GPU imports it before this library's first call: then both run on the one GPU runtime that torch has loaded.
 
@@ -95,7 +95,7 @@ def borrow_tensor(tensor, device: "GpuDevice", nbytes: int) -> BorrowedBuffer:
     tensor's memory goes back to its allocator when its last owner lets go, and is used again in its stream's order (a tensor of another of torch's
     streams: record_stream)."""
     global _lent
-    if getattr(tensor, "requires_grad", False):
+    if floating and getattr(tensor, "requires_grad", False):  # (whole numbers have none; the question costs 0.1 us)
         raise capi.ArrowErrorGPU("ArgumentError", "a tensor that requires gradients: detach() it (nothing here has a backward pass)", capi.ERR_ARG)
     if tensor.get_device() != device.ordinal:  # (of host memory: −1)
         raise capi.ArrowErrorGPU("ArgumentError", f"a tensor on {tensor.device} for a buffer on GPU {device.ordinal}", capi.ERR_ARG)

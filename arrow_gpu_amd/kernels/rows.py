@@ -64,8 +64,9 @@ def _quantised(name: str, stores, rows, where, n: int, pipeline) -> None:
         capi.call(name, pipeline._handle, len(stores), s, r, where.data.ptr, n)
         if where.data._owned or pipeline.own_stream:
             pipeline.keep(where.data)
+    own = pipeline.own_stream
     for store, x in zip(stores, rows):
-        if pipeline.own_stream or store.codes._owned or store.scales._owned or x.data._owned:
+        if own or store.codes._owned or store.scales._owned or x.data._owned:
             _keep(pipeline, store.codes, store.scales, x.data)
 
 
@@ -152,11 +153,12 @@ def take_rows_op(states, indexes: UInt32ArrayGPU, pipeline: ArrowComputePipeline
         if x.gpu_device is not dev:
             _on(pipeline, x)
     capi.call("agpu_take_rows", pipeline._handle, len(states), packed, n_src, indexes.data.ptr, lengths.data.ptr if lengths is not None else None, n)
+    own = pipeline.own_stream
     for x in given:
-        if x.data._owned or pipeline.own_stream:
+        if own or x.data._owned:
             pipeline.keep(x.data)
     for s, o in zip(states, out):
-        if pipeline.own_stream or s.data._owned or o.data._owned:
+        if own or s.data._owned or o.data._owned:
             _keep(pipeline, s.data, o.data)
     return out
 
@@ -207,8 +209,9 @@ def select_beams_op(logits: RowsGPU, beams: int, k: int, pipeline: ArrowComputeP
                             finished.data.ptr if finished is not None else 0, out.scores.data.ptr, out.parents.data.ptr, out.tokens.data.ptr,
                             work.ptr, work.nbytes)
     capi.call("agpu_select_beams", pipeline._handle, args)
+    own = pipeline.own_stream
     for x in given:
-        if x.data._owned or pipeline.own_stream:
+        if own or x.data._owned:
             pipeline.keep(x.data)
     _keep(pipeline, out.scores.data, out.parents.data, out.tokens.data, work)
     return out

@@ -13,6 +13,7 @@ from .array import Float32ArrayGPU, UInt32ArrayGPU
 from .gpu_utils import DeviceBuffer, GpuDevice, borrow_tensor, settle, tensor_type
 
 ITEM_SIZE = {"f32": 4, "f16": 2, "bf16": 2, "i8": 1, "u8": 1, "i16": 2, "u16": 2, "i32": 4, "u32": 4, "i64": 8, "f64": 8}
+_FLOATING = ("f32", "f16", "bf16", "f64")
 ROW_TYPE = {"f32": capi.ROW_F32, "f16": capi.ROW_F16, "bf16": capi.ROW_BF16}
 CODE_TYPE = {"i8": capi.CODE_I8, "i4": capi.CODE_I4, "e4m3": capi.CODE_E4M3}
 _NUMPY = {"f32": np.float32, "f16": np.float16, "bf16": np.uint16, "i8": np.int8, "u8": np.uint8, "i16": np.int16, "u16": np.uint16, "i32": np.int32,
@@ -69,7 +70,7 @@ class RowsGPU:
         if not 2 <= len(shape) <= 4 or (strides[-1] != 1 and shape[-1] > 1):
             return cls(None, gpu_device, shape, t, strides, 0)  # raises
         self = cls.__new__(cls)
-        self.data = data = borrow_tensor(tensor, gpu_device, tensor.numel() * item)
+        self.data = data = borrow_tensor(tensor, gpu_device, tensor.numel() * item, t in _FLOATING)
         self.ptr, self.gpu_device, self.type, self.shape, self.strides, self.item_size = data.ptr, gpu_device, t, shape, strides, item
         self._rows = self._pieces = None
         return self
@@ -222,9 +223,9 @@ class PageMap:
         if tables.type not in ("u32", "i32") or len(tables.shape) != 2:
             raise shape_error("page tables are rows of 32-bit page numbers")
         n = tables.shape[0]
-        for column in (offsets, first):
-            if column is not None and (not isinstance(column, UInt32ArrayGPU) or column.null_buffer is not None):
-                raise capi.OperationNotSupported("offsets and first positions: UInt32ArrayGPUs without nulls")
+        if (not isinstance(offsets, UInt32ArrayGPU) or offsets.null_buffer is not None
+                or (first is not None and (not isinstance(first, UInt32ArrayGPU) or first.null_buffer is not None))):
+            raise capi.OperationNotSupported("offsets and first positions: UInt32ArrayGPUs without nulls")
         if offsets.len != n + 1 or (first is not None and first.len != n):
             raise shape_error(f"{n} page tables need {n + 1} offsets and {n} first positions")
         if not 1 <= page_rows < 1 << 32:
