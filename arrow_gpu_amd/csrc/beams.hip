@@ -2,8 +2,8 @@
 //
 // One pass over the logits.  A row is cut into segments of one WAVE each; the wave streams its segment, adding up exp(x) and keeping the tokens that
 // can be among its k best, and leaves (sum, k best) in the workspace.  A block a request joins the sums and selects among the segments' bests.
-// No wave needs the maximum first: exp is taken relative to the first tile's, and f32 holds it as long as
-// a segment's maximum is at most 60 above that, or 30 below a reference that is no tile's maximum; a segment of another kind is read again.
+// No wave needs the maximum first: exp is taken relative to that of the first tile whose maximum is an ordinary number, and f32 holds it as long as
+// the segment's maximum is at most 60 above that; a segment of another kind is read again.
 //
 // 256 rows x 128256 bf16, 8 beams, k 16 (least and average of 100 launches): segments 22.1 and 23.5 us (66 MB: 3.0 and 2.8 TB/s), join 6.0 and 6.3.  The
 // segments execute 19 vector instructions a logit, 13.3 us of every SIMD — about 12 in the stream, of which the term's exp are 6 and the pair sums, the clamp, the
@@ -16,7 +16,8 @@
 // times what log2 e has beyond f32 (2^-26 of error each), the instruction for 2^f is within 2^-23; 16 are added with 4 roundings, the rest in f64.
 // That bounds a log-sum's error by 2^-23 + ln 2 · 2^-25 + 4 · 2^-24 < 3.8e-7; many different terms are off at random, and it is about 1e-9.
 // What does not count (a masked logit, −infinity, one that a f64 term stands for) is e^-80 of the reference in the f32 sum: at most 8192 of them beside a
-// segment's largest term, which is e^-30 of it or more: 8192 e^-50 < 2e-18, nothing in a f64 sum — a lone token's is exactly 1.
+// segment's largest term, which is the reference's or larger: 8192 e^-80 < 2e-31, nothing in a f64 sum — a lone token's is exactly 1.  A tile before
+// the reference's has no terms: its logits lie more than 60 below the maximum (8192 e^-60 < 8e-23), or the segment is read again.
 #include "common.hpp"
 #include "row_address.hpp"
 
@@ -53,8 +54,7 @@ __device__ __forceinline__ bool is_finished(const BeamArgs& a, uint32_t row) { r
 constexpr float LOG2E = 0x1.715476p+0f, LOG2E_LOW = 0x1.4ae0cp-26f, MAGIC = 0x1.8p23f;
 constexpr double LN2 = 0.69314718055994530942;
 constexpr float REF_MOST = 16384.0f;  // of a reference: MAGIC − k holds its steps
-constexpr float APART = 60.0f;        // of a segment's maximum above its reference
-constexpr float BELOW = 30.0f;        // of it below the reference (0, where the first tile's maximum is no ordinary number)
+constexpr float APART = 60.0f;        // of a segment's maximum above its reference; above a tile that has no terms, at least
 constexpr float LEAST = 80.0f;        // of a term below the reference
 // exp(x) / 2^N, k = MAGIC − N; x log2 e − N within 2^±126
 __device__ __forceinline__ float exp_term(float x, float k) {
@@ -217,7 +217,8 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
   const uint32_t t0 = seg * tiles, row_tiles = (a.vocab + TILE - 1) / TILE, t1 = idle ? t0 : t0 + tiles < row_tiles ? t0 + tiles : row_tiles;
 
   float top[2] = {LOWEST, LOWEST};  // the largest of the lane's first and second eight logits of every tile
-  float floor_v = LOWEST, above = -0x1.fffffep127f, ref_v = 0.0f, k = MAGIC, least = 0.0f;
+  float floor_v = LOWEST, above = -0x1.fffffep127f, ref_v = 0.0f, k = MAGIC, least = 0.0f, without = LOWEST;
+  bool referred = false;
   double sum = 0.0;
   uint64_t nan = 0;
   uint32_t hits[4] = {0, 0, 0, 0};  // a bit a logit of the lane's, tile by tile: it reached the floor
@@ -246,12 +247,18 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
 #pragma unroll
       for (int u = 1; u < U / 2; u++) tm[0] = fmaxf(tm[0], vm[u]), tm[1] = fmaxf(tm[1], vm[U / 2 + u]);
       top[0] = fmaxf(top[0], tm[0]), top[1] = fmaxf(top[1], tm[1]);
-      if (t == t0) {  // the reference: the tile's maximum, as far as it is an ordinary number
+      if (!referred) {  // the reference: the tile's maximum, at most REF_MOST of it (far above that the segment is read again)
         float f = fmaxf(tm[0], tm[1]);
         for (int d = 32; d; d >>= 1) f = fmaxf(f, __shfl_xor(f, d));
-        ref_v = __builtin_fabsf(f) <= REF_MOST ? f : 0.0f;
-        k = MAGIC - __builtin_rintf(ref_v * LOG2E);
-        least = ref_v - LEAST;
+        f = __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, f)));
+        referred = f >= -REF_MOST;
+        if (referred) {
+          ref_v = fminf(f, REF_MOST);
+          k = MAGIC - __builtin_rintf(ref_v * LOG2E);
+          least = ref_v - LEAST;
+        } else {
+          without = fmaxf(without, f);
+        }
       }
     }
     // The floor, after tiles 0 and 2: a value that k logits of the row reach, among the maxima of the block's waves, all of one row
@@ -296,6 +303,7 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
         }
         hits[step / 2] |= h << (step % 2 * EPT + u * VE);
       }
+    if (!referred) continue;
     // the terms (at least e^-80 of the reference, −infinity too), added in pairs of pairs: four roundings on every way
 #pragma unroll
     for (int i = 0; i < EPT; i++) v[i] = exp_term(max_of(v[i], least), k);
@@ -315,7 +323,7 @@ __global__ __launch_bounds__(AGPU_BLOCK) void beam_segment_kernel(BeamArgs a, ui
 #pragma unroll
   for (int i = 0; i < 4; i++) all += (uint32_t)__builtin_popcount(hits[i]);
   for (int d = 32; d; d >>= 1) all += __shfl_xor(all, d);
-  const bool many = all > HITS, again = most > LOWEST && most < __builtin_inff() && (many || most - ref_v > APART || ref_v - most > BELOW);
+  const bool many = all > HITS, again = most > LOWEST && most < __builtin_inff() && (many || !referred || most - ref_v > APART || most - without < APART);
   u32x4 w[U];
   uint32_t m[U];
   const double ref = most;  // (a lone token's term is then exactly 1, its log-sum the logit)

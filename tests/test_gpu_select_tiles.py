@@ -87,6 +87,26 @@ def test_low_logits_behind_a_first_tile_that_holds_none(dev, p, kind, hole):  # 
     assert_selection(sel, want)
 
 
+@pytest.mark.parametrize("sign", [-1, 1])
+@pytest.mark.parametrize("kind", KINDS)
+def test_logits_about_the_largest_reference(dev, p, kind, sign):  # noqa: F811
+    """a reference is an ordinary number up to 16384: tiles below and above -16384 and 16384 in one segment, close to each other and far apart"""
+    import arrow_gpu_amd as ag
+
+    rng = np.random.default_rng(5 + sign)
+    rows, vocab, beams, k = 4096, 8192, 4, 8
+    assert tiles(rows, vocab) == 8
+    x = sign * np.float32(16384) + rng.random((rows, vocab), dtype=np.float32) * 2
+    for r in range(0, rows, beams):  # tile by tile a level of its own, the same in all of a request's rows
+        reach = (2.0, 20.0, 100.0, 3000.0)[r // beams % 4]
+        x[r:r + beams] += np.repeat(rng.uniform(-reach, reach, vocab // 1024), 1024).astype(np.float32)
+    x = R.rounded(x, kind)
+    cum = -np.float32(3) * rng.random(rows).astype(np.float32)
+    sel = ag.select_beams_op(up(x, kind, dev), beams, k, p, scores=f32(cum, dev))
+    p.sync()
+    assert_near(sel, R.select_many(x, beams, k, cum), x, cum)
+
+
 @pytest.mark.parametrize("rows,vocab,beams,k,of", [(2100, 4001, 7, 14, 2), (1040, 16001, 8, 16, 4), (820, 40003, 4, 64, 8), (4100, 8190, 1, 1, 8), (256, 128256, 8, 16, 8)])
 @pytest.mark.parametrize("kind", KINDS)
 def test_a_batch(dev, p, kind, rows, vocab, beams, k, of):  # noqa: F811
