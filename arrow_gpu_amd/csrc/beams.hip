@@ -603,8 +603,8 @@ __global__ __launch_bounds__(MERGE_BLOCK) void beam_merge_kernel(BeamArgs a, Div
 
 // ---------------------------------------------------------------- host
 // Tiles of a segment: the fewer, the more waves share the work; the more, the fewer lists there are to join.  As many as leave 4096 waves (16 a
-// CU), at most 8: 256 rows x 128256 in 4 tiles a segment take 1.2 times as long as in 8 (27.5 us beside 22.9), and 1.5 times to join.  (The type does not enter: the workspace does
-// not depend on it.)
+// CU), at most 8: 256 rows x 128256 in 4 tiles a segment take 1.2 times as long as in 8 (27.5 us beside 22.9), and 1.5 times to join.  (The type does
+// not enter: the workspace does not depend on it.)
 uint32_t segment_tiles(uint64_t rows, uint64_t vocab) {
   uint32_t t = MOST_TILES;
   while (t > 1 && rows * ((vocab + t * TILE - 1) / (t * TILE)) < 4096) t /= 2;

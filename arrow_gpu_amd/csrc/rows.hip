@@ -503,8 +503,9 @@ agpu_status quantised_pages(agpu_pipeline* p, bool put, int32_t n_cols, const ag
 // ---------------------------------------------------------------- take_rows
 // A copy with one indirection: lanes run over the states' accesses of 16 bytes in the order of the destination, two of a lane in flight, all states in
 // one launch (blockIdx.y).  Accesses begin at any byte; the last of a piece that is no multiple of 16 (or of what a length leaves) is the 16 bytes before
-// its end, some of them its neighbour's too, the same.  Bound by memory: 904 MB in 147.8 us at least, 152.0 on average of 100 launches, 6.1 and 5.9 TB/s, where a copy of as many bytes reaches 6.6 (one or four
-// of a lane in flight: 151 and 147, of a short row's 3.6 and 4.8 instead of 3.5); 64 rows of 4000001 f32, no row on 16 bytes, in 349 us, 5.9 TB/s.
+// its end, some of them its neighbour's too, the same.  Bound by memory: 904 MB in 147.8 us at least, 152.0 on average of 100 launches, 6.1 and 5.9 TB/s,
+// where a copy of as many bytes reaches 6.6 (one or four of a lane in flight: 151 and 147 at least, of a short row's 3.6 and 4.8 instead of 3.5); 64 rows of
+// 4000001 f32, no row on 16 bytes, in 349 us, 5.9 TB/s.
 constexpr int MAX_STATES = 8, ROWS_UNROLL = 2;
 struct State {
   const char* src;
