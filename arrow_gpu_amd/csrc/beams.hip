@@ -5,10 +5,10 @@
 // No wave needs the maximum first: exp is taken relative to that of the first tile whose maximum is an ordinary number, and f32 holds it as long as
 // the segment's maximum is at most 60 above that; a segment of another kind is read again.
 //
-// 256 rows x 128256 bf16, 8 beams, k 16 (least and average of 100 launches): segments 22.1 and 23.5 us (66 MB: 3.0 and 2.8 TB/s), join 6.0 and 6.3.  The
-// segments execute 19 vector instructions a logit, 13.3 us of every SIMD — about 12 in the stream, of which the term's exp are 6 and the pair sums, the clamp, the
+// 256 rows x 128256 bf16, 8 beams, k 16 (least and average of 100 launches): segments 22.0 and 23.3 us (66 MB: 3.0 and 2.8 TB/s), join 5.8 and 6.3.  The
+// segments execute 19 vector instructions a logit, 13.5 us of every SIMD — about 12 in the stream, of which the term's exp are 6 and the pair sums, the clamp, the
 // unpacking and the maxima 3.5; the floors and the hits' exact terms are the rest — and the loads alone take 12.6 us; one generation of waves in step
-// overlaps the two in part only.  One request (4 x 32000): 6.0 and 6.5 + 4.8 and 5.3 us, launches and latency.
+// overlaps the two in part only.  One request (4 x 32000): 5.8 and 6.5 + 4.6 and 5.1 us, launches and latency.
 //
 // Precision.  The result is whole numbers, and rows that compete differ by their log-sums only: a log-sum 1e-7 off swaps tokens of two beams.  Scores are
 // compared in f64.  Of the sum, the terms of the tokens that reach the floor — at least the 16 largest of a row, the bulk where it is sharp — are taken in

@@ -69,10 +69,10 @@ struct QuantShape {
 // past the group's end idle), its span found with data-parallel moves inside the wave.  A block takes whole rows, looks their slots up once and
 // keeps them in LDS: a search of the sequence through memory costs microseconds, so it is shared by up to 8 passes of the block (16 passes: 131072
 // rows of 4 bits in 138 us instead of 127).
-// What bounds it is memory (least and average of 100 launches): two columns of 16384 rows of 8 x 128 bf16 go to e4m3 in 17.2 and 19.4 us and come back in 16.9 and
-// 17.8 (102 MB each: 5.9 to 5.3 TB/s, 6.0 to 5.7; a copy of as many bytes takes 19), ragged e4m3 rows of 4 x 96 come back as f16 in 30.6 and 31.9 us (181 MB, 5.9 to
-// 5.7 TB/s), two columns of 131072 rows of 4 bits as bf16 in 127 and 130 us (705 MB, 5.6 to 5.4 TB/s; a u8 -> f32 cast of as many bytes 112).  A token's rows
-// take 2.4 and 2.8 us a call, that is one launch.
+// What bounds it is memory (least and average of 100 launches): two columns of 16384 rows of 8 x 128 bf16 go to e4m3 in 17.1 and 19.8 us and come back in 16.1 and
+// 18.1 (102 MB each: 6.0 to 5.2 TB/s, 6.3 to 5.6; a copy of as many bytes takes 19), ragged e4m3 rows of 4 x 96 come back as f16 in 30.4 and 32.0 us (181 MB, 6.0 to
+// 5.7 TB/s), two columns of 131072 rows of 4 bits as bf16 in 126.7 and 129.6 us (705 MB, 5.6 to 5.4 TB/s; a u8 -> f32 cast of as many bytes 112).  A token's rows
+// take 2.3 and 2.7 us a call, that is one launch.
 constexpr int MAX_COLS = 8, MAX_ROWS = 256;
 struct QuantCols {
   QuantCol c[MAX_COLS];
@@ -503,7 +503,7 @@ agpu_status quantised_pages(agpu_pipeline* p, bool put, int32_t n_cols, const ag
 // ---------------------------------------------------------------- take_rows
 // A copy with one indirection: lanes run over the states' accesses of 16 bytes in the order of the destination, two of a lane in flight, all states in
 // one launch (blockIdx.y).  Accesses begin at any byte; the last of a piece that is no multiple of 16 (or of what a length leaves) is the 16 bytes before
-// its end, some of them its neighbour's too, the same.  Bound by memory: 904 MB in 147.8 us at least, 152.0 on average of 100 launches, 6.1 and 5.9 TB/s,
+// its end, some of them its neighbour's too, the same.  Bound by memory: 904 MB in 146.9 us at least, 151.9 on average of 100 launches, 6.2 and 6.0 TB/s,
 // where a copy of as many bytes reaches 6.6 (one or four of a lane in flight: 151 and 147 at least, of a short row's 3.6 and 4.8 instead of 3.5); 64 rows of
 // 4000001 f32, no row on 16 bytes, in 349 us, 5.9 TB/s.
 constexpr int MAX_STATES = 8, ROWS_UNROLL = 2;
