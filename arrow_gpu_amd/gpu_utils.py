@@ -114,7 +114,7 @@ def _is_lent(x) -> bool:
 
 def _torch_stream(device: "GpuDevice"):
     torch = sys.modules.get("torch")  # (not there: the tensors are another library's)
-    if torch is None:
+    if torch is None or not torch.cuda.is_initialized():
         return None
     if torch.cuda.is_current_stream_capturing():
         raise capi.ArrowErrorGPU("ArgumentError", "a call that waits for torch's stream while torch captures it: record the *_op form", capi.ERR_ARG)

@@ -108,7 +108,7 @@ def test_calls_over_tensors_run_on_torchs_stream(monkeypatch, name):
         raise Made
 
     asked = []
-    fake = types.SimpleNamespace(cuda=types.SimpleNamespace(is_current_stream_capturing=lambda: False, current_stream=lambda ordinal: (asked.append(ordinal), types.SimpleNamespace(cuda_stream=0))[1]))
+    fake = types.SimpleNamespace(cuda=types.SimpleNamespace(is_initialized=lambda: True, is_current_stream_capturing=lambda: False, current_stream=lambda ordinal: (asked.append(ordinal), types.SimpleNamespace(cuda_stream=0))[1]))
     monkeypatch.setitem(sys.modules, "torch", fake)
     monkeypatch.setattr(gpu_utils, "ArrowComputePipeline", make)
     arguments, call = CALLS[name]
@@ -129,7 +129,7 @@ def test_fused_chains_over_tensors_run_on_torchs_stream(monkeypatch):
         made.append(hip_stream)
         raise Made
 
-    monkeypatch.setitem(sys.modules, "torch", types.SimpleNamespace(cuda=types.SimpleNamespace(is_current_stream_capturing=lambda: False, current_stream=lambda o: types.SimpleNamespace(cuda_stream=5))))
+    monkeypatch.setitem(sys.modules, "torch", types.SimpleNamespace(cuda=types.SimpleNamespace(is_initialized=lambda: True, is_current_stream_capturing=lambda: False, current_stream=lambda o: types.SimpleNamespace(cuda_stream=5))))
     monkeypatch.setattr(gpu_utils, "ArrowComputePipeline", make)
     for head, step, other in ((True, False, False), (False, True, False), (False, False, True), (False, False, False)):
         chain = ag.FusedChain(FLOATS(9, head)).add(FLOATS(9, step))
@@ -143,7 +143,7 @@ def test_fused_chains_over_tensors_run_on_torchs_stream(monkeypatch):
 
 def test_reading_back_waits_for_torchs_stream(monkeypatch):
     waited = []
-    fake = types.SimpleNamespace(cuda=types.SimpleNamespace(is_current_stream_capturing=lambda: False, current_stream=lambda o: types.SimpleNamespace(cuda_stream=5, synchronize=lambda: waited.append(o))))
+    fake = types.SimpleNamespace(cuda=types.SimpleNamespace(is_initialized=lambda: True, is_current_stream_capturing=lambda: False, current_stream=lambda o: types.SimpleNamespace(cuda_stream=5, synchronize=lambda: waited.append(o))))
     monkeypatch.setitem(sys.modules, "torch", fake)
 
     def download(*a, **k):
@@ -227,10 +227,27 @@ def test_a_tensor_of_truth_values_is_no_bitmap():
 
 
 def test_a_call_that_waits_is_refused_while_torch_captures(monkeypatch):
-    fake = types.SimpleNamespace(cuda=types.SimpleNamespace(is_current_stream_capturing=lambda: True, current_stream=lambda o: 1 / 0))
+    fake = types.SimpleNamespace(cuda=types.SimpleNamespace(is_initialized=lambda: True, is_current_stream_capturing=lambda: True, current_stream=lambda o: 1 / 0))
     monkeypatch.setitem(sys.modules, "torch", fake)
     for call in (lambda: ag.take_quantised(CACHE(True), INDEX(3, True), out=ROWS((3, 2, 8), True)), lambda: FLOATS(9, True).add(FLOATS(9, False)),
                  lambda: gpu_utils.GpuDevice.retrive_data(DEV, FLOATS(9, True).data)):
         with pytest.raises(ag.ArrowErrorGPU) as e:
             call()
         assert e.value.status == ag._capi.ERR_ARG and "captures" in str(e.value)
+
+
+def test_tensors_of_another_library(monkeypatch):
+    """torch not loaded, or loaded for the CPU alone: a pipeline of the call's own, and torch is not woken"""
+    made = []
+
+    def make(device, label=None, hip_stream=None, fuse=None):
+        made.append(hip_stream)
+        raise Made
+
+    monkeypatch.setattr(gpu_utils, "ArrowComputePipeline", make)
+    for torch in (None, types.SimpleNamespace(cuda=types.SimpleNamespace(is_initialized=lambda: False, current_stream=lambda o: 1 / 0, is_current_stream_capturing=lambda: 1 / 0))):
+        monkeypatch.setitem(sys.modules, "torch", torch)
+        with pytest.raises(Made):
+            FLOATS(9, True).add(FLOATS(9, True))
+        assert made.pop() is None
+        gpu_utils.settle(DEV, FLOATS(9, True))
